@@ -3,8 +3,9 @@
  *
  * Conventions for every entry point:
  *  - Pointers are CUDA device pointers unless named *_host; sizes are element counts.
- *  - All floating-point buffers are fp32, row-major, densely packed unless a leading dimension
- *    (ld*) is given. Index buffers are int32.
+ *  - All floating-point buffers are fp32 (the last section's have the type that its `dtype`
+ *    names), row-major, densely packed unless a leading dimension (ld*) is given. Index buffers
+ *    are int32.
  *  - Outputs are allocated by the caller. No entry point allocates device memory, except
  *    atom_neighbor_list, which uses caller-provided scratch (see its comment).
  *  - `stream` is a cudaStream_t passed as void*; work is stream-ordered and asynchronous.
@@ -34,6 +35,13 @@ enum {
     ATOM_ERR_CUDA = 2,         /* CUDA runtime / launch error */
     ATOM_ERR_CAPACITY = 3,     /* a device-side capacity was exceeded (retry with more room) */
     ATOM_ERR_UNSUPPORTED = 4   /* shape the kernels do not implement */
+};
+
+/* Element types of the typed operators (the last section); everything else is fp32. */
+enum {
+    ATOM_F32 = 0,
+    ATOM_BF16 = 1,
+    ATOM_F16 = 2
 };
 
 /* Copies the last error message of this host thread into buf (NUL-terminated); returns its
@@ -479,6 +487,69 @@ int atom_row_broadcast(const float* v, int64_t N, int C, float scale, float* out
 int atom_orb_zbl(const float* ev, const int* Z, const int* src, const int* tgt, int64_t E,
                  const double* rcov, int nrad, double scale, float* g_ev, double* partials,
                  double* energy, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Typed operators: a gated feed-forward block and low-rank adapters, with their backward
+ * passes, in fp32, bf16 and fp16. No counterparts in the reference (its feed-forwards are
+ * tt_atom/grid.py and tt_atom/spectral.py, it has one set of weights per composition,
+ * tt_atom/bundle_cache.py, and input adjoints only).
+ *
+ * x, y, dy, dx are [M, width] with a leading dimension of at least the width (in elements);
+ * weights and their gradients are dense; one call's operands have one type. Sums are fp32.
+ * Any sizes and element-aligned pointers: operands whose rows do not start on 16 bytes are
+ * copied to the workspace first. `ws`: ws_bytes of device memory, 256-byte aligned, as large as
+ * the *_bytes query says, not used by two calls at a time. M = 0: no rows are written, weight
+ * and adapter gradients are zeroed.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Sizes in bytes, to bytes_host[3]: the workspace of atom_gated_ff_fwd, that of
+ * atom_gated_ff_bwd, and `kept`. */
+int atom_gated_ff_bytes(int dtype, int64_t M, int D, int F, int O, size_t* bytes_host);
+
+/* y = (act(x wg^T) * (x wu^T)) wd^T: x [M, D], wg, wu [F, D], wd [O, F], y [M, O]. act: 0 SiLU,
+ * 1 sigmoid, 2 GELU (erf). The gated row is rounded to the type before the product with wd
+ * (fp32: not). kept (NULL, or device memory, 256-byte aligned): what atom_gated_ff_bwd needs to
+ * spare the first two products. */
+int atom_gated_ff_fwd(int dtype, const void* x, int64_t ldx, int64_t M, int D, int F, int O,
+                      const void* wg, const void* wu, const void* wd, int act, void* y,
+                      int64_t ldy, void* kept, void* ws, size_t ws_bytes, void* stream);
+
+/* VJP of atom_gated_ff_fwd: from dy [M, O], dx [M, D], dwg, dwu [F, D] and dwd [O, F]
+ * (overwritten; each may be NULL). kept: as the forward call on the same inputs left it, or
+ * NULL (the first two products are computed again). */
+int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t M, int D, int F, int O,
+                      const void* wg, const void* wu, const void* wd, int act, const void* dy,
+                      int64_t lddy, const void* kept, void* dx, int64_t lddx, void* dwg,
+                      void* dwu, void* dwd, void* ws, size_t ws_bytes, void* stream);
+
+/* Sizes in bytes, to bytes_host[3]: the workspace of atom_adapted_linear_fwd, that of
+ * atom_adapted_linear_bwd, and `kept`. */
+int atom_adapted_linear_bytes(int dtype, int64_t M, int D, int O, int n_adapters, int R, int nreq,
+                              size_t* bytes_host);
+
+/* Low-rank adapters of many requests beside one projection: for the rows m of request r
+ * (req_ptr[r] <= m < req_ptr[r + 1]) with k = req_adapter[r],
+ *   y[m] = x[m] w^T + scale[k] (x[m] a[k]^T) b[k]^T;
+ * where k is not in 0 .. n_adapters - 1, and for rows of no request, y[m] = x[m] w^T. w [O, D],
+ * a [n_adapters, R, D], b [n_adapters, O, R], scale [n_adapters] fp32, 1 <= R <= 128; req_ptr
+ * [nreq + 1] ascending and req_adapter [nreq] int32 on the device (bounds outside 0 .. M are
+ * clamped). Requests may be empty, and several may have the same adapter. kept (may be NULL):
+ * what atom_adapted_linear_bwd needs to spare the product x a^T. */
+int atom_adapted_linear_fwd(int dtype, const void* x, int64_t ldx, int64_t M, int D, int O,
+                            const void* w, const void* a, const void* b, const float* scale,
+                            int n_adapters, int R, const int* req_ptr, const int* req_adapter,
+                            int nreq, void* y, int64_t ldy, void* kept, void* ws,
+                            size_t ws_bytes, void* stream);
+
+/* VJP of atom_adapted_linear_fwd: from dy [M, O], dx [M, D], da [n_adapters, R, D] and
+ * db [n_adapters, O, R] (overwritten, zeros for an adapter of no request; each may be NULL).
+ * w has no gradient here. kept: as the forward call on the same inputs left it, or NULL. */
+int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, int64_t M, int D, int O,
+                            const void* w, const void* a, const void* b, const float* scale,
+                            int n_adapters, int R, const int* req_ptr, const int* req_adapter,
+                            int nreq, const void* dy, int64_t lddy, const void* kept, void* dx,
+                            int64_t lddx, void* da, void* db, void* ws, size_t ws_bytes,
+                            void* stream);
 
 #ifdef __cplusplus
 }

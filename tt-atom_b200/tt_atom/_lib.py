@@ -17,7 +17,7 @@ ATOM_ERR_CAPACITY = 3
 ATOM_ERR_UNSUPPORTED = 4
 
 c_void_p, c_int, c_int64, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
-c_double = ctypes.c_double
+c_double, c_size_t = ctypes.c_double, ctypes.c_size_t
 
 
 class CellGrid(ctypes.Structure):
@@ -133,6 +133,22 @@ _SIGS = {
     "atom_row_broadcast": (c_void_p, c_int64, c_int, c_float, c_void_p, c_int64, c_int,
                            c_void_p),
     "atom_edge_species": (c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p),
+    "atom_gated_ff_bytes": (c_int, c_int64, c_int, c_int, c_int, c_void_p),
+    "atom_gated_ff_fwd": (c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p,
+                          c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p,
+                          c_size_t, c_void_p),
+    "atom_gated_ff_bwd": (c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p,
+                          c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p,
+                          c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p),
+    "atom_adapted_linear_bytes": (c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p),
+    "atom_adapted_linear_fwd": (c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p,
+                                c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p,
+                                c_int, c_void_p, c_int64, c_void_p, c_void_p, c_size_t,
+                                c_void_p),
+    "atom_adapted_linear_bwd": (c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p,
+                                c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p,
+                                c_int, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
+                                c_void_p, c_void_p, c_size_t, c_void_p),
 }
 
 
