@@ -3,6 +3,50 @@
 
 namespace atom {
 
+// 64 x 64 tile, 16 deep, 4 x 4 outputs a thread.
+__global__ void __launch_bounds__(256) plain_product_kernel(PlainProduct p) {
+    __shared__ float As[16][64 + 1], Bs[16][64 + 1];
+    const long long m0 = (long long)blockIdx.y * 64, n0 = (long long)blockIdx.x * 64;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    float acc[4][4] = {};
+    const long long kp = (p.K + 15) / 16 * 16;
+    for (long long kk = 0; kk < (p.A2 ? 2 * kp : kp); kk += 16) {
+        const void* A = kk < kp ? p.A : p.A2;
+        const void* B = kk < kp ? p.B : p.B2;
+        const long long k0 = kk < kp ? kk : kk - kp;
+        for (int i = threadIdx.x; i < 1024; i += 256) {
+            const int r = p.ak == 1 ? i >> 4 : i & 63, k = p.ak == 1 ? i & 15 : i >> 6;
+            const int rb = p.bk == 1 ? i >> 4 : i & 63, kb = p.bk == 1 ? i & 15 : i >> 6;
+            As[k][r] = m0 + r < p.M && k0 + k < p.K
+                           ? load_f(A, (m0 + r) * p.am + (k0 + k) * p.ak, p.ta) : 0.f;
+            Bs[kb][rb] = n0 + rb < p.N && k0 + kb < p.K
+                             ? load_f(B, (n0 + rb) * p.bn + (k0 + kb) * p.bk, p.tb) : 0.f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[i][j] = fmaf(As[k][ty + 16 * i], Bs[k][tx + 16 * j], acc[i][j]);
+        __syncthreads();
+    }
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 4; ++j) {
+            const long long m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
+            if (m >= p.M || n >= p.N) continue;
+            store_f(p.C, m * p.ldc + n, acc[i][j], p.tc);
+        }
+}
+
+int plain_product(const PlainProduct& p, cudaStream_t st) {
+    if (p.M == 0 || p.N == 0) return ATOM_OK;
+    ATOM_REQUIRE(ceil_div(p.M, 64) < 65536, "too many rows");
+    plain_product_kernel<<<dim3(ceil_div(p.N, 64), ceil_div(p.M, 64)), 256, 0, st>>>(p);
+    return check_launch("plain product");
+}
+
 struct Requests {
     const int* ptr;
     const int* adapter;

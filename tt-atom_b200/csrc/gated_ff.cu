@@ -1,78 +1,310 @@
-// The gated feed-forward block Y = (act(X Wg^T) * (X Wu^T)) Wd^T and its backward pass.
-#include "typed.cuh"
+// The gated feed-forward block Y = (act(X Wg^T) * (X Wu^T)) Wd^T and its backward pass, as pair
+// products (pair_product.cu) with the gate in their epilogues:
+//   forward   [G | U] tiles -> H = act(G) U;  Y = H Wd^T
+//   backward  dH = dY Wd, then [G | U] again with dH in the epilogue -> dG, dU, H (or, with the
+//             forward's G and U kept, dH tiles with G and U in the epilogue);
+//             dX = [dG | dU] [Wg; Wu],  dWg, dWu = [dG | dU]^T X,  dWd = dY^T H
+// The transposed products read their operands as they lie (M/N-major tiles), so nothing is
+// transposed in memory.
+#include <initializer_list>
+
+#include "pair_product.cuh"
 
 namespace atom {
+namespace {
 
-// 64 x 64 tile, 16 deep, 4 x 4 outputs a thread.
-__global__ void __launch_bounds__(256) plain_product_kernel(PlainProduct p) {
-    __shared__ float As[16][64 + 1], Bs[16][64 + 1];
-    const long long m0 = (long long)blockIdx.y * 64, n0 = (long long)blockIdx.x * 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    const long long kp = (p.K + 15) / 16 * 16;
-    for (long long kk = 0; kk < (p.A2 ? 2 * kp : kp); kk += 16) {
-        const void* A = kk < kp ? p.A : p.A2;
-        const void* B = kk < kp ? p.B : p.B2;
-        const long long k0 = kk < kp ? kk : kk - kp;
-        for (int i = threadIdx.x; i < 1024; i += 256) {
-            const int r = p.ak == 1 ? i >> 4 : i & 63, k = p.ak == 1 ? i & 15 : i >> 6;
-            const int rb = p.bk == 1 ? i >> 4 : i & 63, kb = p.bk == 1 ? i & 15 : i >> 6;
-            As[k][r] = m0 + r < p.M && k0 + k < p.K
-                           ? load_f(A, (m0 + r) * p.am + (k0 + k) * p.ak, p.ta) : 0.f;
-            Bs[kb][rb] = n0 + rb < p.N && k0 + kb < p.K
-                             ? load_f(B, (n0 + rb) * p.bn + (k0 + kb) * p.bk, p.tb) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] = fmaf(As[k][ty + 16 * i], Bs[k][tx + 16 * j], acc[i][j]);
-        __syncthreads();
+using namespace pair;
+
+// A 16-bit operand ready for TMA (fp32: its hi plane, the lo plane `plane` elements behind).
+struct Operand {
+    const void* p = nullptr;
+    long long rows = 0, cols = 0, ld = 0, plane = 0;
+    Operand columns(long long c0, long long n) const {
+        Operand o = *this;
+        o.p = static_cast<const __half*>(p) + c0;
+        o.cols = n;
+        return o;
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const long long m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-            if (m >= p.M || n >= p.N) continue;
-            store_f(p.C, m * p.ldc + n, acc[i][j], p.tc);
-        }
-}
+};
 
-int plain_product(const PlainProduct& p, cudaStream_t st) {
-    if (p.M == 0 || p.N == 0) return ATOM_OK;
-    ATOM_REQUIRE(ceil_div(p.M, 64) < 65536, "too many rows");
-    plain_product_kernel<<<dim3(ceil_div(p.N, 64), ceil_div(p.M, 64)), 256, 0, st>>>(p);
-    return check_launch("plain product");
-}
+struct FfSizes {
+    int dtype;
+    long long M;
+    int D, F, O;
+    long long Dp, Fp, Op;       // widths of packed rows
+    bool split;
+    FfSizes(int t, long long m, int d, int f, int o)
+        : dtype(t), M(m), D(d), F(f), O(o), Dp(up(d, 8)), Fp(up(f, 32)), Op(up(o, 8)),
+          split(t == ATOM_F32) {}
+    int nk(long long k) const { return (int)((k + 63) / 64); }
+    Choice gate() const { return choose(M, F, nk(D), 1, true, split, false); }
+    Choice down() const { return choose(M, O, nk(F), 1, false, split, true); }
+    Choice dh() const { return choose(M, F, nk(O), 1, false, split, false); }
+    Choice dx() const { return choose(M, D, 2 * nk(F), 1, false, split, false); }
+    Choice dwgu() const { return choose(F, D, nk(M), 2, false, split, true); }
+    Choice dwd() const { return choose(O, F, nk(M), 1, false, split, true); }
+};
 
-// H = act(G) U; with dH: dG and dU in place of G and U.
-__global__ void gate_kernel(float* G, float* U, const float* dH, float* H, long long n, int act) {
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
-        float a, da;
-        const float u = U[i];
-        act_grad(G[i], act, a, da);
-        H[i] = a * u;
-        if (dH) {
-            G[i] = dH[i] * u * da;
-            U[i] = dH[i] * a;
+// One call's buffers. 16-bit operands are packed only where TMA cannot read them; fp32 ones
+// always become two planes.
+struct FfSpace {
+    __half *x, *wg, *wu, *wd, *dy, *xt, *dyt, *hp, *dgup, *dgut, *ht;
+    float *xr, *dyr, *hr, *dgur, *H32, *dgu32, *dh, *part;
+    __half *H, *dgu;
+    unsigned* max;              // x, wg | wu, wd, dy, dgu, h
+    size_t bytes;
+    FfSpace(void* ws, const FfSizes& z, bool bwd) {
+        memset(this, 0, sizeof(*this));
+        Cursor c(ws);
+        const long long M = z.M, k = z.split ? 2 : 1;
+        x = c.take<__half>(k * M * z.Dp);
+        wg = c.take<__half>(k * z.F * z.Dp);
+        wu = c.take<__half>(k * z.F * z.Dp);
+        wd = c.take<__half>(k * z.O * z.Fp);
+        size_t pf = z.down().part;
+        if (bwd) {
+            pf = z.dwgu().part > z.dwd().part ? z.dwgu().part : z.dwd().part;
+            dy = c.take<__half>(k * M * z.Op);
+            dh = c.take<float>(M * z.Fp);
         }
+        part = c.take<float>(pf);
+        if (!z.split) {
+            H = c.take<__half>(M * z.Fp);
+            if (bwd) dgu = c.take<__half>(2 * M * z.Fp);
+        } else {
+            max = c.take<unsigned>(8);
+            xr = c.take<float>(M);
+            H32 = c.take<float>(M * z.Fp);
+            if (!bwd) {
+                hp = c.take<__half>(2 * M * z.Fp);
+                hr = c.take<float>(M);
+            } else {
+                dyr = c.take<float>(M);
+                dgu32 = c.take<float>(2 * M * z.Fp);
+                dgup = c.take<__half>(4 * M * z.Fp);
+                dgur = c.take<float>(M);
+                xt = c.take<__half>(2 * M * z.Dp);
+                dyt = c.take<__half>(2 * M * z.Op);
+                dgut = c.take<__half>(4 * M * z.Fp);
+                ht = c.take<__half>(2 * M * z.Fp);
+            }
+        }
+        bytes = c.used;
     }
+};
+
+// Fills a map (and, for two planes, the next one).
+int put(Maps& maps, int i, const Operand& o, bool mn, int box_rows, bool split) {
+    for (int pl = 0; pl < (split ? 2 : 1); ++pl)
+        if (int s = make_map(&maps.m[i + pl], static_cast<const __half*>(o.p) + pl * o.plane, o.cols,
+                             o.rows, o.ld, mn ? 64 : box_rows))
+            return s;
+    return ATOM_OK;
 }
 
-static int gate(float* G, float* U, const float* dH, float* H, long long n, int act,
-                cudaStream_t st) {
-    const long long blocks = (n + 255) / 256;
-    gate_kernel<<<(int)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(G, U, dH, H, n, act);
-    return check_launch("gate");
-}
+struct Ff {
+    FfSizes z;
+    FfSpace sp;
+    cudaStream_t st;
+    int act;
+    Operand x, wg, wu, wd, dy;
+    PrepList list;
 
-}  // namespace atom
+    // an operand of this call: as it lies, or through the list's packing / planes
+    Operand take(const void* p, long long rows, long long cols, long long ld, __half* buf,
+                 long long pitch, int mode, float* rinv, unsigned* max) {
+        if (!z.split && tma_ready(p, ld)) return {p, rows, cols, ld, 0};
+        list.add({p, rows, cols, ld, buf, pitch, rows * pitch, rinv, max, z.split ? mode : kPack});
+        return {buf, rows, cols, pitch, rows * pitch};
+    }
+    // weights, x (and dy) brought into the form that the products read
+    int inputs(const void* xp, long long ldx, const void* g, const void* u, const void* d,
+               const void* dyp, long long lddy) {
+        if (z.split) {
+            const cudaError_t e = cudaMemsetAsync(sp.max, 0, 32, st);
+            if (e != cudaSuccess) {
+                set_error("gated_ff: %s", cudaGetErrorString(e));
+                return ATOM_ERR_CUDA;
+            }
+            list.add({g, z.F, z.D, z.D, nullptr, 0, 0, nullptr, sp.max + 1, kMax});
+            list.add({u, z.F, z.D, z.D, nullptr, 0, 0, nullptr, sp.max + 1, kMax});
+            list.add({d, z.O, z.F, z.F, nullptr, 0, 0, nullptr, sp.max + 2, kMax});
+        }
+        x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kRowSplit, sp.xr, sp.max);
+        if (dyp) dy = take(dyp, z.M, z.O, lddy, sp.dy, z.Op, kRowSplit, sp.dyr, sp.max + 3);
+        if (z.split) {
+            if (int s = prepare(list, st)) return s;
+            list.n = 0;
+        }
+        wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kTensorSplit, nullptr, sp.max + 1);
+        wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kTensorSplit, nullptr, sp.max + 1);
+        wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kTensorSplit, nullptr, sp.max + 2);
+        const int s = prepare(list, st);
+        list.n = 0;
+        return s;
+    }
+    Args args(long long M, int N) const {
+        Args p;
+        memset(&p, 0, sizeof(p));
+        p.M = M;
+        p.N = N;
+        p.groups = 1;
+        p.nphase = 1;
+        p.bf16 = z.dtype == ATOM_BF16;
+        p.act = act;
+        p.Fp = (int)z.Fp;
+        p.dtype = z.dtype;
+        p.part = sp.part;
+        return p;
+    }
+    int step() const { return z.split ? 2 : 1; }
+    void output(Args& p, void* C, long long ldc) const {
+        p.C[0] = C;
+        p.ldc = ldc;
+        p.vec = aligned16(C) && ldc * dtype_size(p.dtype) % 16 == 0;
+    }
+    // [G | U] tiles of X
+    int gates(int epilogue, Args& p, void* C, long long ldc) {
+        const Choice c = z.gate();
+        const int k = step();
+        Maps maps;
+        if (int s = put(maps, 0, x, false, 128, z.split)) return s;
+        if (int s = put(maps, k, wg, false, c.bn / 2, z.split)) return s;
+        if (int s = put(maps, 2 * k, wu, false, c.bn / 2, z.split)) return s;
+        p.ph[0] = {0, k, 2 * k, z.nk(z.D), 0, 0, c.bn / 2, 0};
+        p.rinv = sp.xr;
+        p.bmax = sp.max + 1;
+        output(p, C, ldc);
+        return launch(epilogue, c, z.split, maps, p, st);
+    }
+    int forward(void* y, long long ldy, float* kept) {
+        Args p = args(z.M, z.F);
+        p.gu = kept;
+        if (int s = gates(kGate, p, z.split ? (void*)sp.H32 : sp.H, z.Fp)) return s;
+        Operand h{sp.H, z.M, z.F, z.Fp, 0};
+        if (z.split) {
+            list.add({sp.H32, z.M, z.F, z.Fp, sp.hp, z.Fp, z.M * z.Fp, sp.hr, nullptr, kRowSplit});
+            if (int s = prepare(list, st)) return s;
+            h = {sp.hp, z.M, z.F, z.Fp, z.M * z.Fp};
+        }
+        const Choice c = z.down();
+        const int k = step();
+        Maps maps;
+        if (int s = put(maps, 0, h, false, 128, z.split)) return s;
+        if (int s = put(maps, k, wd, false, c.bn / 2, z.split)) return s;
+        Args q = args(z.M, z.O);
+        q.ph[0] = {0, k, k, z.nk(z.F), 0, 0, c.bn, c.bn / 2};
+        q.rinv = sp.hr;
+        q.bmax = sp.max + 2;
+        output(q, y, ldy);
+        return launch(kStore, c, z.split, maps, q, st);
+    }
+    int backward(const float* kept, void* dx, long long lddx, void* dwg, void* dwu, void* dwd) {
+        const int k = step();
+        void* dgu = z.split ? (void*)sp.dgu32 : sp.dgu;
+        void* H = !dwd ? nullptr : z.split ? (void*)sp.H32 : sp.H;
+        {   // dH, and dG, dU, H either in its epilogue or in that of G and U
+            const Choice c = z.dh();
+            Maps maps;
+            if (int s = put(maps, 0, dy, false, 128, z.split)) return s;
+            if (int s = put(maps, k, wd, true, 64, z.split)) return s;
+            Args p = args(z.M, z.F);
+            p.ph[0] = {0, k, k, z.nk(z.O), 0, 1, c.bn, c.bn / 2};
+            p.rinv = sp.dyr;
+            p.bmax = sp.max + 2;
+            p.hmax = sp.max + 4;
+            p.H = H;
+            if (kept) {
+                p.gu = const_cast<float*>(kept);
+                output(p, dgu, 2 * z.Fp);
+                if (int s = launch(kGateBwdDH, c, z.split, maps, p, st)) return s;
+            } else {
+                p.dtype = ATOM_F32;
+                output(p, sp.dh, z.Fp);
+                if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
+                Args q = args(z.M, z.F);
+                q.dh = sp.dh;
+                q.H = H;
+                q.hmax = sp.max + 4;
+                if (int s = gates(kGateBwdGU, q, dgu, 2 * z.Fp)) return s;
+            }
+        }
+        Operand g{sp.dgu, z.M, 2 * z.Fp, 2 * z.Fp, 0}, gt = g, h{sp.H, z.M, z.F, z.Fp, 0};
+        Operand xt = x, dyt = dy;
+        if (z.split) {
+            const long long M = z.M, W = 2 * z.Fp;
+            g = {sp.dgup, M, W, W, M * W};
+            gt = {sp.dgut, M, W, W, M * W};
+            h = {sp.ht, M, z.F, z.Fp, M * z.Fp};
+            if (dx) list.add({sp.dgu32, M, W, W, sp.dgup, W, M * W, sp.dgur, nullptr, kRowSplit});
+            if (dwg || dwu) {
+                list.add({sp.dgu32, M, W, W, sp.dgut, W, M * W, nullptr, sp.max + 4, kTensorSplit});
+                xt.p = sp.xt;
+                list.add({x_src, M, z.D, x_ld, sp.xt, z.Dp, M * z.Dp, nullptr, sp.max,
+                          kTensorSplit});
+            }
+            if (dwd) {
+                list.add({sp.H32, M, z.F, z.Fp, sp.ht, z.Fp, M * z.Fp, nullptr, sp.max + 5,
+                          kTensorSplit});
+                dyt.p = sp.dyt;
+                list.add({dy_src, M, z.O, dy_ld, sp.dyt, z.Op, M * z.Op, nullptr, sp.max + 3,
+                          kTensorSplit});
+            }
+            if (int s = prepare(list, st)) return s;
+        }
+        if (dx) {
+            const Choice c = z.dx();
+            Maps maps;
+            if (int s = put(maps, 0, g.columns(0, z.F), false, 128, z.split)) return s;
+            if (int s = put(maps, k, g.columns(z.Fp, z.F), false, 128, z.split)) return s;
+            if (int s = put(maps, 2 * k, wg, true, 64, z.split)) return s;
+            if (int s = put(maps, 3 * k, wu, true, 64, z.split)) return s;
+            Args p = args(z.M, z.D);
+            p.nphase = 2;
+            p.ph[0] = {0, 2 * k, 2 * k, z.nk(z.F), 0, 1, c.bn, c.bn / 2};
+            p.ph[1] = {k, 3 * k, 3 * k, z.nk(z.F), 0, 1, c.bn, c.bn / 2};
+            p.rinv = sp.dgur;
+            p.bmax = sp.max + 1;
+            output(p, dx, lddx);
+            if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
+        }
+        if (dwg || dwu) {
+            Choice c = z.dwgu();
+            const bool two = dwg && dwu;
+            Maps maps;
+            if (int s = put(maps, 0, gt.columns(dwg ? 0 : z.Fp, z.F), true, 64, z.split)) return s;
+            if (two)
+                if (int s = put(maps, k, gt.columns(z.Fp, z.F), true, 64, z.split)) return s;
+            if (int s = put(maps, 2 * k, xt, true, 64, z.split)) return s;
+            Args p = args(z.F, z.D);
+            p.groups = two ? 2 : 1;
+            p.ph[0] = {0, 2 * k, 2 * k, z.nk(z.M), 1, 1, c.bn, c.bn / 2};
+            p.amax = sp.max + 4;
+            p.bmax = sp.max;
+            output(p, dwg ? dwg : dwu, z.D);
+            p.C[1] = dwu;
+            p.vec = p.vec && aligned16(dwu ? dwu : dwg);
+            if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
+        }
+        if (dwd) {
+            const Choice c = z.dwd();
+            Maps maps;
+            if (int s = put(maps, 0, dyt, true, 64, z.split)) return s;
+            if (int s = put(maps, k, h, true, 64, z.split)) return s;
+            Args p = args(z.O, z.F);
+            p.ph[0] = {0, k, k, z.nk(z.M), 1, 1, c.bn, c.bn / 2};
+            p.amax = sp.max + 3;
+            p.bmax = sp.max + 5;
+            output(p, dwd, z.F);
+            if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
+        }
+        return ATOM_OK;
+    }
+    const void *x_src = nullptr, *dy_src = nullptr;
+    long long x_ld = 0, dy_ld = 0;
+};
 
-using namespace atom;
-
-static int check_ff(int dtype, int64_t M, int D, int F, int O, int act) {
+int check_ff(int dtype, int64_t M, int D, int F, int O, int act) {
     ATOM_REQUIRE(dtype >= ATOM_F32 && dtype <= ATOM_F16, "gated_ff: unknown type %d", dtype);
     ATOM_REQUIRE(M >= 0 && M < (1LL << 31) && D > 0 && F > 0 && O > 0, "gated_ff: bad sizes");
     ATOM_REQUIRE(D < (1 << 24) && F < (1 << 24) && O < (1 << 24), "gated_ff: widths above 2^24");
@@ -80,25 +312,18 @@ static int check_ff(int dtype, int64_t M, int D, int F, int O, int act) {
     return ATOM_OK;
 }
 
-struct FfSpace {
-    float *G, *U, *H, *dH;
-    FfSpace(Cursor& c, int64_t M, int F, bool bwd) {
-        G = c.take<float>(M * F);
-        U = c.take<float>(M * F);
-        H = c.take<float>(M * F);
-        dH = bwd ? c.take<float>(M * F) : nullptr;
-    }
-};
+}  // namespace
+}  // namespace atom
+
+using namespace atom;
 
 extern "C" int atom_gated_ff_bytes(int dtype, int64_t M, int D, int F, int O, size_t* bytes_host) {
     if (int s = check_ff(dtype, M, D, F, O, 0)) return s;
     ATOM_REQUIRE(bytes_host, "gated_ff: bytes_host is NULL");
-    Cursor f(nullptr), b(nullptr);
-    FfSpace(f, M, F, false);
-    FfSpace(b, M, F, true);
-    bytes_host[0] = f.used;
-    bytes_host[1] = b.used;
-    bytes_host[2] = 256;
+    const FfSizes z(dtype, M, D, F, O);
+    bytes_host[0] = FfSpace(nullptr, z, false).bytes;
+    bytes_host[1] = FfSpace(nullptr, z, true).bytes;
+    bytes_host[2] = (size_t)M * 2 * z.Fp * sizeof(float);
     return ATOM_OK;
 }
 
@@ -109,15 +334,12 @@ extern "C" int atom_gated_ff_fwd(int dtype, const void* x, int64_t ldx, int64_t 
     if (int s = check_ff(dtype, M, D, F, O, act)) return s;
     if (M == 0) return ATOM_OK;
     ATOM_REQUIRE(x && wg && wu && wd && y && ldx >= D && ldy >= O, "gated_ff: bad operand");
-    Cursor c(ws);
-    FfSpace sp(c, M, F, false);
-    ATOM_REQUIRE(ws && ws_bytes >= c.used, "gated_ff: the workspace needs %zu bytes", c.used);
-    cudaStream_t st = (cudaStream_t)stream;
-    const int t = dtype;
-    if (int s = plain_product({x, ldx, 1, t, wg, D, 1, t, sp.G, F, 0, M, F, D}, st)) return s;
-    if (int s = plain_product({x, ldx, 1, t, wu, D, 1, t, sp.U, F, 0, M, F, D}, st)) return s;
-    if (int s = gate(sp.G, sp.U, nullptr, sp.H, M * F, act, st)) return s;
-    return plain_product({sp.H, F, 1, 0, wd, F, 1, t, y, ldy, t, M, O, F}, st);
+    const FfSizes z(dtype, M, D, F, O);
+    Ff f{z, FfSpace(ws, z, false), (cudaStream_t)stream, act};
+    ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
+                 f.sp.bytes);
+    if (int s = f.inputs(x, ldx, wg, wu, wd, nullptr, 0)) return s;
+    return f.forward(y, ldy, static_cast<float*>(kept));
 }
 
 extern "C" int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t M, int D, int F,
@@ -127,38 +349,20 @@ extern "C" int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t 
                                  size_t ws_bytes, void* stream) {
     if (int s = check_ff(dtype, M, D, F, O, act)) return s;
     cudaStream_t st = (cudaStream_t)stream;
-    const int t = dtype;
-    if (M > 0) {
-        ATOM_REQUIRE(x && wg && wu && wd && dy && ldx >= D && lddy >= O && (!dx || lddx >= D),
-                     "gated_ff: bad operand");
-        Cursor c(ws);
-        FfSpace sp(c, M, F, true);
-        ATOM_REQUIRE(ws && ws_bytes >= c.used, "gated_ff: the workspace needs %zu bytes", c.used);
-        if (int s = plain_product({x, ldx, 1, t, wg, D, 1, t, sp.G, F, 0, M, F, D}, st))
-            return s;
-        if (int s = plain_product({x, ldx, 1, t, wu, D, 1, t, sp.U, F, 0, M, F, D}, st))
-            return s;
-        if (int s = plain_product({dy, lddy, 1, t, wd, 1, F, t, sp.dH, F, 0, M, F, O}, st))
-            return s;
-        if (int s = gate(sp.G, sp.U, sp.dH, sp.H, M * F, act, st)) return s;
-        if (dx) {
-            if (int s = plain_product({sp.G, F, 1, 0, wg, 1, D, t, dx, lddx, t, M, D, F, sp.U, wu},
-                                      st))
-                return s;
-        }
-        if (dwg)
-            if (int s = plain_product({sp.G, 1, F, 0, x, 1, ldx, t, dwg, D, t, F, D, M}, st))
-                return s;
-        if (dwu)
-            if (int s = plain_product({sp.U, 1, F, 0, x, 1, ldx, t, dwu, D, t, F, D, M}, st))
-                return s;
-        if (dwd)
-            if (int s = plain_product({dy, 1, lddy, t, sp.H, 1, F, 0, dwd, F, t, O, F, M}, st))
-                return s;
-        return ATOM_OK;
+    if (M == 0) {
+        const size_t e = dtype_size(dtype);
+        for (void* p : {dwg, dwu})
+            if (p) cudaMemsetAsync(p, 0, e * F * D, st);
+        if (dwd) cudaMemsetAsync(dwd, 0, e * O * F, st);
+        return check_launch("gated_ff", 0);
     }
-    const size_t e = dtype_size(dtype);
-    for (void* p : {dwg, dwu}) if (p) cudaMemsetAsync(p, 0, e * F * D, st);
-    if (dwd) cudaMemsetAsync(dwd, 0, e * O * F, st);
-    return check_launch("gated_ff", 0);
+    ATOM_REQUIRE(x && wg && wu && wd && dy && ldx >= D && lddy >= O && (!dx || lddx >= D),
+                 "gated_ff: bad operand");
+    const FfSizes z(dtype, M, D, F, O);
+    Ff f{z, FfSpace(ws, z, true), st, act};
+    ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
+                 f.sp.bytes);
+    f.x_src = x, f.x_ld = ldx, f.dy_src = dy, f.dy_ld = lddy;
+    if (int s = f.inputs(x, ldx, wg, wu, wd, dy, lddy)) return s;
+    return f.backward(static_cast<const float*>(kept), dx, lddx, dwg, dwu, dwd);
 }

@@ -1,0 +1,99 @@
+// Host side of the pair products (pair_product.cu): operands, tile choice, launches.
+#pragma once
+
+#include <cuda.h>
+
+#include "typed.cuh"
+
+namespace atom {
+namespace pair {
+
+constexpr int kMaps = 12;
+struct Maps {
+    CUtensorMap m[kMaps];
+};
+
+// One run of K stages: operands by map index (SPLIT: the lo plane's map is the next one).
+struct Phase {
+    int a, b0, b1;           // A; B of CTA 0 and of CTA 1
+    int nk;                  // 64-deep stages
+    int a_mn, b_mn;          // 1: M/N-major
+    int bstep, brank;        // B's first row: column tile * bstep + CTA * brank
+};
+
+enum Epilogue { kStore = 0, kGate = 1, kGateBwdGU = 2, kGateBwdDH = 3 };
+
+struct Args {
+    long long M;             // rows of the output (of one group)
+    int N;                   // its columns (gate epilogues: F)
+    int mtiles, ntiles_n;    // tiles of one group
+    int groups;              // outputs stacked along M: A's map index and C of group g
+    long long tiles;         // all work items
+    int ksplit;
+    int nphase;
+    Phase ph[2];
+    int bf16;                // operand type of the products: 1 bf16, 0 fp16
+    void* C[2];
+    long long ldc;
+    int dtype;               // C's type
+    int vec;                 // C's rows may be stored in 16-byte pieces
+    float* part;             // ksplit > 1: [split][group][M][N] fp32
+    int act;
+    float* gu;               // gate: kept pre-activations [M][2 Fp] (written or read), or NULL
+    const float* dh;         // kGateBwdGU: [M][Fp]
+    void* H;                 // backward: [M][Fp], C[0] is [M][2 Fp]; NULL: not wanted
+    int Fp;
+    const float* rinv;       // SPLIT: 1 / scale of A's rows, or NULL
+    const unsigned* amax;    // SPLIT: finite maximum (bits) of A's tensor where rinv is NULL
+    const unsigned* bmax;    // ... and of B's
+    unsigned* hmax;          // SPLIT gate backward: maxima of dG | dU and of H
+    // low-rank blocks beside the phases: block t + r holds the rows of request r in 256-row tile
+    // t ([256][R] typed, zeros in other rows), multiplied by the request's adapter
+    int ext;                 // stages a request, 0: none
+    int ext_a, ext_b, ext_bmn;
+    const int2* tile_req;    // requests first .. last - 1 of a tile
+    const int* req_adapter;
+    int nad, R;
+    const float* ext_rinv;   // SPLIT: of the low-rank rows
+    const unsigned* ext_bmax;
+    int* err;
+};
+
+// Tile width, K splits and the partial sums' floats of one product.
+struct Choice {
+    int bn, ksplit;
+    size_t part;
+};
+Choice choose(long long M, int N, int nk, int groups, bool gated, bool split, bool may_split);
+
+// Tensor map of a 16-bit matrix [rows, cols] with rows ld elements apart (16-byte aligned), and
+// of `depth` of them `ldz` elements apart where depth > 0. Boxes of 64 x box_rows.
+int make_map(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld,
+             int box_rows, int depth = 0, long long ldz = 0);
+
+// Launches the product: p.tiles etc. are filled in from M, N, groups and the choice.
+int launch(int epilogue, const Choice& c, bool split, const Maps& maps, Args& p, cudaStream_t st);
+
+// Operand preparation, up to 6 matrices a launch.
+enum Prep { kPack = 0, kRowSplit = 1, kMax = 2, kTensorSplit = 3 };
+struct PrepItem {
+    const void* src;
+    long long rows, cols, ld;
+    void* dst;               // [rows][dld], the lo plane `plane` elements behind
+    long long dld, plane;
+    float* rinv;             // kRowSplit: 1 / scale of each row
+    unsigned* max;           // largest finite magnitude: written (kMax, kRowSplit; may be NULL)
+    int mode;                // or read (kTensorSplit)
+};
+struct PrepList {
+    PrepItem it[6];
+    int n = 0;
+    void add(const PrepItem& i) { it[n++] = i; }
+};
+int prepare(const PrepList& l, cudaStream_t st);
+
+inline bool tma_ready(const void* p, long long ld) { return aligned16(p) && ld % 8 == 0; }
+inline long long up(long long n, long long k) { return (n + k - 1) / k * k; }
+
+}  // namespace pair
+}  // namespace atom
