@@ -134,18 +134,6 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Power-of-two scale that puts a largest magnitude (its bits, finite) into [2^14, 2^15).
-__device__ __forceinline__ float pow2_scale(unsigned bits) {
-    const int ex = (int)(bits >> 23);
-    if (bits == 0) return 1.f;
-    int sh = 141 - ex;
-    sh = sh < -126 ? -126 : (sh > 126 ? 126 : sh);
-    return __uint_as_float((unsigned)(sh + 127) << 23);
-}
-__device__ __forceinline__ float pow2_inv(float s) {
-    return __uint_as_float((254u << 23) - (__float_as_uint(s) & 0x7F800000u));
-}
-
 struct Tile {
     int mt, nt, grp, ks;
 };
@@ -165,6 +153,27 @@ __device__ __forceinline__ Tile tile_of(const Args& p, long long t) {
     return ti;
 }
 
+__device__ __forceinline__ bool is_finite(const Args& p, int slot) {
+    const int4 b = p.bad[slot];
+    return (b.x | b.y | b.z | b.w) == 0;
+}
+// Whether row m (a lane's) belongs to a request whose adapter is not finite.
+__device__ __forceinline__ bool spoilt_row(const Args& p, const Tile& ti, long long m, int lane) {
+    const int2 q = p.tile_req[ti.mt];
+    bool bad = false;
+    for (int r = q.x; r < q.y; r += 32) {
+        int4 c = make_int4(-1, 0, 0, 0);
+        if (r + lane < q.y) c = p.piece[ti.mt + r + lane];
+        unsigned found = __ballot_sync(0xffffffffu, c.x >= 0 && !is_finite(p, c.x));
+        for (; found; found &= found - 1) {
+            const int i = __ffs(found) - 1;
+            const int lo = __shfl_sync(0xffffffffu, c.y, i), hi = __shfl_sync(0xffffffffu, c.z, i);
+            bad |= m >= lo && m < hi;
+        }
+    }
+    return bad;
+}
+
 // Walks the stages of a tile: the phases' (this split's share), then the low-rank blocks'.
 struct Stages {
     const Args& p;
@@ -175,7 +184,7 @@ struct Stages {
     __device__ __forceinline__ Stages(const Args& q, const Tile& t) : p(q), ti(t) {
         range();
         r = rend = 0;
-        if (p.ext) {
+        if (p.ext && ti.ks == p.ksplit - 1) {
             const int2 q2 = p.tile_req[ti.mt];
             r = q2.x;
             rend = q2.y;
@@ -197,8 +206,8 @@ struct Stages {
     __device__ __forceinline__ bool ext_stage() {
         if (sub > 0) return true;                       // in the middle of a request's stages
         while (r < rend) {
-            slot = p.req_adapter[r];
-            if (slot >= 0 && slot < p.nad) return true;
+            slot = p.piece[ti.mt + r].x;
+            if (slot >= 0 && is_finite(p, slot)) return true;
             ++r;
         }
         return false;
@@ -262,6 +271,10 @@ __device__ __forceinline__ void store32(void* C, long long off, const float* v, 
         }
     }
 }
+__device__ __forceinline__ void spoil32(float* v) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(0x7FC00000u);
+}
 __device__ __forceinline__ void load32(const float* q, float* v) {
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
@@ -290,11 +303,6 @@ __device__ __forceinline__ void act_both(float g, int act, float& a, float& da) 
     a = act == 1 ? s : g * s;
     da = act == 1 ? s * (1.f - s) : s * (1.f + g * (1.f - s));
 }
-__device__ __forceinline__ unsigned finite_bits(float x) {
-    const unsigned u = __float_as_uint(x) & 0x7FFFFFFFu;
-    return u < 0x7F800000u ? u : 0u;
-}
-
 // The epilogue's last step on 32 columns n.. of row m; v0 (and v1: the u columns of a gate).
 template <int EPI, bool SPLIT>
 __device__ __forceinline__ void finish32(const Args& p, const Tile& ti, long long m, int n,
@@ -549,6 +557,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const Tile ti = tile_of(p, t);
             const long long m = (long long)ti.mt * 256 + rank * 128 + q * 32 + lane;
             const int nb = ti.nt * (GATED ? BN / 2 : BN) + c0;
+            const bool spoilt = EPI == kStore && p.ext && spoilt_row(p, ti, m, lane);
             if constexpr (!SPLIT) {
                 if (!(ok = filled())) break;
                 const uint32_t ta = tmem + lanes + (round & 1u) * CF::kAcc + c0;
@@ -561,6 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     pin32(v0);
                     if (GATED) pin32(v1);
                     if (k == kChunks - 1) drained();
+                    if (EPI == kStore && spoilt) spoil32(v0);
                     finish32<EPI, SPLIT>(p, ti, m, nb + 32 * k, v0, v1, mx0, mx1);
                 }
             } else {
@@ -615,6 +625,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int k = 0; k < kChunks; ++k) {
                     float u[32];         // kGateBwdDH: room for the u that it reads
+                    if (EPI == kStore && spoilt) spoil32(v[k]);
                     finish32<EPI, SPLIT>(p, ti, m, nb + 32 * k, v[k], GATED ? v[kChunks + k] : u,
                                          mx0, mx1);
                 }
@@ -672,8 +683,7 @@ __global__ void __launch_bounds__(256) reduce_kernel(Args p) {
     }
 }
 
-// One warp a row. Split planes: hi = fp16(x s), lo = fp16((x s - hi) 2^11), both zero past the
-// row's end up to the pitch; what is not finite goes into hi alone.
+// One warp a row. Planes are zero past the row's end up to the pitch.
 __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ PrepList l) {
     const PrepItem& it = l.it[blockIdx.y];
     const int lane = threadIdx.x & 31;
@@ -720,13 +730,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ PrepL
             }
             __half h[4], g[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float y = x[j] * s;
-                h[j] = __float2half_rn(y);
-                const float back = __half2float(h[j]);
-                g[j] = finite_bits(back) || back == 0.f ? __float2half_rn((y - back) * 2048.f)
-                                                        : __float2half_rn(0.f);
-            }
+            for (int j = 0; j < 4; ++j) split_half(x[j] * s, h[j], g[j]);
             *reinterpret_cast<uint2*>(hi + c) = *reinterpret_cast<uint2*>(h);
             *reinterpret_cast<uint2*>(lo + c) = *reinterpret_cast<uint2*>(g);
         }

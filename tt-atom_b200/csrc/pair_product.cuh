@@ -52,8 +52,9 @@ struct Args {
     int ext;                 // stages a request, 0: none
     int ext_a, ext_b, ext_bmn;
     const int2* tile_req;    // requests first .. last - 1 of a tile
-    const int* req_adapter;
-    int nad, R;
+    const int4* piece;       // of a block: adapter or -1 (left out), its rows
+    const int4* bad;         // of an adapter: not all zero = not finite, its rows become NaN
+    int R;
     const float* ext_rinv;   // SPLIT: of the low-rank rows
     const unsigned* ext_bmax;
     int* err;

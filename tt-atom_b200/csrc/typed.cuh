@@ -24,17 +24,26 @@ __device__ __forceinline__ void store_f(void* p, long long i, float v, int dtype
     else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-// The gate's activation and its derivative (ACT 0 SiLU, 1 sigmoid, 2 GELU in its erf form).
-__device__ __forceinline__ void act_grad(float g, int act, float& a, float& da) {
-    if (act == 2) {
-        const float phi = 0.5f * erfcf(-0.70710678f * g);
-        a = g * phi;
-        da = phi + g * 0.39894228f * expf(-0.5f * g * g);
-    } else {
-        const float p = sigmoid_f(g);
-        a = act == 1 ? p : g * p;
-        da = act == 1 ? p * (1.f - p) : p * (1.f + g * (1.f - p));
-    }
+// Bits of |x| where x is finite, else 0.
+__device__ __forceinline__ unsigned finite_bits(float x) {
+    const unsigned u = __float_as_uint(x) & 0x7FFFFFFFu;
+    return u < 0x7F800000u ? u : 0u;
+}
+// Power-of-two scale that puts a largest magnitude (its bits, finite) into [2^14, 2^15).
+__device__ __forceinline__ float pow2_scale(unsigned bits) {
+    if (bits == 0) return 1.f;
+    int sh = 141 - (int)(bits >> 23);
+    sh = sh < -126 ? -126 : (sh > 126 ? 126 : sh);
+    return __uint_as_float((unsigned)(sh + 127) << 23);
+}
+__device__ __forceinline__ float pow2_inv(float s) {
+    return __uint_as_float((254u << 23) - (__float_as_uint(s) & 0x7F800000u));
+}
+// y = hi + lo 2^-11 to 22 bits; what is not finite goes into hi alone.
+__device__ __forceinline__ void split_half(float y, __half& hi, __half& lo) {
+    hi = __float2half_rn(y);
+    const float back = __half2float(hi);
+    lo = __float2half_rn(finite_bits(back) || back == 0.f ? (y - back) * 2048.f : 0.f);
 }
 
 // Pieces of a caller's workspace, 256-byte aligned; with base NULL it only adds up the sizes.
@@ -49,25 +58,5 @@ struct Cursor {
         return p;
     }
 };
-
-// C[m, n] = sum_k A[m * am + k * ak] * B[n * bn + k * bk] (+ the same of A2, B2 where A2 is not
-// NULL), types by code, sums in fp32.
-struct PlainProduct {
-    const void* A;
-    long long am, ak;
-    int ta;
-    const void* B;
-    long long bn, bk;
-    int tb;
-    void* C;
-    long long ldc;
-    int tc;
-    long long M, N, K;
-    const void* A2;
-    const void* B2;
-};
-
-__global__ void plain_product_kernel(PlainProduct p);
-int plain_product(const PlainProduct& p, cudaStream_t st);
 
 }  // namespace atom
