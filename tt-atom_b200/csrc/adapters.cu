@@ -313,10 +313,10 @@ __global__ void __launch_bounds__(256) shrink32_kernel(const __grid_constant__ S
         if (in && lane == 0) p.rinv[m] = pow2_inv(sc);
         for (int r = lane; r < p.Rs; r += 32) {
             const float v = in && r < p.R ? out[row * pitch + r] : 0.f;
-            __half h, l;
-            split_half(v * sc, h, l);
-            block[row * p.Rs + r] = h;
-            block[row * p.Rs + r + p.plane] = l;
+            __half2 h, l;
+            split_half2(v * sc, 0.f, h, l);
+            block[row * p.Rs + r] = __low2half(h);
+            block[row * p.Rs + r + p.plane] = __low2half(l);
             if (in && p.compact) static_cast<float*>(p.compact)[(long long)m * p.Rs + r] = v;
         }
     }
@@ -645,7 +645,7 @@ struct Ad {
         p.dtype = z.dtype;
         p.C[0] = out;
         p.ldc = ldo;
-        p.vec = aligned16(out) && ldo * dtype_size(z.dtype) % 16 == 0;
+        p.used = z.on ? (1u << 4 * k) - 1 : (1u << 2 * k) - 1;
         p.part = sp.part;
         p.rinv = sp.rinv;
         p.bmax = sp.max + 1;

@@ -65,7 +65,7 @@ struct FfSpace {
         if (bwd) {
             pf = z.dwgu().part > z.dwd().part ? z.dwgu().part : z.dwd().part;
             dy = c.take<__half>(k * M * z.Op);
-            dh = c.take<float>(M * z.Fp);
+            dh = c.take<float>(up(M, 32) * z.Fp);
         }
         part = c.take<float>(pf);
         if (!z.split) {
@@ -155,16 +155,25 @@ struct Ff {
         p.Fp = (int)z.Fp;
         p.dtype = z.dtype;
         p.part = sp.part;
+        p.used = 0;
         return p;
     }
     int step() const { return z.split ? 2 : 1; }
     void output(Args& p, void* C, long long ldc) const {
         p.C[0] = C;
         p.ldc = ldc;
-        p.vec = aligned16(C) && ldc * dtype_size(p.dtype) % 16 == 0;
+    }
+    // a gate epilogue's output, and what it keeps in lane blocks
+    int gate_output(Maps& maps, Args& p, void* C, long long width, void* H) const {
+        p.gu_half = up(z.M, 32) * z.Fp;
+        p.H = H != nullptr;
+        p.used |= 1u << kOutMap | (unsigned)p.H << kHMap;
+        if (H)
+            if (int s = make_out_map(&maps.m[kHMap], H, z.dtype, z.Fp, z.M, z.Fp)) return s;
+        return make_out_map(&maps.m[kOutMap], C, z.dtype, width, z.M, width);
     }
     // [G | U] tiles of X
-    int gates(int epilogue, Args& p, void* C, long long ldc) {
+    int gates(int epilogue, Args& p, void* C, long long width, void* H) {
         const Choice c = z.gate();
         const int k = step();
         Maps maps;
@@ -174,13 +183,14 @@ struct Ff {
         p.ph[0] = {0, k, 2 * k, z.nk(z.D), 0, 0, c.bn / 2, 0};
         p.rinv = sp.xr;
         p.bmax = sp.max + 1;
-        output(p, C, ldc);
+        p.used = z.split ? 0x3f : 0x7;
+        if (int s = gate_output(maps, p, C, width, H)) return s;
         return launch(epilogue, c, z.split, maps, p, st);
     }
     int forward(void* y, long long ldy, float* kept) {
         Args p = args(z.M, z.F);
         p.gu = kept;
-        if (int s = gates(kGate, p, z.split ? (void*)sp.H32 : sp.H, z.Fp)) return s;
+        if (int s = gates(kGate, p, z.split ? (void*)sp.H32 : sp.H, z.Fp, nullptr)) return s;
         Operand h{sp.H, z.M, z.F, z.Fp, 0};
         if (z.split) {
             list.add({sp.H32, z.M, z.F, z.Fp, sp.hp, z.Fp, z.M * z.Fp, sp.hr, nullptr, kRowSplit});
@@ -213,20 +223,18 @@ struct Ff {
             p.rinv = sp.dyr;
             p.bmax = sp.max + 2;
             p.hmax = sp.max + 4;
-            p.H = H;
+            p.used = z.split ? 0xf : 0x3;
             if (kept) {
                 p.gu = const_cast<float*>(kept);
-                output(p, dgu, 2 * z.Fp);
+                if (int s = gate_output(maps, p, dgu, 2 * z.Fp, H)) return s;
                 if (int s = launch(kGateBwdDH, c, z.split, maps, p, st)) return s;
             } else {
-                p.dtype = ATOM_F32;
-                output(p, sp.dh, z.Fp);
+                p.blocked = sp.dh;
                 if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
                 Args q = args(z.M, z.F);
                 q.dh = sp.dh;
-                q.H = H;
                 q.hmax = sp.max + 4;
-                if (int s = gates(kGateBwdGU, q, dgu, 2 * z.Fp)) return s;
+                if (int s = gates(kGateBwdGU, q, dgu, 2 * z.Fp, H)) return s;
             }
         }
         Operand g{sp.dgu, z.M, 2 * z.Fp, 2 * z.Fp, 0}, gt = g, h{sp.H, z.M, z.F, z.Fp, 0};
@@ -283,7 +291,6 @@ struct Ff {
             p.bmax = sp.max;
             output(p, dwg ? dwg : dwu, z.D);
             p.C[1] = dwu;
-            p.vec = p.vec && aligned16(dwu ? dwu : dwg);
             if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
         }
         if (dwd) {
@@ -323,7 +330,7 @@ extern "C" int atom_gated_ff_bytes(int dtype, int64_t M, int D, int F, int O, si
     const FfSizes z(dtype, M, D, F, O);
     bytes_host[0] = FfSpace(nullptr, z, false).bytes;
     bytes_host[1] = FfSpace(nullptr, z, true).bytes;
-    bytes_host[2] = (size_t)M * 2 * z.Fp * sizeof(float);
+    bytes_host[2] = (size_t)up(M, 32) * 2 * z.Fp * sizeof(float);
     return ATOM_OK;
 }
 

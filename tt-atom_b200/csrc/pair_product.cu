@@ -23,6 +23,8 @@
 // flight land, frees its tensor memory and returns.
 #include <cudaTypedefs.h>
 
+#include <algorithm>
+
 #include "pair_product.cuh"
 
 namespace atom {
@@ -47,23 +49,26 @@ __device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok) : "r"(smem_u32(b)), "r"(parity) : "memory");
     return ok != 0;
 }
-// Bounded wait; false once the budget is spent or any CTA has failed.
+// Bounded wait; false once the budget is spent or any CTA has failed. The clock and the error
+// word (a trip to L2) are looked at every 256 tries only.
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, int* err) {
     if (mbar_try(b, parity)) return true;
     const long long t0 = clock64();
-    while (!mbar_try(b, parity)) {
-        if (clock64() - t0 > kWaitCycles) {
-            atomicCAS(err, 0, ATOM_PAIR_WAIT_CODE);
-            return false;
+    for (uint32_t n = 1;; ++n) {
+        if (mbar_try(b, parity)) return true;
+        if ((n & 255) == 0) {
+            if (clock64() - t0 > kWaitCycles) {
+                atomicCAS(err, 0, ATOM_PAIR_WAIT_CODE);
+                return false;
+            }
+            if (*(volatile int*)err != 0) return false;
         }
-        if (*(volatile int*)err != 0) return false;
     }
-    return true;
 }
 // TMA tile load into this CTA's shared memory, counted on a barrier of the pair's CTA 0.
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y,
@@ -129,6 +134,15 @@ __device__ __forceinline__ void pin32(float* v) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
 }
+// True in one lane of a converged warp. The TMA and product warps walk their loops with all
+// lanes, so that what they compute stays uniform, and one lane issues.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(yes));
+    return yes != 0;
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -174,45 +188,35 @@ __device__ __forceinline__ bool spoilt_row(const Args& p, const Tile& ti, long l
     return bad;
 }
 
-// Walks the stages of a tile: the phases' (this split's share), then the low-rank blocks'.
-struct Stages {
+// A work item's K stages of one phase.
+struct Share {
+    int kt, end;
+    __device__ __forceinline__ Share(const Args& p, const Tile& ti, int f) {
+        const int nk = p.ph[f].nk;
+        kt = p.ksplit == 1 ? 0 : (int)((long long)ti.ks * nk / p.ksplit);
+        end = p.ksplit == 1 ? nk : (int)((long long)(ti.ks + 1) * nk / p.ksplit);
+    }
+};
+// Walks the low-rank blocks of a row tile (of the last K split's item), p.ext stages each.
+struct Blocks {
     const Args& p;
-    Tile ti;
-    int ph = 0, kt, kend;
-    int r, rend, sub = 0, slot = -1;
-    bool ext = false;
-    __device__ __forceinline__ Stages(const Args& q, const Tile& t) : p(q), ti(t) {
-        range();
-        r = rend = 0;
-        if (p.ext && ti.ks == p.ksplit - 1) {
-            const int2 q2 = p.tile_req[ti.mt];
-            r = q2.x;
-            rend = q2.y;
+    int mt, r = 0, end = 0, sub = 0, slot = -1;
+    __device__ __forceinline__ Blocks(const Args& q, const Tile& ti) : p(q), mt(ti.mt) {
+        if (ti.ks == p.ksplit - 1) {
+            const int2 t = p.tile_req[mt];
+            r = t.x;
+            end = t.y;
         }
     }
-    __device__ __forceinline__ void range() {
-        const int nk = p.ph[ph].nk;
-        kt = (int)((long long)ti.ks * nk / p.ksplit);
-        kend = (int)((long long)(ti.ks + 1) * nk / p.ksplit);
-    }
-    // moves to the next stage; false when there is none
-    __device__ __forceinline__ bool phase_stage() {
-        while (kt >= kend) {
-            if (++ph >= p.nphase) return false;
-            range();
-        }
-        return true;
-    }
-    __device__ __forceinline__ bool ext_stage() {
-        if (sub > 0) return true;                       // in the middle of a request's stages
-        while (r < rend) {
-            slot = p.piece[ti.mt + r].x;
+    __device__ __forceinline__ bool any() {
+        if (sub > 0) return true;                       // in the middle of a block
+        for (; r < end; ++r) {
+            slot = p.piece[mt + r].x;
             if (slot >= 0 && is_finite(p, slot)) return true;
-            ++r;
         }
         return false;
     }
-    __device__ __forceinline__ void ext_next() {
+    __device__ __forceinline__ void next() {
         if (++sub == p.ext) {
             sub = 0;
             ++r;
@@ -226,135 +230,208 @@ struct Cfg {
     static constexpr uint32_t kA = 128 * 128, kB = HB * 128;
     static constexpr uint32_t kStage = (SPLIT ? 2 : 1) * (kA + kB);
     static constexpr int S = SPLIT ? 4 : (BN == 256 ? 6 : 8);
-    static constexpr int kAcc = SPLIT ? 2 * BN : BN;    // tensor-memory columns of one buffer
-    static constexpr uint32_t kSmem = S * kStage + 512 + 1024;
-    static_assert(kSmem <= 232448 && 2 * kAcc <= 512, "shared / tensor memory");
+    // tensor memory: two accumulator buffers of BN columns, and SPLIT two for hi lo + lo hi
+    static_assert((SPLIT ? 4 : 2) * BN <= 512, "tensor memory");
+    static constexpr uint32_t kOut = 8 * 4096;
+    static constexpr uint32_t kSmem = S * kStage + kOut + 512 + 1024;
+    static_assert(kSmem <= 232448, "shared memory");
 };
 
-// 32 values of one row from column n on, as far as the row goes.
-__device__ __forceinline__ void store32(void* C, long long off, const float* v, int left,
-                                        int dtype, int vec) {
-    if (dtype == ATOM_F32) {
-        float* q = static_cast<float*>(C) + off;
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-            if (vec && i + 4 <= left) {
-                *reinterpret_cast<float4*>(q + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (i + j < left) q[i + j] = v[i + j];
-            }
-        }
-        return;
+// A warp's way out: 32 x 32 blocks, one row a lane, through a swizzled 4 KB buffer of its own. A
+// lane that stored its row directly would touch 32 lines with every 16 bytes: the gate's tiles
+// took 13,000 clocks that way, more than their products.
+struct Out {
+    uint8_t* buf;
+    uint32_t turn;
+};
+__device__ __forceinline__ uint32_t pack2(float a, float b, int dtype) {
+    if (dtype == ATOM_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
     }
-    unsigned short* q = static_cast<unsigned short*>(C) + off;
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void stage_f32(uint8_t* buf, int lane, const float* v) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-        uint32_t w[4];
+    for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<float4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+            make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+}
+// By TMA, which leaves out what lies past the map's rows and columns. 16-bit blocks take the
+// two halves of the buffer in turn.
+__device__ __forceinline__ void store_tma(Out& o, int lane, const CUtensorMap* map, int x, int y,
+                                          int z, const float* v, int dtype) {
+    uint8_t* b = o.buf;
+    if (dtype == ATOM_F32) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+        stage_f32(b, lane, v);
+    } else {
+        b += (o.turn++ & 1u) * 2048;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (dtype == ATOM_BF16) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
-                w[j] = *reinterpret_cast<const uint32_t*>(&h);
-            } else {
-                const __half2 h = __floats2half2_rn(v[i + 2 * j], v[i + 2 * j + 1]);
-                w[j] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-        }
-        if (vec && i + 8 <= left) {
-            *reinterpret_cast<uint4*>(q + i) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
+        for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4*>(b + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = make_uint4(
+                pack2(v[8 * c], v[8 * c + 1], dtype), pack2(v[8 * c + 2], v[8 * c + 3], dtype),
+                pack2(v[8 * c + 4], v[8 * c + 5], dtype), pack2(v[8 * c + 6], v[8 * c + 7], dtype));
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+        if (z < 0)
+            asm volatile(
+                "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                    reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(b)) : "memory");
+        else
+            asm volatile(
+                "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(b))
+                : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+}
+// Where rows do not start on 16 bytes, or end inside them: row by row, a column a lane.
+__device__ __forceinline__ void store_rows(Out& o, int lane, void* C, long long off, long long ld,
+                                           int rows, int cols, const float* v, int dtype) {
+    __syncwarp();
+    stage_f32(o.buf, lane, v);
+    __syncwarp();
+    for (int r = 0; r < rows; ++r) {
+        const float x = *reinterpret_cast<const float*>(
+            o.buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+        if (lane < cols) store_f(C, off + r * ld + lane, x, dtype);
+    }
+}
+// Buffers that only these kernels read are kept as the lanes have them: 32 x 32 blocks, 16
+// bytes a lane at a time.
+__device__ __forceinline__ float* lane_block(float* p, long long m, int n, int Fp, int lane) {
+    return p + ((m >> 5) * (Fp >> 5) + (n >> 5)) * 1024 + lane * 4;
+}
+__device__ __forceinline__ void store_block(float* q, const float* v) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (i + j < left) q[i + j] = (unsigned short)(w[j >> 1] >> (16 * (j & 1)));
-        }
+    for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<float4*>(q + 128 * j) =
+            make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+}
+__device__ __forceinline__ void load_block(const float* q, float* v) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float4 x = *reinterpret_cast<const float4*>(q + 128 * j);
+        v[4 * j] = x.x, v[4 * j + 1] = x.y, v[4 * j + 2] = x.z, v[4 * j + 3] = x.w;
     }
 }
 __device__ __forceinline__ void spoil32(float* v) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(0x7FC00000u);
 }
-__device__ __forceinline__ void load32(const float* q, float* v) {
+// Activation and derivative: fast intrinsics (a few 2^-23) for 16-bit results, the accurate
+// functions for fp32 ones. GELU's erfc is called, not expanded at each of a row's 32 values.
+__device__ __noinline__ float normal_cdf(float g) { return 0.5f * erfcf(-0.70710678f * g); }
+template <bool EXACT>
+__device__ __forceinline__ float sigmoid_t(float g) {
+    return EXACT ? sigmoid_f(g) : sigmoid_gate(g);
+}
+// h = act(g) u
+template <bool EXACT>
+__device__ __forceinline__ void gate32(float* g, const float* u, int act) {
+    if (act == 0) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(q + i);
-        v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+        for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid_t<EXACT>(g[i]) * u[i];
+    } else if (act == 1) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) g[i] = sigmoid_t<EXACT>(g[i]) * u[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) g[i] = g[i] * normal_cdf(g[i]) * u[i];
+    }
+}
+// (g, u, d = dh) -> (dg, du, h)
+template <bool EXACT>
+__device__ __forceinline__ void gate_bwd32(float* g, float* u, float* d, int act) {
+    auto out = [&](int i, float a, float da) {
+        const float x = u[i];
+        g[i] = d[i] * x * da;
+        u[i] = d[i] * a;
+        d[i] = a * x;
+    };
+    if (act == 0) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float s = sigmoid_t<EXACT>(g[i]);
+            out(i, g[i] * s, s * (1.f + g[i] * (1.f - s)));
+        }
+    } else if (act == 1) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float s = sigmoid_t<EXACT>(g[i]);
+            out(i, s, s * (1.f - s));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float c = normal_cdf(g[i]), x = g[i];
+            out(i, x * c, c + x * 0.39894228f * (EXACT ? expf(-0.5f * x * x) : __expf(-0.5f * x * x)));
+        }
     }
 }
 
-// Activation and derivative: fast intrinsics (a few 2^-23) for 16-bit results, the accurate
-// functions for fp32 ones.
-template <bool EXACT>
-__device__ __forceinline__ float act_of(float g, int act) {
-    if (act == 2) return g * 0.5f * erfcf(-0.70710678f * g);
-    const float s = EXACT ? sigmoid_f(g) : sigmoid_gate(g);
-    return act == 1 ? s : g * s;
-}
-template <bool EXACT>
-__device__ __forceinline__ void act_both(float g, int act, float& a, float& da) {
-    if (act == 2) {
-        const float phi = 0.5f * erfcf(-0.70710678f * g);
-        a = g * phi;
-        da = phi + g * 0.39894228f * (EXACT ? expf(-0.5f * g * g) : __expf(-0.5f * g * g));
-        return;
-    }
-    const float s = EXACT ? sigmoid_f(g) : sigmoid_gate(g);
-    a = act == 1 ? s : g * s;
-    da = act == 1 ? s * (1.f - s) : s * (1.f + g * (1.f - s));
-}
-// The epilogue's last step on 32 columns n.. of row m; v0 (and v1: the u columns of a gate).
+// The epilogue's last step on 32 columns n.. of the warp's rows m.. (m + lane is this lane's);
+// v0 (and v1: the u columns of a gate).
 template <int EPI, bool SPLIT>
-__device__ __forceinline__ void finish32(const Args& p, const Tile& ti, long long m, int n,
-                                         float* v0, float* v1, unsigned& mx0, unsigned& mx1) {
+__device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const Tile& ti, Out& o,
+                                         long long m, int n, int lane, float* v0, float* v1,
+                                         unsigned& mx0, unsigned& mx1) {
     if (m >= p.M || n >= p.N) return;
     const int left = p.N - n;
     if constexpr (EPI == kStore) {
-        if (p.ksplit > 1) {
-            float* q = p.part + ((long long)(ti.ks * p.groups + ti.grp) * p.M + m) * p.N + n;
-            store32(q, 0, v0, left, ATOM_F32, p.N % 4 == 0);
+        if (p.blocked) {
+            store_block(lane_block(p.blocked, m, n, p.Fp, lane), v0);
+        } else if (p.ksplit > 1) {
+            const int z = ti.ks * p.groups + ti.grp;
+            if (p.tma)
+                store_tma(o, lane, &maps.m[kPartMap], n, (int)m, z, v0, ATOM_F32);
+            else
+                store_rows(o, lane, p.part, (z * p.M + m) * p.N + n, p.N,
+                           (int)min(32LL, p.M - m), left, v0, ATOM_F32);
+        } else if (p.tma) {
+            store_tma(o, lane, &maps.m[kOutMap + ti.grp], n, (int)m, -1, v0, p.dtype);
         } else {
-            store32(p.C[ti.grp], m * p.ldc + n, v0, left, p.dtype, p.vec);
+            store_rows(o, lane, p.C[ti.grp], m * p.ldc + n, p.ldc, (int)min(32LL, p.M - m), left,
+                       v0, p.dtype);
         }
     } else if constexpr (EPI == kGate) {
         if (p.gu) {
-            float* q = p.gu + m * 2 * p.Fp + n;
-            store32(q, 0, v0, 32, ATOM_F32, 1);
-            store32(q, p.Fp, v1, 32, ATOM_F32, 1);
+            store_block(lane_block(p.gu, m, n, p.Fp, lane), v0);
+            store_block(lane_block(p.gu, m, n, p.Fp, lane) + p.gu_half, v1);
         }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v0[i] = act_of<SPLIT>(v0[i], p.act) * v1[i];
-        store32(p.C[0], m * p.ldc + n, v0, 32, p.dtype, 1);
+        gate32<SPLIT>(v0, v1, p.act);
+        store_tma(o, lane, &maps.m[kOutMap], n, (int)m, -1, v0, p.dtype);
     } else {
         // v0, v1 = g, u (kGateBwdGU, dh from memory) or v0 = dh (kGateBwdDH, g and u from memory)
         float w[32];
         if constexpr (EPI == kGateBwdGU) {
-            load32(p.dh + m * p.Fp + n, w);
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (i >= left) w[i] = 0.f;      // past the row nothing was written
+            load_block(lane_block(p.dh, m, n, p.Fp, lane), w);
         } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) w[i] = v0[i];
-            load32(p.gu + m * 2 * p.Fp + n, v0);
-            load32(p.gu + m * 2 * p.Fp + p.Fp + n, v1);
+            load_block(lane_block(p.gu, m, n, p.Fp, lane), v0);
+            load_block(lane_block(p.gu, m, n, p.Fp, lane) + p.gu_half, v1);
         }
+        gate_bwd32<SPLIT>(v0, v1, w, p.act);
+        if (SPLIT) {
+            const int mine = m + lane < p.M ? left : 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            float a, da;
-            act_both<SPLIT>(v0[i], p.act, a, da);
-            const float u = v1[i], d = w[i];
-            v0[i] = d * u * da;
-            v1[i] = d * a;
-            w[i] = a * u;
-            if (SPLIT && i < left) {
-                mx0 = max(mx0, max(finite_bits(v0[i]), finite_bits(v1[i])));
-                mx1 = max(mx1, finite_bits(w[i]));
-            }
+            for (int i = 0; i < 32; ++i)
+                if (i < mine) {
+                    mx0 = max(mx0, max(finite_bits(v0[i]), finite_bits(v1[i])));
+                    mx1 = max(mx1, finite_bits(w[i]));
+                }
         }
-        store32(p.C[0], m * 2 * p.Fp + n, v0, 32, p.dtype, 1);
-        store32(p.C[0], m * 2 * p.Fp + p.Fp + n, v1, 32, p.dtype, 1);
-        if (p.H) store32(p.H, m * p.Fp + n, w, 32, p.dtype, 1);
+        store_tma(o, lane, &maps.m[kOutMap], n, (int)m, -1, v0, p.dtype);
+        store_tma(o, lane, &maps.m[kOutMap], p.Fp + n, (int)m, -1, v1, p.dtype);
+        if (p.H) store_tma(o, lane, &maps.m[kHMap], n, (int)m, -1, w, p.dtype);
     }
 }
 
@@ -362,20 +439,21 @@ template <int BN, int EPI, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
     using CF = Cfg<BN, SPLIT>;
-    constexpr int S = CF::S;
+    constexpr int S = CF::S, P = SPLIT ? 2 : 1;      // stages, planes
     // a gate's tile: columns 0 .. BN/2 of the accumulator are g, the others u
     constexpr bool GATED = EPI == kGate || EPI == kGateBwdGU;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * CF::kStage);
+    uint8_t* outbuf = smem + S * CF::kStage;
+    uint64_t* full = reinterpret_cast<uint64_t*>(outbuf + CF::kOut);
     uint64_t* empty = full + S;
     uint64_t* accf = empty + S;      // [2] accumulator buffer full
     uint64_t* acce = accf + 2;       // [2] and free again (CTA 0's: both CTAs' epilogue warps)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acce + 2);
     int* failed = reinterpret_cast<int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     uint32_t rank;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     const int pairs = gridDim.x >> 1, first = blockIdx.x >> 1;
@@ -391,6 +469,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         *failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == 2 && lane < kMaps && (p.used >> lane & 1))
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.m[lane]))
+                     : "memory");
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
             smem_u32(tmem_slot)));
@@ -404,59 +485,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t base = smem_u32(smem);
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
+        {
+            uint32_t it = 0, slot = 0, turn = 0;
             bool ok = true;
+            const uint32_t full0 = peer_addr(smem_u32(full), 0);
             // waits for a free stage and names its barrier of CTA 0
             auto open = [&](uint32_t& dst, uint32_t& bar) {
-                const uint32_t s = it % S, ph = (it / S) & 1u;
-                if (!mbar_wait(&empty[s], ph ^ 1u, p.err)) return false;
-                if (rank == 0)
+                const uint32_t s = slot;
+                if (!mbar_wait(&empty[s], turn ^ 1u, p.err)) return false;
+                if (rank == 0 && elect_one())
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
                                      smem_u32(&full[s])), "r"(2 * CF::kStage) : "memory");
                 dst = base + s * CF::kStage;
-                bar = peer_addr(smem_u32(&full[s]), 0);
+                bar = full0 + s * 8;
                 ++it;
+                if (++slot == S) slot = 0, turn ^= 1u;
                 return true;
             };
             for (long long t = first; ok && t < p.tiles; t += pairs) {
-                Stages st(p, tile_of(p, t));
-                const int m0 = st.ti.mt * 256 + rank * 128;
-                for (; st.phase_stage(); ++st.kt) {
-                    uint32_t dst, bar;
-                    if (!(ok = open(dst, bar))) break;
-                    const Phase& f = p.ph[st.ph];
-                    const int k0 = st.kt * 64, n0 = st.ti.nt * f.bstep + rank * f.brank;
+                const Tile ti = tile_of(p, t);
+                const int m0 = ti.mt * 256 + rank * 128;
+                for (int f = 0; ok && f < p.nphase; ++f) {
+                    const Phase ph = p.ph[f];
+                    const Share sh(p, ti, f);
+                    const int n0 = ti.nt * ph.bstep + rank * ph.brank;
+                    const CUtensorMap* ma = &maps.m[ph.a + P * ti.grp];
+                    const CUtensorMap* mb = &maps.m[rank ? ph.b1 : ph.b0];
+                    for (int kt = sh.kt; kt < sh.end; ++kt) {
+                        uint32_t dst, bar;
+                        if (!(ok = open(dst, bar))) break;
+                        const int k0 = kt * 64;
+                        if (!elect_one()) continue;
 #pragma unroll
-                    for (int pl = 0; pl < (SPLIT ? 2 : 1); ++pl) {
-                        const CUtensorMap* ma = &maps.m[f.a + pl + (SPLIT ? 2 : 1) * st.ti.grp];
-                        const uint32_t da = dst + pl * CF::kA;
-                        if (f.a_mn) {
-                            tma_load(da, ma, m0, k0, bar);
-                            tma_load(da + 8192, ma, m0 + 64, k0, bar);
-                        } else {
-                            tma_load(da, ma, k0, m0, bar);
-                        }
-                        const CUtensorMap* mb = &maps.m[(rank ? f.b1 : f.b0) + pl];
-                        const uint32_t db = dst + (SPLIT ? 2 : 1) * CF::kA + pl * CF::kB;
-                        if (f.b_mn) {
+                        for (int pl = 0; pl < P; ++pl) {
+                            const uint32_t da = dst + pl * CF::kA, db = dst + P * CF::kA + pl * CF::kB;
+                            if (ph.a_mn) {
+                                tma_load(da, ma + pl, m0, k0, bar);
+                                tma_load(da + 8192, ma + pl, m0 + 64, k0, bar);
+                            } else {
+                                tma_load(da, ma + pl, k0, m0, bar);
+                            }
+                            if (ph.b_mn) {
 #pragma unroll
-                            for (int j = 0; j < CF::HB / 64; ++j)
-                                tma_load(db + j * 8192, mb, n0 + 64 * j, k0, bar);
-                        } else {
-                            tma_load(db, mb, k0, n0, bar);
+                                for (int j = 0; j < CF::HB / 64; ++j)
+                                    tma_load(db + j * 8192, mb + pl, n0 + 64 * j, k0, bar);
+                            } else {
+                                tma_load(db, mb + pl, k0, n0, bar);
+                            }
                         }
                     }
                 }
-                for (; ok && p.ext && st.ext_stage(); st.ext_next()) {
+                if (!p.ext) continue;
+                Blocks st(p, ti);
+                for (; ok && st.any(); st.next()) {
                     uint32_t dst, bar;
                     if (!(ok = open(dst, bar))) break;
-                    const int y = (st.ti.mt + st.r) * 256 + rank * 128, k0 = st.sub * 64;
-                    const int n0 = st.ti.nt * BN + rank * CF::HB;
+                    const int y = (ti.mt + st.r) * 256 + rank * 128, k0 = st.sub * 64;
+                    const int n0 = ti.nt * BN + rank * CF::HB;
+                    if (!elect_one()) continue;
 #pragma unroll
-                    for (int pl = 0; pl < (SPLIT ? 2 : 1); ++pl) {
+                    for (int pl = 0; pl < P; ++pl) {
                         tma_load(dst + pl * CF::kA, &maps.m[p.ext_a + pl], k0, y, bar);
-                        const uint32_t db = dst + (SPLIT ? 2 : 1) * CF::kA + pl * CF::kB;
+                        const uint32_t db = dst + P * CF::kA + pl * CF::kB;
                         const CUtensorMap* mb = &maps.m[p.ext_b + pl];
                         if (p.ext_bmn) {
 #pragma unroll
@@ -474,59 +564,91 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (!ok) *(volatile int*)failed = 1;
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            uint32_t it = 0, round = 0;
+        if (rank == 0) {
+            uint32_t slot = 0, turn = 0, round = 0;
             bool ok = true, open = false;
             uint32_t acc = 0, fresh = 0;
+            // SPLIT: hi lo + lo hi gather over all rounds of a tile's phases (and of its blocks),
+            // in two buffers by turns; the rounds' waits cover them
+            uint32_t low = tmem + 2 * BN, low_fresh = 0;
+            const uint64_t base_k = sdesc(base, 0), base_mn = sdesc(base, 1);
             auto begin = [&]() {         // a free accumulator buffer for the next round
                 const uint32_t b = round & 1u;
                 if (!mbar_wait(&acce[b], ((round >> 1) & 1u) ^ 1u, p.err)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                acc = tmem + b * CF::kAcc;
+                acc = tmem + b * BN;
                 fresh = 0;
                 return open = true;
             };
             auto end = [&]() {
-                mma_commit(&accf[round & 1u]);
+                if (elect_one()) mma_commit(&accf[round & 1u]);
                 ++round;
                 open = false;
             };
-            auto stage = [&](int a_mn, int b_mn, int steps) {
-                const uint32_t s = it % S, ph = (it / S) & 1u;
-                if (!mbar_wait(&full[s], ph, p.err)) return false;
+            // One stage's products. Descriptors only add to their address field: one thread issues
+            // a product every ~40 clocks this way, against ~160 building each anew, which had
+            // bound the whole kernel (a product of 256 x 256 x 16 takes 128 clocks).
+            auto stage = [&](uint64_t a, uint64_t b, uint32_t as, uint32_t bs, uint32_t id,
+                             int steps) {
+                if (!mbar_wait(&full[slot], turn, p.err)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t id = idesc(BN, SPLIT ? 0 : p.bf16, a_mn, b_mn);
-                const uint32_t a = base + s * CF::kStage, b = a + (SPLIT ? 2 : 1) * CF::kA;
-                const uint32_t as = a_mn ? 2048 : 32, bs = b_mn ? 2048 : 32;
-                for (int k = 0; k < steps; ++k) {
-                    const uint64_t ad = sdesc(a + k * as, a_mn), bd = sdesc(b + k * bs, b_mn);
-                    mma(acc, ad, bd, id, fresh);
-                    if constexpr (SPLIT) {
-                        const uint64_t al = sdesc(a + CF::kA + k * as, a_mn);
-                        const uint64_t bl = sdesc(b + CF::kB + k * bs, b_mn);
-                        mma(acc + BN, ad, bl, id, fresh);
-                        mma(acc + BN, al, bd, id, 1u);
+                a += slot * (CF::kStage >> 4);
+                b += slot * (CF::kStage >> 4);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (k < steps) {
+                            const uint64_t ad = a + k * as, bd = b + k * bs;
+                            const uint32_t add = k ? 1u : fresh;
+                            mma(acc, ad, bd, id, add);
+                            if constexpr (SPLIT) {
+                                mma(low, ad, bd + (CF::kB >> 4), id, k ? 1u : low_fresh);
+                                mma(low, ad + (CF::kA >> 4), bd, id, 1u);
+                            }
+                        }
                     }
-                    fresh = 1;
+                    mma_commit(&empty[slot]);
                 }
-                mma_commit(&empty[s]);
-                ++it;
+                __syncwarp();
+                fresh = low_fresh = 1;
+                if (++slot == S) slot = 0, turn ^= 1u;
                 return true;
             };
+            auto next_low = [&]() {
+                low = tmem + 2 * BN + (low == tmem + 2 * BN ? BN : 0);
+                low_fresh = 0;
+            };
             for (long long t = first; ok && t < p.tiles; t += pairs) {
-                Stages st(p, tile_of(p, t));
+                const Tile ti = tile_of(p, t);
                 int n = 0;
-                for (; ok && st.phase_stage(); ++st.kt, ++n) {
-                    if (SPLIT && open && n == kRound) end(), n = 0;
-                    ok = (open || begin()) && stage(p.ph[st.ph].a_mn, p.ph[st.ph].b_mn, 4);
+                for (int f = 0; ok && f < p.nphase; ++f) {
+                    const int a_mn = p.ph[f].a_mn, b_mn = p.ph[f].b_mn;
+                    const Share sh(p, ti, f);
+                    const uint64_t a = a_mn ? base_mn : base_k;
+                    const uint64_t b = (b_mn ? base_mn : base_k) + (P * CF::kA >> 4);
+                    const uint32_t as = a_mn ? 2048 >> 4 : 32 >> 4, bs = b_mn ? 2048 >> 4 : 32 >> 4;
+                    const uint32_t id = idesc(BN, SPLIT ? 0 : p.bf16, a_mn, b_mn);
+                    for (int kt = sh.kt; ok && kt < sh.end; ++kt, ++n) {
+                        if (SPLIT && open && n == kRound) end(), n = 0;
+                        ok = (open || begin()) && stage(a, b, as, bs, id, 4);
+                    }
                 }
-                if (SPLIT && ok && open) end(), n = 0;
-                for (; ok && p.ext && st.ext_stage(); st.ext_next(), ++n) {
-                    if (SPLIT && open && n == kRound) end(), n = 0;
-                    ok = (open || begin()) &&
-                         stage(0, p.ext_bmn, (min(64, p.R - 64 * st.sub) + 15) >> 4);
+                if (SPLIT && ok && open) end(), next_low(), n = 0;
+                if (p.ext) {
+                    Blocks st(p, ti);
+                    const uint64_t b = (p.ext_bmn ? base_mn : base_k) + (P * CF::kA >> 4);
+                    const uint32_t bs = p.ext_bmn ? 2048 >> 4 : 32 >> 4;
+                    const uint32_t id = idesc(BN, SPLIT ? 0 : p.bf16, 0, p.ext_bmn);
+                    for (; ok && st.any(); st.next(), ++n) {
+                        if (SPLIT && open && n == kRound) end(), n = 0;
+                        ok = (open || begin()) &&
+                             stage(base_k, b, 32 >> 4, bs, id, (min(64, p.R - 64 * st.sub) + 15) >> 4);
+                    }
                 }
-                if (ok && open) end();
+                if (ok && open) {
+                    end();
+                    if (SPLIT) next_low();
+                }
             }
             if (!ok) *(volatile int*)failed = 1;
         }
@@ -535,12 +657,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         uint32_t round = 0;
         unsigned mx0 = 0, mx1 = 0;
-        auto drained = [&]() {           // this warp has read the round's accumulators
+        const uint32_t acce0 = peer_addr(smem_u32(acce), 0);
+        // This warp has read the round's accumulators. Relaxed: only tensor memory is handed over,
+        // which the fence orders; a release would wait for this warp's stores to memory as well.
+        auto drained = [&]() {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0)
-                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                                 peer_addr(smem_u32(&acce[round & 1u]), 0)) : "memory");
+                asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                 acce0 + 8 * (round & 1u)) : "memory");
             ++round;
         };
         auto filled = [&]() {
@@ -553,14 +678,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         constexpr int kChunks = (GATED ? BN / 4 : BN / 2) / 32;
         const int c0 = half * kChunks * 32;
         bool ok = true;
+        Out out{outbuf + (warp - 2) * 4096, 0};
+        constexpr int kParts = GATED ? 2 * kChunks : kChunks;
+        uint32_t low = 2 * BN;
         for (long long t = first; ok && t < p.tiles; t += pairs) {
             const Tile ti = tile_of(p, t);
-            const long long m = (long long)ti.mt * 256 + rank * 128 + q * 32 + lane;
+            const long long m = (long long)ti.mt * 256 + rank * 128 + q * 32;
             const int nb = ti.nt * (GATED ? BN / 2 : BN) + c0;
-            const bool spoilt = EPI == kStore && p.ext && spoilt_row(p, ti, m, lane);
+            const bool spoilt = EPI == kStore && p.ext && spoilt_row(p, ti, m + lane, lane);
             if constexpr (!SPLIT) {
                 if (!(ok = filled())) break;
-                const uint32_t ta = tmem + lanes + (round & 1u) * CF::kAcc + c0;
+                const uint32_t ta = tmem + lanes + (round & 1u) * BN + c0;
 #pragma unroll 1
                 for (int k = 0; k < kChunks; ++k) {
                     float v0[32], v1[32];
@@ -571,66 +699,82 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (GATED) pin32(v1);
                     if (k == kChunks - 1) drained();
                     if (EPI == kStore && spoilt) spoil32(v0);
-                    finish32<EPI, SPLIT>(p, ti, m, nb + 32 * k, v0, v1, mx0, mx1);
+                    finish32<EPI, SPLIT>(maps, p, ti, out, m, nb + 32 * k, lane, v0, v1, mx0, mx1);
                 }
             } else {
-                // per chunk pair: the tile's rounds summed in registers
-                float v[GATED ? 2 * kChunks : kChunks][32];
+                // the tile's rounds summed in registers
+                float v[kParts][32];
 #pragma unroll
-                for (int k = 0; k < (GATED ? 2 * kChunks : kChunks); ++k)
+                for (int k = 0; k < kParts; ++k)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[k][i] = 0.f;
-                auto add = [&](float f) {
-                    const uint32_t ta = tmem + lanes + (round & 1u) * CF::kAcc + c0;
-#pragma unroll
-                    for (int k = 0; k < (GATED ? 2 * kChunks : kChunks); ++k) {
-                        const uint32_t col =
-                            GATED ? (k / kChunks) * (BN / 2) + (k % kChunks) * 32 : 32 * k;
-                        float x[32], y[32];
-                        tmem_ld32(ta + col, x);
-                        tmem_ld32(ta + BN + col, y);
-                        tmem_wait_ld();
-                        pin32(x);
-                        pin32(y);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            v[k][i] = fmaf(f, fmaf(y[i], 1.f / 2048.f, x[i]), v[k][i]);
-                    }
-                    drained();
+                auto column = [&](int k) {
+                    return GATED ? (k / kChunks) * (BN / 2) + (k % kChunks) * 32 : 32 * k;
                 };
+                // adds f times the next `rounds` rounds
+                auto add = [&](int rounds, float f) {
+                    const uint32_t tl = tmem + lanes + c0;
+                    for (int r = 0; r < rounds; ++r) {
+                        if (!filled()) return false;
+                        const uint32_t ta = tl + (round & 1u) * BN;
+                        float x[2][32];
+#pragma unroll
+                        for (int k = 0; k < kParts; ++k) tmem_ld32(ta + column(k), x[k]);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < kParts; ++k) {
+                            pin32(x[k]);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[k][i] = fmaf(f, x[k][i], v[k][i]);
+                        }
+                        if (r == rounds - 1) {
+#pragma unroll
+                            for (int k = 0; k < kParts; ++k) tmem_ld32(tl + low + column(k), x[k]);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < kParts; ++k) {
+                                pin32(x[k]);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    v[k][i] = fmaf(f * (1.f / 2048.f), x[k][i], v[k][i]);
+                            }
+                            low = low == 2 * BN ? 3 * BN : 2 * BN;
+                        }
+                        drained();
+                    }
+                    return true;
+                };
+                static_assert(!SPLIT || kParts == 2, "parts of a SPLIT tile");
                 const float sb = pow2_inv(pow2_scale(*p.bmax));
-                const float sa = p.rinv ? (m < p.M ? p.rinv[m] : 0.f)
+                const float sa = p.rinv ? (m + lane < p.M ? p.rinv[m + lane] : 0.f)
                                         : pow2_inv(pow2_scale(*p.amax));
                 int stages = 0;
-                for (int f = 0; f < p.nphase; ++f)
-                    stages += (int)((long long)(ti.ks + 1) * p.ph[f].nk / p.ksplit) -
-                              (int)((long long)ti.ks * p.ph[f].nk / p.ksplit);
-                for (int k = 0; ok && k < stages; k += kRound)
-                    if ((ok = filled())) add(1.f);
-                if (!ok) break;
+                for (int f = 0; f < p.nphase; ++f) {
+                    const Share sh(p, ti, f);
+                    stages += sh.end - sh.kt;
+                }
+                if (!(ok = add((stages + kRound - 1) / kRound, 1.f))) break;
 #pragma unroll
-                for (int k = 0; k < (GATED ? 2 * kChunks : kChunks); ++k)
+                for (int k = 0; k < kParts; ++k)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[k][i] = v[k][i] * sa * sb;
                 if (p.ext) {
-                    Stages st(p, ti);
                     int es = 0;
-                    for (; st.ext_stage(); st.ext_next()) ++es;
-                    const float f = (m < p.M ? p.ext_rinv[m] : 0.f) *
+                    for (Blocks st(p, ti); st.any(); st.next()) ++es;
+                    const float f = (m + lane < p.M ? p.ext_rinv[m + lane] : 0.f) *
                                     pow2_inv(pow2_scale(*p.ext_bmax));
-                    for (int k = 0; ok && k < es; k += kRound)
-                        if ((ok = filled())) add(f);
-                    if (!ok) break;
+                    if (!(ok = add((es + kRound - 1) / kRound, f))) break;
                 }
 #pragma unroll
                 for (int k = 0; k < kChunks; ++k) {
                     float u[32];         // kGateBwdDH: room for the u that it reads
                     if (EPI == kStore && spoilt) spoil32(v[k]);
-                    finish32<EPI, SPLIT>(p, ti, m, nb + 32 * k, v[k], GATED ? v[kChunks + k] : u,
-                                         mx0, mx1);
+                    finish32<EPI, SPLIT>(maps, p, ti, out, m, nb + 32 * k, lane, v[k],
+                                         GATED ? v[kChunks + k] : u, mx0, mx1);
                 }
             }
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         if constexpr (SPLIT && (EPI == kGateBwdGU || EPI == kGateBwdDH)) {
             if (p.hmax) {
                 mx0 = __reduce_max_sync(0xffffffffu, mx0);
@@ -683,68 +827,122 @@ __global__ void __launch_bounds__(256) reduce_kernel(Args p) {
     }
 }
 
-// One warp a row. Planes are zero past the row's end up to the pitch.
+__host__ __device__ inline bool prep_wide(const PrepItem& it) {
+    return it.dld > 1024 || it.cols > 1024;
+}
+// A warp a row, or a block where rows are wider than 1024; NV float4 a thread hold a row between
+// its maximum and its planes, so it is read once (up to 8192 columns). Planes and packed rows are
+// zero past the row's end up to the pitch. Bound by memory: the two halves of a value cost five
+// instructions, since what is not finite needs no care (its results are not finite either way)
+// except that a maximum leaves it out.
+template <int NV>
 __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ PrepList l) {
     const PrepItem& it = l.it[blockIdx.y];
-    const int lane = threadIdx.x & 31;
-    unsigned top = 0;
-    for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < it.rows; r += gridDim.x * 8LL) {
-        if (it.mode == kPack) {
+    __shared__ float part[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool wide = prep_wide(it);
+    const int threads = wide ? 256 : 32, me = wide ? threadIdx.x : lane;
+    const long long step = wide ? gridDim.x : gridDim.x * 8LL;
+    const int mode = it.mode;
+    const long long cols = it.cols, dld = it.dld;
+    float top = 0.f;
+    for (long long r = wide ? blockIdx.x : blockIdx.x * 8LL + warp; r < it.rows; r += step) {
+        if (mode == kPack) {
             const unsigned short* src = static_cast<const unsigned short*>(it.src) + r * it.ld;
-            unsigned short* dst = static_cast<unsigned short*>(it.dst) + r * it.dld;
-            for (long long c = lane; c < it.dld; c += 32) dst[c] = c < it.cols ? src[c] : 0;
+            unsigned short* dst = static_cast<unsigned short*>(it.dst) + r * dld;
+            for (long long c0 = 0; c0 < dld; c0 += 8LL * threads) {
+                // eight single loads in flight, then eight stores
+                unsigned short v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const long long c = c0 + j * threads + me;
+                    v[j] = c < cols ? src[c] : 0;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const long long c = c0 + j * threads + me;
+                    if (c < dld) dst[c] = v[j];
+                }
+            }
             continue;
         }
         const float* src = static_cast<const float*>(it.src) + r * it.ld;
-        const bool four = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && it.cols % 4 == 0;
+        const bool four = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && cols % 4 == 0;
+        auto load = [&](long long c) {
+            if (four) return c < cols ? *reinterpret_cast<const float4*>(src + c)
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+            return make_float4(c < cols ? src[c] : 0.f, c + 1 < cols ? src[c + 1] : 0.f,
+                               c + 2 < cols ? src[c + 2] : 0.f, c + 3 < cols ? src[c + 3] : 0.f);
+        };
+        float4 x[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) x[j] = load(4LL * (j * threads + me));
         float s = 1.f;
-        if (it.mode == kTensorSplit) {
+        const long long held = 4LL * NV * threads;
+        if (mode == kTensorSplit) {
             s = pow2_scale(*it.max);
         } else {
-            unsigned mx = 0;
-            if (four) {
-                for (long long c = 4 * lane; c < it.cols; c += 128) {
-                    const float4 x = *reinterpret_cast<const float4*>(src + c);
-                    mx = max(max(mx, max(finite_bits(x.x), finite_bits(x.y))),
-                             max(finite_bits(x.z), finite_bits(x.w)));
+            float mx = 0.f;
+            auto see = [&](const float4& v) {       // fmaxf passes over NaN
+                mx = fmaxf(fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+            };
+            auto see_finite = [&](const float4& v) {
+                for (float y : {v.x, v.y, v.z, v.w}) mx = fmaxf(mx, __uint_as_float(finite_bits(y)));
+            };
+            auto all = [&](auto f) {
+                mx = 0.f;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) f(x[j]);
+                for (long long c = held + 4 * me; c < cols; c += 4 * threads) f(load(c));
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                if (wide) {
+                    __syncthreads();
+                    if (lane == 0) part[warp] = mx;
+                    __syncthreads();
+                    for (int k = 0; k < 8; ++k) mx = fmaxf(mx, part[k]);
                 }
-            } else {
-                for (long long c = lane; c < it.cols; c += 32) mx = max(mx, finite_bits(src[c]));
-            }
-            mx = __reduce_max_sync(0xffffffffu, mx);
-            top = max(top, mx);
-            if (it.mode == kMax) continue;
-            s = pow2_scale(mx);
-            if (lane == 0) it.rinv[r] = pow2_inv(s);
+            };
+            all(see);
+            if (isinf(mx)) all(see_finite);
+            top = fmaxf(top, mx);
+            if (mode == kMax) continue;
+            s = pow2_scale(__float_as_uint(mx));
+            if (me == 0) it.rinv[r] = pow2_inv(s);
         }
-        __half* hi = static_cast<__half*>(it.dst) + r * it.dld;
-        __half* lo = hi + it.plane;
-        for (long long c = 4 * lane; c < it.dld; c += 128) {
-            float x[4];
-            if (four && c < it.cols) {
-                const float4 v = *reinterpret_cast<const float4*>(src + c);
-                x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = c + j < it.cols ? src[c + j] : 0.f;
-            }
-            __half h[4], g[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) split_half(x[j] * s, h[j], g[j]);
+        __half* hi = static_cast<__half*>(it.dst) + r * dld;
+        auto put = [&](long long c, const float4& v) {
+            __half2 h[2], g[2];
+            split_half2(v.x * s, v.y * s, h[0], g[0]);
+            split_half2(v.z * s, v.w * s, h[1], g[1]);
             *reinterpret_cast<uint2*>(hi + c) = *reinterpret_cast<uint2*>(h);
-            *reinterpret_cast<uint2*>(lo + c) = *reinterpret_cast<uint2*>(g);
-        }
+            *reinterpret_cast<uint2*>(hi + it.plane + c) = *reinterpret_cast<uint2*>(g);
+        };
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (4LL * (j * threads + me) < dld) put(4LL * (j * threads + me), x[j]);
+        for (long long c = held + 4 * me; c < dld; c += 4 * threads) put(c, load(c));
     }
-    if (it.max && (it.mode == kMax || it.mode == kRowSplit) && lane == 0 && top)
-        atomicMax(it.max, top);
+    if (it.max && (mode == kMax || mode == kRowSplit) && lane == 0 && top > 0.f)
+        atomicMax(it.max, __float_as_uint(top));
 }
 
 int prepare(const PrepList& l, cudaStream_t st) {
     if (l.n == 0) return ATOM_OK;
-    long long rows = 1;
-    for (int i = 0; i < l.n; ++i) rows = rows < l.it[i].rows ? l.it[i].rows : rows;
+    long long rows = 1, nv = 1;
+    for (int i = 0; i < l.n; ++i) {
+        const PrepItem& it = l.it[i];
+        const bool wide = prep_wide(it);
+        rows = std::max(rows, wide ? 8 * it.rows : it.rows);
+        if (it.mode != kPack)
+            nv = std::max(nv, (std::max(it.dld, it.cols) + (wide ? 1023 : 127)) / (wide ? 1024 : 128));
+    }
     const long long blocks = (rows + 7) / 8;
-    prep_kernel<<<dim3((unsigned)(blocks < 1184 ? blocks : 1184), l.n), 256, 0, st>>>(l);
+    const dim3 grid((unsigned)std::min(blocks, 2368LL), l.n);
+    if (nv <= 1) prep_kernel<1><<<grid, 256, 0, st>>>(l);
+    else if (nv <= 2) prep_kernel<2><<<grid, 256, 0, st>>>(l);
+    else if (nv <= 4) prep_kernel<4><<<grid, 256, 0, st>>>(l);
+    else prep_kernel<8><<<grid, 256, 0, st>>>(l);
     return check_launch("operand preparation");
 }
 
@@ -760,20 +958,23 @@ static PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     return fn;
 }
 
-int make_map(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld,
-             int box_rows, int depth, long long ldz) {
+static int encode_map(CUtensorMap* m, const void* p, bool f32, long long cols, long long rows,
+                      long long depth, long long ld, long long ldz, int box_cols, int box_rows,
+                      CUtensorMapSwizzle swizzle) {
     const auto encode = encoder();
     if (!encode) {
         set_error("cuTensorMapEncodeTiled unavailable");
         return ATOM_ERR_CUDA;
     }
+    const int e = f32 ? 4 : 2;
     cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)depth};
-    cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)ldz * 2};
-    cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+    cuuint64_t strides[2] = {(cuuint64_t)ld * e, (cuuint64_t)ldz * e};
+    cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
     cuuint32_t estr[3] = {1, 1, 1};
-    const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, depth ? 3 : 2,
+    const CUresult r = encode(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : CU_TENSOR_MAP_DATA_TYPE_UINT16, depth ? 3 : 2,
                               const_cast<void*>(p), dims, strides, box, estr,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
@@ -781,6 +982,17 @@ int make_map(CUtensorMap* m, const void* p, long long cols, long long rows, long
         return ATOM_ERR_ARG;
     }
     return ATOM_OK;
+}
+int make_map(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld,
+             int box_rows, int depth, long long ldz) {
+    return encode_map(m, p, false, cols, rows, depth, ld, ldz, 64, box_rows,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int make_out_map(CUtensorMap* m, const void* p, int dtype, long long cols, long long rows,
+                 long long ld) {
+    const bool f32 = dtype == ATOM_F32;
+    return encode_map(m, p, f32, cols, rows, 0, ld, 0, 32, 32,
+                      f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 static int sm_count() {
@@ -847,7 +1059,7 @@ static int run(const Maps& maps, const Args& p, cudaStream_t st) {
     return ATOM_OK;
 }
 
-int launch(int epilogue, const Choice& c, bool split, const Maps& maps, Args& p, cudaStream_t st) {
+int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, cudaStream_t st) {
     const bool gated = epilogue == kGate || epilogue == kGateBwdGU;
     const int w = gated ? c.bn / 2 : c.bn;
     p.mtiles = ceil_div(p.M, 256);
@@ -864,6 +1076,24 @@ int launch(int epilogue, const Choice& c, bool split, const Maps& maps, Args& p,
         return ATOM_ERR_CAPACITY;
     }
     if (p.tiles == 0) return ATOM_OK;
+    if (epilogue == kStore && !p.blocked) {
+        // TMA stores clip at 16 bytes, so columns have to end there too
+        const int e = p.ksplit > 1 ? 4 : dtype_size(p.dtype);
+        p.tma = p.N * e % 16 == 0;
+        for (int g = 0; g < p.groups && p.ksplit == 1; ++g)
+            p.tma = p.tma && aligned16(p.C[g]) && p.ldc * e % 16 == 0;
+        if (p.tma && p.ksplit > 1) {
+            p.used |= 1u << kPartMap;
+            if (int s = encode_map(&maps.m[kPartMap], p.part, true, p.N, p.M, p.ksplit * p.groups,
+                                   p.N, p.M * p.N, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B))
+                return s;
+        }
+        for (int g = 0; p.tma && p.ksplit == 1 && g < p.groups; ++g) {
+            p.used |= 1u << (kOutMap + g);
+            if (int s = make_out_map(&maps.m[kOutMap + g], p.C[g], p.dtype, p.N, p.M, p.ldc))
+                return s;
+        }
+    }
 #define ATOM_PAIR(E)                                            \
     if (epilogue == E) {                                        \
         if (split) return run<128, E, true>(maps, p, st);       \

@@ -9,6 +9,7 @@ namespace atom {
 namespace pair {
 
 constexpr int kMaps = 12;
+constexpr int kOutMap = 8, kHMap = 10, kPartMap = 11;   // outputs (two groups), H, partial sums
 struct Maps {
     CUtensorMap m[kMaps];
 };
@@ -36,12 +37,15 @@ struct Args {
     void* C[2];
     long long ldc;
     int dtype;               // C's type
-    int vec;                 // C's rows may be stored in 16-byte pieces
+    int tma;                 // kStore: C (the partial sums) by TMA
+    unsigned used;           // maps to prefetch
+    float* blocked;          // kStore: fp32 to 32 x 32 lane blocks instead of C
     float* part;             // ksplit > 1: [split][group][M][N] fp32
     int act;
-    float* gu;               // gate: kept pre-activations [M][2 Fp] (written or read), or NULL
-    const float* dh;         // kGateBwdGU: [M][Fp]
-    void* H;                 // backward: [M][Fp], C[0] is [M][2 Fp]; NULL: not wanted
+    float* gu;               // gate: kept g, and u gu_half further, lane blocks, or NULL
+    long long gu_half;
+    float* dh;               // kGateBwdGU: lane blocks
+    int H;                   // gate backward: H wanted (map kHMap; dG | dU: kOutMap, u at Fp)
     int Fp;
     const float* rinv;       // SPLIT: 1 / scale of A's rows, or NULL
     const unsigned* amax;    // SPLIT: finite maximum (bits) of A's tensor where rinv is NULL
@@ -72,8 +76,12 @@ Choice choose(long long M, int N, int nk, int groups, bool gated, bool split, bo
 int make_map(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld,
              int box_rows, int depth = 0, long long ldz = 0);
 
-// Launches the product: p.tiles etc. are filled in from M, N, groups and the choice.
-int launch(int epilogue, const Choice& c, bool split, const Maps& maps, Args& p, cudaStream_t st);
+// Map of an output [rows, cols] that is written in blocks of 32 x 32.
+int make_out_map(CUtensorMap* m, const void* p, int dtype, long long cols, long long rows,
+                 long long ld);
+
+// Launches the product: tiles, C's maps (kStore) etc. are filled in from M, N, C and the choice.
+int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, cudaStream_t st);
 
 // Operand preparation, up to 6 matrices a launch.
 enum Prep { kPack = 0, kRowSplit = 1, kMax = 2, kTensorSplit = 3 };

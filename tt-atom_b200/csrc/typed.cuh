@@ -39,11 +39,11 @@ __device__ __forceinline__ float pow2_scale(unsigned bits) {
 __device__ __forceinline__ float pow2_inv(float s) {
     return __uint_as_float((254u << 23) - (__float_as_uint(s) & 0x7F800000u));
 }
-// y = hi + lo 2^-11 to 22 bits; what is not finite goes into hi alone.
-__device__ __forceinline__ void split_half(float y, __half& hi, __half& lo) {
-    hi = __float2half_rn(y);
-    const float back = __half2float(hi);
-    lo = __float2half_rn(finite_bits(back) || back == 0.f ? (y - back) * 2048.f : 0.f);
+// y = hi + lo 2^-11 to 22 bits (lo is NaN where y is not finite).
+__device__ __forceinline__ void split_half2(float y0, float y1, __half2& hi, __half2& lo) {
+    hi = __floats2half2_rn(y0, y1);
+    const float2 back = __half22float2(hi);
+    lo = __floats2half2_rn((y0 - back.x) * 2048.f, (y1 - back.y) * 2048.f);
 }
 
 // Pieces of a caller's workspace, 256-byte aligned; with base NULL it only adds up the sizes.
