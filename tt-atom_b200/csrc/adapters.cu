@@ -81,7 +81,7 @@ __device__ __forceinline__ bool side_work(const Shrink& p) {
     if (b < 0) return false;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (b == p.q.nad) {
-        for (int t = blockIdx.y * 8 + warp; t < p.tiles; t += 32) {
+        for (int t = blockIdx.y * 8 + warp; t < p.tiles; t += 64) {
             const int first = last_le(p.q.n, t * 256, [&](int r) { return row_of(p.q, r); });
             const int last = last_le(p.q.n, t * 256 + 255, [&](int r) { return row_of(p.q, r); });
             // a request that begins before the tile reaches into it at most as the last such one
@@ -89,6 +89,7 @@ __device__ __forceinline__ bool side_work(const Shrink& p) {
         }
         return true;
     }
+    if (blockIdx.y >= 4) return true;
     int found = 0;
     const long long lo = p.other_n * blockIdx.y / 4, hi = p.other_n * (blockIdx.y + 1) / 4;
     const long long at = (long long)b * p.other_n;
@@ -166,26 +167,28 @@ __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uin
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16-bit: a block of 8 warps has 64 rows of a piece, 16 a warp, and the warps left over split K
-// (all eight do for a piece of 16 rows or fewer). Rows and adapters go from memory into the
-// fragments of m16n8k16 directly: the product does not mind in which order K runs, so each lane
-// reads 8 consecutive elements of its row, half for one instruction and half for the next.
-// Bound by reading x; an adapter's rows come from L1.
+// 16-bit: a block of 8 warps has 32 rows of a piece, 16 a warp, and the warps split K (all eight
+// of them for 16 rows or fewer). Rows and adapters go from memory into the fragments of m16n8k16
+// directly: the product does not mind in which order K runs, so each lane reads 8 consecutive
+// elements of its row, half for one instruction and half for the next. Bound by reading x: an
+// adapter's rows come from L2 and L1, and small blocks, three on an SM, keep enough in flight
+// (with 64 rows and one block an SM 8192 x 2048 rows of rank 32 took 30 us).
 template <bool BF16, int NT>
-__global__ void __launch_bounds__(256) shrink16_kernel(const __grid_constant__ Shrink p) {
+__global__ void __launch_bounds__(256, NT <= 4 ? 3 : 1)
+    shrink16_kernel(const __grid_constant__ Shrink p) {
     extern __shared__ float red[];       // [8 warps][16][8 NT]
     if (side_work(p)) return;
     const Piece c = find_piece(p);
     if (c.slot < 0) return;
-    const int m0 = c.m0 + blockIdx.y * 64, lo = max(c.lo, m0), hi = min(c.hi, m0 + 64);
+    const int m0 = c.m0 + blockIdx.y * 32, lo = max(c.lo, m0), hi = min(c.hi, m0 + 32);
     unsigned short* block = static_cast<unsigned short*>(p.block) +
-                            ((long long)blockIdx.x * 256 + blockIdx.y * 64) * p.Rs;
-    if (lo >= hi) {
-        for (int i = threadIdx.x; i < 64 * p.Rs; i += 256) block[i] = 0;
+                            ((long long)blockIdx.x * 256 + blockIdx.y * 32) * p.Rs;
+    if (lo >= hi) {                      // Rs is a multiple of 8
+        for (int i = threadIdx.x; i < 4 * p.Rs; i += 256)
+            reinterpret_cast<uint4*>(block)[i] = make_uint4(0, 0, 0, 0);
         return;
     }
-    const int g0 = (lo - m0) / 16, groups = (hi - 1 - m0) / 16 - g0 + 1;
-    const int gp = groups == 1 ? 1 : groups == 2 ? 2 : 4, parts = 8 / gp;
+    const int g0 = (lo - m0) / 16, gp = (hi - 1 - m0) / 16 - g0 + 1, parts = 8 / gp;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t8 = (lane & 3) * 8;
     const int grp = warp % gp, part = warp / gp;
@@ -193,7 +196,7 @@ __global__ void __launch_bounds__(256) shrink16_kernel(const __grid_constant__ S
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    if (grp < groups) {
+    {
         const int chunks = (p.K + 31) / 32;
         const int ra = m0 + (g0 + grp) * 16 + g, rb = ra + 8;
         const bool oka = ra >= lo && ra < hi, okb = rb >= lo && rb < hi;
@@ -201,13 +204,14 @@ __global__ void __launch_bounds__(256) shrink16_kernel(const __grid_constant__ S
         const unsigned short* xb = xa + 8 * p.ld;
         const unsigned short* w = static_cast<const unsigned short*>(p.w) + c.slot * p.wa + g * p.wr;
         const uint4 zero = make_uint4(0, 0, 0, 0);
-        constexpr int U = NT <= 4 ? 4 : 1;
-        for (int ch = chunks * part / parts; ch < chunks * (part + 1) / parts; ch += U) {
+        constexpr int U = NT <= 2 ? 3 : NT <= 4 ? 2 : 1;
+        const int end = chunks * (part + 1) / parts;
+        for (int ch = chunks * part / parts; ch < end; ch += U) {
             uint4 a[U], b[U], v[U][NT];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int k = (ch + u) * 32 + t8;
-                const bool in = k < p.K && ch + u < chunks * (part + 1) / parts;
+                const bool in = k < p.K && ch + u < end;
                 a[u] = oka && in ? load8(xa, k, p.K) : zero;
                 b[u] = okb && in ? load8(xb, k, p.K) : zero;
 #pragma unroll
@@ -233,76 +237,80 @@ __global__ void __launch_bounds__(256) shrink16_kernel(const __grid_constant__ S
     }
     __syncthreads();
     const float s = p.scale[c.slot];
-    for (int i = threadIdx.x; i < 64 * p.Rs; i += 256) {
+    for (int i = threadIdx.x; i < 32 * p.Rs; i += 256) {
         const int row = i / p.Rs, r = i - row * p.Rs, m = m0 + row;
         float v = 0.f;
-        const bool in = m >= lo && m < hi && r < p.R;
-        if (in) {
+        const bool in = m >= lo && m < hi;
+        if (in && r < p.R) {
             const float* q = red + ((row / 16 - g0) * 16 + row % 16) * 8 * NT + r;
-            for (int k = 0; k < parts; ++k) v += q[(long long)k * gp * 128 * NT];
+            for (int k = 0; k < parts; ++k) v += q[k * gp * 128 * NT];
             v *= s;
         }
         store_f(block, i, v, p.dtype);
-        if (p.compact && m >= lo && m < hi) store_f(p.compact, (long long)m * p.Rs + r, v, p.dtype);
+        if (p.compact && in) store_f(p.compact, (long long)m * p.Rs + r, v, p.dtype);
     }
 }
 
-// fp32: FMA products of 64 rows by 32 ranks, 32 deep; then each row's planes.
+// fp32: a warp has 8 rows by 8 ranks, its lanes split K, and the 64 sums are added over the lanes
+// by halves (lane l ends with sums 2 l and 2 l + 1); then each row's planes.
+__device__ __forceinline__ void sum_halves(float* v, int lane) {
+#pragma unroll
+    for (int o = 16, n = 32; o > 0; o >>= 1, n >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float mine = up ? v[n + i] : v[i], other = up ? v[i] : v[n + i];
+            v[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+        }
+    }
+}
 __global__ void __launch_bounds__(256) shrink32_kernel(const __grid_constant__ Shrink p) {
-    extern __shared__ float out[];       // [64][R + 1]
-    __shared__ float xs[64][33], ws[32][33];
+    extern __shared__ float out[];       // [32][R + 1]
     if (side_work(p)) return;
     const Piece c = find_piece(p);
     if (c.slot < 0) return;
-    const int m0 = c.m0 + blockIdx.y * 64, lo = max(c.lo, m0), hi = min(c.hi, m0 + 64);
+    const int m0 = c.m0 + blockIdx.y * 32, lo = max(c.lo, m0), hi = min(c.hi, m0 + 32);
     __half* block = static_cast<__half*>(p.block) +
-                    ((long long)blockIdx.x * 256 + blockIdx.y * 64) * p.Rs;
+                    ((long long)blockIdx.x * 256 + blockIdx.y * 32) * p.Rs;
     if (lo >= hi) {
-        for (int i = threadIdx.x; i < 64 * p.Rs; i += 256) {
-            block[i] = __float2half_rn(0.f);
-            block[i + p.plane] = __float2half_rn(0.f);
+        for (int i = threadIdx.x; i < 4 * p.Rs; i += 256) {
+            reinterpret_cast<uint4*>(block)[i] = make_uint4(0, 0, 0, 0);
+            reinterpret_cast<uint4*>(block + p.plane)[i] = make_uint4(0, 0, 0, 0);
         }
         return;
     }
-    const float* x = static_cast<const float*>(p.rows);
-    const float* w = static_cast<const float*>(p.w) + c.slot * p.wa;
-    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    const int pitch = p.R + 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pitch = p.R + 1;
     const float s = p.scale[c.slot];
-    for (int r0 = 0; r0 < p.R; r0 += 32) {
-        float acc[4][2] = {};
-        for (int k0 = 0; k0 < p.K; k0 += 32) {
-            for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-                const int m = m0 + (i >> 5), k = k0 + (i & 31);
-                xs[i >> 5][i & 31] = m >= lo && m < hi && k < p.K ? x[m * p.ld + k] : 0.f;
-            }
-            for (int i = threadIdx.x; i < 32 * 32; i += 256) {
-                const int r = p.wk == 1 ? i >> 5 : i & 31, k = p.wk == 1 ? i & 31 : i >> 5;
-                ws[r][k] = r0 + r < p.R && k0 + k < p.K
-                               ? w[(r0 + r) * p.wr + (k0 + k) * p.wk] : 0.f;
-            }
-            __syncthreads();
+    const int groups = (hi - lo + 7) / 8, ranks = (p.R + 7) / 8;
+    for (int item = warp; item < groups * ranks; item += 8) {
+        const int row0 = lo + item / ranks * 8, r0 = item % ranks * 8;
+        const float* x = static_cast<const float*>(p.rows) + row0 * p.ld;
+        const float* w = static_cast<const float*>(p.w) + c.slot * p.wa + r0 * p.wr;
+        float acc[64];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-                const float b0 = ws[tx][k], b1 = ws[tx + 16][k];
+        for (int i = 0; i < 64; ++i) acc[i] = 0.f;
+        const int nr = min(8, hi - row0), nk = min(8, p.R - r0);
+#pragma unroll 2
+        for (int k = lane; k < p.K; k += 32) {
+            float a[8], b[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = xs[ty + 16 * i][k];
-                    acc[i][0] = fmaf(a, b0, acc[i][0]);
-                    acc[i][1] = fmaf(a, b1, acc[i][1]);
-                }
-            }
-            __syncthreads();
+            for (int i = 0; i < 8; ++i) a[i] = i < nr ? x[i * p.ld + k] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = j < nk ? w[j * p.wr + k * p.wk] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[8 * i + j] = fmaf(a[i], b[j], acc[8 * i + j]);
         }
+        sum_halves(acc, lane);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (r0 + tx + 16 * j < p.R) out[(ty + 16 * i) * pitch + r0 + tx + 16 * j] = s * acc[i][j];
+        for (int e = 0; e < 2; ++e) {
+            const int i = (2 * lane + e) >> 3, j = (2 * lane + e) & 7;
+            if (i < nr && j < nk) out[(row0 - m0 + i) * pitch + r0 + j] = s * acc[e];
+        }
     }
     __syncthreads();
-    const int lane = threadIdx.x & 31;
-    for (int row = threadIdx.x >> 5; row < 64; row += 8) {
+    for (int row = warp; row < 32; row += 8) {
         const int m = m0 + row;
         const bool in = m >= lo && m < hi;
         unsigned mx = 0;
@@ -339,7 +347,9 @@ __global__ void __launch_bounds__(256) transpose_kernel(const unsigned short* sr
     }
 }
 
-// dA[a] = T^T x and dB[a] = (S^T dy)^T over the pieces of adapter a, in their order.
+// dA[a] = T^T x and dB[a] = (S^T dy)^T over the pieces of adapter a, in their order: blocks have
+// all ranks by 128 columns of x or dy, and the pieces are shared out over blocks (`split`) whose
+// sums are added in order by a second pass. Bound by reading x and dy once.
 struct Grads {
     const int4* piece;
     int pieces, nad, R, Rs;
@@ -349,78 +359,209 @@ struct Grads {
     int width[2];            // D, O
     int tiles0;              // 128-column tiles of the first
     void* out[2];
-    float* part;             // split > 1: [split][adapter](R D | R O)
+    float* part;             // split > 1: [split][adapter][R][D + O]
     int split;
     int dtype;
 };
-__global__ void __launch_bounds__(256) grads_kernel(const __grid_constant__ Grads p) {
-    __shared__ float ts[32][36], xs[32][132];
+// Walks an adapter's rows in a block's share of the pieces, `step` at a time (whole warps).
+struct Rows {
+    const int4* piece;
+    int a, b, behind, step;
+    unsigned mine = 0;
+    int m = 0, hi = 0;
+    __device__ __forceinline__ Rows(const Grads& p, int adapter, int rows)
+        : piece(p.piece), a(adapter), step(rows) {
+        b = (int)((long long)p.pieces * blockIdx.z / p.split) - 32;
+        behind = (int)((long long)p.pieces * (blockIdx.z + 1) / p.split);
+    }
+    // the next rows m .. min(m + step, hi) - 1; false when there are none
+    __device__ __forceinline__ bool next() {
+        m += step;
+        if (m < hi) return true;
+        while (mine == 0) {
+            b += 32;
+            if (b >= behind) {
+                b = behind;
+                hi = 0;
+                return false;
+            }
+            const int i = b + (threadIdx.x & 31);
+            mine = __ballot_sync(0xffffffffu, i < behind && piece[i].x == a);
+        }
+        const int4 c = piece[b + __ffs(mine) - 1];
+        mine &= mine - 1;
+        m = c.y;
+        hi = c.z;
+        return true;
+    }
+};
+__device__ __forceinline__ void put_grad(const Grads& p, int which, int a, int r, int k, float v) {
+    const int W = p.width[which];
+    if (r >= p.R || k >= W) return;
+    if (p.split > 1)
+        p.part[(((long long)blockIdx.z * p.nad + a) * p.R + r) * (p.width[0] + p.width[1]) +
+               (which ? p.width[0] : 0) + k] = v;
+    else
+        store_f(p.out[which], (long long)a * p.R * W + (which ? (long long)k * p.R + r
+                                                             : (long long)r * W + k), v, p.dtype);
+}
+
+// 16-bit: 32 rows of both operands a stage, four stages by cp.async, both read transposed into
+// the fragments of m16n8k16. Each of 8 warps has 16 columns and all ranks.
+template <bool BF16, int MT>
+__global__ void __launch_bounds__(256) grads16_kernel(const __grid_constant__ Grads p) {
+    constexpr int kX = 32 * 272, kT = 32 * (32 * MT + 16), kStages = 4;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int which = blockIdx.x >= p.tiles0;
+    const int c0 = (blockIdx.x - (which ? p.tiles0 : 0)) * 128, W = p.width[which];
+    const unsigned short* rows = static_cast<const unsigned short*>(p.rows[which]);
+    const unsigned short* low = static_cast<const unsigned short*>(p.low[which]);
+    const long long ld = p.ld[which];
+    const int a = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    Rows it(p, a, 32);
+    int loaded = 0;
+    bool more = true;
+    auto load = [&]() {
+        if (more && (more = it.next())) {
+            const uint32_t x = base + (loaded % kStages) * (kX + kT), t = x + kX;
+            const int n = min(32, it.hi - it.m);
+            for (int i = threadIdx.x; i < 32 * 16; i += 256) {
+                const int r = i >> 4, c = (i & 15) * 8;
+                // bytes past the row's or the matrix's end are zeros
+                const int bytes = r < n ? max(0, min(16, 2 * (W - c0 - c))) : 0;
+                const void* src = bytes ? rows + (it.m + r) * ld + c0 + c : rows;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(x + r * 272 + c * 2),
+                             "l"(src), "r"(bytes) : "memory");
+            }
+            for (int i = threadIdx.x; i < 32 * 2 * MT; i += 256) {
+                const int r = i / (2 * MT), c = (i % (2 * MT)) * 8;
+                const int bytes = r < n && c < p.Rs ? 16 : 0;
+                const void* src = bytes ? low + (long long)(it.m + r) * p.Rs + c : low;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                 t + r * (32 * MT + 16) + c * 2), "l"(src), "r"(bytes) : "memory");
+            }
+            ++loaded;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float acc[MT][2][4] = {};
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) load();
+    for (int done = 0; done < loaded; ++done) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncthreads();
+        const uint32_t x = base + (done % kStages) * (kX + kT), t = x + kX;
+#pragma unroll
+        for (int k = 0; k < 32; k += 16) {
+            uint32_t b[4];
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3])
+                         : "r"(x + (k + (lane & 7) + ((lane >> 3) & 1) * 8) * 272 +
+                               (warp * 16 + (lane >> 4) * 8) * 2) : "memory");
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                uint32_t f[4];
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3])
+                             : "r"(t + (k + (lane & 7) + (lane >> 4) * 8) * (32 * MT + 16) +
+                                   (i * 16 + ((lane >> 3) & 1) * 8) * 2) : "memory");
+                mma16816<BF16>(acc[i][0], f[0], f[1], f[2], f[3], b[0], b[1]);
+                mma16816<BF16>(acc[i][1], f[0], f[1], f[2], f[3], b[2], b[3]);
+            }
+        }
+        load();
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    const int k0 = c0 + warp * 16 + (lane & 3) * 2;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                put_grad(p, which, a, i * 16 + (lane >> 2) + (e >> 1) * 8, k0 + j * 8 + (e & 1),
+                         acc[i][j][e]);
+}
+
+// fp32: 32 ranks by 128 columns a block, 4 x 4 a thread, 32 rows at a time.
+__global__ void __launch_bounds__(256) grads32_kernel(const __grid_constant__ Grads p) {
+    __shared__ __align__(16) float ts[32][36], xs[32][132];
     const int which = blockIdx.x >= p.tiles0;
     const int c0 = (blockIdx.x - (which ? p.tiles0 : 0)) * 128, W = p.width[which];
     const int chunks = (p.R + 31) / 32;
     const int a = blockIdx.y / chunks, r0 = (blockIdx.y - a * chunks) * 32;
-    const int lane = threadIdx.x & 31;
-    const int ty = threadIdx.x >> 5, tx = lane;      // 4 ranks, 4 columns a thread
+    const float* rows = static_cast<const float*>(p.rows[which]) + c0;
+    const float* low = static_cast<const float*>(p.low[which]) + r0;
+    const long long ld = p.ld[which];
+    const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
     float acc[4][4] = {};
-    const int first = (int)((long long)p.pieces * blockIdx.z / p.split);
-    const int behind = (int)((long long)p.pieces * (blockIdx.z + 1) / p.split);
-    for (int b = first; b < behind; b += 32) {
-        unsigned mine = __ballot_sync(0xffffffffu, b + lane < behind && p.piece[b + lane].x == a);
-        while (mine) {
-            const int4 c = p.piece[b + __ffs(mine) - 1];
-            mine &= mine - 1;
-            for (int m0 = c.y; m0 < c.z; m0 += 32) {
-                for (int i = threadIdx.x; i < 1024; i += 256) {
-                    const int m = m0 + (i >> 5), r = r0 + (i & 31);
-                    ts[i >> 5][i & 31] = m < c.z && r < p.R
-                        ? load_f(p.low[which], (long long)m * p.Rs + r, p.dtype) : 0.f;
-                }
-                for (int i = threadIdx.x; i < 4096; i += 256) {
-                    const int m = m0 + (i >> 7), k = c0 + (i & 127);
-                    xs[i >> 7][i & 127] = m < c.z && k < W
-                        ? load_f(p.rows[which], m * p.ld[which] + k, p.dtype) : 0.f;
-                }
-                __syncthreads();
-#pragma unroll 8
-                for (int k = 0; k < 32; ++k) {
-                    const float4 t = *reinterpret_cast<const float4*>(&ts[k][ty * 4]);
-                    const float4 x = *reinterpret_cast<const float4*>(&xs[k][tx * 4]);
-                    const float tt[4] = {t.x, t.y, t.z, t.w}, xx[4] = {x.x, x.y, x.z, x.w};
+    for (Rows it(p, a, 32); it.next();) {
+        const int n = min(32, it.hi - it.m);
+        float x[16], t[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 16; ++i) {       // warp: rows ty, ty + 8, ..; lanes: columns
+            const int r = ty + 8 * (i >> 2), k = lane + 32 * (i & 3);
+            x[i] = r < n && c0 + k < W ? rows[(it.m + r) * ld + k] : 0.f;
+        }
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(tt[i], xx[j], acc[i][j]);
-                }
-                __syncthreads();
-            }
+        for (int i = 0; i < 4; ++i) {
+            const int r = ty + 8 * i;
+            t[i] = r < n && r0 + lane < p.R ? low[(long long)(it.m + r) * p.Rs + lane] : 0.f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) xs[ty + 8 * (i >> 2)][lane + 32 * (i & 3)] = x[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ts[ty + 8 * i][lane] = t[i];
+        __syncthreads();
+        for (int k = 0; k < n; ++k) {
+            const float4 u = *reinterpret_cast<const float4*>(&ts[k][ty * 4]);
+            const float4 v = *reinterpret_cast<const float4*>(&xs[k][lane * 4]);
+            const float tt[4] = {u.x, u.y, u.z, u.w}, xx[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(tt[i], xx[j], acc[i][j]);
         }
     }
-    const long long per = (long long)p.R * (p.width[0] + p.width[1]);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = r0 + ty * 4 + i, k = c0 + tx * 4 + j;
-            if (r >= p.R || k >= W) continue;
-            const long long e = which ? (long long)k * p.R + r : (long long)r * W + k;
-            if (p.split > 1)
-                p.part[((long long)blockIdx.z * p.nad + a) * per +
-                       (which ? (long long)p.R * p.width[0] : 0) + e] = acc[i][j];
-            else
-                store_f(p.out[which], (long long)a * p.R * W + e, acc[i][j], p.dtype);
-        }
+        for (int j = 0; j < 4; ++j)
+            put_grad(p, which, a, r0 + ty * 4 + i, c0 + lane * 4 + j, acc[i][j]);
 }
 __global__ void __launch_bounds__(256) grads_sum_kernel(const __grid_constant__ Grads p) {
-    const long long n0 = (long long)p.R * p.width[0], per = n0 + (long long)p.R * p.width[1];
-    const long long all = per * p.nad;
+    const int W = p.width[0] + p.width[1];
+    const long long per = (long long)p.R * W, all = per * p.nad;
     for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
         float v = 0.f;
         for (int s = 0; s < p.split; ++s) v += p.part[s * all + i];
         const long long a = i / per, e = i - a * per;
-        const int which = e >= n0;
-        if (p.out[which])
-            store_f(p.out[which], which ? a * (per - n0) + e - n0 : a * n0 + e, v, p.dtype);
+        const int r = (int)(e / W), k = (int)(e - (long long)r * W);
+        if (k < p.width[0])
+            store_f(p.out[0], (a * p.R + r) * p.width[0] + k, v, p.dtype);
+        else
+            store_f(p.out[1], (a * p.width[1] + k - p.width[0]) * p.R + r, v, p.dtype);
     }
+}
+template <bool BF16>
+int grads16(const Grads& p, dim3 grid, cudaStream_t st) {
+#define ATOM_GRADS(N)                                                                             \
+    if (p.R <= 16 * N) {                                                                          \
+        constexpr int smem = 4 * (32 * 272 + 32 * (32 * N + 16));                                 \
+        if (smem > 48 * 1024)                                                                     \
+            cudaFuncSetAttribute(grads16_kernel<BF16, N>,                                         \
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem);              \
+        grads16_kernel<BF16, N><<<grid, 256, smem, st>>>(p);                                      \
+        return check_launch("adapters: gradients");                                               \
+    }
+    ATOM_GRADS(1)
+    ATOM_GRADS(2)
+    ATOM_GRADS(4)
+    ATOM_GRADS(8)
+#undef ATOM_GRADS
+    return ATOM_ERR_UNSUPPORTED;
 }
 
 struct AdSizes {
@@ -430,15 +571,15 @@ struct AdSizes {
     int tiles, pieces, Rs;
     long long Dp, Op;
     bool split, on;
-    AdSizes(int t, long long m, int d, int o, int n, int r, int q)
+    Choice product;
+    AdSizes(int t, long long m, int d, int o, int n, int r, int q, bool bwd)
         : dtype(t), M(m), D(d), O(o), nad(n), R(r), nreq(q), tiles((int)((m + 255) / 256)),
           pieces(tiles + q), Rs((int)up(r, 8)), Dp(up(d, 8)), Op(up(o, 8)), split(t == ATOM_F32),
-          on(n > 0 && q > 0) {}
-    Choice product(bool bwd) const {
-        return choose(M, bwd ? D : O, ((bwd ? O : D) + 63) / 64, 1, false, split, true);
-    }
+          on(n > 0 && q > 0),
+          product(choose(m, bwd ? d : o, ((bwd ? o : d) + 63) / 64, 1, false, t == ATOM_F32, true)) {}
     int grad_split() const {
-        const long long blocks = (long long)nad * ((R + 31) / 32) * ((D + 127) / 128 + (O + 127) / 128);
+        const long long blocks = (long long)nad * (split ? (R + 31) / 32 : 1) *
+                                 ((D + 127) / 128 + (O + 127) / 128);
         const long long s = blocks ? 592 / blocks : 1;
         return (int)std::max(1LL, std::min({s, 16LL, (long long)pieces}));
     }
@@ -458,7 +599,7 @@ struct AdSpace {
         const long long k = z.split ? 2 : 1, e = dtype_size(z.dtype);
         rows = c.take<__half>(k * z.M * (bwd ? z.Op : z.Dp));
         w = c.take<__half>(k * z.O * z.Dp);
-        part = c.take<float>(z.product(bwd).part);
+        part = c.take<float>(z.product.part);
         if (z.split) {
             max = c.take<unsigned>(4);
             rinv = c.take<float>(z.M);
@@ -508,10 +649,10 @@ int shrink16(const Shrink& p, dim3 grid, cudaStream_t st) {
     return ATOM_ERR_UNSUPPORTED;
 }
 int shrink(const Shrink& p, cudaStream_t st) {
-    const dim3 grid(p.pieces + p.q.nad + 1, 4);
+    const dim3 grid(p.pieces + p.q.nad + 1, 8);
     if (p.dtype == ATOM_BF16) return shrink16<true>(p, grid, st);
     if (p.dtype == ATOM_F16) return shrink16<false>(p, grid, st);
-    shrink32_kernel<<<grid, 256, 64 * (p.R + 1) * 4, st>>>(p);
+    shrink32_kernel<<<grid, 256, 32 * (p.R + 1) * 4, st>>>(p);
     return check_launch("adapters: low-rank rows");
 }
 
@@ -613,7 +754,7 @@ struct Ad {
             if (int s = shrink(h, st)) return s;
         }
         if (low_only) return ATOM_OK;
-        const Choice c = z.product(bwd);
+        const Choice c = z.product;
         Maps maps;
         const long long planes[3] = {z.M * Kp, z.O * z.Dp, srows * sp_ld};
         const long long bplane = (long long)z.pieces * 256 * z.Rs;
@@ -684,9 +825,9 @@ extern "C" int atom_adapted_linear_bytes(int dtype, int64_t M, int D, int O, int
                                          int R, int nreq, size_t* bytes_host) {
     if (int s = check_ad(dtype, M, D, O, n_adapters, R, nreq)) return s;
     ATOM_REQUIRE(bytes_host, "adapted_linear: bytes_host is NULL");
-    const AdSizes z(dtype, M, D, O, n_adapters, R, nreq);
+    const AdSizes z(dtype, M, D, O, n_adapters, R, nreq, false);
     bytes_host[0] = AdSpace(nullptr, z, false).bytes;
-    bytes_host[1] = AdSpace(nullptr, z, true).bytes;
+    bytes_host[1] = AdSpace(nullptr, AdSizes(dtype, M, D, O, n_adapters, R, nreq, true), true).bytes;
     bytes_host[2] = (size_t)M * z.Rs * dtype_size(dtype);
     return ATOM_OK;
 }
@@ -700,7 +841,7 @@ extern "C" int atom_adapted_linear_fwd(int dtype, const void* x, int64_t ldx, in
     if (int s = check_ad(dtype, M, D, O, n_adapters, R, nreq)) return s;
     if (M == 0) return ATOM_OK;
     ATOM_REQUIRE(x && w && y && ldx >= D && ldy >= O, "adapted_linear: bad operand");
-    const AdSizes z(dtype, M, D, O, n_adapters, R, nreq);
+    const AdSizes z(dtype, M, D, O, n_adapters, R, nreq, false);
     ATOM_REQUIRE(!z.on || (a && b && scale && req_ptr && req_adapter),
                  "adapted_linear: bad operand");
     Ad f{z, AdSpace(ws, z, false), (cudaStream_t)stream,
@@ -720,7 +861,7 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
     if (int s = check_ad(dtype, M, D, O, n_adapters, R, nreq)) return s;
     cudaStream_t st = (cudaStream_t)stream;
     const size_t e = dtype_size(dtype);
-    const AdSizes z(dtype, M, D, O, n_adapters, R, nreq);
+    const AdSizes z(dtype, M, D, O, n_adapters, R, nreq, true);
     if (M == 0 || !z.on) {
         if (da) cudaMemsetAsync(da, 0, e * n_adapters * R * D, st);
         if (db) cudaMemsetAsync(db, 0, e * n_adapters * R * O, st);
@@ -753,6 +894,17 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
     p.low[0] = f.sp.T, p.low[1] = kept ? kept : f.sp.S;
     p.rows[0] = x, p.rows[1] = dy;
     p.ld[0] = ldx, p.ld[1] = lddy;
+    if (!z.split) {                  // the copies that the products read, where they made one
+        if (!tma_ready(dy, lddy)) p.rows[1] = f.sp.rows, p.ld[1] = z.Op;
+        if (da && !tma_ready(x, ldx)) {
+            if (kept || !db) {
+                PrepList l;
+                l.add({x, M, D, ldx, f.sp.x, z.Dp, 0, nullptr, nullptr, kPack});
+                if (int s = prepare(l, st)) return s;
+            }
+            p.rows[0] = f.sp.x, p.ld[0] = z.Dp;
+        }
+    }
     p.width[0] = da ? D : 0, p.width[1] = db ? O : 0;
     p.tiles0 = ceil_div(p.width[0], 128);
     p.out[0] = da, p.out[1] = db;
@@ -760,9 +912,15 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
     p.split = z.grad_split();
     p.dtype = dtype;
     const int tiles = p.tiles0 + ceil_div(p.width[1], 128);
-    const long long ny = (long long)n_adapters * ((R + 31) / 32);
-    grads_kernel<<<dim3(tiles, (unsigned)ny, p.split), 256, 0, st>>>(p);
-    ATOM_CHECK_LAUNCH("adapters: gradients");
+    const dim3 grid(tiles, (unsigned)n_adapters * (z.split ? (R + 31) / 32 : 1), p.split);
+    int rc;
+    if (dtype == ATOM_BF16) rc = grads16<true>(p, grid, st);
+    else if (dtype == ATOM_F16) rc = grads16<false>(p, grid, st);
+    else {
+        grads32_kernel<<<grid, 256, 0, st>>>(p);
+        rc = check_launch("adapters: gradients");
+    }
+    if (rc) return rc;
     if (p.split > 1) {
         grads_sum_kernel<<<592, 256, 0, st>>>(p);
         ATOM_CHECK_LAUNCH("adapters: gradient sums");

@@ -33,16 +33,21 @@ struct FfSizes {
     int D, F, O;
     long long Dp, Fp, Op;       // widths of packed rows
     bool split;
-    FfSizes(int t, long long m, int d, int f, int o)
+    Choice gate{}, down{}, dh{}, dx{}, dwgu{}, dwd{};
+    FfSizes(int t, long long m, int d, int f, int o, bool bwd)
         : dtype(t), M(m), D(d), F(f), O(o), Dp(up(d, 8)), Fp(up(f, 32)), Op(up(o, 8)),
-          split(t == ATOM_F32) {}
+          split(t == ATOM_F32) {
+        gate = choose(M, F, nk(D), 1, true, split, false);
+        if (!bwd) {
+            down = choose(M, O, nk(F), 1, false, split, true);
+        } else {
+            dh = choose(M, F, nk(O), 1, false, split, false);
+            dx = choose(M, D, 2 * nk(F), 1, false, split, false);
+            dwgu = choose(F, D, nk(M), 2, false, split, true);
+            dwd = choose(O, F, nk(M), 1, false, split, true);
+        }
+    }
     int nk(long long k) const { return (int)((k + 63) / 64); }
-    Choice gate() const { return choose(M, F, nk(D), 1, true, split, false); }
-    Choice down() const { return choose(M, O, nk(F), 1, false, split, true); }
-    Choice dh() const { return choose(M, F, nk(O), 1, false, split, false); }
-    Choice dx() const { return choose(M, D, 2 * nk(F), 1, false, split, false); }
-    Choice dwgu() const { return choose(F, D, nk(M), 2, false, split, true); }
-    Choice dwd() const { return choose(O, F, nk(M), 1, false, split, true); }
 };
 
 // One call's buffers. 16-bit operands are packed only where TMA cannot read them; fp32 ones
@@ -61,9 +66,9 @@ struct FfSpace {
         wg = c.take<__half>(k * z.F * z.Dp);
         wu = c.take<__half>(k * z.F * z.Dp);
         wd = c.take<__half>(k * z.O * z.Fp);
-        size_t pf = z.down().part;
+        size_t pf = z.down.part;
         if (bwd) {
-            pf = z.dwgu().part > z.dwd().part ? z.dwgu().part : z.dwd().part;
+            pf = z.dwgu.part > z.dwd.part ? z.dwgu.part : z.dwd.part;
             dy = c.take<__half>(k * M * z.Op);
             dh = c.take<float>(up(M, 32) * z.Fp);
         }
@@ -174,7 +179,7 @@ struct Ff {
     }
     // [G | U] tiles of X
     int gates(int epilogue, Args& p, void* C, long long width, void* H) {
-        const Choice c = z.gate();
+        const Choice c = z.gate;
         const int k = step();
         Maps maps;
         if (int s = put(maps, 0, x, false, 128, z.split)) return s;
@@ -197,7 +202,7 @@ struct Ff {
             if (int s = prepare(list, st)) return s;
             h = {sp.hp, z.M, z.F, z.Fp, z.M * z.Fp};
         }
-        const Choice c = z.down();
+        const Choice c = z.down;
         const int k = step();
         Maps maps;
         if (int s = put(maps, 0, h, false, 128, z.split)) return s;
@@ -214,7 +219,7 @@ struct Ff {
         void* dgu = z.split ? (void*)sp.dgu32 : sp.dgu;
         void* H = !dwd ? nullptr : z.split ? (void*)sp.H32 : sp.H;
         {   // dH, and dG, dU, H either in its epilogue or in that of G and U
-            const Choice c = z.dh();
+            const Choice c = z.dh;
             Maps maps;
             if (int s = put(maps, 0, dy, false, 128, z.split)) return s;
             if (int s = put(maps, k, wd, true, 64, z.split)) return s;
@@ -261,7 +266,7 @@ struct Ff {
             if (int s = prepare(list, st)) return s;
         }
         if (dx) {
-            const Choice c = z.dx();
+            const Choice c = z.dx;
             Maps maps;
             if (int s = put(maps, 0, g.columns(0, z.F), false, 128, z.split)) return s;
             if (int s = put(maps, k, g.columns(z.Fp, z.F), false, 128, z.split)) return s;
@@ -277,7 +282,7 @@ struct Ff {
             if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
         }
         if (dwg || dwu) {
-            Choice c = z.dwgu();
+            Choice c = z.dwgu;
             const bool two = dwg && dwu;
             Maps maps;
             if (int s = put(maps, 0, gt.columns(dwg ? 0 : z.Fp, z.F), true, 64, z.split)) return s;
@@ -294,7 +299,7 @@ struct Ff {
             if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
         }
         if (dwd) {
-            const Choice c = z.dwd();
+            const Choice c = z.dwd;
             Maps maps;
             if (int s = put(maps, 0, dyt, true, 64, z.split)) return s;
             if (int s = put(maps, k, h, true, 64, z.split)) return s;
@@ -327,9 +332,9 @@ using namespace atom;
 extern "C" int atom_gated_ff_bytes(int dtype, int64_t M, int D, int F, int O, size_t* bytes_host) {
     if (int s = check_ff(dtype, M, D, F, O, 0)) return s;
     ATOM_REQUIRE(bytes_host, "gated_ff: bytes_host is NULL");
-    const FfSizes z(dtype, M, D, F, O);
+    const FfSizes z(dtype, M, D, F, O, false);
     bytes_host[0] = FfSpace(nullptr, z, false).bytes;
-    bytes_host[1] = FfSpace(nullptr, z, true).bytes;
+    bytes_host[1] = FfSpace(nullptr, FfSizes(dtype, M, D, F, O, true), true).bytes;
     bytes_host[2] = (size_t)up(M, 32) * 2 * z.Fp * sizeof(float);
     return ATOM_OK;
 }
@@ -341,7 +346,7 @@ extern "C" int atom_gated_ff_fwd(int dtype, const void* x, int64_t ldx, int64_t 
     if (int s = check_ff(dtype, M, D, F, O, act)) return s;
     if (M == 0) return ATOM_OK;
     ATOM_REQUIRE(x && wg && wu && wd && y && ldx >= D && ldy >= O, "gated_ff: bad operand");
-    const FfSizes z(dtype, M, D, F, O);
+    const FfSizes z(dtype, M, D, F, O, false);
     Ff f{z, FfSpace(ws, z, false), (cudaStream_t)stream, act};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
                  f.sp.bytes);
@@ -365,7 +370,7 @@ extern "C" int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t 
     }
     ATOM_REQUIRE(x && wg && wu && wd && dy && ldx >= D && lddy >= O && (!dx || lddx >= D),
                  "gated_ff: bad operand");
-    const FfSizes z(dtype, M, D, F, O);
+    const FfSizes z(dtype, M, D, F, O, true);
     Ff f{z, FfSpace(ws, z, true), st, act};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
                  f.sp.bytes);

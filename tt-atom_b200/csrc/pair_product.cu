@@ -996,9 +996,14 @@ int make_out_map(CUtensorMap* m, const void* p, int dtype, long long cols, long 
 }
 
 static int sm_count() {
-    int dev = 0, n = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    static std::atomic<int> count[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    int n = count[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n = 148;
+        count[dev].store(n, std::memory_order_relaxed);
+    }
     return n;
 }
 
@@ -1033,10 +1038,10 @@ Choice choose(long long M, int N, int nk, int groups, bool gated, bool split, bo
 template <int BN, int EPI, bool SPLIT>
 static int run(const Maps& maps, const Args& p, cudaStream_t st) {
     using CF = Cfg<BN, SPLIT>;
-    static bool set[64] = {};
+    static std::atomic<bool> set[64];
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !set[dev]) {
+    if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_relaxed)) {
         const cudaError_t e = cudaFuncSetAttribute(
             pair_kernel<BN, EPI, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
             (int)CF::kSmem);
@@ -1045,7 +1050,7 @@ static int run(const Maps& maps, const Args& p, cudaStream_t st) {
                       cudaGetErrorString(e));
             return ATOM_ERR_CUDA;
         }
-        if (dev >= 0 && dev < 64) set[dev] = true;
+        if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
     }
     const long long pairs = sm_count() / 2;
     const int grid = 2 * (int)(p.tiles < pairs ? p.tiles : pairs);

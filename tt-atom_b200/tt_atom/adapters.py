@@ -9,41 +9,40 @@ kernels are behind ``atom_adapted_linear_fwd`` / ``atom_adapted_linear_bwd``.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib as L
-from .feedforward import buffer, check_like, check_rows, dtype_code, row_stride
+from .feedforward import buffer, check_kept, check_like, on_device, row_stride, rows_code
 
 
-def _int32(name, t, x, n=None):
-    if t.dtype != torch.int32 or t.device != x.device or t.dim() != 1 or not t.is_contiguous():
-        raise ValueError(f"{name} must be a dense int32 vector on {x.device}")
-    if n is not None and t.numel() != n:
-        raise ValueError(f"{name} has {t.numel()} entries: expected {n}")
+def _vector(name, t, dtype, n, x):
+    if t.dtype != dtype or t.device != x.device or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a dense {dtype} vector of {n} on {x.device}")
 
 
 def _shapes(x, w, a, b, scale, req_ptr, req_adapter):
-    check_rows("x", x)
-    code = dtype_code("x", x)
-    if w.dim() != 2 or a.dim() != 3:
-        raise ValueError("w must be [O, D], a [n, R, D] and b [n, O, R]")
-    (M, D), O, (n, R) = x.shape, w.shape[0], a.shape[:2]  # noqa: E741
+    code = rows_code(x)
+    if w.dim() != 2 or a.dim() != 3 or req_adapter.dim() != 1:
+        raise ValueError("w must be [O, D], a [n, R, D], b [n, O, R] and req_adapter a vector")
+    (M, D), O, (n, R, _) = x.shape, w.shape[0], a.shape  # noqa: E741
+    nreq = req_adapter.shape[0]
     check_like("w", w, (O, D), x)
     check_like("a", a, (n, R, D), x)
     check_like("b", b, (n, O, R), x)
-    if scale.dtype != torch.float32 or scale.device != x.device or tuple(scale.shape) != (n,) \
-            or not scale.is_contiguous():
-        raise ValueError(f"scale must be a dense float32 vector of {n} on {x.device}")
-    _int32("req_adapter", req_adapter, x)
-    _int32("req_ptr", req_ptr, x, req_adapter.numel() + 1)
-    return code, M, D, O, n, R, req_adapter.numel()
+    _vector("scale", scale, torch.float32, n, x)
+    _vector("req_adapter", req_adapter, torch.int32, nreq, x)
+    _vector("req_ptr", req_ptr, torch.int32, nreq + 1, x)
+    return code, M, D, O, n, R, nreq
 
 
-def _bytes(code, M, D, O, n, R, nreq):  # noqa: E741
+@functools.lru_cache(maxsize=1024)
+def _bytes(device, *sizes):
+    """Workspace and kept sizes, by sizes and the GPU they are for."""
     out = (ctypes.c_size_t * 3)()
-    L.call("atom_adapted_linear_bytes", code, M, D, O, n, R, nreq, out)
-    return out
+    L.call("atom_adapted_linear_bytes", *sizes, out)
+    return tuple(out)
 
 
 def adapted_linear(x, w, a, b, scale, req_ptr, req_adapter, keep=False):
@@ -54,15 +53,18 @@ def adapted_linear(x, w, a, b, scale, req_ptr, req_adapter, keep=False):
     req_adapter [nreq] int32, all on x's device: a replayed graph sees what they hold then.
     Requests may be empty and may share an adapter. Sums in float32. With ``keep`` returns
     (y, kept): what ``adapted_linear_bwd`` needs to spare the product x a^T."""
-    code, M, D, O, n, R, nreq = _shapes(x, w, a, b, scale, req_ptr, req_adapter)  # noqa: E741
-    with torch.cuda.device(x.device):
-        nb = _bytes(code, M, D, O, n, R, nreq)
+    sizes = code, M, D, O, n, R, nreq = _shapes(x, w, a, b, scale, req_ptr,  # noqa: E741
+                                                req_adapter)
+    ldx = row_stride("x", x)
+    here, stream = on_device(x)
+    with here:
+        nb = _bytes(x.device.index, *sizes)
         y = torch.empty(M, O, dtype=x.dtype, device=x.device)
-        ws, kept = buffer(nb[0], x), buffer(nb[2], x) if keep else None
-        L.call("atom_adapted_linear_fwd", code, x.data_ptr(), row_stride(x), M, D, O,
-               w.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), n, R,
-               req_ptr.data_ptr(), req_adapter.data_ptr(), nreq, y.data_ptr(), O, L.ptr(kept),
-               L.ptr(ws), nb[0], L.stream_ptr())
+        ws, at = buffer(nb[0], x)
+        kept, kept_at = buffer(nb[2], x) if keep else (None, None)
+        L.call("atom_adapted_linear_fwd", code, x.data_ptr(), ldx, M, D, O, w.data_ptr(),
+               a.data_ptr(), b.data_ptr(), scale.data_ptr(), n, R, req_ptr.data_ptr(),
+               req_adapter.data_ptr(), nreq, y.data_ptr(), O, kept_at, at, nb[0], stream)
     return (y, kept) if keep else y
 
 
@@ -72,21 +74,21 @@ def adapted_linear_bwd(x, w, a, b, scale, req_ptr, req_adapter, dy, kept=None,
     no gradient here (it is what the adapters leave fixed). An adapter of no request has zeros.
     Without ``adapter_grads`` the last two are None. ``kept``: what
     ``adapted_linear(..., keep=True)`` returned for the same inputs."""
-    code, M, D, O, n, R, nreq = _shapes(x, w, a, b, scale, req_ptr, req_adapter)  # noqa: E741
-    check_rows("dy", dy, x, (M, O))
-    with torch.cuda.device(x.device):
-        nb = _bytes(code, M, D, O, n, R, nreq)
-        if kept is not None and (kept.dtype != torch.uint8 or kept.numel() != nb[2]
-                                 or kept.device != x.device):
-            raise ValueError("kept is not what adapted_linear(..., keep=True) returns for these "
-                             "inputs")
+    sizes = code, M, D, O, n, R, nreq = _shapes(x, w, a, b, scale, req_ptr,  # noqa: E741
+                                                req_adapter)
+    check_like("dy", dy, (M, O), x, dense=False)
+    ldx, lddy = row_stride("x", x), row_stride("dy", dy)
+    here, stream = on_device(x)
+    with here:
+        nb = _bytes(x.device.index, *sizes)
+        if kept is not None:
+            check_kept(kept, nb[2], x, "adapted_linear")
         dx = torch.empty(M, D, dtype=x.dtype, device=x.device)
         da = torch.empty_like(a) if adapter_grads else None
         db = torch.empty_like(b) if adapter_grads else None
-        ws = buffer(nb[1], x)
-        L.call("atom_adapted_linear_bwd", code, x.data_ptr(), row_stride(x), M, D, O,
-               w.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), n, R,
-               req_ptr.data_ptr(), req_adapter.data_ptr(), nreq, dy.data_ptr(), row_stride(dy),
-               L.ptr(kept), dx.data_ptr(), D, L.ptr(da), L.ptr(db), L.ptr(ws), nb[1],
-               L.stream_ptr())
+        ws, at = buffer(nb[1], x)
+        L.call("atom_adapted_linear_bwd", code, x.data_ptr(), ldx, M, D, O, w.data_ptr(),
+               a.data_ptr(), b.data_ptr(), scale.data_ptr(), n, R, req_ptr.data_ptr(),
+               req_adapter.data_ptr(), nreq, dy.data_ptr(), lddy, L.ptr(kept), dx.data_ptr(), D,
+               L.ptr(da), L.ptr(db), at, nb[1], stream)
     return dx, da, db

@@ -8,7 +8,9 @@ reference, whose feed-forwards are ungated MLPs (tt_atom/grid.py) or the spectra
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -16,52 +18,64 @@ from . import _lib as L
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTS = {"silu": 0, "sigmoid": 1, "gelu": 2}
+_SAME = contextlib.nullcontext()
 
 
-def dtype_code(name, t):
-    """The C ABI's type code of a tensor; ValueError for a type it does not have."""
-    code = DTYPES.get(t.dtype)
+def rows_code(x):
+    """Checks the matrix x of rows and returns the C ABI's code of its type."""
+    if x.dim() != 2:
+        raise ValueError(f"x must be a matrix [rows, width], got {x.dim()} dimensions")
+    if not x.is_cuda:
+        raise ValueError("x must be on a CUDA device")
+    code = DTYPES.get(x.dtype)
     if code is None:
-        raise ValueError(f"{name} is {t.dtype}: expected float32, bfloat16 or float16")
+        raise ValueError(f"x is {x.dtype}: expected float32, bfloat16 or float16")
     return code
 
 
-def check_like(name, t, shape, x):
-    """A dense operand of ``shape`` with x's type, on x's device."""
+def row_stride(name, t):
+    """The stride of a matrix's rows, which have to be dense."""
+    rows, width = t.shape
+    if rows <= 1:
+        if width > 1 and t.stride(1) != 1:
+            raise ValueError(f"{name} must have dense rows (strides {t.stride()})")
+        return width
+    s0, s1 = t.stride()
+    if width > 1 and s1 != 1 or s0 < width:
+        raise ValueError(f"{name} must have dense rows (strides {t.stride()})")
+    return s0
+
+
+def check_like(name, t, shape, x, dense=True):
+    """An operand of ``shape`` with x's type, on x's device."""
     if t.dtype != x.dtype or t.device != x.device:
         raise ValueError(f"{name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}: expected {tuple(shape)}")
-    if not t.is_contiguous():
+    if dense and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
 
 
-def check_rows(name, t, x=None, shape=None):
-    """A matrix whose rows are dense (any row stride of at least their width)."""
-    if t.dim() != 2:
-        raise ValueError(f"{name} must be a matrix [rows, width], got {t.dim()} dimensions")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be on a CUDA device")
-    if x is not None and (t.dtype != x.dtype or t.device != x.device):
-        raise ValueError(f"{name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}: expected {tuple(shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"{name} must have dense rows (strides {t.stride()})")
-
-
-def row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def on_device(x):
+    """Context with x's device current, and x's current stream there."""
+    i = x.device.index
+    return (_SAME if i == torch.cuda.current_device() else torch.cuda.device(i),
+            torch._C._cuda_getCurrentRawStream(i))
 
 
 def buffer(nbytes, x):
-    """A scratch tensor on x's device, from the current stream's pool (None for 0 bytes)."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    """Scratch on x's device from the current stream's pool, and its address."""
+    t = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    return t, t.data_ptr()
+
+
+def check_kept(kept, nbytes, x, maker):
+    if kept.dtype != torch.uint8 or kept.numel() != nbytes or kept.device != x.device:
+        raise ValueError(f"kept is not what {maker}(..., keep=True) returns for these inputs")
 
 
 def _shapes(x, wg, wu, wd, act):
-    check_rows("x", x)
-    code = dtype_code("x", x)
+    code = rows_code(x)
     if act not in ACTS:
         raise ValueError(f"unknown activation {act!r}: expected one of {', '.join(ACTS)}")
     if wg.dim() != 2 or wd.dim() != 2:
@@ -73,10 +87,12 @@ def _shapes(x, wg, wu, wd, act):
     return code, M, D, F, O
 
 
-def _bytes(code, M, D, F, O):  # noqa: E741
+@functools.lru_cache(maxsize=1024)
+def _bytes(device, *sizes):
+    """Workspace and kept sizes, by sizes and the GPU they are for."""
     out = (ctypes.c_size_t * 3)()
-    L.call("atom_gated_ff_bytes", code, M, D, F, O, out)
-    return out
+    L.call("atom_gated_ff_bytes", *sizes, out)
+    return tuple(out)
 
 
 def gated_ff(x, wg, wu, wd, act="silu", keep=False):
@@ -87,13 +103,15 @@ def gated_ff(x, wg, wu, wd, act="silu", keep=False):
     (y, kept): what ``gated_ff_bwd`` needs to spare the first two products. Runs on the current
     stream of x's device, without synchronising."""
     code, M, D, F, O = _shapes(x, wg, wu, wd, act)  # noqa: E741
-    with torch.cuda.device(x.device):
-        n = _bytes(code, M, D, F, O)
+    ldx = row_stride("x", x)
+    here, stream = on_device(x)
+    with here:
+        n = _bytes(x.device.index, code, M, D, F, O)
         y = torch.empty(M, O, dtype=x.dtype, device=x.device)
-        ws, kept = buffer(n[0], x), buffer(n[2], x) if keep else None
-        L.call("atom_gated_ff_fwd", code, x.data_ptr(), row_stride(x), M, D, F, O, wg.data_ptr(),
-               wu.data_ptr(), wd.data_ptr(), ACTS[act], y.data_ptr(), O, L.ptr(kept), L.ptr(ws),
-               n[0], L.stream_ptr())
+        ws, at = buffer(n[0], x)
+        kept, kept_at = buffer(n[2], x) if keep else (None, None)
+        L.call("atom_gated_ff_fwd", code, x.data_ptr(), ldx, M, D, F, O, wg.data_ptr(),
+               wu.data_ptr(), wd.data_ptr(), ACTS[act], y.data_ptr(), O, kept_at, at, n[0], stream)
     return (y, kept) if keep else y
 
 
@@ -103,16 +121,17 @@ def gated_ff_bwd(x, wg, wu, wd, dy, act="silu", kept=None, weight_grads=True):
     ``kept`` is what ``gated_ff(..., keep=True)`` returned for the same inputs; without it the
     first two products are computed again."""
     code, M, D, F, O = _shapes(x, wg, wu, wd, act)  # noqa: E741
-    check_rows("dy", dy, x, (M, O))
-    with torch.cuda.device(x.device):
-        n = _bytes(code, M, D, F, O)
-        if kept is not None and (kept.dtype != torch.uint8 or kept.numel() != n[2]
-                                 or kept.device != x.device):
-            raise ValueError("kept is not what gated_ff(..., keep=True) returns for these inputs")
+    check_like("dy", dy, (M, O), x, dense=False)
+    ldx, lddy = row_stride("x", x), row_stride("dy", dy)
+    here, stream = on_device(x)
+    with here:
+        n = _bytes(x.device.index, code, M, D, F, O)
+        if kept is not None:
+            check_kept(kept, n[2], x, "gated_ff")
         dx = torch.empty(M, D, dtype=x.dtype, device=x.device)
         dw = [torch.empty_like(w) for w in (wg, wu, wd)] if weight_grads else [None] * 3
-        ws = buffer(n[1], x)
-        L.call("atom_gated_ff_bwd", code, x.data_ptr(), row_stride(x), M, D, F, O, wg.data_ptr(),
-               wu.data_ptr(), wd.data_ptr(), ACTS[act], dy.data_ptr(), row_stride(dy),
-               L.ptr(kept), dx.data_ptr(), D, *map(L.ptr, dw), L.ptr(ws), n[1], L.stream_ptr())
+        ws, at = buffer(n[1], x)
+        L.call("atom_gated_ff_bwd", code, x.data_ptr(), ldx, M, D, F, O, wg.data_ptr(),
+               wu.data_ptr(), wd.data_ptr(), ACTS[act], dy.data_ptr(), lddy, L.ptr(kept),
+               dx.data_ptr(), D, *map(L.ptr, dw), at, n[1], stream)
     return (dx, *dw)
