@@ -14,6 +14,7 @@
 // is not is found in the shrink pass, left out, and its own rows are set to NaN.
 #include <algorithm>
 
+#include "few_rows.cuh"
 #include "pair_product.cuh"
 
 namespace atom {
@@ -30,25 +31,6 @@ struct Requests {
 // Rows of request r, kept within 0 .. M whatever the table holds.
 __device__ __forceinline__ int row_of(const Requests& q, int r) {
     return min(max(q.ptr[r], 0), q.M);
-}
-
-// The last r in 0 .. n - 1 with value(r) <= key, or -1; value ascending, one warp.
-template <typename V>
-__device__ __forceinline__ int last_le(int n, int key, V value) {
-    const int lane = threadIdx.x & 31;
-    int lo = 0;
-    while (n > 0) {
-        const int step = (n + 31) / 32, i = lo + lane * step;
-        const unsigned yes = __ballot_sync(0xffffffffu, lane * step < n && value(i) <= key);
-        const int count = __popc(yes);
-        if (count == 0) return lo - 1;
-        if (step == 1) return lo + count - 1;
-        lo += (count - 1) * step;
-        n = min(step, n - (count - 1) * step);
-        // value(lo) <= key holds: look behind it
-        if (n == 1) return lo;
-    }
-    return lo - 1;
 }
 
 struct Shrink {
@@ -252,18 +234,7 @@ __global__ void __launch_bounds__(256, NT <= 4 ? 3 : 1)
 }
 
 // fp32: a warp has 8 rows by 8 ranks, its lanes split K, and the 64 sums are added over the lanes
-// by halves (lane l ends with sums 2 l and 2 l + 1); then each row's planes.
-__device__ __forceinline__ void sum_halves(float* v, int lane) {
-#pragma unroll
-    for (int o = 16, n = 32; o > 0; o >>= 1, n >>= 1) {
-        const bool up = lane & o;
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-            const float mine = up ? v[n + i] : v[i], other = up ? v[i] : v[n + i];
-            v[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
-        }
-    }
-}
+// by halves; then each row's planes.
 __global__ void __launch_bounds__(256) shrink32_kernel(const __grid_constant__ Shrink p) {
     extern __shared__ float out[];       // [32][R + 1]
     if (side_work(p)) return;
@@ -591,6 +562,8 @@ struct AdSpace {
     void *S, *T;
     int4 *piece, *bad;
     int2* tile_req;
+    float* few_S;
+    int* few_slot;
     unsigned* max;           // rows, w, adapters
     size_t bytes;
     AdSpace(void* ws, const AdSizes& z, bool bwd) {
@@ -605,6 +578,10 @@ struct AdSpace {
             rinv = c.take<float>(z.M);
         }
         if (z.on) {
+            if (!bwd && z.M <= few::kFewRows) {
+                few_S = c.take<float>(z.M * z.R);
+                few_slot = c.take<int>(z.M);
+            }
             piece = c.take<int4>(z.pieces);
             bad = c.take<int4>(z.nad);
             tile_req = c.take<int2>(z.tiles);
@@ -848,6 +825,16 @@ extern "C" int atom_adapted_linear_fwd(int dtype, const void* x, int64_t ldx, in
          {req_ptr, req_adapter, nreq, n_adapters, (int)M}, scale, w, a, b};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "adapted_linear: the workspace needs %zu bytes",
                  f.sp.bytes);
+    if (few::suits(dtype, M, D, x, ldx, w, a)) {
+        // a few rows: the low-rank values first, then the projection with them in its epilogue;
+        // nothing is kept, the backward pass computes S again
+        if (z.on)
+            if (int s = few::low_rank({x, ldx, (int)M, D, a, R, scale, req_ptr, req_adapter, nreq,
+                                       n_adapters, f.sp.few_S, f.sp.few_slot, dtype}, f.st))
+                return s;
+        return few::product({x, ldx, (int)M, D, {w, nullptr}, O, 0, y, ldy, dtype,
+                             z.on ? f.sp.few_S : nullptr, f.sp.few_slot, b, R, z.on}, f.st);
+    }
     return f.run(x, ldx, false, y, ldy, kept, false);
 }
 
@@ -877,6 +864,7 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "adapted_linear: the workspace needs %zu bytes",
                  f.sp.bytes);
     const bool grads = z.on && (da || db);
+    if (few::suits(dtype, M, D, x, ldx, w, a)) kept = nullptr;
     if (grads && db && !kept) {      // S again
         AdSpace fs = f.sp;
         fs.rows = f.sp.x;            // x's copy, where it needs one

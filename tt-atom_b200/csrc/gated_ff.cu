@@ -8,6 +8,7 @@
 // transposed in memory.
 #include <initializer_list>
 
+#include "few_rows.cuh"
 #include "pair_product.cuh"
 
 namespace atom {
@@ -316,6 +317,14 @@ struct Ff {
     long long x_ld = 0, dy_ld = 0;
 };
 
+// Whether the forward pass runs as two products of a few rows. It keeps nothing then: the backward
+// pass, which sees the same operands, computes G and U again.
+bool few_rows(const FfSizes& z, const void* x, long long ldx, const void* wg, const void* wu,
+              const void* wd) {
+    return few::suits(z.dtype, z.M, z.D, x, ldx, wg, wu) &&
+           few::suits(z.dtype, z.M, z.F, nullptr, z.Fp, wd, nullptr);
+}
+
 int check_ff(int dtype, int64_t M, int D, int F, int O, int act) {
     ATOM_REQUIRE(dtype >= ATOM_F32 && dtype <= ATOM_F16, "gated_ff: unknown type %d", dtype);
     ATOM_REQUIRE(M >= 0 && M < (1LL << 31) && D > 0 && F > 0 && O > 0, "gated_ff: bad sizes");
@@ -350,6 +359,14 @@ extern "C" int atom_gated_ff_fwd(int dtype, const void* x, int64_t ldx, int64_t 
     Ff f{z, FfSpace(ws, z, false), (cudaStream_t)stream, act};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
                  f.sp.bytes);
+    void* h = z.split ? (void*)f.sp.H32 : f.sp.H;
+    if (few_rows(z, x, ldx, wg, wu, wd)) {
+        if (int s = few::product({x, ldx, (int)M, D, {wg, wu}, F, act, h, z.Fp, dtype, nullptr,
+                                  nullptr, nullptr, 0, 0}, f.st))
+            return s;
+        return few::product({h, z.Fp, (int)M, F, {wd, nullptr}, O, 0, y, ldy, dtype, nullptr,
+                             nullptr, nullptr, 0, 1}, f.st);
+    }
     if (int s = f.inputs(x, ldx, wg, wu, wd, nullptr, 0)) return s;
     return f.forward(y, ldy, static_cast<float*>(kept));
 }
@@ -376,5 +393,6 @@ extern "C" int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t 
                  f.sp.bytes);
     f.x_src = x, f.x_ld = ldx, f.dy_src = dy, f.dy_ld = lddy;
     if (int s = f.inputs(x, ldx, wg, wu, wd, dy, lddy)) return s;
+    if (few_rows(z, x, ldx, wg, wu, wd)) kept = nullptr;
     return f.backward(static_cast<const float*>(kept), dx, lddx, dwg, dwu, dwd);
 }

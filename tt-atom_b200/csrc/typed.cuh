@@ -46,6 +46,43 @@ __device__ __forceinline__ void split_half2(float y0, float y1, __half2& hi, __h
     lo = __floats2half2_rn((y0 - back.x) * 2048.f, (y1 - back.y) * 2048.f);
 }
 
+// The last r in 0 .. n - 1 with value(r) <= key, or -1; value ascending, one warp.
+template <typename V>
+__device__ __forceinline__ int last_le(int n, int key, V value) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0;
+    while (n > 0) {
+        const int step = (n + 31) / 32, i = lo + lane * step;
+        const unsigned yes = __ballot_sync(0xffffffffu, lane * step < n && value(i) <= key);
+        const int count = __popc(yes);
+        if (count == 0) return lo - 1;
+        if (step == 1) return lo + count - 1;
+        lo += (count - 1) * step;
+        n = min(step, n - (count - 1) * step);
+        // value(lo) <= key holds: look behind it
+        if (n == 1) return lo;
+    }
+    return lo - 1;
+}
+
+// Adds 64 values over a warp: lane l ends with sums 2 l and 2 l + 1 in v[0], v[1].
+__device__ __forceinline__ void sum_halves(float* v, int lane) {
+#pragma unroll
+    for (int o = 16, n = 32; o > 0; o >>= 1, n >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float mine = up ? v[n + i] : v[i], other = up ? v[i] : v[n + i];
+            v[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+        }
+    }
+}
+// Two 16-bit values of a word.
+__device__ __forceinline__ float2 pair_f(uint32_t w, int dtype) {
+    return dtype == ATOM_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w))
+                              : __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
 // Pieces of a caller's workspace, 256-byte aligned; with base NULL it only adds up the sizes.
 struct Cursor {
     char* base;
