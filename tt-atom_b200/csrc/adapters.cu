@@ -159,6 +159,8 @@ template <bool BF16, int NT>
 __global__ void __launch_bounds__(256, NT <= 4 ? 3 : 1)
     shrink16_kernel(const __grid_constant__ Shrink p) {
     extern __shared__ float red[];       // [8 warps][16][8 NT]
+    let_next_start();
+    wait_before();
     if (side_work(p)) return;
     const Piece c = find_piece(p);
     if (c.slot < 0) return;
@@ -237,6 +239,8 @@ __global__ void __launch_bounds__(256, NT <= 4 ? 3 : 1)
 // by halves; then each row's planes.
 __global__ void __launch_bounds__(256) shrink32_kernel(const __grid_constant__ Shrink p) {
     extern __shared__ float out[];       // [32][R + 1]
+    let_next_start();
+    wait_before();
     if (side_work(p)) return;
     const Piece c = find_piece(p);
     if (c.slot < 0) return;
@@ -304,6 +308,8 @@ __global__ void __launch_bounds__(256) shrink32_kernel(const __grid_constant__ S
 // dst[a][r][o] = src[a][o][r], 16-bit, dst's rows `pitch` apart and zero-filled.
 __global__ void __launch_bounds__(256) transpose_kernel(const unsigned short* src, int O, int R,
                                                         int pitch, unsigned short* dst) {
+    let_next_start();
+    wait_before();
     __shared__ unsigned short tile[32][33];
     const long long a = blockIdx.z;
     const int o0 = blockIdx.x * 32, r0 = blockIdx.y * 32;
@@ -383,6 +389,8 @@ template <bool BF16, int MT>
 __global__ void __launch_bounds__(256) grads16_kernel(const __grid_constant__ Grads p) {
     constexpr int kX = 32 * 272, kT = 32 * (32 * MT + 16), kStages = 4;
     extern __shared__ __align__(16) uint8_t smem[];
+    let_next_start();
+    wait_before();
     const int which = blockIdx.x >= p.tiles0;
     const int c0 = (blockIdx.x - (which ? p.tiles0 : 0)) * 128, W = p.width[which];
     const unsigned short* rows = static_cast<const unsigned short*>(p.rows[which]);
@@ -458,6 +466,8 @@ __global__ void __launch_bounds__(256) grads16_kernel(const __grid_constant__ Gr
 // fp32: 32 ranks by 128 columns a block, 4 x 4 a thread, 32 rows at a time.
 __global__ void __launch_bounds__(256) grads32_kernel(const __grid_constant__ Grads p) {
     __shared__ __align__(16) float ts[32][36], xs[32][132];
+    let_next_start();
+    wait_before();
     const int which = blockIdx.x >= p.tiles0;
     const int c0 = (blockIdx.x - (which ? p.tiles0 : 0)) * 128, W = p.width[which];
     const int chunks = (p.R + 31) / 32;
@@ -503,6 +513,8 @@ __global__ void __launch_bounds__(256) grads32_kernel(const __grid_constant__ Gr
             put_grad(p, which, a, r0 + ty * 4 + i, c0 + lane * 4 + j, acc[i][j]);
 }
 __global__ void __launch_bounds__(256) grads_sum_kernel(const __grid_constant__ Grads p) {
+    let_next_start();
+    wait_before();
     const int W = p.width[0] + p.width[1];
     const long long per = (long long)p.R * W, all = per * p.nad;
     for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
@@ -517,15 +529,14 @@ __global__ void __launch_bounds__(256) grads_sum_kernel(const __grid_constant__ 
     }
 }
 template <bool BF16>
-int grads16(const Grads& p, dim3 grid, cudaStream_t st) {
+int grads16(const Grads& p, dim3 grid, Chain& st) {
 #define ATOM_GRADS(N)                                                                             \
     if (p.R <= 16 * N) {                                                                          \
         constexpr int smem = 4 * (32 * 272 + 32 * (32 * N + 16));                                 \
         if (smem > 48 * 1024)                                                                     \
             cudaFuncSetAttribute(grads16_kernel<BF16, N>,                                         \
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem);              \
-        grads16_kernel<BF16, N><<<grid, 256, smem, st>>>(p);                                      \
-        return check_launch("adapters: gradients");                                               \
+        return st.launch("adapters: gradients", grads16_kernel<BF16, N>, grid, 256, smem, p);     \
     }
     ATOM_GRADS(1)
     ATOM_GRADS(2)
@@ -558,7 +569,7 @@ struct AdSizes {
 
 struct AdSpace {
     __half *rows, *x, *w, *ad, *ext, *block, *bt;
-    float *rinv, *ext_rinv, *part, *gpart;
+    float *rinv, *wr, *ext_rinv, *part, *gpart;
     void *S, *T;
     int4 *piece, *bad;
     int2* tile_req;
@@ -574,8 +585,10 @@ struct AdSpace {
         w = c.take<__half>(k * z.O * z.Dp);
         part = c.take<float>(z.product.part);
         if (z.split) {
+            rinv = c.take<float>(up(z.M, 32));
+            if (!bwd) wr = c.take<float>(up(z.O, 32));
             max = c.take<unsigned>(4);
-            rinv = c.take<float>(z.M);
+            ext_rinv = c.take<float>(z.on ? z.M : 0);
         }
         if (z.on) {
             if (!bwd && z.M <= few::kFewRows) {
@@ -589,7 +602,6 @@ struct AdSpace {
             if (!z.split) ad = c.take<__half>((long long)z.nad * z.R * (bwd ? z.Op : z.Dp));
             ext = c.take<__half>(k * z.nad * (bwd ? z.R * z.Dp : (long long)z.O * z.Rs));
             block = c.take<__half>(k * z.pieces * 256 * z.Rs);
-            if (z.split) ext_rinv = c.take<float>(z.M);
             if (bwd) {
                 if (!z.split) {
                     x = c.take<__half>(z.M * z.Dp);
@@ -606,7 +618,7 @@ struct AdSpace {
 };
 
 template <bool BF16>
-int shrink16(const Shrink& p, dim3 grid, cudaStream_t st) {
+int shrink16(const Shrink& p, dim3 grid, Chain& st) {
     const int nt = (p.R + 7) / 8;
 #define ATOM_SHRINK(N)                                                                       \
     if (nt <= N) {                                                                           \
@@ -614,8 +626,7 @@ int shrink16(const Shrink& p, dim3 grid, cudaStream_t st) {
         if (smem > 48 * 1024)                                                                \
             cudaFuncSetAttribute(shrink16_kernel<BF16, N>,                                   \
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem);         \
-        shrink16_kernel<BF16, N><<<grid, 256, smem, st>>>(p);                                \
-        return check_launch("adapters: low-rank rows");                                      \
+        return st.launch("adapters: low-rank rows", shrink16_kernel<BF16, N>, grid, 256, smem, p); \
     }
     ATOM_SHRINK(1)
     ATOM_SHRINK(2)
@@ -625,12 +636,11 @@ int shrink16(const Shrink& p, dim3 grid, cudaStream_t st) {
 #undef ATOM_SHRINK
     return ATOM_ERR_UNSUPPORTED;
 }
-int shrink(const Shrink& p, cudaStream_t st) {
+int shrink(const Shrink& p, Chain& st) {
     const dim3 grid(p.pieces + p.q.nad + 1, 8);
     if (p.dtype == ATOM_BF16) return shrink16<true>(p, grid, st);
     if (p.dtype == ATOM_F16) return shrink16<false>(p, grid, st);
-    shrink32_kernel<<<grid, 256, 32 * (p.R + 1) * 4, st>>>(p);
-    return check_launch("adapters: low-rank rows");
+    return st.launch("adapters: low-rank rows", shrink32_kernel, grid, 256, 32 * (p.R + 1) * 4, p);
 }
 
 // One direction: out [M, N] = rows [M, K] W' + (low-rank rows) (adapters), where forward has
@@ -638,7 +648,7 @@ int shrink(const Shrink& p, cudaStream_t st) {
 struct Ad {
     AdSizes z;
     AdSpace sp;
-    cudaStream_t st;
+    Chain st;
     Requests q;
     const float* scale;
     const void *w, *a, *b;
@@ -662,33 +672,42 @@ struct Ad {
         const bool both = z.on && !low_only;
         if (z.split && low_only) {
         } else if (z.split) {
-            cudaMemsetAsync(sp.max, 0, 16, st);
-            if (z.on) cudaMemsetAsync(sp.ext_rinv, 0, z.M * sizeof(float), st);
-            l.add({w, z.O, z.D, z.D, nullptr, 0, 0, nullptr, sp.max + 1, kMax});
-            if (z.on) l.add({second, srows, scols, scols, nullptr, 0, 0, nullptr, sp.max + 2, kMax});
-            l.add({rows, z.M, K, ld, sp.rows, Kp, z.M * Kp, sp.rinv, nullptr, kRowSplit});
+            // the largest w and adapters, and no scales for rows without low-rank values
+            if (int s = st.zero("adapters", sp.max,
+                                (char*)(sp.ext_rinv + (z.on ? z.M : 0)) - (char*)sp.max))
+                return s;
+            if (bwd) l.add({w, z.O, z.D, z.D, nullptr, 0, 0, nullptr, sp.max + 1, kMax, nullptr});
+            if (z.on)
+                l.add({second, srows, scols, scols, nullptr, 0, 0, nullptr, sp.max + 2, kMax,
+                       nullptr});
+            l.add({rows, z.M, K, ld, sp.rows, Kp, z.M * Kp, sp.rinv, nullptr, kRowSplit, nullptr});
+            if (!bwd)
+                l.add({w, z.O, z.D, z.D, sp.w, z.Dp, z.O * z.Dp, sp.wr, nullptr, kRowSplit,
+                       nullptr});
             if (int s = prepare(l, st)) return s;
             l.n = 0;
-            l.add({w, z.O, z.D, z.D, sp.w, z.Dp, z.O * z.Dp, nullptr, sp.max + 1, kTensorSplit});
+            if (bwd)
+                l.add({w, z.O, z.D, z.D, sp.w, z.Dp, z.O * z.Dp, nullptr, sp.max + 1, kTensorSplit,
+                       nullptr});
             if (z.on)
                 l.add({second, srows, scols, scols, sp.ext, sp_ld, srows * sp_ld, nullptr,
-                       sp.max + 2, kTensorSplit});
+                       sp.max + 2, kTensorSplit, nullptr});
         } else {
             if (!tma_ready(rows, ld)) {
-                l.add({rows, z.M, K, ld, sp.rows, Kp, 0, nullptr, nullptr, kPack});
+                l.add({rows, z.M, K, ld, sp.rows, Kp, 0, nullptr, nullptr, kPack, nullptr});
                 xr = sp.rows, xld = Kp;
             }
             if (!low_only && !tma_ready(w, z.D)) {
-                l.add({w, z.O, z.D, z.D, sp.w, z.Dp, 0, nullptr, nullptr, kPack});
+                l.add({w, z.O, z.D, z.D, sp.w, z.Dp, 0, nullptr, nullptr, kPack, nullptr});
                 wp = sp.w, wld = z.Dp;
             }
             if (both && !tma_ready(second, scols)) {
-                l.add({second, srows, scols, scols, sp.ext, sp_ld, 0, nullptr, nullptr, kPack});
+                l.add({second, srows, scols, scols, sp.ext, sp_ld, 0, nullptr, nullptr, kPack, nullptr});
                 sec = sp.ext, sec_ld = sp_ld;
             }
             if (z.on && !bwd && !tma_ready(first, z.D)) {
                 l.add({first, (long long)z.nad * z.R, z.D, z.D, sp.ad, z.Dp, 0, nullptr, nullptr,
-                       kPack});
+                       kPack, nullptr});
                 first = sp.ad;
             }
         }
@@ -705,10 +724,11 @@ struct Ad {
             if (bwd && z.split) {
                 h.wa = (long long)z.O * z.R, h.wr = 1, h.wk = z.R;
             } else if (bwd) {
-                transpose_kernel<<<dim3(ceil_div(z.Op, 32), ceil_div(z.R, 32), z.nad), 256, 0, st>>>(
-                    static_cast<const unsigned short*>(b), z.O, z.R, (int)z.Op,
-                    reinterpret_cast<unsigned short*>(sp.ad));
-                if (int s = check_launch("adapters: transpose")) return s;
+                if (int s = st.launch("adapters: transpose", transpose_kernel,
+                                      dim3(ceil_div(z.Op, 32), ceil_div(z.R, 32), z.nad), 256, 0,
+                                      static_cast<const unsigned short*>(b), z.O, z.R, (int)z.Op,
+                                      reinterpret_cast<unsigned short*>(sp.ad)))
+                    return s;
                 h.w = sp.ad;
                 h.wa = z.R * z.Op, h.wr = z.Op, h.wk = 1;
             } else {
@@ -766,7 +786,8 @@ struct Ad {
         p.used = z.on ? (1u << 4 * k) - 1 : (1u << 2 * k) - 1;
         p.part = sp.part;
         p.rinv = sp.rinv;
-        p.bmax = sp.max + 1;
+        p.cinv[0] = sp.wr;
+        if (z.split && bwd) p.bmax = sp.max + 1;
         if (z.on) {
             p.ext = (z.R + 63) / 64;
             p.ext_a = 2 * k, p.ext_b = 3 * k, p.ext_bmn = bwd ? 1 : 0;
@@ -833,7 +854,7 @@ extern "C" int atom_adapted_linear_fwd(int dtype, const void* x, int64_t ldx, in
                                        n_adapters, f.sp.few_S, f.sp.few_slot, dtype}, f.st))
                 return s;
         return few::product({x, ldx, (int)M, D, {w, nullptr}, O, 0, y, ldy, dtype,
-                             z.on ? f.sp.few_S : nullptr, f.sp.few_slot, b, R, z.on}, f.st);
+                             z.on ? f.sp.few_S : nullptr, f.sp.few_slot, b, R}, f.st);
     }
     return f.run(x, ldx, false, y, ldy, kept, false);
 }
@@ -872,6 +893,7 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
         Ad g = f;
         g.sp = fs;
         if (int s = g.run(x, ldx, false, nullptr, 0, f.sp.S, true)) return s;
+        f.st = g.st;
     }
     if (int s = f.run(dy, lddy, true, dx, lddx, grads ? f.sp.T : nullptr, !dx)) return s;
     if (!grads) return ATOM_OK;
@@ -887,8 +909,8 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
         if (da && !tma_ready(x, ldx)) {
             if (kept || !db) {
                 PrepList l;
-                l.add({x, M, D, ldx, f.sp.x, z.Dp, 0, nullptr, nullptr, kPack});
-                if (int s = prepare(l, st)) return s;
+                l.add({x, M, D, ldx, f.sp.x, z.Dp, 0, nullptr, nullptr, kPack, nullptr});
+                if (int s = prepare(l, f.st)) return s;
             }
             p.rows[0] = f.sp.x, p.ld[0] = z.Dp;
         }
@@ -902,16 +924,11 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
     const int tiles = p.tiles0 + ceil_div(p.width[1], 128);
     const dim3 grid(tiles, (unsigned)n_adapters * (z.split ? (R + 31) / 32 : 1), p.split);
     int rc;
-    if (dtype == ATOM_BF16) rc = grads16<true>(p, grid, st);
-    else if (dtype == ATOM_F16) rc = grads16<false>(p, grid, st);
-    else {
-        grads32_kernel<<<grid, 256, 0, st>>>(p);
-        rc = check_launch("adapters: gradients");
-    }
+    if (dtype == ATOM_BF16) rc = grads16<true>(p, grid, f.st);
+    else if (dtype == ATOM_F16) rc = grads16<false>(p, grid, f.st);
+    else rc = f.st.launch("adapters: gradients", grads32_kernel, grid, 256, 0, p);
     if (rc) return rc;
-    if (p.split > 1) {
-        grads_sum_kernel<<<592, 256, 0, st>>>(p);
-        ATOM_CHECK_LAUNCH("adapters: gradient sums");
-    }
+    if (p.split > 1)
+        return f.st.launch("adapters: gradient sums", grads_sum_kernel, dim3(592), 256, 0, p);
     return ATOM_OK;
 }

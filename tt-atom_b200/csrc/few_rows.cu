@@ -26,14 +26,6 @@ __device__ __forceinline__ void mma(float* c, uint32_t a0, uint32_t a1, uint32_t
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Waits for the kernel before this one in the stream (a launch without overlap: at once).
-__device__ __forceinline__ void wait_before() {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void let_next_start() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 // The block's sums of 16 rows by 8 columns (red: [warp][matrix][16][8]) into out.
 template <bool GATED>
 __device__ __forceinline__ void finish(const Args& p, const float* red, int n0) {
@@ -81,7 +73,7 @@ __global__ void __launch_bounds__(256) few16_kernel(const __grid_constant__ Args
     const uint4 zero = make_uint4(0, 0, 0, 0);
     const int chunks = (p.K + 31) / 32, end = chunks * (warp + 1) / 8;
     float acc[kMats][4] = {};
-    bool waited = !p.after;
+    bool waited = false;
     for (int c = chunks * warp / 8; c < end || !waited; c += U) {
         uint4 v[U][kMats], a[U], b[U];
 #pragma unroll
@@ -130,7 +122,7 @@ __global__ void __launch_bounds__(256) few32_kernel(const __grid_constant__ Args
     let_next_start();
     const int chunks = (p.K + 127) / 128, first = chunks * warp / 8, end = chunks * (warp + 1) / 8;
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    bool waited = !p.after;
+    bool waited = false;
     for (int m0 = 0; m0 < 16; m0 += 8) {
 #pragma unroll
         for (int j = 0; j < kMats; ++j) {
@@ -174,6 +166,7 @@ __global__ void __launch_bounds__(256) few32_kernel(const __grid_constant__ Args
 __global__ void __launch_bounds__(256) low_kernel(const __grid_constant__ LowArgs p) {
     const int lane = threadIdx.x & 31, m = blockIdx.y, r = blockIdx.x * 8 + (threadIdx.x >> 5);
     let_next_start();
+    wait_before();
     const int q = last_le(p.nreq, m, [&](int i) { return min(max(p.ptr[i], 0), p.M); });
     int a = -1;
     if (q >= 0 && m < p.ptr[q + 1]) a = p.adapter[q];
@@ -217,23 +210,7 @@ bool suits(int dtype, long long M, int K, const void* x, long long ldx, const vo
            aligned16(w1);
 }
 
-template <typename A>
-static int start(void (*kernel)(A), const A& p, dim3 grid, bool after, const char* what,
-                 cudaStream_t st) {
-    cudaLaunchConfig_t c{};
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    c.gridDim = grid;
-    c.blockDim = dim3(256);
-    c.stream = st;
-    c.attrs = &at;
-    c.numAttrs = after ? 1 : 0;
-    cudaLaunchKernelEx(&c, kernel, p);
-    return check_launch(what);
-}
-
-int product(const Args& p, cudaStream_t st) {
+int product(const Args& p, Chain& st) {
     const dim3 grid((p.N + 7) / 8);
     const bool gated = p.w[1] != nullptr, half = p.M <= 8;
     void (*k)(Args) = nullptr;
@@ -252,11 +229,11 @@ int product(const Args& p, cudaStream_t st) {
         ATOM_FEW(false, false, false)
     }
 #undef ATOM_FEW
-    return start(k, p, grid, p.after, "product of a few rows", st);
+    return st.launch("product of a few rows", k, grid, 256, 0, p);
 }
 
-int low_rank(const LowArgs& p, cudaStream_t st) {
-    return start(low_kernel, p, dim3((p.R + 7) / 8, p.M), false, "low-rank part of a few rows", st);
+int low_rank(const LowArgs& p, Chain& st) {
+    return st.launch("low-rank part of a few rows", low_kernel, dim3((p.R + 7) / 8, p.M), 256, 0, p);
 }
 
 }  // namespace few

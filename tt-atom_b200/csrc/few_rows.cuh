@@ -23,12 +23,11 @@ struct Args {
     const int* slot;         // [M], -1: none
     const void* b;           // [adapters][N][R]
     int R;
-    int after;               // launched to overlap with the kernel before, which writes x or S
 };
 // Whether the matrices suit: 16-byte loads along rows of K.
 bool suits(int dtype, long long M, int K, const void* x, long long ldx, const void* w0,
            const void* w1);
-int product(const Args& p, cudaStream_t st);
+int product(const Args& p, Chain& st);
 
 // S[m, r] = scale x[m] . a[slot][r], and each row's adapter.
 struct LowArgs {
@@ -45,7 +44,7 @@ struct LowArgs {
     int* slot;
     int dtype;
 };
-int low_rank(const LowArgs& p, cudaStream_t st);
+int low_rank(const LowArgs& p, Chain& st);
 
 }  // namespace few
 }  // namespace atom

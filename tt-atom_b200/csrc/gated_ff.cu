@@ -54,15 +54,15 @@ struct FfSizes {
 // One call's buffers. 16-bit operands are packed only where TMA cannot read them; fp32 ones
 // always become two planes.
 struct FfSpace {
-    __half *x, *wg, *wu, *wd, *dy, *xt, *dyt, *hp, *dgup, *dgut, *ht;
-    float *xr, *dyr, *hr, *dgur, *H32, *dgu32, *dh, *part;
+    __half *x, *wg, *wu, *wd, *dy, *xt, *dyt, *hp, *dgup;
+    float *xr, *wgr, *wur, *wdr, *dyr, *hr, *dgur, *H32, *dgu32, *dh, *part;
     __half *H, *dgu;
-    unsigned* max;              // x, wg | wu, wd, dy, dgu, h
+    unsigned* max;              // x'' factor, wg | wu, wd, dy'' factor
     size_t bytes;
     FfSpace(void* ws, const FfSizes& z, bool bwd) {
         memset(this, 0, sizeof(*this));
         Cursor c(ws);
-        const long long M = z.M, k = z.split ? 2 : 1;
+        const long long M = z.M, k = z.split ? 2 : 1, M32 = up(M, 32);
         x = c.take<__half>(k * M * z.Dp);
         wg = c.take<__half>(k * z.F * z.Dp);
         wu = c.take<__half>(k * z.F * z.Dp);
@@ -71,7 +71,7 @@ struct FfSpace {
         if (bwd) {
             pf = z.dwgu.part > z.dwd.part ? z.dwgu.part : z.dwd.part;
             dy = c.take<__half>(k * M * z.Op);
-            dh = c.take<float>(up(M, 32) * z.Fp);
+            dh = c.take<float>(M32 * z.Fp);
         }
         part = c.take<float>(pf);
         if (!z.split) {
@@ -79,20 +79,21 @@ struct FfSpace {
             if (bwd) dgu = c.take<__half>(2 * M * z.Fp);
         } else {
             max = c.take<unsigned>(8);
-            xr = c.take<float>(M);
+            xr = c.take<float>(M32);
             H32 = c.take<float>(M * z.Fp);
+            hp = c.take<__half>(2 * M * z.Fp);
+            hr = c.take<float>(M32);
             if (!bwd) {
-                hp = c.take<__half>(2 * M * z.Fp);
-                hr = c.take<float>(M);
+                wgr = c.take<float>(up(z.F, 32));
+                wur = c.take<float>(up(z.F, 32));
+                wdr = c.take<float>(up(z.O, 32));
             } else {
-                dyr = c.take<float>(M);
+                dyr = c.take<float>(M32);
                 dgu32 = c.take<float>(2 * M * z.Fp);
                 dgup = c.take<__half>(4 * M * z.Fp);
-                dgur = c.take<float>(M);
+                dgur = c.take<float>(M32);
                 xt = c.take<__half>(2 * M * z.Dp);
                 dyt = c.take<__half>(2 * M * z.Op);
-                dgut = c.take<__half>(4 * M * z.Fp);
-                ht = c.take<__half>(2 * M * z.Fp);
             }
         }
         bytes = c.used;
@@ -111,7 +112,7 @@ int put(Maps& maps, int i, const Operand& o, bool mn, int box_rows, bool split) 
 struct Ff {
     FfSizes z;
     FfSpace sp;
-    cudaStream_t st;
+    Chain st;
     int act;
     Operand x, wg, wu, wd, dy;
     PrepList list;
@@ -120,31 +121,39 @@ struct Ff {
     Operand take(const void* p, long long rows, long long cols, long long ld, __half* buf,
                  long long pitch, int mode, float* rinv, unsigned* max) {
         if (!z.split && tma_ready(p, ld)) return {p, rows, cols, ld, 0};
-        list.add({p, rows, cols, ld, buf, pitch, rows * pitch, rinv, max, z.split ? mode : kPack});
+        list.add({p, rows, cols, ld, buf, pitch, rows * pitch, rinv, max, z.split ? mode : kPack,
+                  nullptr});
         return {buf, rows, cols, pitch, rows * pitch};
     }
-    // weights, x (and dy) brought into the form that the products read
-    int inputs(const void* xp, long long ldx, const void* g, const void* u, const void* d,
-               const void* dyp, long long lddy) {
+    // Weights and rows brought into the form that the products read. fp32 forward: every operand
+    // scaled row by row, in one launch. fp32 backward: the weights are read across their rows, so
+    // each of them (Wg and Wu together) has one scale, from a launch before; x is needed only for
+    // G and U, and beside its scales in the weights' gradients later.
+    int inputs(const void* xp, long long ldx, const void* g, const void* u, const void* d) {
+        x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kRowSplit, sp.xr, nullptr);
+        wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kRowSplit, sp.wgr, nullptr);
+        wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kRowSplit, sp.wur, nullptr);
+        wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kRowSplit, sp.wdr, nullptr);
+        return flush();
+    }
+    int inputs_bwd(const void* xp, long long ldx, const void* g, const void* u, const void* d,
+                   const void* dyp, long long lddy, bool kept) {
         if (z.split) {
-            const cudaError_t e = cudaMemsetAsync(sp.max, 0, 32, st);
-            if (e != cudaSuccess) {
-                set_error("gated_ff: %s", cudaGetErrorString(e));
-                return ATOM_ERR_CUDA;
-            }
-            list.add({g, z.F, z.D, z.D, nullptr, 0, 0, nullptr, sp.max + 1, kMax});
-            list.add({u, z.F, z.D, z.D, nullptr, 0, 0, nullptr, sp.max + 1, kMax});
-            list.add({d, z.O, z.F, z.F, nullptr, 0, 0, nullptr, sp.max + 2, kMax});
+            if (int s = st.zero("gated_ff", sp.max, 32)) return s;
+            list.add({g, z.F, z.D, z.D, nullptr, 0, 0, nullptr, sp.max + 1, kMax, nullptr});
+            list.add({u, z.F, z.D, z.D, nullptr, 0, 0, nullptr, sp.max + 1, kMax, nullptr});
+            list.add({d, z.O, z.F, z.F, nullptr, 0, 0, nullptr, sp.max + 2, kMax, nullptr});
         }
-        x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kRowSplit, sp.xr, sp.max);
-        if (dyp) dy = take(dyp, z.M, z.O, lddy, sp.dy, z.Op, kRowSplit, sp.dyr, sp.max + 3);
-        if (z.split) {
-            if (int s = prepare(list, st)) return s;
-            list.n = 0;
-        }
+        x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kept ? kRowScale : kRowSplit, sp.xr, nullptr);
+        dy = take(dyp, z.M, z.O, lddy, sp.dy, z.Op, kRowSplit, sp.dyr, nullptr);
+        if (z.split)
+            if (int s = flush()) return s;
         wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kTensorSplit, nullptr, sp.max + 1);
         wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kTensorSplit, nullptr, sp.max + 1);
         wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kTensorSplit, nullptr, sp.max + 2);
+        return flush();
+    }
+    int flush() {
         const int s = prepare(list, st);
         list.n = 0;
         return s;
@@ -188,7 +197,8 @@ struct Ff {
         if (int s = put(maps, 2 * k, wu, false, c.bn / 2, z.split)) return s;
         p.ph[0] = {0, k, 2 * k, z.nk(z.D), 0, 0, c.bn / 2, 0};
         p.rinv = sp.xr;
-        p.bmax = sp.max + 1;
+        if (sp.wgr) p.cinv[0] = sp.wgr, p.cinv[1] = sp.wur;
+        else if (z.split) p.bmax = sp.max + 1;
         p.used = z.split ? 0x3f : 0x7;
         if (int s = gate_output(maps, p, C, width, H)) return s;
         return launch(epilogue, c, z.split, maps, p, st);
@@ -199,8 +209,9 @@ struct Ff {
         if (int s = gates(kGate, p, z.split ? (void*)sp.H32 : sp.H, z.Fp, nullptr)) return s;
         Operand h{sp.H, z.M, z.F, z.Fp, 0};
         if (z.split) {
-            list.add({sp.H32, z.M, z.F, z.Fp, sp.hp, z.Fp, z.M * z.Fp, sp.hr, nullptr, kRowSplit});
-            if (int s = prepare(list, st)) return s;
+            list.add({sp.H32, z.M, z.F, z.Fp, sp.hp, z.Fp, z.M * z.Fp, sp.hr, nullptr, kRowSplit,
+                      nullptr});
+            if (int s = flush()) return s;
             h = {sp.hp, z.M, z.F, z.Fp, z.M * z.Fp};
         }
         const Choice c = z.down;
@@ -211,7 +222,7 @@ struct Ff {
         Args q = args(z.M, z.O);
         q.ph[0] = {0, k, k, z.nk(z.F), 0, 0, c.bn, c.bn / 2};
         q.rinv = sp.hr;
-        q.bmax = sp.max + 2;
+        q.cinv[0] = sp.wdr;
         output(q, y, ldy);
         return launch(kStore, c, z.split, maps, q, st);
     }
@@ -227,8 +238,7 @@ struct Ff {
             Args p = args(z.M, z.F);
             p.ph[0] = {0, k, k, z.nk(z.O), 0, 1, c.bn, c.bn / 2};
             p.rinv = sp.dyr;
-            p.bmax = sp.max + 2;
-            p.hmax = sp.max + 4;
+            if (z.split) p.bmax = sp.max + 2;
             p.used = z.split ? 0xf : 0x3;
             if (kept) {
                 p.gu = const_cast<float*>(kept);
@@ -239,32 +249,35 @@ struct Ff {
                 if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
                 Args q = args(z.M, z.F);
                 q.dh = sp.dh;
-                q.hmax = sp.max + 4;
                 if (int s = gates(kGateBwdGU, q, dgu, 2 * z.Fp, H)) return s;
             }
         }
-        Operand g{sp.dgu, z.M, 2 * z.Fp, 2 * z.Fp, 0}, gt = g, h{sp.H, z.M, z.F, z.Fp, 0};
+        Operand g{sp.dgu, z.M, 2 * z.Fp, 2 * z.Fp, 0}, h{sp.H, z.M, z.F, z.Fp, 0};
         Operand xt = x, dyt = dy;
         if (z.split) {
+            // dG | dU and H are scaled row by row. In the weights' gradients, sums over rows, the
+            // rows' scales s cancel against x (and dy) rows divided by them: what is left is one
+            // power of two, the largest of the rows' x (dy) and dG | dU (H) scales together, and
+            // rows lose bits only as far as they are small in the sum.
             const long long M = z.M, W = 2 * z.Fp;
             g = {sp.dgup, M, W, W, M * W};
-            gt = {sp.dgut, M, W, W, M * W};
-            h = {sp.ht, M, z.F, z.Fp, M * z.Fp};
-            if (dx) list.add({sp.dgu32, M, W, W, sp.dgup, W, M * W, sp.dgur, nullptr, kRowSplit});
+            h = {sp.hp, M, z.F, z.Fp, M * z.Fp};
+            list.add({sp.dgu32, M, W, W, sp.dgup, W, M * W, sp.dgur, sp.max, kRowSplit, sp.xr});
+            if (dwd)
+                list.add({sp.H32, M, z.F, z.Fp, sp.hp, z.Fp, M * z.Fp, sp.hr, sp.max + 3,
+                          kRowSplit, sp.dyr});
+            if (int s = flush()) return s;
             if (dwg || dwu) {
-                list.add({sp.dgu32, M, W, W, sp.dgut, W, M * W, nullptr, sp.max + 4, kTensorSplit});
-                xt.p = sp.xt;
-                list.add({x_src, M, z.D, x_ld, sp.xt, z.Dp, M * z.Dp, nullptr, sp.max,
-                          kTensorSplit});
+                xt = {sp.xt, M, z.D, z.Dp, M * z.Dp};
+                list.add({x_src, M, z.D, x_ld, sp.xt, z.Dp, M * z.Dp, nullptr, sp.max, kWeighted,
+                          sp.dgur});
             }
             if (dwd) {
-                list.add({sp.H32, M, z.F, z.Fp, sp.ht, z.Fp, M * z.Fp, nullptr, sp.max + 5,
-                          kTensorSplit});
-                dyt.p = sp.dyt;
+                dyt = {sp.dyt, M, z.O, z.Op, M * z.Op};
                 list.add({dy_src, M, z.O, dy_ld, sp.dyt, z.Op, M * z.Op, nullptr, sp.max + 3,
-                          kTensorSplit});
+                          kWeighted, sp.hr});
             }
-            if (int s = prepare(list, st)) return s;
+            if (int s = flush()) return s;
         }
         if (dx) {
             const Choice c = z.dx;
@@ -278,7 +291,7 @@ struct Ff {
             p.ph[0] = {0, 2 * k, 2 * k, z.nk(z.F), 0, 1, c.bn, c.bn / 2};
             p.ph[1] = {k, 3 * k, 3 * k, z.nk(z.F), 0, 1, c.bn, c.bn / 2};
             p.rinv = sp.dgur;
-            p.bmax = sp.max + 1;
+            if (z.split) p.bmax = sp.max + 1;
             output(p, dx, lddx);
             if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
         }
@@ -286,15 +299,14 @@ struct Ff {
             Choice c = z.dwgu;
             const bool two = dwg && dwu;
             Maps maps;
-            if (int s = put(maps, 0, gt.columns(dwg ? 0 : z.Fp, z.F), true, 64, z.split)) return s;
+            if (int s = put(maps, 0, g.columns(dwg ? 0 : z.Fp, z.F), true, 64, z.split)) return s;
             if (two)
-                if (int s = put(maps, k, gt.columns(z.Fp, z.F), true, 64, z.split)) return s;
+                if (int s = put(maps, k, g.columns(z.Fp, z.F), true, 64, z.split)) return s;
             if (int s = put(maps, 2 * k, xt, true, 64, z.split)) return s;
             Args p = args(z.F, z.D);
             p.groups = two ? 2 : 1;
             p.ph[0] = {0, 2 * k, 2 * k, z.nk(z.M), 1, 1, c.bn, c.bn / 2};
-            p.amax = sp.max + 4;
-            p.bmax = sp.max;
+            p.factor = reinterpret_cast<const float*>(sp.max);
             output(p, dwg ? dwg : dwu, z.D);
             p.C[1] = dwu;
             if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
@@ -306,8 +318,7 @@ struct Ff {
             if (int s = put(maps, k, h, true, 64, z.split)) return s;
             Args p = args(z.O, z.F);
             p.ph[0] = {0, k, k, z.nk(z.M), 1, 1, c.bn, c.bn / 2};
-            p.amax = sp.max + 3;
-            p.bmax = sp.max + 5;
+            p.factor = reinterpret_cast<const float*>(sp.max + 3);
             output(p, dwd, z.F);
             if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
         }
@@ -362,12 +373,12 @@ extern "C" int atom_gated_ff_fwd(int dtype, const void* x, int64_t ldx, int64_t 
     void* h = z.split ? (void*)f.sp.H32 : f.sp.H;
     if (few_rows(z, x, ldx, wg, wu, wd)) {
         if (int s = few::product({x, ldx, (int)M, D, {wg, wu}, F, act, h, z.Fp, dtype, nullptr,
-                                  nullptr, nullptr, 0, 0}, f.st))
+                                  nullptr, nullptr, 0}, f.st))
             return s;
         return few::product({h, z.Fp, (int)M, F, {wd, nullptr}, O, 0, y, ldy, dtype, nullptr,
-                             nullptr, nullptr, 0, 1}, f.st);
+                             nullptr, nullptr, 0}, f.st);
     }
-    if (int s = f.inputs(x, ldx, wg, wu, wd, nullptr, 0)) return s;
+    if (int s = f.inputs(x, ldx, wg, wu, wd)) return s;
     return f.forward(y, ldy, static_cast<float*>(kept));
 }
 
@@ -392,7 +403,7 @@ extern "C" int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t 
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
                  f.sp.bytes);
     f.x_src = x, f.x_ld = ldx, f.dy_src = dy, f.dy_ld = lddy;
-    if (int s = f.inputs(x, ldx, wg, wu, wd, dy, lddy)) return s;
     if (few_rows(z, x, ldx, wg, wu, wd)) kept = nullptr;
+    if (int s = f.inputs_bwd(x, ldx, wg, wu, wd, dy, lddy, kept != nullptr)) return s;
     return f.backward(static_cast<const float*>(kept), dx, lddx, dwg, dwu, dwd);
 }

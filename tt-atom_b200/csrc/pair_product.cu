@@ -326,29 +326,24 @@ __device__ __forceinline__ void spoil32(float* v) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(0x7FC00000u);
 }
-// Activation and derivative: fast intrinsics (a few 2^-23) for 16-bit results, the accurate
-// functions for fp32 ones. GELU's erfc is called, not expanded at each of a row's 32 values.
+// The gate and its gradient. Sigmoids from ex2.approx and rcp.approx, each good to 2 units in the
+// last place; what the exponent's own rounding adds, |g| 2^-24, is far below the products' own
+// error of 5e-7. GELU's erfc is called, not expanded at each of a row's 32 values.
 __device__ __noinline__ float normal_cdf(float g) { return 0.5f * erfcf(-0.70710678f * g); }
-template <bool EXACT>
-__device__ __forceinline__ float sigmoid_t(float g) {
-    return EXACT ? sigmoid_f(g) : sigmoid_gate(g);
-}
 // h = act(g) u
-template <bool EXACT>
 __device__ __forceinline__ void gate32(float* g, const float* u, int act) {
     if (act == 0) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid_t<EXACT>(g[i]) * u[i];
+        for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid_gate(g[i]) * u[i];
     } else if (act == 1) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) g[i] = sigmoid_t<EXACT>(g[i]) * u[i];
+        for (int i = 0; i < 32; ++i) g[i] = sigmoid_gate(g[i]) * u[i];
     } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) g[i] = g[i] * normal_cdf(g[i]) * u[i];
     }
 }
 // (g, u, d = dh) -> (dg, du, h)
-template <bool EXACT>
 __device__ __forceinline__ void gate_bwd32(float* g, float* u, float* d, int act) {
     auto out = [&](int i, float a, float da) {
         const float x = u[i];
@@ -359,20 +354,20 @@ __device__ __forceinline__ void gate_bwd32(float* g, float* u, float* d, int act
     if (act == 0) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            const float s = sigmoid_t<EXACT>(g[i]);
+            const float s = sigmoid_gate(g[i]);
             out(i, g[i] * s, s * (1.f + g[i] * (1.f - s)));
         }
     } else if (act == 1) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            const float s = sigmoid_t<EXACT>(g[i]);
+            const float s = sigmoid_gate(g[i]);
             out(i, s, s * (1.f - s));
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const float c = normal_cdf(g[i]), x = g[i];
-            out(i, x * c, c + x * 0.39894228f * (EXACT ? expf(-0.5f * x * x) : __expf(-0.5f * x * x)));
+            out(i, x * c, c + x * 0.39894228f * __expf(-0.5f * x * x));
         }
     }
 }
@@ -381,8 +376,7 @@ __device__ __forceinline__ void gate_bwd32(float* g, float* u, float* d, int act
 // v0 (and v1: the u columns of a gate).
 template <int EPI, bool SPLIT>
 __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const Tile& ti, Out& o,
-                                         long long m, int n, int lane, float* v0, float* v1,
-                                         unsigned& mx0, unsigned& mx1) {
+                                         long long m, int n, int lane, float* v0, float* v1) {
     if (m >= p.M || n >= p.N) return;
     const int left = p.N - n;
     if constexpr (EPI == kStore) {
@@ -406,7 +400,7 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
             store_block(lane_block(p.gu, m, n, p.Fp, lane), v0);
             store_block(lane_block(p.gu, m, n, p.Fp, lane) + p.gu_half, v1);
         }
-        gate32<SPLIT>(v0, v1, p.act);
+        gate32(v0, v1, p.act);
         store_tma(o, lane, &maps.m[kOutMap], n, (int)m, -1, v0, p.dtype);
     } else {
         // v0, v1 = g, u (kGateBwdGU, dh from memory) or v0 = dh (kGateBwdDH, g and u from memory)
@@ -419,16 +413,7 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
             load_block(lane_block(p.gu, m, n, p.Fp, lane), v0);
             load_block(lane_block(p.gu, m, n, p.Fp, lane) + p.gu_half, v1);
         }
-        gate_bwd32<SPLIT>(v0, v1, w, p.act);
-        if (SPLIT) {
-            const int mine = m + lane < p.M ? left : 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (i < mine) {
-                    mx0 = max(mx0, max(finite_bits(v0[i]), finite_bits(v1[i])));
-                    mx1 = max(mx1, finite_bits(w[i]));
-                }
-        }
+        gate_bwd32(v0, v1, w, p.act);
         store_tma(o, lane, &maps.m[kOutMap], n, (int)m, -1, v0, p.dtype);
         store_tma(o, lane, &maps.m[kOutMap], p.Fp + n, (int)m, -1, v1, p.dtype);
         if (p.H) store_tma(o, lane, &maps.m[kHMap], n, (int)m, -1, w, p.dtype);
@@ -457,6 +442,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     uint32_t rank;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     const int pairs = gridDim.x >> 1, first = blockIdx.x >> 1;
+    let_next_start();
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 1);
@@ -483,6 +469,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
     const uint32_t base = smem_u32(smem);
+    wait_before();
 
     if (warp == 0) {
         {
@@ -656,7 +643,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int q = warp & 3, half = (warp - 2) >> 2;
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         uint32_t round = 0;
-        unsigned mx0 = 0, mx1 = 0;
         const uint32_t acce0 = peer_addr(smem_u32(acce), 0);
         // This warp has read the round's accumulators. Relaxed: only tensor memory is handed over,
         // which the fence orders; a release would wait for this warp's stores to memory as well.
@@ -699,7 +685,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (GATED) pin32(v1);
                     if (k == kChunks - 1) drained();
                     if (EPI == kStore && spoilt) spoil32(v0);
-                    finish32<EPI, SPLIT>(maps, p, ti, out, m, nb + 32 * k, lane, v0, v1, mx0, mx1);
+                    finish32<EPI, SPLIT>(maps, p, ti, out, m, nb + 32 * k, lane, v0, v1);
                 }
             } else {
                 // the tile's rounds summed in registers
@@ -745,9 +731,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     return true;
                 };
                 static_assert(!SPLIT || kParts == 2, "parts of a SPLIT tile");
-                const float sb = pow2_inv(pow2_scale(*p.bmax));
-                const float sa = p.rinv ? (m + lane < p.M ? p.rinv[m + lane] : 0.f)
-                                        : pow2_inv(pow2_scale(*p.amax));
+                const float sb = p.bmax ? pow2_inv(pow2_scale(*p.bmax)) : 1.f;
+                const float sa = p.rinv ? (m + lane < p.M ? p.rinv[m + lane] : 0.f) : *p.factor;
                 int stages = 0;
                 for (int f = 0; f < p.nphase; ++f) {
                     const Share sh(p, ti, f);
@@ -758,6 +743,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 for (int k = 0; k < kParts; ++k)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[k][i] = v[k][i] * sa * sb;
+                if (p.cinv[0]) {
+#pragma unroll
+                    for (int k = 0; k < kParts; ++k) {
+                        const int n = nb + 32 * (GATED ? k % kChunks : k);
+                        const float* c = p.cinv[GATED && k >= kChunks] + n;
+                        if (n >= p.N) continue;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 x = __ldg(reinterpret_cast<const float4*>(c + i));
+                            v[k][i] *= x.x, v[k][i + 1] *= x.y;
+                            v[k][i + 2] *= x.z, v[k][i + 3] *= x.w;
+                        }
+                    }
+                }
                 if (p.ext) {
                     int es = 0;
                     for (Blocks st(p, ti); st.any(); st.next()) ++es;
@@ -770,21 +769,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     float u[32];         // kGateBwdDH: room for the u that it reads
                     if (EPI == kStore && spoilt) spoil32(v[k]);
                     finish32<EPI, SPLIT>(maps, p, ti, out, m, nb + 32 * k, lane, v[k],
-                                         GATED ? v[kChunks + k] : u, mx0, mx1);
+                                         GATED ? v[kChunks + k] : u);
                 }
             }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        if constexpr (SPLIT && (EPI == kGateBwdGU || EPI == kGateBwdDH)) {
-            if (p.hmax) {
-                mx0 = __reduce_max_sync(0xffffffffu, mx0);
-                mx1 = __reduce_max_sync(0xffffffffu, mx1);
-                if (lane == 0) {
-                    atomicMax(p.hmax, mx0);
-                    atomicMax(p.hmax + 1, mx1);
-                }
-            }
-        }
         if (!ok && lane == 0) *(volatile int*)failed = 1;
     }
     __syncthreads();
@@ -804,6 +793,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // C[g][m, n] = sum over the splits, in order.
 __global__ void __launch_bounds__(256) reduce_kernel(Args p) {
+    let_next_start();
+    wait_before();
     const long long per = p.M * p.N, all = per * p.groups;
     const bool four = p.N % 4 == 0;
     for (long long i = (blockIdx.x * 256LL + threadIdx.x) * 4; i < all; i += gridDim.x * 1024LL) {
@@ -837,6 +828,8 @@ __host__ __device__ inline bool prep_wide(const PrepItem& it) {
 // except that a maximum leaves it out.
 template <int NV>
 __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ PrepList l) {
+    let_next_start();
+    wait_before();
     const PrepItem& it = l.it[blockIdx.y];
     __shared__ float part[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -881,6 +874,9 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ PrepL
         const long long held = 4LL * NV * threads;
         if (mode == kTensorSplit) {
             s = pow2_scale(*it.max);
+        } else if (mode == kWeighted) {
+            // a row whose partner is zero may have any weight
+            s = fminf(it.weight[r] * pow2_inv(__uint_as_float(*it.max)), 0x1p126f);
         } else {
             float mx = 0.f;
             auto see = [&](const float4& v) {       // fmaxf passes over NaN
@@ -905,10 +901,15 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ PrepL
             };
             all(see);
             if (isinf(mx)) all(see_finite);
-            top = fmaxf(top, mx);
-            if (mode == kMax) continue;
+            if (mode == kMax) {
+                top = fmaxf(top, mx);
+                continue;
+            }
             s = pow2_scale(__float_as_uint(mx));
-            if (me == 0) it.rinv[r] = pow2_inv(s);
+            const float inv = mx > 0.f ? pow2_inv(s) : 0.f;
+            if (me == 0) it.rinv[r] = inv;
+            if (it.weight) top = fmaxf(top, fminf(inv * it.weight[r], 0x1p126f));
+            if (mode == kRowScale) continue;
         }
         __half* hi = static_cast<__half*>(it.dst) + r * dld;
         auto put = [&](long long c, const float4& v) {
@@ -923,11 +924,14 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ PrepL
             if (4LL * (j * threads + me) < dld) put(4LL * (j * threads + me), x[j]);
         for (long long c = held + 4 * me; c < dld; c += 4 * threads) put(c, load(c));
     }
+    // the epilogue reads scales of columns 32 at a time
+    if (mode == kRowSplit && blockIdx.x == 0 && threadIdx.x < 32 && it.rows + lane < (it.rows + 31) / 32 * 32)
+        it.rinv[it.rows + lane] = 0.f;
     if (it.max && (mode == kMax || mode == kRowSplit) && lane == 0 && top > 0.f)
         atomicMax(it.max, __float_as_uint(top));
 }
 
-int prepare(const PrepList& l, cudaStream_t st) {
+int prepare(const PrepList& l, Chain& st) {
     if (l.n == 0) return ATOM_OK;
     long long rows = 1, nv = 1;
     for (int i = 0; i < l.n; ++i) {
@@ -939,11 +943,8 @@ int prepare(const PrepList& l, cudaStream_t st) {
     }
     const long long blocks = (rows + 7) / 8;
     const dim3 grid((unsigned)std::min(blocks, 2368LL), l.n);
-    if (nv <= 1) prep_kernel<1><<<grid, 256, 0, st>>>(l);
-    else if (nv <= 2) prep_kernel<2><<<grid, 256, 0, st>>>(l);
-    else if (nv <= 4) prep_kernel<4><<<grid, 256, 0, st>>>(l);
-    else prep_kernel<8><<<grid, 256, 0, st>>>(l);
-    return check_launch("operand preparation");
+    return st.launch("operand preparation", nv <= 1 ? prep_kernel<1> : nv <= 2 ? prep_kernel<2>
+                     : nv <= 4 ? prep_kernel<4> : prep_kernel<8>, grid, 256, 0, l);
 }
 
 static PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -1036,7 +1037,7 @@ Choice choose(long long M, int N, int nk, int groups, bool gated, bool split, bo
 }
 
 template <int BN, int EPI, bool SPLIT>
-static int run(const Maps& maps, const Args& p, cudaStream_t st) {
+static int run(const Maps& maps, const Args& p, Chain& st) {
     using CF = Cfg<BN, SPLIT>;
     static std::atomic<bool> set[64];
     int dev = 0;
@@ -1054,17 +1055,18 @@ static int run(const Maps& maps, const Args& p, cudaStream_t st) {
     }
     const long long pairs = sm_count() / 2;
     const int grid = 2 * (int)(p.tiles < pairs ? p.tiles : pairs);
-    pair_kernel<BN, EPI, SPLIT><<<grid, kThreads, CF::kSmem, st>>>(maps, p);
-    if (int s = check_launch("pair product")) return s;
+    if (int s = st.launch("pair product", pair_kernel<BN, EPI, SPLIT>, dim3(grid), kThreads,
+                          CF::kSmem, maps, p))
+        return s;
     if (p.ksplit > 1) {
         const long long blocks = (p.M * p.N * p.groups + 1023) / 1024;
-        reduce_kernel<<<(unsigned)(blocks < 1184 ? blocks : 1184), 256, 0, st>>>(p);
-        return check_launch("pair product sums");
+        return st.launch("pair product sums", reduce_kernel,
+                         dim3((unsigned)(blocks < 1184 ? blocks : 1184)), 256, 0, p);
     }
     return ATOM_OK;
 }
 
-int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, cudaStream_t st) {
+int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain& st) {
     const bool gated = epilogue == kGate || epilogue == kGateBwdGU;
     const int w = gated ? c.bn / 2 : c.bn;
     p.mtiles = ceil_div(p.M, 256);

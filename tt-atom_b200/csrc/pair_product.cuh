@@ -47,10 +47,10 @@ struct Args {
     float* dh;               // kGateBwdGU: lane blocks
     int H;                   // gate backward: H wanted (map kHMap; dG | dU: kOutMap, u at Fp)
     int Fp;
-    const float* rinv;       // SPLIT: 1 / scale of A's rows, or NULL
-    const unsigned* amax;    // SPLIT: finite maximum (bits) of A's tensor where rinv is NULL
-    const unsigned* bmax;    // ... and of B's
-    unsigned* hmax;          // SPLIT gate backward: maxima of dG | dU and of H
+    const float* rinv;       // SPLIT: 1 / scale of A's rows; NULL: `factor` for all of them
+    const float* factor;     // ... and the planes' scales together
+    const float* cinv[2];    // 1 / scale of B's rows (columns of C; u's second), or NULL:
+    const unsigned* bmax;    // B's tensor was scaled by this finite maximum (bits)
     // low-rank blocks beside the phases: block t + r holds the rows of request r in 256-row tile
     // t ([256][R] typed, zeros in other rows), multiplied by the request's adapter
     int ext;                 // stages a request, 0: none
@@ -81,25 +81,29 @@ int make_out_map(CUtensorMap* m, const void* p, int dtype, long long cols, long 
                  long long ld);
 
 // Launches the product: tiles, C's maps (kStore) etc. are filled in from M, N, C and the choice.
-int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, cudaStream_t st);
+int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain& st);
 
 // Operand preparation, up to 6 matrices a launch.
-enum Prep { kPack = 0, kRowSplit = 1, kMax = 2, kTensorSplit = 3 };
+// kPack: 16-bit copy. kRowSplit: planes scaled row by row. kRowScale: the scales alone. kMax: the
+// largest finite magnitude. kTensorSplit: planes scaled by that. kWeighted: planes of row r times
+// weight[r] / max (a power of two).
+enum Prep { kPack = 0, kRowSplit = 1, kMax = 2, kTensorSplit = 3, kRowScale = 4, kWeighted = 5 };
 struct PrepItem {
     const void* src;
     long long rows, cols, ld;
     void* dst;               // [rows][dld], the lo plane `plane` elements behind
     long long dld, plane;
-    float* rinv;             // kRowSplit: 1 / scale of each row
-    unsigned* max;           // largest finite magnitude: written (kMax, kRowSplit; may be NULL)
-    int mode;                // or read (kTensorSplit)
+    float* rinv;             // kRowSplit, kRowScale: 1 / scale of each row, 0 for a row of zeros
+    unsigned* max;           // written by kMax; by kRowSplit (with weight): the largest
+    int mode;                // rinv[r] * weight[r]; read by kTensorSplit and kWeighted
+    const float* weight;
 };
 struct PrepList {
     PrepItem it[6];
     int n = 0;
     void add(const PrepItem& i) { it[n++] = i; }
 };
-int prepare(const PrepList& l, cudaStream_t st);
+int prepare(const PrepList& l, Chain& st);
 
 inline bool tma_ready(const void* p, long long ld) { return aligned16(p) && ld % 8 == 0; }
 inline long long up(long long n, long long k) { return (n + k - 1) / k * k; }

@@ -83,6 +83,45 @@ __device__ __forceinline__ float2 pair_f(uint32_t w, int dtype) {
                               : __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
+// A call's kernels on its stream. Each after the first starts while the one before it still runs
+// (it sets up, then waits in wait_before() for what that one writes), which hides the launches.
+struct Chain {
+    cudaStream_t st;
+    bool after = false;
+    Chain(cudaStream_t s) : st(s) {}
+    template <typename... P, typename... A>
+    int launch(const char* what, void (*kernel)(P...), dim3 grid, int block, size_t smem,
+               const A&... args) {
+        cudaLaunchConfig_t c{};
+        cudaLaunchAttribute at;
+        at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at.val.programmaticStreamSerializationAllowed = 1;
+        c.gridDim = grid;
+        c.blockDim = dim3(block);
+        c.dynamicSmemBytes = smem;
+        c.stream = st;
+        c.attrs = &at;
+        c.numAttrs = after ? 1 : 0;
+        cudaLaunchKernelEx(&c, kernel, args...);
+        after = true;
+        return check_launch(what);
+    }
+    int zero(const char* what, void* p, size_t n) {
+        const cudaError_t e = n ? cudaMemsetAsync(p, 0, n, st) : cudaSuccess;
+        after = false;
+        if (e == cudaSuccess) return ATOM_OK;
+        set_error("%s: %s", what, cudaGetErrorString(e));
+        return ATOM_ERR_CUDA;
+    }
+};
+// Waits for the kernel before this one (a launch without overlap: at once).
+__device__ __forceinline__ void wait_before() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_start() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // Pieces of a caller's workspace, 256-byte aligned; with base NULL it only adds up the sizes.
 struct Cursor {
     char* base;
