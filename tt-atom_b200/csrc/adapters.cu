@@ -6,8 +6,8 @@
 // r in row tile t (t + r grows along the requests, so it names a piece without a table). The
 // shrink pass writes S of each piece as a block of 256 rows, zeros where the rows are not the
 // request's, and the shared projection's product (pair_product.cu) then takes each piece of its
-// row tile as one more K stage, S's block times the request's B: the adapters cost their own
-// multiplications and no pass over y. The backward pass is the same with T = s (dy B), W and A in
+// row tile as more of K, S's block times the request's B, in slices of 16 ranks of which four make
+// a stage: the adapters cost their own multiplications and no pass over y. The backward pass is the same with T = s (dy B), W and A in
 // the place of S, W^T and B, and dA = T^T x, dB = dy^T S summed by pieces in their order.
 //
 // Zeros in a block keep other requests' rows as they are only where B is finite; an adapter that
@@ -36,6 +36,7 @@ __device__ __forceinline__ int row_of(const Requests& q, int r) {
 struct Shrink {
     Requests q;
     int pieces;              // row tiles + requests
+    int rb;                  // rows of a piece that a block has (32 .. 256, grid.y = 256 / rb)
     const void* rows;        // [M, K]
     long long ld;
     int K;
@@ -63,7 +64,7 @@ __device__ __forceinline__ bool side_work(const Shrink& p) {
     if (b < 0) return false;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (b == p.q.nad) {
-        for (int t = blockIdx.y * 8 + warp; t < p.tiles; t += 64) {
+        for (int t = blockIdx.y * 8 + warp; t < p.tiles; t += 8 * gridDim.y) {
             const int first = last_le(p.q.n, t * 256, [&](int r) { return row_of(p.q, r); });
             const int last = last_le(p.q.n, t * 256 + 255, [&](int r) { return row_of(p.q, r); });
             // a request that begins before the tile reaches into it at most as the last such one
@@ -71,9 +72,10 @@ __device__ __forceinline__ bool side_work(const Shrink& p) {
         }
         return true;
     }
-    if (blockIdx.y >= 4) return true;
+    const int parts = min(4, gridDim.y);
+    if (blockIdx.y >= parts) return true;
     int found = 0;
-    const long long lo = p.other_n * blockIdx.y / 4, hi = p.other_n * (blockIdx.y + 1) / 4;
+    const long long lo = p.other_n * blockIdx.y / parts, hi = p.other_n * (blockIdx.y + 1) / parts;
     const long long at = (long long)b * p.other_n;
     if (p.dtype == ATOM_F32) {
         const unsigned* v = static_cast<const unsigned*>(p.other) + at;
@@ -98,7 +100,8 @@ __device__ __forceinline__ bool side_work(const Shrink& p) {
         for (; i < hi; i += 256) found |= (v[i] & top) == top;
     }
     found = __syncthreads_or(found);
-    if (threadIdx.x == 0) reinterpret_cast<int*>(p.bad + b)[blockIdx.y] = found;
+    for (int i = blockIdx.y; i < 4 && threadIdx.x == 0; i += parts)
+        reinterpret_cast<int*>(p.bad + b)[i] = i == blockIdx.y ? found : 0;
     return true;
 }
 
@@ -164,13 +167,14 @@ __global__ void __launch_bounds__(256, NT <= 4 ? 3 : 1)
     if (side_work(p)) return;
     const Piece c = find_piece(p);
     if (c.slot < 0) return;
-    const int m0 = c.m0 + blockIdx.y * 32, lo = max(c.lo, m0), hi = min(c.hi, m0 + 32);
+    for (int m0 = c.m0 + blockIdx.y * p.rb, behind = m0 + p.rb; m0 < behind; m0 += 32) {
+    const int lo = max(c.lo, m0), hi = min(c.hi, m0 + 32);
     unsigned short* block = static_cast<unsigned short*>(p.block) +
-                            ((long long)blockIdx.x * 256 + blockIdx.y * 32) * p.Rs;
+                            ((long long)blockIdx.x * 256 + m0 - c.m0) * p.Rs;
     if (lo >= hi) {                      // Rs is a multiple of 8
         for (int i = threadIdx.x; i < 4 * p.Rs; i += 256)
             reinterpret_cast<uint4*>(block)[i] = make_uint4(0, 0, 0, 0);
-        return;
+        continue;
     }
     const int g0 = (lo - m0) / 16, gp = (hi - 1 - m0) / 16 - g0 + 1, parts = 8 / gp;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -233,75 +237,101 @@ __global__ void __launch_bounds__(256, NT <= 4 ? 3 : 1)
         store_f(block, i, v, p.dtype);
         if (p.compact && in) store_f(p.compact, (long long)m * p.Rs + r, v, p.dtype);
     }
+    __syncthreads();                     // red is free for the next 32 rows
+    }
 }
 
-// fp32: a warp has 8 rows by 8 ranks, its lanes split K, and the 64 sums are added over the lanes
+// fp32: a warp has 8 rows by 4 ranks, its lanes split K, and the 32 sums are added over the lanes
 // by halves; then each row's planes.
-__global__ void __launch_bounds__(256) shrink32_kernel(const __grid_constant__ Shrink p) {
+__global__ void __launch_bounds__(256, 2) shrink32_kernel(const __grid_constant__ Shrink p) {
     extern __shared__ float out[];       // [32][R + 1]
     let_next_start();
     wait_before();
     if (side_work(p)) return;
     const Piece c = find_piece(p);
     if (c.slot < 0) return;
-    const int m0 = c.m0 + blockIdx.y * 32, lo = max(c.lo, m0), hi = min(c.hi, m0 + 32);
-    __half* block = static_cast<__half*>(p.block) +
-                    ((long long)blockIdx.x * 256 + blockIdx.y * 32) * p.Rs;
-    if (lo >= hi) {
-        for (int i = threadIdx.x; i < 4 * p.Rs; i += 256) {
-            reinterpret_cast<uint4*>(block)[i] = make_uint4(0, 0, 0, 0);
-            reinterpret_cast<uint4*>(block + p.plane)[i] = make_uint4(0, 0, 0, 0);
-        }
-        return;
-    }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pitch = p.R + 1;
     const float s = p.scale[c.slot];
-    const int groups = (hi - lo + 7) / 8, ranks = (p.R + 7) / 8;
-    for (int item = warp; item < groups * ranks; item += 8) {
-        const int row0 = lo + item / ranks * 8, r0 = item % ranks * 8;
-        const float* x = static_cast<const float*>(p.rows) + row0 * p.ld;
-        const float* w = static_cast<const float*>(p.w) + c.slot * p.wa + r0 * p.wr;
-        float acc[64];
-#pragma unroll
-        for (int i = 0; i < 64; ++i) acc[i] = 0.f;
-        const int nr = min(8, hi - row0), nk = min(8, p.R - r0);
-#pragma unroll 2
-        for (int k = lane; k < p.K; k += 32) {
-            float a[8], b[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] = i < nr ? x[i * p.ld + k] : 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = j < nk ? w[j * p.wr + k * p.wk] : 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) acc[8 * i + j] = fmaf(a[i], b[j], acc[8 * i + j]);
+    const bool xvec = p.K % 4 == 0 && p.ld % 4 == 0 && aligned16(p.rows);
+    const bool wvec = p.K % 4 == 0 && p.wk == 1 && aligned16(p.w);
+    const bool wrow = p.wr == 1 && p.R % 4 == 0 && aligned16(p.w);
+    // four consecutive elements a lane, whatever the strides: the sums' order stays the same
+    auto four = [&](const float* q, long long step, int k, bool in, bool vec) {
+        if (!in) return make_float4(0.f, 0.f, 0.f, 0.f);
+        if (vec) return *reinterpret_cast<const float4*>(q + k);
+        return make_float4(q[k * step], k + 1 < p.K ? q[(k + 1) * step] : 0.f,
+                           k + 2 < p.K ? q[(k + 2) * step] : 0.f,
+                           k + 3 < p.K ? q[(k + 3) * step] : 0.f);
+    };
+    for (int m0 = c.m0 + blockIdx.y * p.rb, behind = m0 + p.rb; m0 < behind; m0 += 32) {
+        const int lo = max(c.lo, m0), hi = min(c.hi, m0 + 32);
+        __half* block = static_cast<__half*>(p.block) +
+                        ((long long)blockIdx.x * 256 + m0 - c.m0) * p.Rs;
+        if (lo >= hi) {
+            for (int i = threadIdx.x; i < 4 * p.Rs; i += 256) {
+                reinterpret_cast<uint4*>(block)[i] = make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(block + p.plane)[i] = make_uint4(0, 0, 0, 0);
+            }
+            continue;
         }
-        sum_halves(acc, lane);
+        const int groups = (hi - lo + 7) / 8, ranks = (p.R + 3) / 4;
+        for (int item = warp; item < groups * ranks; item += 8) {
+            const int row0 = lo + item / ranks * 8, r0 = item % ranks * 4;
+            const float* x = static_cast<const float*>(p.rows) + row0 * p.ld;
+            const float* w = static_cast<const float*>(p.w) + c.slot * p.wa + r0 * p.wr;
+            const int nr = min(8, hi - row0), nk = min(4, p.R - r0);
+            float acc[32];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int i = (2 * lane + e) >> 3, j = (2 * lane + e) & 7;
-            if (i < nr && j < nk) out[(row0 - m0 + i) * pitch + r0 + j] = s * acc[e];
+            for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+            for (int k = lane * 4; k < p.K; k += 128) {
+                float4 a[8], d[4];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[i] = four(x + i * p.ld, 1, k, i < nr, xvec);
+                if (wrow && k + 3 < p.K) {       // the ranks of a K element lie side by side
+                    float4 t[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        t[e] = *reinterpret_cast<const float4*>(w + (k + e) * p.wk);
+                    d[0] = make_float4(t[0].x, t[1].x, t[2].x, t[3].x);
+                    d[1] = make_float4(t[0].y, t[1].y, t[2].y, t[3].y);
+                    d[2] = make_float4(t[0].z, t[1].z, t[2].z, t[3].z);
+                    d[3] = make_float4(t[0].w, t[1].w, t[2].w, t[3].w);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) d[j] = four(w + j * p.wr, p.wk, k, j < nk, wvec);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[4 * i + j] = fmaf(a[i].x, d[j].x, fmaf(a[i].y, d[j].y,
+                                         fmaf(a[i].z, d[j].z, fmaf(a[i].w, d[j].w, acc[4 * i + j]))));
+            }
+            sum_halves<32>(acc, lane);
+            const int i = lane >> 2, j = lane & 3;
+            if (i < nr && j < nk) out[(row0 - m0 + i) * pitch + r0 + j] = s * acc[0];
         }
-    }
-    __syncthreads();
-    for (int row = warp; row < 32; row += 8) {
-        const int m = m0 + row;
-        const bool in = m >= lo && m < hi;
-        unsigned mx = 0;
-        if (in)
-            for (int r = lane; r < p.R; r += 32) mx = max(mx, finite_bits(out[row * pitch + r]));
-        mx = __reduce_max_sync(0xffffffffu, mx);
-        const float sc = pow2_scale(mx);
-        if (in && lane == 0) p.rinv[m] = pow2_inv(sc);
-        for (int r = lane; r < p.Rs; r += 32) {
-            const float v = in && r < p.R ? out[row * pitch + r] : 0.f;
-            __half2 h, l;
-            split_half2(v * sc, 0.f, h, l);
-            block[row * p.Rs + r] = __low2half(h);
-            block[row * p.Rs + r + p.plane] = __low2half(l);
-            if (in && p.compact) static_cast<float*>(p.compact)[(long long)m * p.Rs + r] = v;
+        __syncthreads();
+        for (int row = warp; row < 32; row += 8) {
+            const int m = m0 + row;
+            const bool in = m >= lo && m < hi;
+            unsigned mx = 0;
+            if (in)
+                for (int r = lane; r < p.R; r += 32)
+                    mx = max(mx, finite_bits(out[row * pitch + r]));
+            mx = __reduce_max_sync(0xffffffffu, mx);
+            const float sc = pow2_scale(mx);
+            if (in && lane == 0) p.rinv[m] = pow2_inv(sc);
+            for (int r = lane; r < p.Rs; r += 32) {
+                const float v = in && r < p.R ? out[row * pitch + r] : 0.f;
+                __half2 h, l;
+                split_half2(v * sc, 0.f, h, l);
+                block[row * p.Rs + r] = __low2half(h);
+                block[row * p.Rs + r + p.plane] = __low2half(l);
+                if (in && p.compact) static_cast<float*>(p.compact)[(long long)m * p.Rs + r] = v;
+            }
         }
+        __syncthreads();                 // out is free for the next 32 rows
     }
 }
 
@@ -562,7 +592,7 @@ struct AdSizes {
     int grad_split() const {
         const long long blocks = (long long)nad * (split ? (R + 31) / 32 : 1) *
                                  ((D + 127) / 128 + (O + 127) / 128);
-        const long long s = blocks ? 592 / blocks : 1;
+        const long long s = blocks ? 1184 / blocks : 1;
         return (int)std::max(1LL, std::min({s, 16LL, (long long)pieces}));
     }
 };
@@ -637,7 +667,7 @@ int shrink16(const Shrink& p, dim3 grid, Chain& st) {
     return ATOM_ERR_UNSUPPORTED;
 }
 int shrink(const Shrink& p, Chain& st) {
-    const dim3 grid(p.pieces + p.q.nad + 1, 8);
+    const dim3 grid(p.pieces + p.q.nad + 1, 256 / p.rb);
     if (p.dtype == ATOM_BF16) return shrink16<true>(p, grid, st);
     if (p.dtype == ATOM_F16) return shrink16<false>(p, grid, st);
     return st.launch("adapters: low-rank rows", shrink32_kernel, grid, 256, 32 * (p.R + 1) * 4, p);
@@ -717,6 +747,11 @@ struct Ad {
             memset(&h, 0, sizeof(h));
             h.q = q;
             h.pieces = z.pieces;
+            // Small blocks for large requests, but no more than eight blocks an SM: most of a small
+            // request's piece is zeros, and finding its rows costs a block some two microseconds
+            // (12,011 rows of 512 requests, fp32: 54 us with 4,800 blocks, SHRINKUS with 1,200).
+            for (h.rb = 32; h.rb < 256 && z.pieces * (256 / h.rb) > 8 * 148; h.rb *= 2) {
+            }
             h.rows = z.split ? rows : xr;
             h.ld = z.split ? ld : xld;
             h.K = K;
@@ -766,13 +801,13 @@ struct Ad {
                                  z.split ? z.Dp : wld, bwd ? 64 : c.bn / 2))
                 return s;
             if (!z.on) continue;
-            if (int s = make_map(&maps.m[2 * k + pl], at(sp.block, bplane), z.R,
-                                 (long long)z.pieces * 256, z.Rs, 128))
+            if (int s = make_slice_map(&maps.m[2 * k + pl], at(sp.block, bplane), z.R,
+                                       (long long)z.pieces * 256, z.Rs, 128, false, 0, 0))
                 return s;
             const long long sl = z.split ? sp_ld : sec_ld;
-            if (int s = make_map(&maps.m[3 * k + pl], at(z.split ? sp.ext : sec, planes[2]), scols,
-                                 bwd ? z.R : z.O, sl, bwd ? 64 : c.bn / 2, z.nad,
-                                 (bwd ? z.R : z.O) * sl))
+            if (int s = make_slice_map(&maps.m[3 * k + pl], at(z.split ? sp.ext : sec, planes[2]),
+                                       scols, bwd ? z.R : z.O, sl, c.bn / 2, bwd, z.nad,
+                                       (bwd ? z.R : z.O) * sl))
                 return s;
         }
         Args p;
@@ -789,12 +824,11 @@ struct Ad {
         p.cinv[0] = sp.wr;
         if (z.split && bwd) p.bmax = sp.max + 1;
         if (z.on) {
-            p.ext = (z.R + 63) / 64;
+            p.ext = (z.R + 15) / 16;
             p.ext_a = 2 * k, p.ext_b = 3 * k, p.ext_bmn = bwd ? 1 : 0;
             p.tile_req = sp.tile_req;
             p.piece = sp.piece;
             p.bad = sp.bad;
-            p.R = z.R;
             p.ext_rinv = sp.ext_rinv;
             p.ext_bmax = sp.max + 2;
         }

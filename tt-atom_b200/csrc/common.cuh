@@ -52,7 +52,7 @@ inline int check_launch(const char* what, int launches = 1) {
         if (_s != ATOM_OK) return _s;             \
     } while (0)
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+__host__ __device__ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

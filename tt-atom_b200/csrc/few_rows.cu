@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(256) few32_kernel(const __grid_constant__ Args
                                          fmaf(a.z, b[n].z, fmaf(a.w, b[n].w, acc[8 * i + n]))));
                 }
             }
-            sum_halves(acc, lane);
+            sum_halves<64>(acc, lane);
             *reinterpret_cast<float2*>(red + (warp * kMats + j) * 128 + m0 * 8 + 2 * lane) =
                 make_float2(acc[0], acc[1]);
         }

@@ -95,6 +95,16 @@ __device__ __forceinline__ uint64_t sdesc(uint32_t saddr, int mn) {
     d |= (uint64_t)2 << 61;
     return d;
 }
+// A low-rank slice, 16 deep: K-major rows of 32 bytes in 32-byte swizzle (8-row groups 256 bytes
+// apart), or M/N-major like a stage's but with 64-element blocks 2048 bytes apart.
+__device__ __forceinline__ uint64_t sdesc_slice(uint32_t saddr, int mn) {
+    uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFF);
+    d |= (uint64_t)(mn ? 2048 >> 4 : 1) << 16;
+    d |= (uint64_t)((mn ? 1024 : 256) >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)(mn ? 2 : 6) << 61;
+    return d;
+}
 // Instruction descriptor (kind::f16): D fp32, M = 256 over the pair, N = n.
 __device__ __forceinline__ uint32_t idesc(int n, int bf16, int a_mn, int b_mn) {
     return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_mn << 15) |
@@ -197,7 +207,8 @@ struct Share {
         end = p.ksplit == 1 ? nk : (int)((long long)(ti.ks + 1) * nk / p.ksplit);
     }
 };
-// Walks the low-rank blocks of a row tile (of the last K split's item), p.ext stages each.
+// Walks the low-rank blocks of a row tile (of the last K split's item) in slices of 16 ranks,
+// p.ext of them each; four slices of whatever blocks make a stage.
 struct Blocks {
     const Args& p;
     int mt, r = 0, end = 0, sub = 0, slot = -1;
@@ -328,8 +339,17 @@ __device__ __forceinline__ void spoil32(float* v) {
 }
 // The gate and its gradient. Sigmoids from ex2.approx and rcp.approx, each good to 2 units in the
 // last place; what the exponent's own rounding adds, |g| 2^-24, is far below the products' own
-// error of 5e-7. GELU's erfc is called, not expanded at each of a row's 32 values.
-__device__ __noinline__ float normal_cdf(float g) { return 0.5f * erfcf(-0.70710678f * g); }
+// error of 5e-7. GELU's normal distribution function from Abramowitz and Stegun's 7.1.26 (its
+// error at most 8e-8), whose exponential is the density that the derivative needs.
+__device__ __forceinline__ void normal(float g, float& cdf, float& bell) {
+    const float x = fabsf(g) * 0.70710678f;
+    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+    bell = __expf(-x * x);
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f),
+                                                1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * poly * bell;
+    cdf = g < 0.f ? tail : 1.f - tail;
+}
 // h = act(g) u
 __device__ __forceinline__ void gate32(float* g, const float* u, int act) {
     if (act == 0) {
@@ -340,7 +360,11 @@ __device__ __forceinline__ void gate32(float* g, const float* u, int act) {
         for (int i = 0; i < 32; ++i) g[i] = sigmoid_gate(g[i]) * u[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) g[i] = g[i] * normal_cdf(g[i]) * u[i];
+        for (int i = 0; i < 32; ++i) {
+            float c, bell;
+            normal(g[i], c, bell);
+            g[i] = g[i] * c * u[i];
+        }
     }
 }
 // (g, u, d = dh) -> (dg, du, h)
@@ -366,8 +390,10 @@ __device__ __forceinline__ void gate_bwd32(float* g, float* u, float* d, int act
     } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            const float c = normal_cdf(g[i]), x = g[i];
-            out(i, x * c, c + x * 0.39894228f * __expf(-0.5f * x * x));
+            const float x = g[i];
+            float c, bell;
+            normal(x, c, bell);
+            out(i, x * c, c + x * 0.39894228f * bell);
         }
     }
 }
@@ -477,12 +503,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             bool ok = true;
             const uint32_t full0 = peer_addr(smem_u32(full), 0);
             // waits for a free stage and names its barrier of CTA 0
-            auto open = [&](uint32_t& dst, uint32_t& bar) {
+            auto open = [&](uint32_t& dst, uint32_t& bar, uint32_t bytes = CF::kStage) {
                 const uint32_t s = slot;
                 if (!mbar_wait(&empty[s], turn ^ 1u, p.err)) return false;
                 if (rank == 0 && elect_one())
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
-                                     smem_u32(&full[s])), "r"(2 * CF::kStage) : "memory");
+                                     smem_u32(&full[s])), "r"(2 * bytes) : "memory");
                 dst = base + s * CF::kStage;
                 bar = full0 + s * 8;
                 ++it;
@@ -524,23 +550,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 if (!p.ext) continue;
                 Blocks st(p, ti);
-                for (; ok && st.any(); st.next()) {
+                while (ok && st.any()) {
                     uint32_t dst, bar;
-                    if (!(ok = open(dst, bar))) break;
-                    const int y = (ti.mt + st.r) * 256 + rank * 128, k0 = st.sub * 64;
+                    int n = 0;
+                    Blocks ahead = st;           // how many slices this stage gets
+                    for (; n < 4 && ahead.any(); ++n) ahead.next();
+                    if (!(ok = open(dst, bar, n * (CF::kStage / 4)))) break;
                     const int n0 = ti.nt * BN + rank * CF::HB;
-                    if (!elect_one()) continue;
+                    for (int i = 0; i < n; ++i, st.next()) {
+                        st.any();
+                        if (!elect_one()) continue;
+                        const int y = (ti.mt + st.r) * 256 + rank * 128, k0 = st.sub * 16;
 #pragma unroll
-                    for (int pl = 0; pl < P; ++pl) {
-                        tma_load(dst + pl * CF::kA, &maps.m[p.ext_a + pl], k0, y, bar);
-                        const uint32_t db = dst + P * CF::kA + pl * CF::kB;
-                        const CUtensorMap* mb = &maps.m[p.ext_b + pl];
-                        if (p.ext_bmn) {
+                        for (int pl = 0; pl < P; ++pl) {
+                            tma_load(dst + pl * CF::kA + i * (CF::kA / 4), &maps.m[p.ext_a + pl],
+                                     k0, y, bar);
+                            const uint32_t db = dst + P * CF::kA + pl * CF::kB + i * (CF::kB / 4);
+                            const CUtensorMap* mb = &maps.m[p.ext_b + pl];
+                            if (p.ext_bmn) {
 #pragma unroll
-                            for (int j = 0; j < CF::HB / 64; ++j)
-                                tma_load3(db + j * 8192, mb, n0 + 64 * j, k0, st.slot, bar);
-                        } else {
-                            tma_load3(db, mb, k0, n0, st.slot, bar);
+                                for (int j = 0; j < CF::HB / 64; ++j)
+                                    tma_load3(db + j * 2048, mb, n0 + 64 * j, k0, st.slot, bar);
+                            } else {
+                                tma_load3(db, mb, k0, n0, st.slot, bar);
+                            }
                         }
                     }
                 }
@@ -622,14 +655,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 if (SPLIT && ok && open) end(), next_low(), n = 0;
                 if (p.ext) {
-                    Blocks st(p, ti);
-                    const uint64_t b = (p.ext_bmn ? base_mn : base_k) + (P * CF::kA >> 4);
-                    const uint32_t bs = p.ext_bmn ? 2048 >> 4 : 32 >> 4;
+                    const uint64_t a = sdesc_slice(base, 0);
+                    const uint64_t b = sdesc_slice(base + P * CF::kA, p.ext_bmn);
                     const uint32_t id = idesc(BN, SPLIT ? 0 : p.bf16, 0, p.ext_bmn);
-                    for (; ok && st.any(); st.next(), ++n) {
+                    for (Blocks st(p, ti); ok && st.any(); ++n) {
+                        int k = 0;
+                        for (; k < 4 && st.any(); ++k) st.next();
                         if (SPLIT && open && n == kRound) end(), n = 0;
                         ok = (open || begin()) &&
-                             stage(base_k, b, 32 >> 4, bs, id, (min(64, p.R - 64 * st.sub) + 15) >> 4);
+                             stage(a, b, CF::kA >> 6, CF::kB >> 6, id, k);
                     }
                 }
                 if (ok && open) {
@@ -760,6 +794,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (p.ext) {
                     int es = 0;
                     for (Blocks st(p, ti); st.any(); st.next()) ++es;
+                    es = (es + 3) >> 2;
                     const float f = (m + lane < p.M ? p.ext_rinv[m + lane] : 0.f) *
                                     pow2_inv(pow2_scale(*p.ext_bmax));
                     if (!(ok = add((es + kRound - 1) / kRound, f))) break;
@@ -985,9 +1020,15 @@ static int encode_map(CUtensorMap* m, const void* p, bool f32, long long cols, l
     return ATOM_OK;
 }
 int make_map(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld,
-             int box_rows, int depth, long long ldz) {
-    return encode_map(m, p, false, cols, rows, depth, ld, ldz, 64, box_rows,
-                      CU_TENSOR_MAP_SWIZZLE_128B);
+             int box_rows) {
+    return encode_map(m, p, false, cols, rows, 0, ld, 0, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int make_slice_map(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld,
+                   int box_rows, bool mn, int depth, long long ldz) {
+    return mn ? encode_map(m, p, false, cols, rows, depth, ld, ldz, 64, 16,
+                           CU_TENSOR_MAP_SWIZZLE_128B)
+              : encode_map(m, p, false, cols, rows, depth, ld, ldz, 16, box_rows,
+                           CU_TENSOR_MAP_SWIZZLE_32B);
 }
 int make_out_map(CUtensorMap* m, const void* p, int dtype, long long cols, long long rows,
                  long long ld) {

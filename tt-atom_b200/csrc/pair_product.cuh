@@ -53,12 +53,11 @@ struct Args {
     const unsigned* bmax;    // B's tensor was scaled by this finite maximum (bits)
     // low-rank blocks beside the phases: block t + r holds the rows of request r in 256-row tile
     // t ([256][R] typed, zeros in other rows), multiplied by the request's adapter
-    int ext;                 // stages a request, 0: none
+    int ext;                 // 16-rank slices a request, 0: none
     int ext_a, ext_b, ext_bmn;
     const int2* tile_req;    // requests first .. last - 1 of a tile
     const int4* piece;       // of a block: adapter or -1 (left out), its rows
     const int4* bad;         // of an adapter: not all zero = not finite, its rows become NaN
-    int R;
     const float* ext_rinv;   // SPLIT: of the low-rank rows
     const unsigned* ext_bmax;
     int* err;
@@ -71,10 +70,14 @@ struct Choice {
 };
 Choice choose(long long M, int N, int nk, int groups, bool gated, bool split, bool may_split);
 
-// Tensor map of a 16-bit matrix [rows, cols] with rows ld elements apart (16-byte aligned), and
-// of `depth` of them `ldz` elements apart where depth > 0. Boxes of 64 x box_rows.
+// Tensor map of a 16-bit matrix [rows, cols] with rows ld elements apart (16-byte aligned); boxes
+// of 64 x box_rows.
 int make_map(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld,
-             int box_rows, int depth = 0, long long ldz = 0);
+             int box_rows);
+// The same for low-rank slices, of `depth` matrices `ldz` elements apart where depth > 0: boxes of
+// 16 x box_rows, or of 64 x 16 where K runs along the rows (mn).
+int make_slice_map(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld,
+                   int box_rows, bool mn, int depth, long long ldz);
 
 // Map of an output [rows, cols] that is written in blocks of 32 x 32.
 int make_out_map(CUtensorMap* m, const void* p, int dtype, long long cols, long long rows,

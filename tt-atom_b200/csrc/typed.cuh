@@ -65,10 +65,12 @@ __device__ __forceinline__ int last_le(int n, int key, V value) {
     return lo - 1;
 }
 
-// Adds 64 values over a warp: lane l ends with sums 2 l and 2 l + 1 in v[0], v[1].
+// Adds N values (64 or 32) over a warp by halves: lane l ends with sum l N / 32 and, of 64, the one
+// behind it in v[0], v[1].
+template <int N>
 __device__ __forceinline__ void sum_halves(float* v, int lane) {
 #pragma unroll
-    for (int o = 16, n = 32; o > 0; o >>= 1, n >>= 1) {
+    for (int o = 16, n = N / 2; o > 0; o >>= 1, n >>= 1) {
         const bool up = lane & o;
 #pragma unroll
         for (int i = 0; i < n; ++i) {
