@@ -18,8 +18,8 @@
 // (added there to nearest) every kRound stages: 8 additions, which holds an fp32 result near 5e-7
 // of itself (2-norm) at any K; one accumulator at K = 1024 is 3.5e-6 off, 16 additions 9.7e-7.
 //
-// 320 threads: warp 0 TMA, warp 1 tensor memory and the products (CTA 0's issues for both), warps
-// 2..9 the epilogue. Every wait is bounded: on expiry the kernel records a code, lets copies in
+// Warp 0 has TMA, warp 1 tensor memory and the products (CTA 0's issues for both), warps 2.. the
+// epilogue. Every wait is bounded: on expiry the kernel records a code, lets copies in
 // flight land, frees its tensor memory and returns.
 #include <cudaTypedefs.h>
 
@@ -30,7 +30,6 @@
 namespace atom {
 namespace pair {
 
-constexpr int kThreads = 320;
 constexpr int kRound = 2;                            // stages between two drains of a SPLIT tile
 constexpr long long kWaitCycles = 2000000000LL;      // ~1 s
 
@@ -163,17 +162,21 @@ struct Tile {
 };
 // Work item -> tile. Eight row tiles by all column tiles at a time, so that the pairs at work
 // share both operands' tiles in L2.
-__device__ __forceinline__ Tile tile_of(const Args& p, long long t) {
+__device__ __forceinline__ Tile tile_of(const Args& p, long long item) {
     Tile ti;
-    ti.ks = (int)(t % p.ksplit);
-    int u = (int)(t / p.ksplit);
-    const int all = p.mtiles * p.groups, band = 8 * p.ntiles_n;
-    const int b = u / band, r = u - b * band;
-    const int high = min(8, all - b * 8);
-    ti.mt = b * 8 + r % high;
-    ti.nt = r / high;
-    ti.grp = ti.mt / p.mtiles;
-    ti.mt -= ti.grp * p.mtiles;
+    uint32_t u = (uint32_t)item;         // 32-bit: every warp divides here, tile by tile
+    ti.ks = 0;
+    if (p.ksplit > 1) {
+        ti.ks = u % (uint32_t)p.ksplit;
+        u /= (uint32_t)p.ksplit;
+    }
+    const uint32_t all = p.mtiles * p.groups, band = 8u * p.ntiles_n;
+    const uint32_t b = u / band, r = u - b * band;
+    const uint32_t high = min(8u, all - b * 8);
+    ti.nt = high == 8 ? r >> 3 : r / high;
+    ti.mt = b * 8 + r - ti.nt * high;
+    ti.grp = 0;
+    if (ti.mt >= p.mtiles) ti.grp = 1, ti.mt -= p.mtiles;
     return ti;
 }
 
@@ -235,15 +238,21 @@ struct Blocks {
     }
 };
 
-template <int BN, bool SPLIT>
+template <int BN, int EPI, bool SPLIT>
 struct Cfg {
+    // Epilogue warps: 16 for a wide gate, whose arithmetic is more than its products at small K
+    // (60,000 x 256 x 1024 bf16: 78 us with 8, GATE16 us with 16; two groups of 8 on alternate
+    // tiles hold accumulators longer, 80 us), at the cost of a stage's room; 8 elsewhere (plain
+    // tiles lose 4 % to the shorter ring).
+    static constexpr int EW = EPI == kGate && BN == 256 ? 16 : 8;
+    static constexpr int kThreads = 64 + 32 * EW;
     static constexpr int HB = BN / 2;
     static constexpr uint32_t kA = 128 * 128, kB = HB * 128;
     static constexpr uint32_t kStage = (SPLIT ? 2 : 1) * (kA + kB);
-    static constexpr int S = SPLIT ? 4 : (BN == 256 ? 6 : 8);
+    static constexpr int S = SPLIT ? 4 : (EW == 16 ? 160 : 192) * 1024 / kStage;
     // tensor memory: two accumulator buffers of BN columns, and SPLIT two for hi lo + lo hi
     static_assert((SPLIT ? 4 : 2) * BN <= 512, "tensor memory");
-    static constexpr uint32_t kOut = 8 * 4096;
+    static constexpr uint32_t kOut = EW * 4096;
     static constexpr uint32_t kSmem = S * kStage + kOut + 512 + 1024;
     static_assert(kSmem <= 232448, "shared memory");
 };
@@ -341,6 +350,16 @@ __device__ __forceinline__ void spoil32(float* v) {
 // last place; what the exponent's own rounding adds, |g| 2^-24, is far below the products' own
 // error of 5e-7. GELU's normal distribution function from Abramowitz and Stegun's 7.1.26 (its
 // error at most 8e-8), whose exponential is the density that the derivative needs.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ void normal(float g, float& cdf, float& bell) {
     const float x = fabsf(g) * 0.70710678f;
     const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
@@ -350,14 +369,27 @@ __device__ __forceinline__ void normal(float g, float& cdf, float& bell) {
     const float tail = 0.5f * poly * bell;
     cdf = g < 0.f ? tail : 1.f - tail;
 }
+// Two sigmoids with one reciprocal, 1 / (a b): a multiprocessor has 16 results of ex2 and rcp a
+// clock, and a gate needs both for every value. Exponentials stay below 2^60, where a sigmoid is
+// nothing beside its own rounding, so that a b is finite.
+__device__ __forceinline__ void sigmoid2(float g0, float g1, float& s0, float& s1) {
+    const float a = 1.f + exp2_fast(fminf(-1.4426950f * g0, 60.f));
+    const float b = 1.f + exp2_fast(fminf(-1.4426950f * g1, 60.f));
+    const float r = rcp_fast(a * b);
+    s0 = r * b;
+    s1 = r * a;
+}
 // h = act(g) u
 __device__ __forceinline__ void gate32(float* g, const float* u, int act) {
-    if (act == 0) {
+    if (act < 2) {
+        const bool silu = act == 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid_gate(g[i]) * u[i];
-    } else if (act == 1) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) g[i] = sigmoid_gate(g[i]) * u[i];
+        for (int i = 0; i < 32; i += 2) {
+            float s0, s1;
+            sigmoid2(g[i], g[i + 1], s0, s1);
+            g[i] = (silu ? g[i] : 1.f) * s0 * u[i];
+            g[i + 1] = (silu ? g[i + 1] : 1.f) * s1 * u[i + 1];
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
@@ -375,17 +407,12 @@ __device__ __forceinline__ void gate_bwd32(float* g, float* u, float* d, int act
         u[i] = d[i] * a;
         d[i] = a * x;
     };
-    if (act == 0) {
+    if (act < 2) {
+        const bool silu = act == 0;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            const float s = sigmoid_gate(g[i]);
-            out(i, g[i] * s, s * (1.f + g[i] * (1.f - s)));
-        }
-    } else if (act == 1) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const float s = sigmoid_gate(g[i]);
-            out(i, s, s * (1.f - s));
+            const float x = g[i], s = sigmoid_gate(x), ds = s * (1.f - s);
+            out(i, silu ? x * s : s, silu ? fmaf(x, ds, s) : ds);
         }
     } else {
 #pragma unroll
@@ -447,9 +474,9 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
 }
 
 template <int BN, int EPI, bool SPLIT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>::kThreads, 1)
     pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
-    using CF = Cfg<BN, SPLIT>;
+    using CF = Cfg<BN, EPI, SPLIT>;
     constexpr int S = CF::S, P = SPLIT ? 2 : 1;      // stages, planes
     // a gate's tile: columns 0 .. BN/2 of the accumulator are g, the others u
     constexpr bool GATED = EPI == kGate || EPI == kGateBwdGU;
@@ -476,7 +503,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&accf[b], 1);
-            mbar_init(&acce[b], 16);
+            mbar_init(&acce[b], 2 * CF::EW);
         }
         *failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -674,7 +701,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (!ok) *(volatile int*)failed = 1;
         }
     } else {
-        const int q = warp & 3, half = (warp - 2) >> 2;
+        const int q = warp & 3, part = (warp - 2) >> 2;     // rows' quarter, columns' share
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         uint32_t round = 0;
         const uint32_t acce0 = peer_addr(smem_u32(acce), 0);
@@ -695,8 +722,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             return ok;
         };
         // first column of this warp's k-th 32-column chunk (of g, for a gate; u: BN/2 further)
-        constexpr int kChunks = (GATED ? BN / 4 : BN / 2) / 32;
-        const int c0 = half * kChunks * 32;
+        constexpr int kChunks = (GATED ? BN / 2 : BN) / (CF::EW / 4) / 32;
+        const int c0 = part * kChunks * 32;
         bool ok = true;
         Out out{outbuf + (warp - 2) * 4096, 0};
         constexpr int kParts = GATED ? 2 * kChunks : kChunks;
@@ -1079,7 +1106,7 @@ Choice choose(long long M, int N, int nk, int groups, bool gated, bool split, bo
 
 template <int BN, int EPI, bool SPLIT>
 static int run(const Maps& maps, const Args& p, Chain& st) {
-    using CF = Cfg<BN, SPLIT>;
+    using CF = Cfg<BN, EPI, SPLIT>;
     static std::atomic<bool> set[64];
     int dev = 0;
     cudaGetDevice(&dev);
@@ -1096,7 +1123,7 @@ static int run(const Maps& maps, const Args& p, Chain& st) {
     }
     const long long pairs = sm_count() / 2;
     const int grid = 2 * (int)(p.tiles < pairs ? p.tiles : pairs);
-    if (int s = st.launch("pair product", pair_kernel<BN, EPI, SPLIT>, dim3(grid), kThreads,
+    if (int s = st.launch("pair product", pair_kernel<BN, EPI, SPLIT>, dim3(grid), CF::kThreads,
                           CF::kSmem, maps, p))
         return s;
     if (p.ksplit > 1) {
