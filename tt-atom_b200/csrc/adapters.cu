@@ -592,7 +592,7 @@ struct AdSizes {
     int grad_split() const {
         const long long blocks = (long long)nad * (split ? (R + 31) / 32 : 1) *
                                  ((D + 127) / 128 + (O + 127) / 128);
-        const long long s = blocks ? 1184 / blocks : 1;
+        const long long s = blocks ? (split ? 592 : 1184) / blocks : 1;
         return (int)std::max(1LL, std::min({s, 16LL, (long long)pieces}));
     }
 };
@@ -747,10 +747,12 @@ struct Ad {
             memset(&h, 0, sizeof(h));
             h.q = q;
             h.pieces = z.pieces;
-            // Small blocks for large requests, but no more than eight blocks an SM: most of a small
-            // request's piece is zeros, and finding its rows costs a block some two microseconds
-            // (12,011 rows of 512 requests, fp32: 54 us with 4,800 blocks, SHRINKUS with 1,200).
-            for (h.rb = 32; h.rb < 256 && z.pieces * (256 / h.rb) > 8 * 148; h.rb *= 2) {
+            // Small blocks for large requests, but no more than eight blocks an SM (fp32, whose blocks
+            // are larger: two): most of a small request's piece is zeros, and finding its rows costs
+            // a block some two microseconds (12,011 rows of 512 requests, fp32: 54 us with 4,800
+            // blocks, 25 us with 1,200, SHRINKUS us with 600).
+            for (h.rb = 32; h.rb < 256 && z.pieces * (256 / h.rb) > (z.split ? 2 : 8) * 148;
+                 h.rb *= 2) {
             }
             h.rows = z.split ? rows : xr;
             h.ld = z.split ? ld : xld;

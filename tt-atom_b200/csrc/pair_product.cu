@@ -241,7 +241,7 @@ struct Blocks {
 template <int BN, int EPI, bool SPLIT>
 struct Cfg {
     // Epilogue warps: 16 for a wide gate, whose arithmetic is more than its products at small K
-    // (60,000 x 256 x 1024 bf16: 78 us with 8, GATE16 us with 16; two groups of 8 on alternate
+    // (60,000 x 256 x 1024 bf16: 78 us with 8, 69 us with 16; two groups of 8 on alternate
     // tiles hold accumulators longer, 80 us), at the cost of a stage's room; 8 elsewhere (plain
     // tiles lose 4 % to the shorter ring).
     static constexpr int EW = EPI == kGate && BN == 256 ? 16 : 8;
@@ -880,133 +880,234 @@ __global__ void __launch_bounds__(256) reduce_kernel(Args p) {
     }
 }
 
+// Operand preparation. A warp has eight float4 a lane: one row of up to 1024 columns, or two, four
+// or eight narrower ones, so that narrow rows keep as much in flight; wider rows take a block. Rows
+// stay in registers between their maximum and their planes (up to 8192 columns) and are read once.
+// Planes and packed rows are zero past the row's end up to the pitch. Bound by memory: the two
+// halves of a value cost five instructions, since what is not finite needs no care (its results are
+// not finite either way) except that a maximum leaves it out.
+constexpr int kNV = 8;
+__host__ __device__ inline int prep_slots(const PrepItem& it) {      // float4 a lane of one row
+    const long long c = it.dld > it.cols ? it.dld : it.cols;
+    return c <= 128 ? 1 : c <= 256 ? 2 : c <= 512 ? 4 : 8;
+}
 __host__ __device__ inline bool prep_wide(const PrepItem& it) {
     return it.dld > 1024 || it.cols > 1024;
 }
-// A warp a row, or a block where rows are wider than 1024; NV float4 a thread hold a row between
-// its maximum and its planes, so it is read once (up to 8192 columns). Planes and packed rows are
-// zero past the row's end up to the pitch. Bound by memory: the two halves of a value cost five
-// instructions, since what is not finite needs no care (its results are not finite either way)
-// except that a maximum leaves it out.
-template <int NV>
-__global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ PrepList l) {
-    let_next_start();
-    wait_before();
-    const PrepItem& it = l.it[blockIdx.y];
-    __shared__ float part[8];
+__device__ __forceinline__ float4 prep_load(const float* src, int c, int cols, bool four) {
+    if (four) return c < cols ? *reinterpret_cast<const float4*>(src + c)
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
+    return make_float4(c < cols ? src[c] : 0.f, c + 1 < cols ? src[c + 1] : 0.f,
+                       c + 2 < cols ? src[c + 2] : 0.f, c + 3 < cols ? src[c + 3] : 0.f);
+}
+__device__ __forceinline__ void prep_put(__half* hi, long long plane, const float4& v, float s) {
+    __half2 h[2], g[2];
+    split_half2(v.x * s, v.y * s, h[0], g[0]);
+    split_half2(v.z * s, v.w * s, h[1], g[1]);
+    *reinterpret_cast<uint2*>(hi) = *reinterpret_cast<uint2*>(h);
+    *reinterpret_cast<uint2*>(hi + plane) = *reinterpret_cast<uint2*>(g);
+}
+__device__ __forceinline__ float max_abs(float m, const float4& v) {      // passes over NaN
+    return fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+}
+__device__ __forceinline__ float max_finite(float m, const float4& v) {
+    return fmaxf(fmaxf(m, __uint_as_float(max(finite_bits(v.x), finite_bits(v.y)))),
+                 __uint_as_float(max(finite_bits(v.z), finite_bits(v.w))));
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// A row's scale from its maximum; its inverse and what goes into `max` on the way.
+__device__ __forceinline__ float row_scale(const PrepItem& it, long long r, float mx, bool writes,
+                                           float& top) {
+    const float s = pow2_scale(__float_as_uint(mx)), inv = mx > 0.f ? pow2_inv(s) : 0.f;
+    if (writes) it.rinv[r] = inv;
+    if (it.weight) top = fmaxf(top, fminf(inv * it.weight[r], 0x1p126f));
+    return s;
+}
+__device__ __forceinline__ float fixed_scale(const PrepItem& it, long long r) {
+    if (it.mode == kTensorSplit) return pow2_scale(*it.max);
+    // kWeighted; a row whose partner is zero may have any weight
+    return fminf(it.weight[r] * pow2_inv(__uint_as_float(*it.max)), 0x1p126f);
+}
+
+__device__ __forceinline__ void prep_narrow(const PrepItem& it, float& top) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const bool wide = prep_wide(it);
-    const int threads = wide ? 256 : 32, me = wide ? threadIdx.x : lane;
-    const long long step = wide ? gridDim.x : gridDim.x * 8LL;
-    const int mode = it.mode;
-    const long long cols = it.cols, dld = it.dld;
-    float top = 0.f;
-    for (long long r = wide ? blockIdx.x : blockIdx.x * 8LL + warp; r < it.rows; r += step) {
-        if (mode == kPack) {
-            const unsigned short* src = static_cast<const unsigned short*>(it.src) + r * it.ld;
-            unsigned short* dst = static_cast<unsigned short*>(it.dst) + r * dld;
-            for (long long c0 = 0; c0 < dld; c0 += 8LL * threads) {
-                // eight single loads in flight, then eight stores
-                unsigned short v[8];
+    const int nv = prep_slots(it), rows = kNV / nv, shift = 31 - __clz(nv);
+    const int cols = (int)it.cols, dld = (int)it.dld, mode = it.mode;
+    const bool scans = mode == kRowSplit || mode == kMax || mode == kRowScale;
+    for (long long r0 = (blockIdx.x * 8LL + warp) * rows; r0 < it.rows; r0 += gridDim.x * 8LL * rows) {
+        float4 x[kNV];
+        const float* src = static_cast<const float*>(it.src) + r0 * it.ld;
+        const bool four = aligned16(it.src) && it.ld % 4 == 0 && cols % 4 == 0;
+        // slot j: row r0 + j / nv, columns 4 (j % nv * 32 + lane) ..
+        if (four) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const long long c = c0 + j * threads + me;
-                    v[j] = c < cols ? src[c] : 0;
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const long long c = c0 + j * threads + me;
-                    if (c < dld) dst[c] = v[j];
-                }
+            for (int j = 0; j < kNV; ++j) {
+                const int i = j >> shift, c = (((j & (nv - 1)) << 5) + lane) * 4;
+                x[j] = r0 + i < it.rows && c < cols
+                           ? *reinterpret_cast<const float4*>(src + i * it.ld + c)
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            continue;
-        }
-        const float* src = static_cast<const float*>(it.src) + r * it.ld;
-        const bool four = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && cols % 4 == 0;
-        auto load = [&](long long c) {
-            if (four) return c < cols ? *reinterpret_cast<const float4*>(src + c)
-                                      : make_float4(0.f, 0.f, 0.f, 0.f);
-            return make_float4(c < cols ? src[c] : 0.f, c + 1 < cols ? src[c + 1] : 0.f,
-                               c + 2 < cols ? src[c + 2] : 0.f, c + 3 < cols ? src[c + 3] : 0.f);
-        };
-        float4 x[NV];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) x[j] = load(4LL * (j * threads + me));
-        float s = 1.f;
-        const long long held = 4LL * NV * threads;
-        if (mode == kTensorSplit) {
-            s = pow2_scale(*it.max);
-        } else if (mode == kWeighted) {
-            // a row whose partner is zero may have any weight
-            s = fminf(it.weight[r] * pow2_inv(__uint_as_float(*it.max)), 0x1p126f);
         } else {
+#pragma unroll
+            for (int j = 0; j < kNV; ++j) {
+                const int i = j >> shift, c = (((j & (nv - 1)) << 5) + lane) * 4;
+                x[j] = prep_load(src + i * it.ld, c, r0 + i < it.rows ? cols : 0, false);
+            }
+        }
+        float m[kNV];
+        if (scans) {
+            bool wild = false;
+#pragma unroll
+            for (int j = 0; j < kNV; ++j) {
+                m[j] = max_abs(0.f, x[j]);
+                wild |= isinf(m[j]);
+            }
+            if (__any_sync(0xffffffffu, wild))
+#pragma unroll
+                for (int j = 0; j < kNV; ++j) m[j] = max_finite(0.f, x[j]);
+            // over a row's slots, then over the lanes
+#pragma unroll
+            for (int o = 1; o < kNV; o *= 2)
+                if (o < nv)
+#pragma unroll
+                    for (int j = 0; j < kNV; ++j)
+                        if (!(j & o)) m[j] = m[j | o] = fmaxf(m[j], m[j | o]);
+#pragma unroll
+            for (int j = 0; j < kNV; ++j)
+                if ((j & (nv - 1)) == 0) m[j] = warp_max(m[j]);
+#pragma unroll
+            for (int o = kNV / 2; o > 0; o /= 2)
+                if (o < nv)
+#pragma unroll
+                    for (int j = 0; j < kNV; ++j)
+                        if ((j & (2 * o - 1)) == o) m[j] = m[j ^ o];
+            if (mode == kMax) {
+#pragma unroll
+                for (int j = 0; j < kNV; ++j) top = fmaxf(top, m[j]);
+                continue;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kNV; ++j) {
+            const int i = j >> shift, k = j & (nv - 1), c = ((k << 5) + lane) * 4;
+            const long long r = r0 + i;
+            if (r >= it.rows) continue;
+            const float s = scans ? row_scale(it, r, m[j], k == 0 && lane == 0, top)
+                                  : fixed_scale(it, r);
+            if (mode != kRowScale && c < dld)
+                prep_put(static_cast<__half*>(it.dst) + r * dld + c, it.plane, x[j], s);
+        }
+    }
+}
+
+__device__ __forceinline__ void prep_block(const PrepItem& it, float* part, float& top) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = threadIdx.x;
+    const int cols = (int)it.cols, dld = (int)it.dld, mode = it.mode;
+    const bool scans = mode == kRowSplit || mode == kMax || mode == kRowScale;
+    for (long long r = blockIdx.x; r < it.rows; r += gridDim.x) {
+        const float* src = static_cast<const float*>(it.src) + r * it.ld;
+        const bool four = aligned16(src) && cols % 4 == 0;
+        float4 x[kNV];
+        if (four) {
+#pragma unroll
+            for (int j = 0; j < kNV; ++j) x[j] = prep_load(src, 4 * (j * 256 + me), cols, true);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kNV; ++j) x[j] = prep_load(src, 4 * (j * 256 + me), cols, false);
+        }
+        const int held = 4 * kNV * 256;
+        float s;
+        if (scans) {
             float mx = 0.f;
-            auto see = [&](const float4& v) {       // fmaxf passes over NaN
-                mx = fmaxf(fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-            };
-            auto see_finite = [&](const float4& v) {
-                for (float y : {v.x, v.y, v.z, v.w}) mx = fmaxf(mx, __uint_as_float(finite_bits(y)));
-            };
-            auto all = [&](auto f) {
+            for (int pass = 0; pass < 2; ++pass) {
                 mx = 0.f;
 #pragma unroll
-                for (int j = 0; j < NV; ++j) f(x[j]);
-                for (long long c = held + 4 * me; c < cols; c += 4 * threads) f(load(c));
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                if (wide) {
-                    __syncthreads();
-                    if (lane == 0) part[warp] = mx;
-                    __syncthreads();
-                    for (int k = 0; k < 8; ++k) mx = fmaxf(mx, part[k]);
+                for (int j = 0; j < kNV; ++j) mx = pass ? max_finite(mx, x[j]) : max_abs(mx, x[j]);
+                for (int c = held + 4 * me; c < cols; c += 1024) {
+                    const float4 v = prep_load(src, c, cols, four);
+                    mx = pass ? max_finite(mx, v) : max_abs(mx, v);
                 }
-            };
-            all(see);
-            if (isinf(mx)) all(see_finite);
+                mx = warp_max(mx);
+                __syncthreads();
+                if (lane == 0) part[warp] = mx;
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mx = fmaxf(mx, part[k]);
+                if (!isinf(mx)) break;
+            }
             if (mode == kMax) {
                 top = fmaxf(top, mx);
                 continue;
             }
-            s = pow2_scale(__float_as_uint(mx));
-            const float inv = mx > 0.f ? pow2_inv(s) : 0.f;
-            if (me == 0) it.rinv[r] = inv;
-            if (it.weight) top = fmaxf(top, fminf(inv * it.weight[r], 0x1p126f));
+            s = row_scale(it, r, mx, me == 0, top);
             if (mode == kRowScale) continue;
+        } else {
+            s = fixed_scale(it, r);
         }
         __half* hi = static_cast<__half*>(it.dst) + r * dld;
-        auto put = [&](long long c, const float4& v) {
-            __half2 h[2], g[2];
-            split_half2(v.x * s, v.y * s, h[0], g[0]);
-            split_half2(v.z * s, v.w * s, h[1], g[1]);
-            *reinterpret_cast<uint2*>(hi + c) = *reinterpret_cast<uint2*>(h);
-            *reinterpret_cast<uint2*>(hi + it.plane + c) = *reinterpret_cast<uint2*>(g);
-        };
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (4LL * (j * threads + me) < dld) put(4LL * (j * threads + me), x[j]);
-        for (long long c = held + 4 * me; c < dld; c += 4 * threads) put(c, load(c));
+        for (int j = 0; j < kNV; ++j) {
+            const int c = 4 * (j * 256 + me);
+            if (c < dld) prep_put(hi + c, it.plane, x[j], s);
+        }
+        for (int c = held + 4 * me; c < dld; c += 1024)
+            prep_put(hi + c, it.plane, prep_load(src, c, cols, four), s);
     }
+}
+
+// 16-bit rows to an aligned pitch; eight single loads in flight, then eight stores.
+__device__ __forceinline__ void prep_pack(const PrepItem& it) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int cols = (int)it.cols, dld = (int)it.dld;
+    for (long long r = blockIdx.x * 8LL + warp; r < it.rows; r += gridDim.x * 8LL) {
+        const unsigned short* src = static_cast<const unsigned short*>(it.src) + r * it.ld;
+        unsigned short* dst = static_cast<unsigned short*>(it.dst) + r * dld;
+        for (int c0 = 0; c0 < dld; c0 += 256) {
+            unsigned short v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = c0 + j * 32 + lane < cols ? src[c0 + j * 32 + lane] : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c0 + j * 32 + lane < dld) dst[c0 + j * 32 + lane] = v[j];
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256, 3) prep_kernel(const __grid_constant__ PrepList l) {
+    __shared__ float part[8];
+    let_next_start();
+    wait_before();
+    const PrepItem& it = l.it[blockIdx.y];
+    const int lane = threadIdx.x & 31;
+    float top = 0.f;
+    if (it.mode == kPack) prep_pack(it);
+    else if (prep_wide(it)) prep_block(it, part, top);
+    else prep_narrow(it, top);
     // the epilogue reads scales of columns 32 at a time
-    if (mode == kRowSplit && blockIdx.x == 0 && threadIdx.x < 32 && it.rows + lane < (it.rows + 31) / 32 * 32)
+    if (it.mode == kRowSplit && blockIdx.x == 0 && threadIdx.x < 32 &&
+        it.rows + lane < (it.rows + 31) / 32 * 32)
         it.rinv[it.rows + lane] = 0.f;
-    if (it.max && (mode == kMax || mode == kRowSplit) && lane == 0 && top > 0.f)
-        atomicMax(it.max, __float_as_uint(top));
+    if (it.max && (it.mode == kMax || it.mode == kRowSplit)) {
+        top = warp_max(top);
+        if (lane == 0 && top > 0.f) atomicMax(it.max, __float_as_uint(top));
+    }
 }
 
 int prepare(const PrepList& l, Chain& st) {
     if (l.n == 0) return ATOM_OK;
-    long long rows = 1, nv = 1;
+    long long blocks = 1;
     for (int i = 0; i < l.n; ++i) {
         const PrepItem& it = l.it[i];
-        const bool wide = prep_wide(it);
-        rows = std::max(rows, wide ? 8 * it.rows : it.rows);
-        if (it.mode != kPack)
-            nv = std::max(nv, (std::max(it.dld, it.cols) + (wide ? 1023 : 127)) / (wide ? 1024 : 128));
+        const int rows = it.mode == kPack ? 8 : prep_wide(it) ? 1 : 8 * (kNV / prep_slots(it));
+        blocks = std::max(blocks, (it.rows + rows - 1) / rows);
     }
-    const long long blocks = (rows + 7) / 8;
-    const dim3 grid((unsigned)std::min(blocks, 2368LL), l.n);
-    return st.launch("operand preparation", nv <= 1 ? prep_kernel<1> : nv <= 2 ? prep_kernel<2>
-                     : nv <= 4 ? prep_kernel<4> : prep_kernel<8>, grid, 256, 0, l);
+    return st.launch("operand preparation", prep_kernel,
+                     dim3((unsigned)std::min(blocks, 2368LL), l.n), 256, 0, l);
 }
 
 static PFN_cuTensorMapEncodeTiled_v12000 encoder() {
