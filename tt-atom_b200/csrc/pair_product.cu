@@ -27,6 +27,8 @@
 
 #include "pair_product.cuh"
 
+#pragma nv_diag_suppress 128      // loops that an instantiation has no way to
+
 namespace atom {
 namespace pair {
 
@@ -102,6 +104,16 @@ __device__ __forceinline__ uint64_t sdesc_slice(uint32_t saddr, int mn) {
     d |= (uint64_t)((mn ? 1024 : 256) >> 4) << 32;
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)(mn ? 2 : 6) << 61;
+    return d;
+}
+// kLow's M/N-major slices: 64 rows of 32 bytes in 32-byte swizzle, 16-element blocks 2048 bytes
+// apart, 8-deep groups 256 bytes apart.
+__device__ __forceinline__ uint64_t sdesc_low(uint32_t saddr) {
+    uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFF);
+    d |= (uint64_t)(2048 >> 4) << 16;
+    d |= (uint64_t)(256 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)6 << 61;
     return d;
 }
 // Instruction descriptor (kind::f16): D fp32, M = 256 over the pair, N = n.
@@ -185,12 +197,12 @@ __device__ __forceinline__ bool is_finite(const Args& p, int slot) {
     return (b.x | b.y | b.z | b.w) == 0;
 }
 // Whether row m (a lane's) belongs to a request whose adapter is not finite.
-__device__ __forceinline__ bool spoilt_row(const Args& p, const Tile& ti, long long m, int lane) {
-    const int2 q = p.tile_req[ti.mt];
+__device__ __noinline__ bool spoilt_row(const Args& p, int mt, long long m, int lane) {
+    const int4 q = p.tile_req[mt];
     bool bad = false;
     for (int r = q.x; r < q.y; r += 32) {
         int4 c = make_int4(-1, 0, 0, 0);
-        if (r + lane < q.y) c = p.piece[ti.mt + r + lane];
+        if (r + lane < q.y) c = p.piece[mt + r + lane];
         unsigned found = __ballot_sync(0xffffffffu, c.x >= 0 && !is_finite(p, c.x));
         for (; found; found &= found - 1) {
             const int i = __ffs(found) - 1;
@@ -201,6 +213,22 @@ __device__ __forceinline__ bool spoilt_row(const Args& p, const Tile& ti, long l
     return bad;
 }
 
+// What a warp knows of its tiles' requests: a lane a tile, 32 tiles ahead, so that no tile waits
+// for its own (a load takes two microseconds beside the tiles' traffic).
+struct Ahead {
+    int4 mine;
+    __device__ __forceinline__ int4 get(const Args& p, uint32_t k, uint32_t first, uint32_t pairs) {
+        if ((k & 31) == 0) {
+            const long long t = first + (long long)(k + (threadIdx.x & 31)) * pairs;
+            mine = make_int4(0, 0, 0, 0);
+            if (t < p.tiles) mine = p.tile_req[tile_of(p, t).mt];
+        }
+        const int l = k & 31;
+        return make_int4(__shfl_sync(0xffffffffu, mine.x, l), __shfl_sync(0xffffffffu, mine.y, l),
+                         __shfl_sync(0xffffffffu, mine.z, l), __shfl_sync(0xffffffffu, mine.w, l));
+    }
+};
+
 // A work item's K stages of one phase.
 struct Share {
     int kt, end;
@@ -210,31 +238,123 @@ struct Share {
         end = p.ksplit == 1 ? nk : (int)((long long)(ti.ks + 1) * nk / p.ksplit);
     }
 };
-// Walks the low-rank blocks of a row tile (of the last K split's item) in slices of 16 ranks,
-// p.ext of them each; four slices of whatever blocks make a stage.
+// Walks the low-rank blocks of a row tile in slices of 16 ranks, p.ext of them each; four slices of
+// whatever blocks make a stage. The adapters of the first 32 requests, one a lane, are asked for
+// when the walk is made and needed when it begins.
 struct Blocks {
     const Args& p;
-    int mt, r = 0, end = 0, sub = 0, slot = -1;
-    __device__ __forceinline__ Blocks(const Args& q, const Tile& ti) : p(q), mt(ti.mt) {
-        if (ti.ks == p.ksplit - 1) {
-            const int2 t = p.tile_req[mt];
-            r = t.x;
-            end = t.y;
-        }
+    int mt, base, behind, mine, left_in = -1, sub = 0, r = 0, slot = 0;
+    unsigned left = 0;
+    __device__ __forceinline__ Blocks(const Args& q, int tile, const int4& t)
+        : p(q), mt(tile), base(t.x), behind(t.z ? t.y : t.x) {
+        ask();
     }
-    __device__ __forceinline__ bool any() {
-        if (sub > 0) return true;                       // in the middle of a block
-        for (; r < end; ++r) {
-            slot = p.piece[mt + r].x;
-            if (slot >= 0 && is_finite(p, slot)) return true;
-        }
-        return false;
+    __device__ __forceinline__ void ask() {
+        const int i = base + (threadIdx.x & 31);
+        mine = i < behind ? p.usable[mt + i] : -1;
     }
-    __device__ __forceinline__ void next() {
-        if (++sub == p.ext) {
-            sub = 0;
-            ++r;
+    // the next slice (r, at(), slot); false when there is none
+    __device__ __forceinline__ bool next() {
+        if (sub > 0 && sub < p.ext) {
+            ++sub;
+            return true;
         }
+        if (left_in != base) left = __ballot_sync(0xffffffffu, mine >= 0), left_in = base;
+        while (left == 0) {
+            if (base + 32 >= behind) return false;
+            base += 32;
+            ask();
+            left = __ballot_sync(0xffffffffu, mine >= 0);
+            left_in = base;
+        }
+        const int i = __ffs(left) - 1;
+        left &= left - 1;
+        r = base + i;
+        slot = __shfl_sync(0xffffffffu, mine, i);
+        sub = 1;
+        return true;
+    }
+    __device__ __forceinline__ int at() const { return (sub - 1) * 16; }     // first rank
+};
+
+// A row tile's pieces, 32 requests at a time, one a lane. Whole warps.
+struct Window {
+    const Args& p;
+    int mt, first, behind, base = 0;
+    int4 c;                  // this lane's piece
+    unsigned mask = 0;       // the lanes whose piece has an adapter
+    __device__ __forceinline__ Window(const Args& q, int tile) : p(q), mt(tile) {
+        const int4 t = p.tile_req[mt];
+        first = t.x;
+        behind = t.y;
+        look(first);
+    }
+    __device__ __forceinline__ void look(int r) {
+        base = r;
+        const int i = r + (threadIdx.x & 31);
+        c = i < behind ? p.piece[mt + i] : make_int4(-1, 0, 0, 0);
+        mask = __ballot_sync(0xffffffffu, c.x >= 0);
+    }
+    __device__ __forceinline__ int count() {         // of all requests; ends on the first again
+        int n = __popc(mask);
+        if (behind - first > 32) {
+            for (int r = first + 32; r < behind; r += 32) {
+                look(r);
+                n += __popc(mask);
+            }
+            look(first);
+        }
+        return n;
+    }
+    // writes down which pieces the product beside the projection takes
+    __device__ __forceinline__ void settle() {
+        int n = 0, spoilt = 0;
+        for (int r = first; r < behind; r += 32) {
+            look(r);
+            const bool ok = c.x >= 0 && is_finite(p, c.x);
+            n += __popc(__ballot_sync(0xffffffffu, ok));
+            spoilt |= __ballot_sync(0xffffffffu, c.x >= 0 && !ok) != 0;
+            const int i = r + (threadIdx.x & 31);
+            if (i < behind) p.usable[mt + i] = ok ? c.x : -1;
+        }
+        if ((threadIdx.x & 31) == 0) {
+            p.tile_req[mt].z = n;
+            p.tile_req[mt].w = spoilt;
+        }
+        look(first);
+    }
+};
+
+// kLow: groups of a row tile's pieces whose slices of 16 ranks fill 128 columns (a piece's slices
+// stay together); with few row tiles, `ksplit` work items share a tile's groups.
+struct Low {
+    Window w;
+    int count, slices, each, before = 0;         // pieces; slices a piece; pieces a group
+    __device__ __forceinline__ Low(const Args& p, int tile) : w(p, tile) {
+        slices = p.ext;
+        each = 8 / slices;
+        count = w.count();
+    }
+    __device__ __forceinline__ int groups() const { return (count + each - 1) / each; }
+    __device__ __forceinline__ int used(int g) const {          // slices of group g
+        return min(each, count - g * each) * slices;
+    }
+    // the piece of slice i of group g: its adapter and rows, and in w its request
+    __device__ __forceinline__ int4 piece(int g, int i) {
+        int j = g * each + i / slices;
+        if (j < before) {
+            before = 0;
+            w.look(w.first);
+        }
+        while (j >= before + __popc(w.mask)) {
+            before += __popc(w.mask);
+            w.look(w.base + 32);
+        }
+        unsigned v = w.mask;
+        for (j -= before; j > 0; --j) v &= v - 1;
+        const int l = __ffs(v) - 1;
+        return make_int4(__shfl_sync(0xffffffffu, w.c.x, l), __shfl_sync(0xffffffffu, w.c.y, l),
+                         __shfl_sync(0xffffffffu, w.c.z, l), w.base + l);
     }
 };
 
@@ -473,6 +593,46 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
     }
 }
 
+// kLow: a lane's row of the four slices that a warp has of group g, times the adapter's scale and f:
+// into the pieces' blocks (zeros outside a piece's rows), and into the rows' own places.
+__device__ __forceinline__ void low_store(const Args& p, Low& low, int g, int part,
+                                          long long m0, int lane, float (*v)[32], float f) {
+    const int used = low.used(g);
+    const long long m = m0 + lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int slice = part * 4 + i;
+        if (slice >= used) break;
+        const int4 piece = low.piece(g, slice);
+        const int c0 = slice % p.ext * 16;
+        const bool in = m >= piece.y && m < piece.z;
+        const float s = p.low_scale[piece.x] * f;
+        float* x = v[i >> 1] + (i & 1) * 16;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = in ? x[j] * s : 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {                // eight ranks at a time: Rs is a multiple of 8
+            const int c = c0 + 8 * h;
+            if (c >= p.Rs) break;
+            const float* y = x + 8 * h;
+            if (p.dtype == ATOM_F32) {
+                float* q = static_cast<float*>(p.low_rows) + m * p.Rs + c;
+                if (in) {
+                    *reinterpret_cast<float4*>(q) = make_float4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<float4*>(q + 4) = make_float4(y[4], y[5], y[6], y[7]);
+                }
+                continue;
+            }
+            const uint4 w = make_uint4(pack2(y[0], y[1], p.dtype), pack2(y[2], y[3], p.dtype),
+                                       pack2(y[4], y[5], p.dtype), pack2(y[6], y[7], p.dtype));
+            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.low_block) +
+                                      ((long long)(low.w.mt + piece.w) * 256 + (m & 255)) * p.Rs + c) = w;
+            if (p.low_rows && in)
+                *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.low_rows) + m * p.Rs + c) = w;
+        }
+    }
+}
+
 template <int BN, int EPI, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>::kThreads, 1)
     pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
@@ -542,9 +702,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 if (++slot == S) slot = 0, turn ^= 1u;
                 return true;
             };
-            for (long long t = first; ok && t < p.tiles; t += pairs) {
+            Ahead ahead;
+            uint32_t mine_k = 0;
+            for (long long t = first; ok && t < p.tiles; t += pairs, ++mine_k) {
                 const Tile ti = tile_of(p, t);
                 const int m0 = ti.mt * 256 + rank * 128;
+                int4 req = make_int4(0, 0, 0, 0);
+                if (EPI == kStore && p.ext) {
+                    req = ahead.get(p, mine_k, first, pairs);
+                    if (ti.ks != p.ksplit - 1) req.z = 0;
+                }
+                Blocks st(p, ti.mt, req);
+                if constexpr (EPI == kLow) {
+                    Low low(p, ti.mt);
+                    const bool mn = p.ph[0].b_mn;
+                    for (int g = ti.ks; ok && g < low.groups(); g += p.ksplit) {
+                        const int n = low.used(g), mine = min(4, max(0, n - 4 * (int)rank));
+                        int slot[4], r16[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            slot[i] = i < mine ? low.piece(g, 4 * rank + i).x : 0;
+                            r16[i] = (4 * rank + i) % p.ext * 16;
+                        }
+                        for (int kt = 0; kt < p.ph[0].nk; ++kt) {
+                            uint32_t dst, bar;
+                            if (!(ok = open(dst, bar, P * (CF::kA + n * 1024)))) break;
+                            if (!elect_one()) continue;
+                            const int k0 = kt * 64;
+#pragma unroll
+                            for (int pl = 0; pl < P; ++pl) {
+                                tma_load(dst + pl * CF::kA, &maps.m[p.ph[0].a + pl], k0, m0, bar);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const uint32_t db = dst + P * CF::kA + pl * CF::kB + i * 2048;
+                                    if (i < mine)
+                                        tma_load3(db, &maps.m[p.ph[0].b0 + pl], mn ? r16[i] : k0,
+                                                  mn ? k0 : r16[i], slot[i], bar);
+                                }
+                            }
+                        }
+                    }
+                    continue;
+                }
                 for (int f = 0; ok && f < p.nphase; ++f) {
                     const Phase ph = p.ph[f];
                     const Share sh(p, ti, f);
@@ -576,18 +775,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     }
                 }
                 if (!p.ext) continue;
-                Blocks st(p, ti);
-                while (ok && st.any()) {
+                const int n0 = ti.nt * BN + rank * CF::HB;
+                while (ok) {
+                    int rs[4], slots[4], ks[4], n = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (n == i && st.next()) rs[i] = st.r, slots[i] = st.slot, ks[i] = st.at(), ++n;
                     uint32_t dst, bar;
-                    int n = 0;
-                    Blocks ahead = st;           // how many slices this stage gets
-                    for (; n < 4 && ahead.any(); ++n) ahead.next();
-                    if (!(ok = open(dst, bar, n * (CF::kStage / 4)))) break;
-                    const int n0 = ti.nt * BN + rank * CF::HB;
-                    for (int i = 0; i < n; ++i, st.next()) {
-                        st.any();
-                        if (!elect_one()) continue;
-                        const int y = (ti.mt + st.r) * 256 + rank * 128, k0 = st.sub * 16;
+                    if (n == 0 || !(ok = open(dst, bar, n * (CF::kStage / 4)))) break;
+                    if (!elect_one()) continue;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (i >= n) break;
+                        const int y = (ti.mt + rs[i]) * 256 + rank * 128, k0 = ks[i];
 #pragma unroll
                         for (int pl = 0; pl < P; ++pl) {
                             tma_load(dst + pl * CF::kA + i * (CF::kA / 4), &maps.m[p.ext_a + pl],
@@ -597,9 +797,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                             if (p.ext_bmn) {
 #pragma unroll
                                 for (int j = 0; j < CF::HB / 64; ++j)
-                                    tma_load3(db + j * 2048, mb, n0 + 64 * j, k0, st.slot, bar);
+                                    tma_load3(db + j * 2048, mb, n0 + 64 * j, k0, slots[i], bar);
                             } else {
-                                tma_load3(db, mb, k0, n0, st.slot, bar);
+                                tma_load3(db, mb, k0, n0, slots[i], bar);
                             }
                         }
                     }
@@ -665,9 +865,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 low = tmem + 2 * BN + (low == tmem + 2 * BN ? BN : 0);
                 low_fresh = 0;
             };
-            for (long long t = first; ok && t < p.tiles; t += pairs) {
+            Ahead ahead;
+            uint32_t mine_k = 0;
+            for (long long t = first; ok && t < p.tiles; t += pairs, ++mine_k) {
                 const Tile ti = tile_of(p, t);
-                int n = 0;
+                int n = 0, left = 0;
+                if (EPI == kStore && p.ext) {
+                    left = ahead.get(p, mine_k, first, pairs).z * p.ext;
+                    if (ti.ks != p.ksplit - 1) left = 0;
+                }
+                if constexpr (EPI == kLow) {
+                    const int groups = Low(p, ti.mt).groups(), mn = p.ph[0].b_mn;
+                    const uint64_t b = mn ? sdesc_low(base + P * CF::kA)
+                                          : base_k + (P * CF::kA >> 4);
+                    const uint32_t id = idesc(BN, SPLIT ? 0 : p.bf16, 0, mn);
+                    for (int g = ti.ks; ok && g < groups; g += p.ksplit) {
+                        for (int kt = 0; ok && kt < p.ph[0].nk; ++kt, ++n) {
+                            if (SPLIT && open && n == kRound) end(), n = 0;
+                            ok = (open || begin()) &&
+                                 stage(base_k, b, 32 >> 4, mn ? 512 >> 4 : 32 >> 4, id, 4);
+                        }
+                        if (ok) end(), n = 0;
+                        if (SPLIT) next_low();
+                    }
+                    continue;
+                }
                 for (int f = 0; ok && f < p.nphase; ++f) {
                     const int a_mn = p.ph[f].a_mn, b_mn = p.ph[f].b_mn;
                     const Share sh(p, ti, f);
@@ -685,12 +907,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     const uint64_t a = sdesc_slice(base, 0);
                     const uint64_t b = sdesc_slice(base + P * CF::kA, p.ext_bmn);
                     const uint32_t id = idesc(BN, SPLIT ? 0 : p.bf16, 0, p.ext_bmn);
-                    for (Blocks st(p, ti); ok && st.any(); ++n) {
-                        int k = 0;
-                        for (; k < 4 && st.any(); ++k) st.next();
+                    for (; ok && left > 0; left -= 4, ++n) {
                         if (SPLIT && open && n == kRound) end(), n = 0;
                         ok = (open || begin()) &&
-                             stage(a, b, CF::kA >> 6, CF::kB >> 6, id, k);
+                             stage(a, b, CF::kA >> 6, CF::kB >> 6, id, min(4, left));
                     }
                 }
                 if (ok && open) {
@@ -728,12 +948,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
         Out out{outbuf + (warp - 2) * 4096, 0};
         constexpr int kParts = GATED ? 2 * kChunks : kChunks;
         uint32_t low = 2 * BN;
-        for (long long t = first; ok && t < p.tiles; t += pairs) {
+        Ahead ahead;
+        uint32_t mine_k = 0;
+        for (long long t = first; ok && t < p.tiles; t += pairs, ++mine_k) {
             const Tile ti = tile_of(p, t);
             const long long m = (long long)ti.mt * 256 + rank * 128 + q * 32;
             const int nb = ti.nt * (GATED ? BN / 2 : BN) + c0;
-            const bool spoilt = EPI == kStore && p.ext && spoilt_row(p, ti, m + lane, lane);
-            if constexpr (!SPLIT) {
+            int4 req = make_int4(0, 0, 0, 0);
+            if (EPI == kStore && p.ext) req = ahead.get(p, mine_k, first, pairs);
+            const bool spoilt = EPI == kStore && req.w && spoilt_row(p, ti.mt, m + lane, lane);
+            if (EPI == kLow && warp == 2 && rank == 0 && ti.ks == 0 && p.usable)
+                Window(p, ti.mt).settle();
+            if constexpr (EPI == kLow && !SPLIT) {
+                Low low_(p, ti.mt);
+                for (int g = ti.ks; g < low_.groups(); g += p.ksplit) {
+                    if (!(ok = filled())) break;
+                    const uint32_t ta = tmem + lanes + (round & 1u) * BN + c0;
+                    float v[2][32];
+                    tmem_ld32(ta, v[0]);
+                    tmem_ld32(ta + 32, v[1]);
+                    tmem_wait_ld();
+                    pin32(v[0]);
+                    pin32(v[1]);
+                    drained();
+                    low_store(p, low_, g, part, m, lane, v, 1.f);
+                }
+            } else if constexpr (!SPLIT) {
                 if (!(ok = filled())) break;
                 const uint32_t ta = tmem + lanes + (round & 1u) * BN + c0;
 #pragma unroll 1
@@ -751,10 +991,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
             } else {
                 // the tile's rounds summed in registers
                 float v[kParts][32];
+                auto clear = [&]() {
 #pragma unroll
-                for (int k = 0; k < kParts; ++k)
+                    for (int k = 0; k < kParts; ++k)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[k][i] = 0.f;
+                        for (int i = 0; i < 32; ++i) v[k][i] = 0.f;
+                };
+                clear();
                 auto column = [&](int k) {
                     return GATED ? (k / kChunks) * (BN / 2) + (k % kChunks) * 32 : 32 * k;
                 };
@@ -794,6 +1037,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 static_assert(!SPLIT || kParts == 2, "parts of a SPLIT tile");
                 const float sb = p.bmax ? pow2_inv(pow2_scale(*p.bmax)) : 1.f;
                 const float sa = p.rinv ? (m + lane < p.M ? p.rinv[m + lane] : 0.f) : *p.factor;
+                if constexpr (EPI == kLow) {
+                    Low low_(p, ti.mt);
+                    for (int g = ti.ks; g < low_.groups(); g += p.ksplit) {
+                        clear();
+                        if (!(ok = add((p.ph[0].nk + kRound - 1) / kRound, 1.f))) break;
+                        low_store(p, low_, g, part, m, lane, v, sa * sb);
+                    }
+                    if (!ok) break;
+                    continue;
+                }
                 int stages = 0;
                 for (int f = 0; f < p.nphase; ++f) {
                     const Share sh(p, ti, f);
@@ -819,9 +1072,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     }
                 }
                 if (p.ext) {
-                    int es = 0;
-                    for (Blocks st(p, ti); st.any(); st.next()) ++es;
-                    es = (es + 3) >> 2;
+                    const int es = ti.ks == p.ksplit - 1 ? (req.z * p.ext + 3) >> 2 : 0;
                     const float f = (m + lane < p.M ? p.ext_rinv[m + lane] : 0.f) *
                                     pow2_inv(pow2_scale(*p.ext_bmax));
                     if (!(ok = add((es + kRound - 1) / kRound, f))) break;
@@ -1158,6 +1409,13 @@ int make_slice_map(CUtensorMap* m, const void* p, long long cols, long long rows
               : encode_map(m, p, false, cols, rows, depth, ld, ldz, 16, box_rows,
                            CU_TENSOR_MAP_SWIZZLE_32B);
 }
+int make_low_map(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld, bool mn,
+                 int depth, long long ldz) {
+    return mn ? encode_map(m, p, false, cols, rows, depth, ld, ldz, 16, 64,
+                           CU_TENSOR_MAP_SWIZZLE_32B)
+              : encode_map(m, p, false, cols, rows, depth, ld, ldz, 64, 16,
+                           CU_TENSOR_MAP_SWIZZLE_128B);
+}
 int make_out_map(CUtensorMap* m, const void* p, int dtype, long long cols, long long rows,
                  long long ld) {
     const bool f32 = dtype == ATOM_F32;
@@ -1227,7 +1485,7 @@ static int run(const Maps& maps, const Args& p, Chain& st) {
     if (int s = st.launch("pair product", pair_kernel<BN, EPI, SPLIT>, dim3(grid), CF::kThreads,
                           CF::kSmem, maps, p))
         return s;
-    if (p.ksplit > 1) {
+    if (EPI != kLow && p.ksplit > 1) {
         const long long blocks = (p.M * p.N * p.groups + 1023) / 1024;
         return st.launch("pair product sums", reduce_kernel,
                          dim3((unsigned)(blocks < 1184 ? blocks : 1184)), 256, 0, p);
@@ -1252,6 +1510,8 @@ int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain
         return ATOM_ERR_CAPACITY;
     }
     if (p.tiles == 0) return ATOM_OK;
+    if (epilogue == kLow)
+        return split ? run<128, kLow, true>(maps, p, st) : run<128, kLow, false>(maps, p, st);
     if (epilogue == kStore && !p.blocked) {
         // TMA stores clip at 16 bytes, so columns have to end there too
         const int e = p.ksplit > 1 ? 4 : dtype_size(p.dtype);

@@ -22,7 +22,9 @@ struct Phase {
     int bstep, brank;        // B's first row: column tile * bstep + CTA * brank
 };
 
-enum Epilogue { kStore = 0, kGate = 1, kGateBwdGU = 2, kGateBwdDH = 3 };
+// kLow: the requests' low-rank rows themselves: of each row tile, times the adapters of its pieces,
+// 16 columns a slice (ph[0].b0: the adapters' map).
+enum Epilogue { kStore = 0, kGate = 1, kGateBwdGU = 2, kGateBwdDH = 3, kLow = 4 };
 
 struct Args {
     long long M;             // rows of the output (of one group)
@@ -55,9 +57,15 @@ struct Args {
     // t ([256][R] typed, zeros in other rows), multiplied by the request's adapter
     int ext;                 // 16-rank slices a request, 0: none
     int ext_a, ext_b, ext_bmn;
-    const int2* tile_req;    // requests first .. last - 1 of a tile
-    const int4* piece;       // of a block: adapter or -1 (left out), its rows
+    int4* tile_req;          // of a row tile: its requests' first and behind; and, from kLow on,
+                             // how many pieces count and whether one's adapter is not finite
+    const int4* piece;       // of a block: adapter or -1 (none), its rows
+    int* usable;             // from kLow on: the same adapter, -1 also where it is not finite
     const int4* bad;         // of an adapter: not all zero = not finite, its rows become NaN
+    const float* low_scale;  // kLow: per adapter
+    void* low_block;         // kLow: [block][256][Rs] typed, or NULL (SPLIT)
+    void* low_rows;          // kLow: [M][Rs] typed, or NULL
+    int Rs;
     const float* ext_rinv;   // SPLIT: of the low-rank rows
     const unsigned* ext_bmax;
     int* err;
@@ -78,7 +86,9 @@ int make_map(CUtensorMap* m, const void* p, long long cols, long long rows, long
 // 16 x box_rows, or of 64 x 16 where K runs along the rows (mn).
 int make_slice_map(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld,
                    int box_rows, bool mn, int depth, long long ldz);
-
+// kLow's adapters [depth][rows = R][cols = K], or [depth][rows = K][cols = R] (mn).
+int make_low_map(CUtensorMap* m, const void* p, long long cols, long long rows, long long ld, bool mn,
+                 int depth, long long ldz);
 // Map of an output [rows, cols] that is written in blocks of 32 x 32.
 int make_out_map(CUtensorMap* m, const void* p, int dtype, long long cols, long long rows,
                  long long ld);
