@@ -22,88 +22,8 @@ namespace {
 
 using namespace pair;
 
-struct Requests {
-    const int* ptr;
-    const int* adapter;
-    int n, nad;
-    int M;
-};
-// Rows of request r, kept within 0 .. M whatever the table holds.
-__device__ __forceinline__ int row_of(const Requests& q, int r) {
-    return min(max(q.ptr[r], 0), q.M);
-}
-
-struct Pieces {
-    Requests q;
-    int tiles, pieces;       // row tiles; and requests
-    int4* piece;             // adapter or -1, first row, behind the last row
-    int4* tile_req;          // requests first .. behind that reach into a row tile
-    const void* other;       // the matrix of each adapter beside the projection: `other_n` values
-    long long other_n;
-    int4* bad;               // per adapter: a quarter of them is not finite
-    int dtype;
-};
-// Blocks of 8 warps: a piece a warp, a row tile a warp, then four blocks an adapter.
-__global__ void __launch_bounds__(256) pieces_kernel(const __grid_constant__ Pieces p) {
-    let_next_start();
-    wait_before();
-    const int lane = threadIdx.x & 31, w = blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lookups = (p.pieces + p.tiles + 7) / 8;
-    auto begins = [&](int r) { return row_of(p.q, r); };
-    if (blockIdx.x < lookups) {
-        if (w < p.pieces) {
-            // t + r grows with r at each request's first tile t: the last request at or before w
-            const int r = last_le(p.q.n, w, [&](int i) { return row_of(p.q, i) / 256 + i; });
-            int4 c = make_int4(-1, 0, 0, 0);
-            if (r >= 0 && w - r < p.tiles) {
-                const int m0 = (w - r) * 256, a = p.q.adapter[r];
-                c.y = max(row_of(p.q, r), m0);
-                c.z = min(row_of(p.q, r + 1), m0 + 256);
-                if (c.y < c.z && a >= 0 && a < p.q.nad) c.x = a;
-            }
-            if (lane == 0) p.piece[w] = c;
-        } else if (w < p.pieces + p.tiles) {
-            const int t = w - p.pieces;
-            const int first = last_le(p.q.n, t * 256, begins);
-            const int last = last_le(p.q.n, t * 256 + 255, begins);
-            // a request that begins before the tile reaches into it at most as the last such one
-            if (lane == 0) p.tile_req[t] = make_int4(max(first, 0), last + 1, 0, 0);
-        }
-        return;
-    }
-    const int a = (blockIdx.x - lookups) >> 2, part = (blockIdx.x - lookups) & 3;
-    int found = 0;
-    const long long lo = p.other_n * part / 4, hi = p.other_n * (part + 1) / 4;
-    const long long at = (long long)a * p.other_n;
-    if (p.dtype == ATOM_F32) {
-        const unsigned* v = static_cast<const unsigned*>(p.other) + at;
-#pragma unroll 16
-        for (long long i = lo + threadIdx.x; i < hi; i += 256)
-            found |= (v[i] & 0x7F800000u) == 0x7F800000u;
-    } else {
-        const unsigned short top = p.dtype == ATOM_BF16 ? 0x7F80 : 0x7C00;
-        const unsigned short* v = static_cast<const unsigned short*>(p.other) + at;
-        long long i = lo + threadIdx.x;
-        if ((reinterpret_cast<uintptr_t>(v + lo) & 15) == 0) {
-            const unsigned two = top * 0x10001u;
-            const long long n8 = (hi - lo) / 8;
-#pragma unroll 8
-            for (long long j = threadIdx.x; j < n8; j += 256) {
-                const uint4 x = *reinterpret_cast<const uint4*>(v + lo + 8 * j);
-                const unsigned w4[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    found |= (w4[k] & top) == top || ((w4[k] & two) >> 16) == top;
-            }
-            i = lo + 8 * n8 + threadIdx.x;
-        }
-        for (; i < hi; i += 256) found |= (v[i] & top) == top;
-    }
-    found = __syncthreads_or(found);
-    if (threadIdx.x == 0) reinterpret_cast<int*>(p.bad + a)[part] = found;
-}
-
-// fp32: the pieces' blocks as planes, scaled row by row, from the low-rank rows. A block a piece.
+// fp32, more than 64 ranks: the pieces' blocks as planes, scaled row by row, from the low-rank
+// rows. A block a piece.
 __global__ void __launch_bounds__(256) blocks32_kernel(const int4* pieces, const float* rows, int R,
                                                        int Rs, __half* block, long long plane,
                                                        float* rinv) {
@@ -350,12 +270,12 @@ __global__ void __launch_bounds__(256) grads_sum_kernel(const __grid_constant__ 
     let_next_start();
     wait_before();
     const int W = p.width[0] + p.width[1], groups = (p.R + 3) / 4;
+    const int k = blockIdx.x * 256 + threadIdx.x;
+    if (k >= W) return;
     const long long per = (long long)p.R * W, all = per * p.nad;
-    const long long items = (long long)p.nad * groups * W;
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < items; i += gridDim.x * 256LL) {
-        const int k = (int)(i % W);
-        const long long q = i / W, a = q / groups;
-        const int r0 = (int)(q - a * groups) * 4, n = min(4, p.R - r0);
+    const bool first = k < p.width[0], vec = aligned16(p.out[1]);
+    for (int i = blockIdx.y; i < p.nad * groups; i += gridDim.y) {
+        const int a = i / groups, r0 = (i - a * groups) * 4, n = min(4, p.R - r0);
         const float* part = p.part + a * per + (long long)r0 * W + k;
         float v[4] = {};
 #pragma unroll 4
@@ -363,13 +283,22 @@ __global__ void __launch_bounds__(256) grads_sum_kernel(const __grid_constant__ 
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (j < n) v[j] += part[s * all + (long long)j * W];
-        const bool first = k < p.width[0];
-        const long long at = first ? (a * p.R + r0) * p.width[0] + k
-                                   : (a * p.width[1] + k - p.width[0]) * p.R + r0;
+        const long long at = first ? ((long long)a * p.R + r0) * p.width[0] + k
+                                   : ((long long)a * p.width[1] + k - p.width[0]) * p.R + r0;
         const long long step = first ? p.width[0] : 1;
+        if (!first && p.R % 4 == 0 && vec) {         // four ranks at once
+            if (p.dtype == ATOM_F32)
+                *reinterpret_cast<float4*>(static_cast<float*>(p.out[1]) + at) =
+                    make_float4(v[0], v[1], v[2], v[3]);
+            else
+                *reinterpret_cast<uint2*>(static_cast<unsigned short*>(p.out[1]) + at) =
+                    make_uint2(pair_w(v[0], v[1], p.dtype), pair_w(v[2], v[3], p.dtype));
+            continue;
+        }
+        void* out = first ? p.out[0] : p.out[1];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (j < n) store_f(p.out[!first], at + j * step, v[j], p.dtype);
+            if (j < n) store_f(out, at + j * step, v[j], p.dtype);
     }
 }
 template <bool BF16>
@@ -419,7 +348,8 @@ struct AdSpace {
     void *S, *T;
     int4 *piece, *bad, *tile_req;
     int *usable, *few_slot;
-    unsigned* max;           // w, the adapters beside it, the adapters of the low-rank rows
+    unsigned *max, *maxima[3];       // of w, of the adapters beside it, of those of the low-rank
+                                     // rows; and the blocks' own
     size_t bytes;
     AdSpace(void* ws, const AdSizes& z, bool bwd) {
         memset(this, 0, sizeof(*this));
@@ -432,7 +362,8 @@ struct AdSpace {
         if (z.split) {
             rinv = c.take<float>(up(z.M, 32));
             if (!bwd) wr = c.take<float>(up(z.O, 32));
-            max = c.take<unsigned>(8);
+            max = c.take<unsigned>(4);
+            for (unsigned*& m : maxima) m = c.take<unsigned>(kPrepBlocks);
             ext_rinv = c.take<float>(z.on ? z.M : 0);
         }
         if (z.on) {
@@ -467,22 +398,13 @@ struct Ad {
     AdSizes z;
     AdSpace sp;
     Chain st;
-    Requests q;
+    const int *req_ptr, *req_adapter;
     const float* scale;
     const void *w, *a, *b;
 
-    // the pieces of the requests' rows, and which adapters `other` (beside the projection) are not
-    // finite
-    int find_pieces(const void* other, long long other_n) {
-        Pieces p;
-        memset(&p, 0, sizeof(p));
-        p.q = q;
-        p.tiles = z.tiles, p.pieces = z.pieces;
-        p.piece = sp.piece, p.tile_req = sp.tile_req, p.bad = sp.bad;
-        p.other = other, p.other_n = other_n;
-        p.dtype = z.dtype;
-        const int blocks = (z.pieces + z.tiles + 7) / 8 + (other ? 4 * z.nad : 0);
-        return st.launch("adapters: pieces", pieces_kernel, dim3(blocks), 256, 0, p);
+    Pieces pieces(const void* other, long long other_n) const {
+        return {req_ptr, req_adapter, z.nreq, z.nad, (int)z.M, z.tiles, z.pieces, sp.piece,
+                sp.tile_req, other, other_n, sp.bad, z.dtype};
     }
 
     // A direction's operands: rows, the shared matrix, the adapters that make the low-rank rows
@@ -524,8 +446,11 @@ struct Ad {
         p.ph[0] = {0, k, k, (K + 63) / 64, 0, bwd ? 1 : 0, 0, 0};
         p.used = (1u << 2 * k) - 1;
         p.low_scale = scale;
-        p.low_block = sp.block;
-        p.low_rows = z.split && !kept ? sp.T : kept;
+        const bool planes = z.split && z.R <= 64;        // written by the product
+        p.low_block = !z.split || (blocks && planes) ? sp.block : nullptr;
+        p.low_plane = (long long)z.pieces * 256 * z.Rs;
+        p.low_rinv = sp.ext_rinv;
+        p.low_rows = z.split && !planes && !kept ? sp.T : kept;
         if (!blocks) p.usable = nullptr;
         p.Rs = z.Rs;
         p.rinv = rinv;
@@ -534,7 +459,7 @@ struct Ad {
         const int groups = std::min(16, (z.nreq * p.ext + 7) / 8);
         const int share = std::max(1, std::min(groups, 74 / z.tiles));
         if (int s = launch(kLow, {128, share, 0}, z.split, maps, p, st)) return s;
-        if (!z.split || !blocks) return ATOM_OK;
+        if (!z.split || !blocks || planes) return ATOM_OK;
         return st.launch("adapters: blocks", blocks32_kernel, dim3(z.pieces), 256, 0,
                          (const int4*)sp.piece, (const float*)p.low_rows, z.R, z.Rs, sp.block,
                          (long long)z.pieces * 256 * z.Rs, sp.ext_rinv);
@@ -552,36 +477,38 @@ struct Ad {
         const bool product = out != nullptr;
         Operands o{rows, w, first, second, ld, z.D, fcols, scols, 0, 0, 0, 0};
         PrepList l;
+        const Pieces found = pieces(product ? second : nullptr, (long long)z.R * (bwd ? z.D : z.O));
         if (z.split) {
             o = {sp.rows, sp.w, sp.first, sp.ext, Kp, z.Dp, fp, spp,
                  z.M * Kp, z.O * z.Dp, frows * fp, srows * spp};
-            // the largest w and adapters, and no scales for rows without low-rank values
-            if (int s = st.zero("adapters", sp.max,
-                                (char*)(sp.ext_rinv + (z.on ? z.M : 0)) - (char*)sp.max))
-                return s;
+            int parts[3] = {};
+            auto largest = [&](const void* p, long long n, long long cols, int m) {
+                PrepItem it{p, n, cols, cols, nullptr, 0, 0, nullptr, nullptr, kMax, nullptr,
+                            sp.maxima[m], 0};
+                parts[m] = prep_blocks(it);
+                l.add(it);
+            };
+            auto planes = [&](const void* p, long long n, long long cols, __half* dst,
+                              long long pitch, int m) {
+                l.add({p, n, cols, cols, dst, pitch, n * pitch, nullptr, sp.max + m, kTensorSplit,
+                       nullptr, sp.maxima[m], parts[m]});
+            };
             l.add({rows, z.M, K, ld, sp.rows, Kp, z.M * Kp, sp.rinv, nullptr, kRowSplit, nullptr});
-            if (product && bwd)
-                l.add({w, z.O, z.D, z.D, nullptr, 0, 0, nullptr, sp.max, kMax, nullptr});
+            if (product && bwd) largest(w, z.O, z.D, 0);
             if (product && !bwd)
                 l.add({w, z.O, z.D, z.D, sp.w, z.Dp, z.O * z.Dp, sp.wr, nullptr, kRowSplit,
                        nullptr});
             if (z.on) {
-                l.add({second, srows, scols, scols, nullptr, 0, 0, nullptr, sp.max + 1, kMax,
-                       nullptr});
-                l.add({first, frows, fcols, fcols, nullptr, 0, 0, nullptr, sp.max + 2, kMax,
-                       nullptr});
+                largest(second, srows, scols, 1);
+                largest(first, frows, fcols, 2);
+            }
+            if (int s = prepare(l, st, z.on ? &found : nullptr)) return s;
+            if (product && bwd) planes(w, z.O, z.D, sp.w, z.Dp, 0);
+            if (z.on) {
+                planes(second, srows, scols, sp.ext, spp, 1);
+                planes(first, frows, fcols, sp.first, fp, 2);
             }
             if (int s = prepare(l, st)) return s;
-            l.n = 0;
-            if (product && bwd)
-                l.add({w, z.O, z.D, z.D, sp.w, z.Dp, z.O * z.Dp, nullptr, sp.max, kTensorSplit,
-                       nullptr});
-            if (z.on) {
-                l.add({second, srows, scols, scols, sp.ext, spp, srows * spp, nullptr, sp.max + 1,
-                       kTensorSplit, nullptr});
-                l.add({first, frows, fcols, fcols, sp.first, fp, frows * fp, nullptr, sp.max + 2,
-                       kTensorSplit, nullptr});
-            }
         } else {
             auto take = [&](const void*& p, long long& pld, long long n, long long cols, __half* buf,
                             long long pitch) {
@@ -596,13 +523,11 @@ struct Ad {
                 if (product) take(o.second, o.second_ld, srows, scols, sp.ext, spp);
             }
         }
-        if (int s = prepare(l, st)) return s;
-        if (z.on) {
-            if (int s = find_pieces(product ? second : nullptr, (long long)z.R * (bwd ? z.D : z.O)))
-                return s;
+        if (!z.split)
+            if (int s = prepare(l, st, z.on ? &found : nullptr)) return s;
+        if (z.on)
             if (int s = low_rows(o, bwd, sp.rinv, z.split ? sp.max + 2 : nullptr, kept, product))
                 return s;
-        }
         if (!product) return ATOM_OK;
         const Choice c = z.product;
         Maps maps;
@@ -649,8 +574,8 @@ struct Ad {
             o = {sp.x, nullptr, sp.first2, nullptr, z.Dp, 0, z.Dp, 0, z.M * z.Dp, 0, an * z.Dp, 0};
             l.add({x, z.M, z.D, ldx, sp.x, z.Dp, z.M * z.Dp, sp.xinv, nullptr, kRowSplit, nullptr});
             // a's maximum is there: a is beside the projection in this direction
-            l.add({a, an, z.D, z.D, sp.first2, z.Dp, an * z.Dp, nullptr, sp.max + 1, kTensorSplit,
-                   nullptr});
+            l.add({a, an, z.D, z.D, sp.first2, z.Dp, an * z.Dp, nullptr, sp.max + 3, kTensorSplit,
+                   nullptr, sp.max + 1, 1});
         } else {
             if (!tma_ready(x, ldx)) {
                 l.add({x, z.M, z.D, ldx, sp.x, z.Dp, 0, nullptr, nullptr, kPack, nullptr});
@@ -662,7 +587,7 @@ struct Ad {
             }
         }
         if (int s = prepare(l, st)) return s;
-        return low_rows(o, false, sp.xinv, z.split ? sp.max + 1 : nullptr, sp.S, false);
+        return low_rows(o, false, sp.xinv, z.split ? sp.max + 3 : nullptr, sp.S, false);
     }
 };
 
@@ -706,8 +631,7 @@ extern "C" int atom_adapted_linear_fwd(int dtype, const void* x, int64_t ldx, in
     const AdSizes z(dtype, M, D, O, n_adapters, R, nreq, false);
     ATOM_REQUIRE(!z.on || (a && b && scale && req_ptr && req_adapter),
                  "adapted_linear: bad operand");
-    Ad f{z, AdSpace(ws, z, false), (cudaStream_t)stream,
-         {req_ptr, req_adapter, nreq, n_adapters, (int)M}, scale, w, a, b};
+    Ad f{z, AdSpace(ws, z, false), (cudaStream_t)stream, req_ptr, req_adapter, scale, w, a, b};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "adapted_linear: the workspace needs %zu bytes",
                  f.sp.bytes);
     if (few::suits(dtype, M, D, x, ldx, w, a)) {
@@ -744,8 +668,7 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
                  "adapted_linear: bad operand");
     ATOM_REQUIRE(!z.on || (a && b && scale && req_ptr && req_adapter),
                  "adapted_linear: bad operand");
-    Ad f{z, AdSpace(ws, z, true), st, {req_ptr, req_adapter, nreq, n_adapters, (int)M}, scale, w,
-         a, b};
+    Ad f{z, AdSpace(ws, z, true), st, req_ptr, req_adapter, scale, w, a, b};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "adapted_linear: the workspace needs %zu bytes",
                  f.sp.bytes);
     const bool grads = z.on && (da || db);
@@ -788,6 +711,8 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
     else rc = f.st.launch("adapters: gradients", grads32_kernel, grid, 256, 0, p);
     if (rc) return rc;
     if (p.split > 1)
-        return f.st.launch("adapters: gradient sums", grads_sum_kernel, dim3(1184), 256, 0, p);
+        return f.st.launch("adapters: gradient sums", grads_sum_kernel,
+                           dim3(ceil_div(p.width[0] + p.width[1], 256),
+                                std::min(n_adapters * ((R + 3) / 4), 65535)), 256, 0, p);
     return ATOM_OK;
 }

@@ -57,7 +57,7 @@ struct FfSpace {
     __half *x, *wg, *wu, *wd, *dy, *xt, *dyt, *hp, *dgup;
     float *xr, *wgr, *wur, *wdr, *dyr, *hr, *dgur, *H32, *dgu32, *dh, *part;
     __half *H, *dgu;
-    unsigned* max;              // x'' factor, wg | wu, wd, dy'' factor
+    unsigned *max, *maxima[4];  // of wg | wu, of wd, x'' factor, dy'' factor; and the blocks' own
     size_t bytes;
     FfSpace(void* ws, const FfSizes& z, bool bwd) {
         memset(this, 0, sizeof(*this));
@@ -78,7 +78,8 @@ struct FfSpace {
             H = c.take<__half>(M * z.Fp);
             if (bwd) dgu = c.take<__half>(2 * M * z.Fp);
         } else {
-            max = c.take<unsigned>(8);
+            max = c.take<unsigned>(4);
+            for (unsigned*& m : maxima) m = bwd ? c.take<unsigned>(2 * kPrepBlocks) : nullptr;
             xr = c.take<float>(M32);
             H32 = c.take<float>(M * z.Fp);
             hp = c.take<__half>(2 * M * z.Fp);
@@ -116,47 +117,51 @@ struct Ff {
     int act;
     Operand x, wg, wu, wd, dy;
     PrepList list;
+    int parts[4] = {};          // blocks' maxima so far
 
-    // an operand of this call: as it lies, or through the list's packing / planes
+    // an operand of this call: as it lies, or through the list's packing / planes; kTensorSplit:
+    // by maximum `m` of parts[m] blocks
     Operand take(const void* p, long long rows, long long cols, long long ld, __half* buf,
-                 long long pitch, int mode, float* rinv, unsigned* max) {
+                 long long pitch, int mode, float* rinv, int m = 0) {
         if (!z.split && tma_ready(p, ld)) return {p, rows, cols, ld, 0};
-        list.add({p, rows, cols, ld, buf, pitch, rows * pitch, rinv, max, z.split ? mode : kPack,
-                  nullptr});
+        list.add({p, rows, cols, ld, buf, pitch, rows * pitch, rinv, sp.max + m,
+                  z.split ? mode : kPack, nullptr, sp.maxima[m], parts[m]});
+        if (mode == kRowSplit || !z.split) list.it[list.n - 1].part = nullptr;
         return {buf, rows, cols, pitch, rows * pitch};
+    }
+    // an item whose blocks' maxima go behind those that maximum m has
+    void gather(PrepItem it, int m) {
+        it.part = sp.maxima[m] + parts[m];
+        parts[m] += prep_blocks(it);
+        list.add(it);
     }
     // Weights and rows brought into the form that the products read. fp32 forward: every operand
     // scaled row by row, in one launch. fp32 backward: the weights are read across their rows, so
     // each of them (Wg and Wu together) has one scale, from a launch before; x is needed only for
     // G and U, and beside its scales in the weights' gradients later.
     int inputs(const void* xp, long long ldx, const void* g, const void* u, const void* d) {
-        x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kRowSplit, sp.xr, nullptr);
-        wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kRowSplit, sp.wgr, nullptr);
-        wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kRowSplit, sp.wur, nullptr);
-        wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kRowSplit, sp.wdr, nullptr);
-        return flush();
+        x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kRowSplit, sp.xr);
+        wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kRowSplit, sp.wgr);
+        wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kRowSplit, sp.wur);
+        wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kRowSplit, sp.wdr);
+        return prepare(list, st);
     }
     int inputs_bwd(const void* xp, long long ldx, const void* g, const void* u, const void* d,
                    const void* dyp, long long lddy, bool kept) {
         if (z.split) {
-            if (int s = st.zero("gated_ff", sp.max, 32)) return s;
-            list.add({g, z.F, z.D, z.D, nullptr, 0, 0, nullptr, sp.max + 1, kMax, nullptr});
-            list.add({u, z.F, z.D, z.D, nullptr, 0, 0, nullptr, sp.max + 1, kMax, nullptr});
-            list.add({d, z.O, z.F, z.F, nullptr, 0, 0, nullptr, sp.max + 2, kMax, nullptr});
+            gather({g, z.F, z.D, z.D, nullptr, 0, 0, nullptr, nullptr, kMax, nullptr}, 0);
+            gather({u, z.F, z.D, z.D, nullptr, 0, 0, nullptr, nullptr, kMax, nullptr}, 0);
+            gather({d, z.O, z.F, z.F, nullptr, 0, 0, nullptr, nullptr, kMax, nullptr}, 1);
         }
-        x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kept ? kRowScale : kRowSplit, sp.xr, nullptr);
-        dy = take(dyp, z.M, z.O, lddy, sp.dy, z.Op, kRowSplit, sp.dyr, nullptr);
+        x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kept ? kRowScale : kRowSplit, sp.xr);
+        if (z.split) list.it[list.n - 1].part = nullptr;
+        dy = take(dyp, z.M, z.O, lddy, sp.dy, z.Op, kRowSplit, sp.dyr);
         if (z.split)
-            if (int s = flush()) return s;
-        wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kTensorSplit, nullptr, sp.max + 1);
-        wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kTensorSplit, nullptr, sp.max + 1);
-        wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kTensorSplit, nullptr, sp.max + 2);
-        return flush();
-    }
-    int flush() {
-        const int s = prepare(list, st);
-        list.n = 0;
-        return s;
+            if (int s = prepare(list, st)) return s;
+        wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kTensorSplit, nullptr, 0);
+        wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kTensorSplit, nullptr, 0);
+        wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kTensorSplit, nullptr, 1);
+        return prepare(list, st);
     }
     Args args(long long M, int N) const {
         Args p;
@@ -198,7 +203,7 @@ struct Ff {
         p.ph[0] = {0, k, 2 * k, z.nk(z.D), 0, 0, c.bn / 2, 0};
         p.rinv = sp.xr;
         if (sp.wgr) p.cinv[0] = sp.wgr, p.cinv[1] = sp.wur;
-        else if (z.split) p.bmax = sp.max + 1;
+        else if (z.split) p.bmax = sp.max;
         p.used = z.split ? 0x3f : 0x7;
         if (int s = gate_output(maps, p, C, width, H)) return s;
         return launch(epilogue, c, z.split, maps, p, st);
@@ -211,7 +216,7 @@ struct Ff {
         if (z.split) {
             list.add({sp.H32, z.M, z.F, z.Fp, sp.hp, z.Fp, z.M * z.Fp, sp.hr, nullptr, kRowSplit,
                       nullptr});
-            if (int s = flush()) return s;
+            if (int s = prepare(list, st)) return s;
             h = {sp.hp, z.M, z.F, z.Fp, z.M * z.Fp};
         }
         const Choice c = z.down;
@@ -238,7 +243,7 @@ struct Ff {
             Args p = args(z.M, z.F);
             p.ph[0] = {0, k, k, z.nk(z.O), 0, 1, c.bn, c.bn / 2};
             p.rinv = sp.dyr;
-            if (z.split) p.bmax = sp.max + 2;
+            if (z.split) p.bmax = sp.max + 1;
             p.used = z.split ? 0xf : 0x3;
             if (kept) {
                 p.gu = const_cast<float*>(kept);
@@ -262,22 +267,22 @@ struct Ff {
             const long long M = z.M, W = 2 * z.Fp;
             g = {sp.dgup, M, W, W, M * W};
             h = {sp.hp, M, z.F, z.Fp, M * z.Fp};
-            list.add({sp.dgu32, M, W, W, sp.dgup, W, M * W, sp.dgur, sp.max, kRowSplit, sp.xr});
+            gather({sp.dgu32, M, W, W, sp.dgup, W, M * W, sp.dgur, nullptr, kRowSplit, sp.xr}, 2);
             if (dwd)
-                list.add({sp.H32, M, z.F, z.Fp, sp.hp, z.Fp, M * z.Fp, sp.hr, sp.max + 3,
-                          kRowSplit, sp.dyr});
-            if (int s = flush()) return s;
+                gather({sp.H32, M, z.F, z.Fp, sp.hp, z.Fp, M * z.Fp, sp.hr, nullptr, kRowSplit,
+                        sp.dyr}, 3);
+            if (int s = prepare(list, st)) return s;
             if (dwg || dwu) {
                 xt = {sp.xt, M, z.D, z.Dp, M * z.Dp};
-                list.add({x_src, M, z.D, x_ld, sp.xt, z.Dp, M * z.Dp, nullptr, sp.max, kWeighted,
-                          sp.dgur});
+                list.add({x_src, M, z.D, x_ld, sp.xt, z.Dp, M * z.Dp, nullptr, sp.max + 2, kWeighted,
+                          sp.dgur, sp.maxima[2], parts[2]});
             }
             if (dwd) {
                 dyt = {sp.dyt, M, z.O, z.Op, M * z.Op};
                 list.add({dy_src, M, z.O, dy_ld, sp.dyt, z.Op, M * z.Op, nullptr, sp.max + 3,
-                          kWeighted, sp.hr});
+                          kWeighted, sp.hr, sp.maxima[3], parts[3]});
             }
-            if (int s = flush()) return s;
+            if (int s = prepare(list, st)) return s;
         }
         if (dx) {
             const Choice c = z.dx;
@@ -291,7 +296,7 @@ struct Ff {
             p.ph[0] = {0, 2 * k, 2 * k, z.nk(z.F), 0, 1, c.bn, c.bn / 2};
             p.ph[1] = {k, 3 * k, 3 * k, z.nk(z.F), 0, 1, c.bn, c.bn / 2};
             p.rinv = sp.dgur;
-            if (z.split) p.bmax = sp.max + 1;
+            if (z.split) p.bmax = sp.max;
             output(p, dx, lddx);
             if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
         }
@@ -306,7 +311,7 @@ struct Ff {
             Args p = args(z.F, z.D);
             p.groups = two ? 2 : 1;
             p.ph[0] = {0, 2 * k, 2 * k, z.nk(z.M), 1, 1, c.bn, c.bn / 2};
-            p.factor = reinterpret_cast<const float*>(sp.max);
+            p.factor = reinterpret_cast<const float*>(sp.max + 2);
             output(p, dwg ? dwg : dwu, z.D);
             p.C[1] = dwu;
             if (int s = launch(kStore, c, z.split, maps, p, st)) return s;

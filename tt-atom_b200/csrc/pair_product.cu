@@ -329,19 +329,25 @@ struct Window {
 // stay together); with few row tiles, `ksplit` work items share a tile's groups.
 struct Low {
     Window w;
-    int count, slices, each, before = 0;         // pieces; slices a piece; pieces a group
+    int count, slices, half, each, before = 0;   // pieces; slices a piece; pieces a half, a group
     __device__ __forceinline__ Low(const Args& p, int tile) : w(p, tile) {
         slices = p.ext;
-        each = 8 / slices;
+        half = slices <= 4 ? 4 / slices : 0;
+        each = slices <= 4 ? 2 * half : 1;
         count = w.count();
     }
     __device__ __forceinline__ int groups() const { return (count + each - 1) / each; }
-    __device__ __forceinline__ int used(int g) const {          // slices of group g
-        return min(each, count - g * each) * slices;
+    // slices of group g in half h (64 columns; slice i of a group is i % 4 of half i / 4)
+    __device__ __forceinline__ int used(int g, int h) const {
+        if (slices > 4) return h ? slices - 4 : 4;
+        return max(0, min(half, count - g * each - h * half)) * slices;
     }
-    // the piece of slice i of group g: its adapter and rows, and in w its request
+    __device__ __forceinline__ int sub(int i) const {           // which of its piece's slices i is
+        return slices > 4 ? i : (i & 3) % slices;
+    }
+    // the piece of slice i of group g: its adapter and rows, and its request
     __device__ __forceinline__ int4 piece(int g, int i) {
-        int j = g * each + i / slices;
+        int j = g * each + (slices > 4 ? 0 : (i >> 2) * half + (i & 3) / slices);
         if (j < before) {
             before = 0;
             w.look(w.first);
@@ -384,14 +390,6 @@ struct Out {
     uint8_t* buf;
     uint32_t turn;
 };
-__device__ __forceinline__ uint32_t pack2(float a, float b, int dtype) {
-    if (dtype == ATOM_BF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ void stage_f32(uint8_t* buf, int lane, const float* v) {
 #pragma unroll
     for (int c = 0; c < 8; ++c)
@@ -414,8 +412,8 @@ __device__ __forceinline__ void store_tma(Out& o, int lane, const CUtensorMap* m
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             *reinterpret_cast<uint4*>(b + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = make_uint4(
-                pack2(v[8 * c], v[8 * c + 1], dtype), pack2(v[8 * c + 2], v[8 * c + 3], dtype),
-                pack2(v[8 * c + 4], v[8 * c + 5], dtype), pack2(v[8 * c + 6], v[8 * c + 7], dtype));
+                pair_w(v[8 * c], v[8 * c + 1], dtype), pair_w(v[8 * c + 2], v[8 * c + 3], dtype),
+                pair_w(v[8 * c + 4], v[8 * c + 5], dtype), pair_w(v[8 * c + 6], v[8 * c + 7], dtype));
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -594,42 +592,68 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
 }
 
 // kLow: a lane's row of the four slices that a warp has of group g, times the adapter's scale and f:
-// into the pieces' blocks (zeros outside a piece's rows), and into the rows' own places.
+// into the pieces' blocks (zeros outside a piece's rows), and into the rows' own places. fp32
+// blocks are planes, scaled row by row: a piece's slices are all in one warp then (ranks of 64 at
+// most; larger ones have a kernel of their own, from the rows).
 __device__ __forceinline__ void low_store(const Args& p, Low& low, int g, int part,
                                           long long m0, int lane, float (*v)[32], float f) {
-    const int used = low.used(g);
+    const int used = low.used(g, part);
     const long long m = m0 + lane;
+    float largest = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int slice = part * 4 + i;
-        if (slice >= used) break;
-        const int4 piece = low.piece(g, slice);
-        const int c0 = slice % p.ext * 16;
+        if (i >= used) break;
+        const int4 piece = low.piece(g, part * 4 + i);
+        const int sub = low.sub(part * 4 + i), c0 = sub * 16;
         const bool in = m >= piece.y && m < piece.z;
         const float s = p.low_scale[piece.x] * f;
         float* x = v[i >> 1] + (i & 1) * 16;
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = in ? x[j] * s : 0.f;
+        const long long row = ((long long)(low.w.mt + piece.w) * 256 + (m & 255)) * p.Rs;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                // eight ranks at a time: Rs is a multiple of 8
             const int c = c0 + 8 * h;
             if (c >= p.Rs) break;
             const float* y = x + 8 * h;
             if (p.dtype == ATOM_F32) {
-                float* q = static_cast<float*>(p.low_rows) + m * p.Rs + c;
-                if (in) {
+                if (p.low_rows && in) {
+                    float* q = static_cast<float*>(p.low_rows) + m * p.Rs + c;
                     *reinterpret_cast<float4*>(q) = make_float4(y[0], y[1], y[2], y[3]);
                     *reinterpret_cast<float4*>(q + 4) = make_float4(y[4], y[5], y[6], y[7]);
                 }
                 continue;
             }
-            const uint4 w = make_uint4(pack2(y[0], y[1], p.dtype), pack2(y[2], y[3], p.dtype),
-                                       pack2(y[4], y[5], p.dtype), pack2(y[6], y[7], p.dtype));
-            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.low_block) +
-                                      ((long long)(low.w.mt + piece.w) * 256 + (m & 255)) * p.Rs + c) = w;
+            const uint4 w = make_uint4(pair_w(y[0], y[1], p.dtype), pair_w(y[2], y[3], p.dtype),
+                                       pair_w(y[4], y[5], p.dtype), pair_w(y[6], y[7], p.dtype));
+            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.low_block) + row + c) = w;
             if (p.low_rows && in)
                 *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.low_rows) + m * p.Rs + c) = w;
         }
+        if (p.dtype != ATOM_F32 || !p.low_block) continue;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(x[j]));
+        if (sub < p.ext - 1) continue;               // the piece's last slice: its planes
+        const float scale = pow2_scale(finite_bits(largest));
+        if (in) p.low_rinv[m] = pow2_inv(scale);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k > i || k < i - sub) continue;
+            const float* y = v[k >> 1] + (k & 1) * 16;
+            const int c = (k - i + sub) * 16;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (c + 8 * h >= p.Rs) break;
+                __half2 hi[4], lo[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    split_half2(y[8 * h + 2 * j] * scale, y[8 * h + 2 * j + 1] * scale, hi[j], lo[j]);
+                __half* q = static_cast<__half*>(p.low_block) + row + c + 8 * h;
+                *reinterpret_cast<uint4*>(q) = *reinterpret_cast<uint4*>(hi);
+                *reinterpret_cast<uint4*>(q + p.low_plane) = *reinterpret_cast<uint4*>(lo);
+            }
+        }
+        largest = 0.f;
     }
 }
 
@@ -717,12 +741,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     Low low(p, ti.mt);
                     const bool mn = p.ph[0].b_mn;
                     for (int g = ti.ks; ok && g < low.groups(); g += p.ksplit) {
-                        const int n = low.used(g), mine = min(4, max(0, n - 4 * (int)rank));
+                        const int n = low.used(g, 0) + low.used(g, 1), mine = low.used(g, rank);
                         int slot[4], r16[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             slot[i] = i < mine ? low.piece(g, 4 * rank + i).x : 0;
-                            r16[i] = (4 * rank + i) % p.ext * 16;
+                            r16[i] = low.sub(4 * rank + i) * 16;
                         }
                         for (int kt = 0; kt < p.ph[0].nk; ++kt) {
                             uint32_t dst, bar;
@@ -1073,8 +1097,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 }
                 if (p.ext) {
                     const int es = ti.ks == p.ksplit - 1 ? (req.z * p.ext + 3) >> 2 : 0;
-                    const float f = (m + lane < p.M ? p.ext_rinv[m + lane] : 0.f) *
-                                    pow2_inv(pow2_scale(*p.ext_bmax));
+                    // rows of no piece have no scale, and sums of zero
+                    float f = m + lane < p.M ? p.ext_rinv[m + lane] : 0.f;
+                    f = (finite_bits(f) ? f : 0.f) * pow2_inv(pow2_scale(*p.ext_bmax));
                     if (!(ok = add((es + kRound - 1) / kRound, f))) break;
                 }
 #pragma unroll
@@ -1104,30 +1129,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
 }
 
 
-// C[g][m, n] = sum over the splits, in order.
-__global__ void __launch_bounds__(256) reduce_kernel(Args p) {
+// C[g][m, n] = sum over the splits, in order. Split products are small (fewer tiles than pairs of
+// SMs), so 32-bit indexes do.
+__global__ void __launch_bounds__(256) reduce_kernel(const __grid_constant__ Args p) {
     let_next_start();
     wait_before();
-    const long long per = p.M * p.N, all = per * p.groups;
-    const bool four = p.N % 4 == 0;
-    for (long long i = (blockIdx.x * 256LL + threadIdx.x) * 4; i < all; i += gridDim.x * 1024LL) {
+    const uint32_t M = (uint32_t)p.M, N = p.N, all = M * N * p.groups;
+    const uint32_t step = N % 4 ? 1 : 4;
+    for (uint32_t i = (blockIdx.x * 256u + threadIdx.x) * step; i < all; i += gridDim.x * 256u * step) {
         float v[4] = {};
-        const int n = (int)min(4LL, all - i);
-        for (int s = 0; s < p.ksplit; ++s) {
-            const float* q = p.part + s * all + i;
-            if (four) {
-                const float4 x = *reinterpret_cast<const float4*>(q);
+        if (step == 4) {
+#pragma unroll 4
+            for (int s = 0; s < p.ksplit; ++s) {
+                const float4 x = *reinterpret_cast<const float4*>(p.part + (long long)s * all + i);
                 v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
-            } else {
-                for (int j = 0; j < n; ++j) v[j] += q[j];
             }
+        } else {
+#pragma unroll 4
+            for (int s = 0; s < p.ksplit; ++s) v[0] += p.part[(long long)s * all + i];
         }
-        for (int j = 0; j < n; ++j) {
-            const long long e = i + j;
-            const int g = (int)(e / per);
-            const long long r = e - g * per;
-            store_f(p.C[g], r / p.N * p.ldc + r % p.N, v[j], p.dtype);
-        }
+        const uint32_t row = i / N, n = i - row * N, g = row >= M;
+        const long long at = (row - g * M) * p.ldc + n;
+        for (uint32_t j = 0; j < step; ++j) store_f(p.C[g], at + j, v[j], p.dtype);
     }
 }
 
@@ -1179,18 +1202,20 @@ __device__ __forceinline__ float row_scale(const PrepItem& it, long long r, floa
     if (it.weight) top = fmaxf(top, fminf(inv * it.weight[r], 0x1p126f));
     return s;
 }
-__device__ __forceinline__ float fixed_scale(const PrepItem& it, long long r) {
-    if (it.mode == kTensorSplit) return pow2_scale(*it.max);
-    // kWeighted; a row whose partner is zero may have any weight
-    return fminf(it.weight[r] * pow2_inv(__uint_as_float(*it.max)), 0x1p126f);
+// kTensorSplit's scale, or what kWeighted divides a row's weight by, from the maxima.
+__device__ __forceinline__ float fixed_scale(const PrepItem& it, long long r, unsigned max) {
+    if (it.mode == kTensorSplit) return pow2_scale(max);
+    // a row whose partner is zero may have any weight
+    return fminf(it.weight[r] * pow2_inv(__uint_as_float(max)), 0x1p126f);
 }
 
-__device__ __forceinline__ void prep_narrow(const PrepItem& it, float& top) {
+__device__ __forceinline__ void prep_narrow(const PrepItem& it, int blocks, unsigned max,
+                                            float& top) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int nv = prep_slots(it), rows = kNV / nv, shift = 31 - __clz(nv);
     const int cols = (int)it.cols, dld = (int)it.dld, mode = it.mode;
     const bool scans = mode == kRowSplit || mode == kMax || mode == kRowScale;
-    for (long long r0 = (blockIdx.x * 8LL + warp) * rows; r0 < it.rows; r0 += gridDim.x * 8LL * rows) {
+    for (long long r0 = (blockIdx.x * 8LL + warp) * rows; r0 < it.rows; r0 += blocks * 8LL * rows) {
         float4 x[kNV];
         const float* src = static_cast<const float*>(it.src) + r0 * it.ld;
         const bool four = aligned16(it.src) && it.ld % 4 == 0 && cols % 4 == 0;
@@ -1249,18 +1274,19 @@ __device__ __forceinline__ void prep_narrow(const PrepItem& it, float& top) {
             const long long r = r0 + i;
             if (r >= it.rows) continue;
             const float s = scans ? row_scale(it, r, m[j], k == 0 && lane == 0, top)
-                                  : fixed_scale(it, r);
+                                  : fixed_scale(it, r, max);
             if (mode != kRowScale && c < dld)
                 prep_put(static_cast<__half*>(it.dst) + r * dld + c, it.plane, x[j], s);
         }
     }
 }
 
-__device__ __forceinline__ void prep_block(const PrepItem& it, float* part, float& top) {
+__device__ __forceinline__ void prep_block(const PrepItem& it, int blocks, float* part,
+                                           unsigned max, float& top) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = threadIdx.x;
     const int cols = (int)it.cols, dld = (int)it.dld, mode = it.mode;
     const bool scans = mode == kRowSplit || mode == kMax || mode == kRowScale;
-    for (long long r = blockIdx.x; r < it.rows; r += gridDim.x) {
+    for (long long r = blockIdx.x; r < it.rows; r += blocks) {
         const float* src = static_cast<const float*>(it.src) + r * it.ld;
         const bool four = aligned16(src) && cols % 4 == 0;
         float4 x[kNV];
@@ -1298,7 +1324,7 @@ __device__ __forceinline__ void prep_block(const PrepItem& it, float* part, floa
             s = row_scale(it, r, mx, me == 0, top);
             if (mode == kRowScale) continue;
         } else {
-            s = fixed_scale(it, r);
+            s = fixed_scale(it, r, max);
         }
         __half* hi = static_cast<__half*>(it.dst) + r * dld;
 #pragma unroll
@@ -1312,10 +1338,10 @@ __device__ __forceinline__ void prep_block(const PrepItem& it, float* part, floa
 }
 
 // 16-bit rows to an aligned pitch; eight single loads in flight, then eight stores.
-__device__ __forceinline__ void prep_pack(const PrepItem& it) {
+__device__ __forceinline__ void prep_pack(const PrepItem& it, int blocks) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int cols = (int)it.cols, dld = (int)it.dld;
-    for (long long r = blockIdx.x * 8LL + warp; r < it.rows; r += gridDim.x * 8LL) {
+    for (long long r = blockIdx.x * 8LL + warp; r < it.rows; r += blocks * 8LL) {
         const unsigned short* src = static_cast<const unsigned short*>(it.src) + r * it.ld;
         unsigned short* dst = static_cast<unsigned short*>(it.dst) + r * dld;
         for (int c0 = 0; c0 < dld; c0 += 256) {
@@ -1329,36 +1355,126 @@ __device__ __forceinline__ void prep_pack(const PrepItem& it) {
     }
 }
 
-__global__ void __launch_bounds__(256, 3) prep_kernel(const __grid_constant__ PrepList l) {
+// Finds pieces: a piece a warp, a row tile a warp, then four blocks an adapter.
+__device__ __forceinline__ void find_pieces(const Pieces& p) {
+    const int lane = threadIdx.x & 31, w = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lookups = (p.pieces + p.tiles + 7) / 8;
+    // rows are kept within 0 .. M whatever the table holds
+    auto begins = [&](int r) { return min(::max(p.ptr[r], 0), p.M); };
+    if (blockIdx.x < lookups) {
+        if (w < p.pieces) {
+            // t + r grows with r at each request's first tile t: the last request at or before w
+            const int r = last_le(p.n, w, [&](int i) { return begins(i) / 256 + i; });
+            int4 c = make_int4(-1, 0, 0, 0);
+            if (r >= 0 && w - r < p.tiles) {
+                const int m0 = (w - r) * 256, a = p.adapter[r];
+                c.y = ::max(begins(r), m0);
+                c.z = min(begins(r + 1), m0 + 256);
+                if (c.y < c.z && a >= 0 && a < p.nad) c.x = a;
+            }
+            if (lane == 0) p.piece[w] = c;
+        } else if (w < p.pieces + p.tiles) {
+            const int t = w - p.pieces;
+            const int first = last_le(p.n, t * 256, begins);
+            const int last = last_le(p.n, t * 256 + 255, begins);
+            // a request that begins before the tile reaches into it at most as the last such one
+            if (lane == 0) p.tile_req[t] = make_int4(::max(first, 0), last + 1, 0, 0);
+        }
+        return;
+    }
+    const int a = (blockIdx.x - lookups) >> 2, part = (blockIdx.x - lookups) & 3;
+    if (!p.other || a >= p.nad) return;
+    int found = 0;
+    const long long lo = p.other_n * part / 4, hi = p.other_n * (part + 1) / 4;
+    const long long at = (long long)a * p.other_n;
+    if (p.dtype == ATOM_F32) {
+        const unsigned* v = static_cast<const unsigned*>(p.other) + at;
+#pragma unroll 16
+        for (long long i = lo + threadIdx.x; i < hi; i += 256)
+            found |= (v[i] & 0x7F800000u) == 0x7F800000u;
+    } else {
+        const unsigned short top = p.dtype == ATOM_BF16 ? 0x7F80 : 0x7C00;
+        const unsigned short* v = static_cast<const unsigned short*>(p.other) + at;
+        long long i = lo + threadIdx.x;
+        if ((reinterpret_cast<uintptr_t>(v + lo) & 15) == 0) {
+            const unsigned two = top * 0x10001u;
+            const long long n8 = (hi - lo) / 8;
+#pragma unroll 8
+            for (long long j = threadIdx.x; j < n8; j += 256) {
+                const uint4 x = *reinterpret_cast<const uint4*>(v + lo + 8 * j);
+                const unsigned w4[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    found |= (w4[k] & top) == top || ((w4[k] & two) >> 16) == top;
+            }
+            i = lo + 8 * n8 + threadIdx.x;
+        }
+        for (; i < hi; i += 256) found |= (v[i] & top) == top;
+    }
+    found = __syncthreads_or(found);
+    if (threadIdx.x == 0) reinterpret_cast<int*>(p.bad + a)[part] = found;
+}
+
+__global__ void __launch_bounds__(256, 3)
+    prep_kernel(const __grid_constant__ PrepList l, const __grid_constant__ Pieces pieces) {
     __shared__ float part[8];
     let_next_start();
     wait_before();
+    if (blockIdx.y == l.n) {
+        find_pieces(pieces);
+        return;
+    }
     const PrepItem& it = l.it[blockIdx.y];
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (blockIdx.x >= l.blocks[blockIdx.y]) return;
     float top = 0.f;
-    if (it.mode == kPack) prep_pack(it);
-    else if (prep_wide(it)) prep_block(it, part, top);
-    else prep_narrow(it, top);
+    auto over_block = [&](float v) {             // the block's largest, in every thread
+        v = warp_max(v);
+        if (lane == 0) part[warp] = v;
+        __syncthreads();
+        v = part[lane & 7];
+        __syncthreads();
+        return warp_max(v);
+    };
+    unsigned max = 0;
+    if (it.mode == kTensorSplit || it.mode == kWeighted) {
+        float v = 0.f;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < it.parts; i += 256) v = fmaxf(v, __uint_as_float(it.part[i]));
+        max = __float_as_uint(over_block(v));
+        if (blockIdx.x == 0 && threadIdx.x == 0) *it.max = max;
+    }
+    const int blocks = l.blocks[blockIdx.y];
+    if (it.mode == kPack) prep_pack(it, blocks);
+    else if (prep_wide(it)) prep_block(it, blocks, part, max, top);
+    else prep_narrow(it, blocks, max, top);
     // the epilogue reads scales of columns 32 at a time
     if (it.mode == kRowSplit && blockIdx.x == 0 && threadIdx.x < 32 &&
         it.rows + lane < (it.rows + 31) / 32 * 32)
         it.rinv[it.rows + lane] = 0.f;
-    if (it.max && (it.mode == kMax || it.mode == kRowSplit)) {
-        top = warp_max(top);
-        if (lane == 0 && top > 0.f) atomicMax(it.max, __float_as_uint(top));
+    if (it.part && (it.mode == kMax || it.mode == kRowSplit)) {
+        __syncthreads();
+        top = over_block(top);
+        if (threadIdx.x == 0) it.part[blockIdx.x] = __float_as_uint(top);
     }
 }
 
-int prepare(const PrepList& l, Chain& st) {
-    if (l.n == 0) return ATOM_OK;
-    long long blocks = 1;
-    for (int i = 0; i < l.n; ++i) {
-        const PrepItem& it = l.it[i];
-        const int rows = it.mode == kPack ? 8 : prep_wide(it) ? 1 : 8 * (kNV / prep_slots(it));
-        blocks = std::max(blocks, (it.rows + rows - 1) / rows);
-    }
-    return st.launch("operand preparation", prep_kernel,
-                     dim3((unsigned)std::min(blocks, 2368LL), l.n), 256, 0, l);
+int prep_blocks(const PrepItem& it) {
+    const int rows = it.mode == kPack ? 8 : prep_wide(it) ? 1 : 8 * (kNV / prep_slots(it));
+    return (int)std::max(1LL, std::min((it.rows + rows - 1) / rows, (long long)kPrepBlocks));
+}
+int prepare(PrepList& l, Chain& st, const Pieces* pieces) {
+    if (l.n == 0 && !pieces) return ATOM_OK;
+    int grid = 1;
+    for (int i = 0; i < l.n; ++i) grid = std::max(grid, l.blocks[i] = prep_blocks(l.it[i]));
+    Pieces none{};
+    if (pieces)
+        grid = std::max(grid, (pieces->pieces + pieces->tiles + 7) / 8 +
+                                  (pieces->other ? 4 * pieces->nad : 0));
+    const int s = st.launch("operand preparation", prep_kernel, dim3(grid, l.n + (pieces != nullptr)),
+                            256, 0, l, pieces ? *pieces : none);
+    l.n = 0;
+    return s;
 }
 
 static PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -1486,9 +1602,9 @@ static int run(const Maps& maps, const Args& p, Chain& st) {
                           CF::kSmem, maps, p))
         return s;
     if (EPI != kLow && p.ksplit > 1) {
-        const long long blocks = (p.M * p.N * p.groups + 1023) / 1024;
+        const long long blocks = (p.M * p.N * p.groups / (p.N % 4 ? 1 : 4) + 255) / 256;
         return st.launch("pair product sums", reduce_kernel,
-                         dim3((unsigned)(blocks < 1184 ? blocks : 1184)), 256, 0, p);
+                         dim3((unsigned)std::min(std::max(blocks, 1LL), 1184LL)), 256, 0, p);
     }
     return ATOM_OK;
 }

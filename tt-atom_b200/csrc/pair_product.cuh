@@ -63,7 +63,9 @@ struct Args {
     int* usable;             // from kLow on: the same adapter, -1 also where it is not finite
     const int4* bad;         // of an adapter: not all zero = not finite, its rows become NaN
     const float* low_scale;  // kLow: per adapter
-    void* low_block;         // kLow: [block][256][Rs] typed, or NULL (SPLIT)
+    void* low_block;         // kLow: [block][256][Rs] typed (SPLIT: planes low_plane apart, NULL
+    long long low_plane;     // for more than 64 ranks), and SPLIT 1 / scale of the rows
+    float* low_rinv;
     void* low_rows;          // kLow: [M][Rs] typed, or NULL
     int Rs;
     const float* ext_rinv;   // SPLIT: of the low-rank rows
@@ -107,16 +109,37 @@ struct PrepItem {
     void* dst;               // [rows][dld], the lo plane `plane` elements behind
     long long dld, plane;
     float* rinv;             // kRowSplit, kRowScale: 1 / scale of each row, 0 for a row of zeros
-    unsigned* max;           // written by kMax; by kRowSplit (with weight): the largest
-    int mode;                // rinv[r] * weight[r]; read by kTensorSplit and kWeighted
+    // kMax, and kRowSplit with a weight (the largest rinv[r] * weight[r]): a maximum of each block
+    // goes to part[block]. kTensorSplit, kWeighted: the largest of part[0 .. parts - 1], which its
+    // first block leaves in *max for the products
+    unsigned* max;
+    int mode;
     const float* weight;
+    unsigned* part = nullptr;
+    int parts = 0;
 };
+constexpr int kPrepBlocks = 1184;            // of one launch and item, at most
+int prep_blocks(const PrepItem& it);          // how many maxima an item writes
 struct PrepList {
     PrepItem it[6];
-    int n = 0;
+    int n = 0, blocks[6];
     void add(const PrepItem& i) { it[n++] = i; }
 };
-int prepare(const PrepList& l, Chain& st);
+
+// The pieces of an adapters call's requests (adapters.cu), found in a preparation launch beside its
+// matrices.
+struct Pieces {
+    const int *ptr, *adapter;
+    int n, nad, M;           // requests, adapters, rows
+    int tiles, pieces;       // row tiles; and requests
+    int4* piece;             // adapter or -1, first row, behind the last row
+    int4* tile_req;          // requests first .. behind that reach into a row tile
+    const void* other;       // the matrix of each adapter beside the projection: `other_n` values
+    long long other_n;
+    int4* bad;               // per adapter: a quarter of them is not finite
+    int dtype;
+};
+int prepare(PrepList& l, Chain& st, const Pieces* pieces = nullptr);      // empties the list
 
 inline bool tma_ready(const void* p, long long ld) { return aligned16(p) && ld % 8 == 0; }
 inline long long up(long long n, long long k) { return (n + k - 1) / k * k; }

@@ -85,6 +85,15 @@ __device__ __forceinline__ float2 pair_f(uint32_t w, int dtype) {
                               : __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
+__device__ __forceinline__ uint32_t pair_w(float a, float b, int dtype) {
+    if (dtype == ATOM_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // A call's kernels on its stream. Each after the first starts while the one before it still runs
 // (it sets up, then waits in wait_before() for what that one writes), which hides the launches.
 struct Chain {
@@ -107,13 +116,6 @@ struct Chain {
         cudaLaunchKernelEx(&c, kernel, args...);
         after = true;
         return check_launch(what);
-    }
-    int zero(const char* what, void* p, size_t n) {
-        const cudaError_t e = n ? cudaMemsetAsync(p, 0, n, st) : cudaSuccess;
-        after = false;
-        if (e == cudaSuccess) return ATOM_OK;
-        set_error("%s: %s", what, cudaGetErrorString(e));
-        return ATOM_ERR_CUDA;
     }
 };
 // Waits for the kernel before this one (a launch without overlap: at once).
