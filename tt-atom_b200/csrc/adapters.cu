@@ -344,7 +344,7 @@ struct AdSizes {
 // second time where the forward pass kept no S.
 struct AdSpace {
     __half *rows, *x, *w, *first, *first2, *ext, *block;
-    float *rinv, *xinv, *wr, *ext_rinv, *part, *gpart, *few_S;
+    float *rinv, *xinv, *wr, *ext_rinv, *part, *gpart, *few_S, *few_T, *few_dx;
     void *S, *T;
     int4 *piece, *bad, *tile_req;
     int *usable, *few_slot;
@@ -355,6 +355,14 @@ struct AdSpace {
         memset(this, 0, sizeof(*this));
         Cursor c(ws);
         const long long k = z.split ? 2 : 1, e = dtype_size(z.dtype);
+        if (z.M <= few::kFewRows) {
+            few_S = c.take<float>(z.M * z.R);
+            few_T = c.take<float>(bwd ? z.M * z.R : 0);
+            few_slot = c.take<int>(z.M);
+            if (bwd) few_dx = c.take<float>(few::down_shares(z.O, z.D, z.dtype) * z.M * z.D);
+            bytes = c.used;
+            return;
+        }
         const long long a_n = (long long)z.nad * z.R * z.Dp, b_n = (long long)z.nad * z.O * z.Rs;
         rows = c.take<__half>(k * z.M * (bwd ? z.Op : z.Dp));
         w = c.take<__half>(k * z.O * z.Dp);
@@ -367,10 +375,6 @@ struct AdSpace {
             ext_rinv = c.take<float>(z.on ? z.M : 0);
         }
         if (z.on) {
-            if (!bwd && z.M <= few::kFewRows) {
-                few_S = c.take<float>(z.M * z.R);
-                few_slot = c.take<int>(z.M);
-            }
             piece = c.take<int4>(z.pieces);
             bad = c.take<int4>(z.nad);
             tile_req = c.take<int4>(z.tiles);
@@ -634,15 +638,20 @@ extern "C" int atom_adapted_linear_fwd(int dtype, const void* x, int64_t ldx, in
     Ad f{z, AdSpace(ws, z, false), (cudaStream_t)stream, req_ptr, req_adapter, scale, w, a, b};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "adapted_linear: the workspace needs %zu bytes",
                  f.sp.bytes);
-    if (few::suits(dtype, M, D, x, ldx, w, a)) {
+    if (M <= few::kFewRows) {
         // a few rows: the low-rank values first, then the projection with them in its epilogue;
         // nothing is kept, the backward pass computes S again
         if (z.on)
             if (int s = few::low_rank({x, ldx, (int)M, D, a, R, scale, req_ptr, req_adapter, nreq,
                                        n_adapters, f.sp.few_S, f.sp.few_slot, dtype}, f.st))
                 return s;
-        return few::product({x, ldx, (int)M, D, {w, nullptr}, O, 0, y, ldy, dtype,
-                             z.on ? f.sp.few_S : nullptr, f.sp.few_slot, b, R}, f.st);
+        few::Args p{};
+        p.x = x, p.ldx = ldx, p.M = (int)M, p.K = D, p.N = O;
+        p.w[0] = w;
+        p.out = y, p.ldo = ldy;
+        p.dtype = dtype;
+        p.S = z.on ? f.sp.few_S : nullptr, p.slot = f.sp.few_slot, p.b = b, p.R = R;
+        return few::product(p, f.st);
     }
     return f.run(x, ldx, false, y, ldy, kept);
 }
@@ -672,7 +681,27 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "adapted_linear: the workspace needs %zu bytes",
                  f.sp.bytes);
     const bool grads = z.on && (da || db);
-    if (few::suits(dtype, M, D, x, ldx, w, a)) kept = nullptr;
+    if (M <= few::kFewRows) {
+        const int m = (int)M, shares = few::down_shares(O, D, dtype);
+        if (z.on) {
+            if (int s = few::low_rank({x, ldx, m, D, a, R, scale, req_ptr, req_adapter, nreq,
+                                       n_adapters, f.sp.few_S, f.sp.few_slot, dtype}, f.st))
+                return s;
+            if (int s = few::low_rank_back({dy, lddy, m, O, b, R, scale, f.sp.few_slot, f.sp.few_T,
+                                            dtype}, f.st))
+                return s;
+        }
+        if (grads)
+            if (int s = few::adapter_grads({f.sp.few_T, f.sp.few_S, f.sp.few_slot, x, dy, ldx, lddy,
+                                            m, D, O, R, n_adapters, da, db, dtype}, f.st))
+                return s;
+        if (!dx) return ATOM_OK;
+        if (int s = few::down({{dy, nullptr}, lddy, 0, m, O, {w, nullptr}, D, shares, f.sp.few_dx,
+                               dtype}, f.st))
+            return s;
+        return few::sum({f.sp.few_dx, shares, m, D, dx, lddx, z.on ? f.sp.few_T : nullptr,
+                         f.sp.few_slot, a, R, dtype}, f.st);
+    }
     if (grads || dx)
         if (int s = f.run(dy, lddy, true, dx, lddx, grads ? f.sp.T : nullptr)) return s;
     const bool again = grads && db && !kept;

@@ -5,6 +5,10 @@
 // rows of W the 8; K runs in the order that the loads give, which both operands share), so a block
 // has all its bytes of W in flight after a few instructions. Bound by HBM or L2: the launch that
 // follows in an operator starts early and has its first weights before it waits for the rows.
+// The backward pass sums down the columns of W (down_kernel: fp32 sums in registers, K shared out
+// over warps and blocks) and writes outer products of the rows (outer_kernel), in fp32 throughout.
+#include <algorithm>
+
 #include "few_rows.cuh"
 
 namespace atom {
@@ -26,6 +30,27 @@ __device__ __forceinline__ void mma(float* c, uint32_t a0, uint32_t a1, uint32_t
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// 8 (fp32: 4) elements of a row from k on, zeros past its end.
+__device__ __forceinline__ uint4 load16(const unsigned short* row, int k, int K, bool vec) {
+    if (vec) return *reinterpret_cast<const uint4*>(row + k);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        w[j] = (k + 2 * j < K ? row[k + 2 * j] : 0u) |
+               (k + 2 * j + 1 < K ? (uint32_t)row[k + 2 * j + 1] << 16 : 0u);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ float4 load16(const float* row, int k, int K, bool vec) {
+    if (vec) return *reinterpret_cast<const float4*>(row + k);
+    return make_float4(row[k], k + 1 < K ? row[k + 1] : 0.f, k + 2 < K ? row[k + 2] : 0.f,
+                       k + 3 < K ? row[k + 3] : 0.f);
+}
+// Whether rows of K elements, ld apart, start on 16 bytes and end there.
+__device__ __forceinline__ bool rows16(const void* p, int K, long long ld, int dtype) {
+    const int e = dtype == ATOM_F32 ? 4 : 8;
+    return aligned16(p) && K % e == 0 && ld % e == 0;
+}
+
 // The block's sums of 16 rows by 8 columns (red: [warp][matrix][16][8]) into out.
 template <bool GATED>
 __device__ __forceinline__ void finish(const Args& p, const float* red, int n0) {
@@ -38,6 +63,24 @@ __device__ __forceinline__ void finish(const Args& p, const float* red, int n0) 
     for (int k = 0; k < 8; ++k) {
         v += red[k * kMats * 128 + i];
         if (GATED) u += red[k * kMats * 128 + 128 + i];
+    }
+    if (GATED && p.dh) {
+        float d = 0.f, a, da;
+        const long long at = (long long)m * p.N + n, all = (long long)p.M * p.N;
+        for (int k = 0; k < p.dh_parts; ++k) d += p.dh[k * all + at];
+        if (p.act == 2) {
+            const float phi = 0.5f * erfcf(-0.70710678f * v);
+            a = v * phi;
+            da = phi + v * 0.39894228f * expf(-0.5f * v * v);
+        } else {
+            const float s = sigmoid_f(v);
+            a = p.act == 1 ? s : v * s;
+            da = p.act == 1 ? s * (1.f - s) : s * (1.f + v * (1.f - s));
+        }
+        p.grads[at] = d * u * da;
+        p.grads[all + at] = d * a;
+        p.grads[2 * all + at] = a * u;
+        return;
     }
     if (GATED) {
         if (p.act == 2) v *= 0.5f * erfcf(-0.70710678f * v);
@@ -70,6 +113,8 @@ __global__ void __launch_bounds__(256) few16_kernel(const __grid_constant__ Args
     const unsigned short* x0 = static_cast<const unsigned short*>(p.x) + g * p.ldx;
     const unsigned short* x1 = x0 + 8 * p.ldx;
     const bool in0 = g < p.M, in1 = !HALF && g + 8 < p.M;
+    const bool xv = rows16(p.x, p.K, p.ldx, p.dtype), wv = rows16(p.w[0], p.K, p.K, p.dtype) &&
+                                                           (!GATED || aligned16(p.w[kMats - 1]));
     const uint4 zero = make_uint4(0, 0, 0, 0);
     const int chunks = (p.K + 31) / 32, end = chunks * (warp + 1) / 8;
     float acc[kMats][4] = {};
@@ -82,7 +127,7 @@ __global__ void __launch_bounds__(256) few16_kernel(const __grid_constant__ Args
             const bool in = c + u < end && k < p.K;
 #pragma unroll
             for (int j = 0; j < kMats; ++j)
-                v[u][j] = in && in_w ? __ldg(reinterpret_cast<const uint4*>(w[j] + k)) : zero;
+                v[u][j] = in && in_w ? load16(w[j], k, p.K, wv) : zero;
         }
         if (!waited) {
             wait_before();
@@ -92,8 +137,8 @@ __global__ void __launch_bounds__(256) few16_kernel(const __grid_constant__ Args
         for (int u = 0; u < U; ++u) {
             const int k = (c + u) * 32 + t8;
             const bool in = c + u < end && k < p.K;
-            a[u] = in && in0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
-            b[u] = in && in1 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
+            a[u] = in && in0 ? load16(x0, k, p.K, xv) : zero;
+            b[u] = in && in1 ? load16(x1, k, p.K, xv) : zero;
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -121,6 +166,8 @@ __global__ void __launch_bounds__(256) few32_kernel(const __grid_constant__ Args
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n0 = blockIdx.x * 8;
     let_next_start();
     const int chunks = (p.K + 127) / 128, first = chunks * warp / 8, end = chunks * (warp + 1) / 8;
+    const bool xv = rows16(p.x, p.K, p.ldx, ATOM_F32), wv = rows16(p.w[0], p.K, p.K, ATOM_F32) &&
+                                                            (!GATED || aligned16(p.w[kMats - 1]));
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
     bool waited = false;
     for (int m0 = 0; m0 < 16; m0 += 8) {
@@ -137,9 +184,7 @@ __global__ void __launch_bounds__(256) few32_kernel(const __grid_constant__ Args
                 float4 b[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    b[i] = in && n0 + i < p.N
-                               ? __ldg(reinterpret_cast<const float4*>(w + (long long)i * p.K + k))
-                               : zero;
+                    b[i] = in && n0 + i < p.N ? load16(w + (long long)i * p.K, k, p.K, wv) : zero;
                 if (!waited) {
                     wait_before();
                     waited = true;
@@ -147,7 +192,7 @@ __global__ void __launch_bounds__(256) few32_kernel(const __grid_constant__ Args
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     if (m0 + i >= p.M) break;
-                    const float4 a = in ? *reinterpret_cast<const float4*>(x + i * p.ldx + k) : zero;
+                    const float4 a = in ? load16(x + i * p.ldx, k, p.K, xv) : zero;
 #pragma unroll
                     for (int n = 0; n < 8; ++n)
                         acc[8 * i + n] = fmaf(a.x, b[n].x, fmaf(a.y, b[n].y,
@@ -175,13 +220,13 @@ __global__ void __launch_bounds__(256) low_kernel(const __grid_constant__ LowArg
     if (a < 0 || r >= p.R) return;
     float v = 0.f;
     const long long at = ((long long)a * p.R + r) * p.K;
+    const bool xv = rows16(p.x, p.K, p.ldx, p.dtype), wv = rows16(p.a, p.K, p.K, p.dtype);
     if (p.dtype == ATOM_F32) {
         const float* x = static_cast<const float*>(p.x) + m * p.ldx;
         const float* w = static_cast<const float*>(p.a) + at;
 #pragma unroll 4
         for (int k = lane * 4; k < p.K; k += 128) {
-            const float4 c = *reinterpret_cast<const float4*>(x + k);
-            const float4 d = *reinterpret_cast<const float4*>(w + k);
+            const float4 c = load16(x, k, p.K, xv), d = load16(w, k, p.K, wv);
             v = fmaf(c.x, d.x, fmaf(c.y, d.y, fmaf(c.z, d.z, fmaf(c.w, d.w, v))));
         }
     } else {
@@ -189,8 +234,7 @@ __global__ void __launch_bounds__(256) low_kernel(const __grid_constant__ LowArg
         const unsigned short* w = static_cast<const unsigned short*>(p.a) + at;
 #pragma unroll 4
         for (int k = lane * 8; k < p.K; k += 256) {
-            const uint4 c = *reinterpret_cast<const uint4*>(x + k);
-            const uint4 d = *reinterpret_cast<const uint4*>(w + k);
+            const uint4 c = load16(x, k, p.K, xv), d = load16(w, k, p.K, wv);
             const uint32_t cc[4] = {c.x, c.y, c.z, c.w}, dd[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -203,11 +247,241 @@ __global__ void __launch_bounds__(256) low_kernel(const __grid_constant__ LowArg
     if (lane == 0) p.S[m * p.R + r] = v * p.scale[a];
 }
 
-bool suits(int dtype, long long M, int K, const void* x, long long ldx, const void* w0,
-           const void* w1) {
-    const int e = dtype == ATOM_F32 ? 4 : 8;
-    return M <= kFewRows && K % e == 0 && ldx % e == 0 && aligned16(x) && aligned16(w0) &&
-           aligned16(w1);
+// A block a row: threads have eight ranks and a share of O.
+__global__ void __launch_bounds__(256) low_back_kernel(const __grid_constant__ LowBackArgs p) {
+    __shared__ float red[256][9];
+    let_next_start();
+    wait_before();
+    const int m = blockIdx.x, a = p.slot[m];
+    if (a < 0) return;
+    const int chunks = (p.R + 7) / 8, groups = 256 / chunks;
+    const int g = threadIdx.x / chunks, r0 = (threadIdx.x - g * chunks) * 8;
+    float acc[8] = {};
+    const bool vec = p.R % 8 == 0 && aligned16(p.b);
+    if (g < groups) {
+        const int n = min(8, p.R - r0);
+        const long long at = (long long)a * p.O * p.R + r0;
+#pragma unroll 8
+        for (int o = g; o < p.O; o += groups) {
+            const float y = load_f(p.dy, m * p.ld + o, p.dtype);
+            const long long e = at + (long long)o * p.R;
+            float v[8];
+            if (vec && p.dtype != ATOM_F32) {
+                const uint4 w = *reinterpret_cast<const uint4*>(
+                    static_cast<const unsigned short*>(p.b) + e);
+                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = pair_f(ww[j], p.dtype);
+                    v[2 * j] = f.x, v[2 * j + 1] = f.y;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = j < n ? load_f(p.b, e + j, p.dtype) : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] = fmaf(y, v[j], acc[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) red[threadIdx.x][j] = acc[j];
+    __syncthreads();
+    for (int r = threadIdx.x >> 5; r < p.R; r += 8) {        // a warp a rank
+        float v = 0.f;
+        for (int k = threadIdx.x & 31; k < groups; k += 32) v += red[k * chunks + (r >> 3)][r & 7];
+        v = warp_sum(v);
+        if ((threadIdx.x & 31) == 0) p.T[m * p.R + r] = v * p.scale[a];
+    }
+}
+
+// A block has 32 lanes' columns (8 a lane, fp32 4) and a share of K, of which its 8 warps take
+// every eighth row; the warps' sums are added in order through shared memory.
+template <int DT, int MR>
+__global__ void __launch_bounds__(256) down_kernel(const __grid_constant__ DownArgs p) {
+    constexpr int C = DT == ATOM_F32 ? 4 : 8, kW = 32 * C, kK = 128;
+    __shared__ __align__(16) float as[kK][MR];
+    __shared__ float red[MR][kW];
+    let_next_start();
+    wait_before();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.x * kW + lane * C;
+    const int lo = (int)((long long)p.K * blockIdx.y / p.shares);
+    const int hi = (int)((long long)p.K * (blockIdx.y + 1) / p.shares);
+    const bool vec = rows16(p.w[0], p.N, p.N, DT) && (!p.a[1] || aligned16(p.w[1]));
+    float acc[MR][C];
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[m][c] = 0.f;
+    for (int j = 0; j < (p.a[1] ? 2 : 1); ++j)
+        for (int k0 = lo; k0 < hi; k0 += kK) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < kK * MR; i += 256) {
+                const int k = k0 + i % kK, m = i / kK;
+                as[i % kK][m] = k < hi && m < p.M
+                    ? load_f(p.a[j], m * p.lda + k, p.a32 ? ATOM_F32 : DT) : 0.f;
+            }
+            __syncthreads();
+            if (n >= p.N) continue;
+#pragma unroll 4
+            for (int i = warp; i < min(kK, hi - k0); i += 8) {
+                float w[C];
+                const long long at = (long long)(k0 + i) * p.N;
+                if constexpr (DT == ATOM_F32) {
+                    const float4 v = load16(static_cast<const float*>(p.w[j]) + at, n, p.N, vec);
+                    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                } else {
+                    const uint4 v = load16(static_cast<const unsigned short*>(p.w[j]) + at, n, p.N,
+                                           vec);
+                    const uint32_t ww[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float2 f = pair_f(ww[c], DT);
+                        w[2 * c] = f.x, w[2 * c + 1] = f.y;
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < MR; m += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(&as[i][m]);
+                    const float xx[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int c = 0; c < C; ++c) acc[m + e][c] = fmaf(xx[e], w[c], acc[m + e][c]);
+                }
+            }
+        }
+    for (int k = 0; k < 8; ++k) {
+        __syncthreads();
+        if (warp == k)
+#pragma unroll
+            for (int m = 0; m < MR; ++m)
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    float* q = &red[m][c * 32 + lane];       // a bank a lane
+                    *q = k ? *q + acc[m][c] : acc[m][c];
+                }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.M * kW; i += 256) {
+        const int m = i / kW, j = i % kW, col = blockIdx.x * kW + j;
+        if (col < p.N)
+            p.part[((long long)blockIdx.y * p.M + m) * p.N + col] = red[m][j % C * 32 + j / C];
+    }
+}
+__global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumArgs p) {
+    let_next_start();
+    wait_before();
+    const int n = blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
+    if (n >= p.N) return;
+    float v = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < p.shares; ++k) v += p.part[((long long)k * p.M + m) * p.N + n];
+    const int a = p.T ? p.slot[m] : -1;
+    if (a >= 0) {
+        const long long at = (long long)a * p.R * p.N + n;
+#pragma unroll 8
+        for (int r = 0; r < p.R; ++r)
+            v = fmaf(p.T[m * p.R + r], load_f(p.a, at + (long long)r * p.N, p.dtype), v);
+    }
+    store_f(p.out, m * p.ldo + n, v, p.dtype);
+}
+
+// 32 rows by 256 columns a block, 4 by 8 a thread. Bound by writing.
+__global__ void __launch_bounds__(256) outer_kernel(const __grid_constant__ OuterArgs p) {
+    __shared__ float ps[kFewRows][32];
+    __shared__ float qs[kFewRows][256];
+    let_next_start();
+    wait_before();
+    int k = 0;
+    while (k + 1 < p.n && blockIdx.x >= p.first[k + 1]) ++k;
+    const OuterItem& it = p.it[k];
+    const int tiles = (it.J + 255) / 256, b = blockIdx.x - p.first[k];
+    const int i0 = b / tiles * 32, j0 = b % tiles * 256;
+    for (int i = threadIdx.x; i < p.M * 32; i += 256) {
+        const int m = i >> 5, c = i0 + (i & 31);
+        ps[m][i & 31] = c < it.I ? load_f(it.p, m * it.ldp + c, it.p32 ? ATOM_F32 : p.dtype) : 0.f;
+    }
+    for (int i = threadIdx.x; i < p.M * 256; i += 256) {
+        const int m = i >> 8, c = j0 + (i & 255);
+        qs[m][i & 255] = c < it.J ? load_f(it.q, m * it.ldq + c, it.q32 ? ATOM_F32 : p.dtype) : 0.f;
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float acc[4][8] = {};
+    for (int m = 0; m < p.M; ++m) {
+        float x[4], y[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = ps[m][warp * 4 + i];
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(&qs[m][lane * 8 + j]);
+            y[j] = v.x, y[j + 1] = v.y, y[j + 2] = v.z, y[j + 3] = v.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+    }
+    const bool vec = rows16(it.out, it.J, it.J, p.dtype);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i0 + warp * 4 + i, c = j0 + lane * 8;
+        if (r >= it.I || c >= it.J) continue;
+        const long long at = (long long)r * it.J + c;
+        if (vec && c + 8 <= it.J) {
+            if (p.dtype == ATOM_F32) {
+                float4* q = reinterpret_cast<float4*>(static_cast<float*>(it.out) + at);
+                q[0] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+                q[1] = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
+            } else {
+                *reinterpret_cast<uint4*>(static_cast<unsigned short*>(it.out) + at) = make_uint4(
+                    pair_w(acc[i][0], acc[i][1], p.dtype), pair_w(acc[i][2], acc[i][3], p.dtype),
+                    pair_w(acc[i][4], acc[i][5], p.dtype), pair_w(acc[i][6], acc[i][7], p.dtype));
+            }
+        } else {
+            for (int j = 0; j < 8; ++j)
+                if (c + j < it.J) store_f(it.out, at + j, acc[i][j], p.dtype);
+        }
+    }
+}
+
+// Blocks of 256 columns of x, which write all ranks of dA, then blocks of 2,048 elements of dB.
+__global__ void __launch_bounds__(256) adapter_grads_kernel(const __grid_constant__ GradArgs p) {
+    let_next_start();
+    wait_before();
+    const int a = blockIdx.y, xb = p.da ? (p.D + 255) / 256 : 0;
+    unsigned mine = 0;
+#pragma unroll
+    for (int m = 0; m < kFewRows; ++m)
+        if (m < p.M && p.slot[m] == a) mine |= 1u << m;
+    if ((int)blockIdx.x < xb) {
+        const int k = blockIdx.x * 256 + threadIdx.x;
+        if (k >= p.D) return;
+        float v[kFewRows];
+#pragma unroll
+        for (int m = 0; m < kFewRows; ++m)
+            v[m] = mine >> m & 1 ? load_f(p.x, m * p.ldx + k, p.dtype) : 0.f;
+        for (int r = 0; r < p.R; ++r) {
+            float s = 0.f;
+#pragma unroll
+            for (int m = 0; m < kFewRows; ++m)
+                if (mine >> m & 1) s = fmaf(p.T[m * p.R + r], v[m], s);
+            store_f(p.da, ((long long)a * p.R + r) * p.D + k, s, p.dtype);
+        }
+        return;
+    }
+    const long long all = (long long)p.O * p.R, at = (long long)(blockIdx.x - xb) * 2048 + threadIdx.x;
+#pragma unroll 2
+    for (int j = 0; j < 8; ++j) {
+        const long long i = at + 256 * j;
+        if (i >= all) return;
+        const int o = (int)((unsigned)i / (unsigned)p.R), r = (int)(i - (long long)o * p.R);
+        float s = 0.f;
+        for (int m = 0; m < p.M; ++m)
+            if (mine >> m & 1)
+                s = fmaf(p.S[m * p.R + r], load_f(p.dy, m * p.lddy + o, p.dtype), s);
+        store_f(p.db, a * all + i, s, p.dtype);
+    }
 }
 
 int product(const Args& p, Chain& st) {
@@ -234,6 +508,41 @@ int product(const Args& p, Chain& st) {
 
 int low_rank(const LowArgs& p, Chain& st) {
     return st.launch("low-rank part of a few rows", low_kernel, dim3((p.R + 7) / 8, p.M), 256, 0, p);
+}
+int low_rank_back(const LowBackArgs& p, Chain& st) {
+    return st.launch("low-rank part of a few rows", low_back_kernel, dim3(p.M), 256, 0, p);
+}
+
+// Shares of K that give the GPU some three blocks an SM, 64 rows each at least.
+int down_shares(int K, int N, int dtype) {
+    const int w = dtype == ATOM_F32 ? 128 : 256, tiles = (N + w - 1) / w;
+    return std::max(1, std::min({444 / tiles, K / 64, 32}));
+}
+int down(const DownArgs& p, Chain& st) {
+    const int w = p.dtype == ATOM_F32 ? 128 : 256;
+    const bool half = p.M <= 8;
+    void (*k)(DownArgs) =
+        p.dtype == ATOM_F32    ? (half ? down_kernel<ATOM_F32, 8> : down_kernel<ATOM_F32, 16>)
+        : p.dtype == ATOM_BF16 ? (half ? down_kernel<ATOM_BF16, 8> : down_kernel<ATOM_BF16, 16>)
+                               : (half ? down_kernel<ATOM_F16, 8> : down_kernel<ATOM_F16, 16>);
+    return st.launch("product of a few rows", k, dim3((p.N + w - 1) / w, p.shares), 256, 0, p);
+}
+int sum(const SumArgs& p, Chain& st) {
+    return st.launch("sums of a few rows", sum_kernel, dim3((p.N + 255) / 256, p.M), 256, 0, p);
+}
+int outer(OuterArgs p, Chain& st) {
+    int n = 0;
+    for (int i = 0; i < p.n; ++i) {
+        p.first[i] = n;
+        n += (p.it[i].I + 31) / 32 * ((p.it[i].J + 255) / 256);
+    }
+    return n ? st.launch("outer products of a few rows", outer_kernel, dim3(n), 256, 0, p) : ATOM_OK;
+}
+int adapter_grads(const GradArgs& p, Chain& st) {
+    const long long n = (p.da ? (p.D + 255) / 256 : 0) +
+                        (p.db ? ((long long)p.O * p.R + 2047) / 2048 : 0);
+    return st.launch("adapters' gradients of a few rows", adapter_grads_kernel, dim3(n, p.nad), 256,
+                     0, p);
 }
 
 }  // namespace few

@@ -6,6 +6,7 @@
 //             dX = [dG | dU] [Wg; Wu],  dWg, dWu = [dG | dU]^T X,  dWd = dY^T H
 // The transposed products read their operands as they lie (M/N-major tiles), so nothing is
 // transposed in memory.
+#include <algorithm>
 #include <initializer_list>
 
 #include "few_rows.cuh"
@@ -43,7 +44,7 @@ struct FfSizes {
             down = choose(M, O, nk(F), 1, false, split, true);
         } else {
             dh = choose(M, F, nk(O), 1, false, split, false);
-            dx = choose(M, D, 2 * nk(F), 1, false, split, false);
+            dx = choose(M, D, 2 * nk(F), 1, false, split, true);
             dwgu = choose(F, D, nk(M), 2, false, split, true);
             dwd = choose(O, F, nk(M), 1, false, split, true);
         }
@@ -57,19 +58,33 @@ struct FfSpace {
     __half *x, *wg, *wu, *wd, *dy, *xt, *dyt, *hp, *dgup;
     float *xr, *wgr, *wur, *wdr, *dyr, *hr, *dgur, *H32, *dgu32, *dh, *part;
     __half *H, *dgu;
+    float *few_dh, *few_dx, *few_grads;
     unsigned *max, *maxima[4];  // of wg | wu, of wd, x'' factor, dy'' factor; and the blocks' own
     size_t bytes;
     FfSpace(void* ws, const FfSizes& z, bool bwd) {
         memset(this, 0, sizeof(*this));
         Cursor c(ws);
         const long long M = z.M, k = z.split ? 2 : 1, M32 = up(M, 32);
+        if (M <= few::kFewRows) {
+            if (bwd) {
+                few_dh = c.take<float>(few::down_shares(z.O, z.F, z.dtype) * M * z.F);
+                few_dx = c.take<float>(few::down_shares(z.F, z.D, z.dtype) * M * z.D);
+                few_grads = c.take<float>(3 * M * z.F);
+            } else if (z.split) {
+                H32 = c.take<float>(M * z.Fp);
+            } else {
+                H = c.take<__half>(M * z.Fp);
+            }
+            bytes = c.used;
+            return;
+        }
         x = c.take<__half>(k * M * z.Dp);
         wg = c.take<__half>(k * z.F * z.Dp);
         wu = c.take<__half>(k * z.F * z.Dp);
         wd = c.take<__half>(k * z.O * z.Fp);
         size_t pf = z.down.part;
         if (bwd) {
-            pf = z.dwgu.part > z.dwd.part ? z.dwgu.part : z.dwd.part;
+            pf = std::max({z.dx.part, z.dwgu.part, z.dwd.part});
             dy = c.take<__half>(k * M * z.Op);
             dh = c.take<float>(M32 * z.Fp);
         }
@@ -333,12 +348,57 @@ struct Ff {
     long long x_ld = 0, dy_ld = 0;
 };
 
-// Whether the forward pass runs as two products of a few rows. It keeps nothing then: the backward
-// pass, which sees the same operands, computes G and U again.
-bool few_rows(const FfSizes& z, const void* x, long long ldx, const void* wg, const void* wu,
-              const void* wd) {
-    return few::suits(z.dtype, z.M, z.D, x, ldx, wg, wu) &&
-           few::suits(z.dtype, z.M, z.F, nullptr, z.Fp, wd, nullptr);
+// A few rows: two products forward, which keep nothing; back, dH, then G and U again with dG, dU
+// and H from them in fp32, dX and the weights' outer products.
+int few_forward(Ff& f, const void* x, long long ldx, const void* wg, const void* wu, const void* wd,
+                void* y, long long ldy) {
+    const FfSizes& z = f.z;
+    void* h = z.split ? (void*)f.sp.H32 : f.sp.H;
+    few::Args p{};
+    p.x = x, p.ldx = ldx, p.M = (int)z.M, p.K = z.D, p.N = z.F;
+    p.w[0] = wg, p.w[1] = wu;
+    p.act = f.act;
+    p.out = h, p.ldo = z.Fp;
+    p.dtype = z.dtype;
+    if (int s = few::product(p, f.st)) return s;
+    few::Args q{};
+    q.x = h, q.ldx = z.Fp, q.M = (int)z.M, q.K = z.F, q.N = z.O;
+    q.w[0] = wd;
+    q.out = y, q.ldo = ldy;
+    q.dtype = z.dtype;
+    return few::product(q, f.st);
+}
+int few_backward(Ff& f, const void* x, long long ldx, const void* wg, const void* wu,
+                 const void* wd, const void* dy, long long lddy, void* dx, long long lddx,
+                 void* dwg, void* dwu, void* dwd) {
+    const FfSizes& z = f.z;
+    const int M = (int)z.M, t = z.dtype;
+    const int s1 = few::down_shares(z.O, z.F, t), s2 = few::down_shares(z.F, z.D, t);
+    if (int s = few::down({{dy, nullptr}, lddy, 0, M, z.O, {wd, nullptr}, z.F, s1, f.sp.few_dh, t},
+                          f.st))
+        return s;
+    few::Args p{};
+    p.x = x, p.ldx = ldx, p.M = M, p.K = z.D, p.N = z.F;
+    p.w[0] = wg, p.w[1] = wu;
+    p.act = f.act;
+    p.dtype = t;
+    p.dh = f.sp.few_dh, p.dh_parts = s1, p.grads = f.sp.few_grads;
+    if (int s = few::product(p, f.st)) return s;
+    const long long n = (long long)M * z.F;
+    const float *dg = f.sp.few_grads, *du = dg + n, *h = du + n;
+    if (dx) {
+        if (int s = few::down({{dg, du}, z.F, 1, M, z.F, {wg, wu}, z.D, s2, f.sp.few_dx, t}, f.st))
+            return s;
+        if (int s = few::sum({f.sp.few_dx, s2, M, z.D, dx, lddx, nullptr, nullptr, nullptr, 0, t},
+                             f.st))
+            return s;
+    }
+    few::OuterArgs o{};
+    o.M = M, o.dtype = t;
+    if (dwg) o.it[o.n++] = {dg, z.F, 1, z.F, x, ldx, 0, z.D, dwg};
+    if (dwu) o.it[o.n++] = {du, z.F, 1, z.F, x, ldx, 0, z.D, dwu};
+    if (dwd) o.it[o.n++] = {dy, lddy, 0, z.O, h, z.F, 1, z.F, dwd};
+    return few::outer(o, f.st);
 }
 
 int check_ff(int dtype, int64_t M, int D, int F, int O, int act) {
@@ -375,14 +435,7 @@ extern "C" int atom_gated_ff_fwd(int dtype, const void* x, int64_t ldx, int64_t 
     Ff f{z, FfSpace(ws, z, false), (cudaStream_t)stream, act};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
                  f.sp.bytes);
-    void* h = z.split ? (void*)f.sp.H32 : f.sp.H;
-    if (few_rows(z, x, ldx, wg, wu, wd)) {
-        if (int s = few::product({x, ldx, (int)M, D, {wg, wu}, F, act, h, z.Fp, dtype, nullptr,
-                                  nullptr, nullptr, 0}, f.st))
-            return s;
-        return few::product({h, z.Fp, (int)M, F, {wd, nullptr}, O, 0, y, ldy, dtype, nullptr,
-                             nullptr, nullptr, 0}, f.st);
-    }
+    if (M <= few::kFewRows) return few_forward(f, x, ldx, wg, wu, wd, y, ldy);
     if (int s = f.inputs(x, ldx, wg, wu, wd)) return s;
     return f.forward(y, ldy, static_cast<float*>(kept));
 }
@@ -408,7 +461,8 @@ extern "C" int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t 
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
                  f.sp.bytes);
     f.x_src = x, f.x_ld = ldx, f.dy_src = dy, f.dy_ld = lddy;
-    if (few_rows(z, x, ldx, wg, wu, wd)) kept = nullptr;
+    if (M <= few::kFewRows)
+        return few_backward(f, x, ldx, wg, wu, wd, dy, lddy, dx, lddx, dwg, dwu, dwd);
     if (int s = f.inputs_bwd(x, ldx, wg, wu, wd, dy, lddy, kept != nullptr)) return s;
     return f.backward(static_cast<const float*>(kept), dx, lddx, dwg, dwu, dwd);
 }
