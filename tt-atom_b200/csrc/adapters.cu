@@ -278,11 +278,19 @@ __global__ void __launch_bounds__(256) grads_sum_kernel(const __grid_constant__ 
         const int a = i / groups, r0 = (i - a * groups) * 4, n = min(4, p.R - r0);
         const float* part = p.part + a * per + (long long)r0 * W + k;
         float v[4] = {};
-#pragma unroll 4
-        for (int s = 0; s < p.split; ++s)
+        for (int s0 = 0; s0 < p.split; s0 += 8) {    // 32 loads at once
+            float t[8][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < n) v[j] += part[s * all + (long long)j * W];
+            for (int s = 0; s < 8; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    t[s][j] = j < n && s0 + s < p.split
+                        ? part[(s0 + s) * all + (long long)j * W] : 0.f;
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += t[s][j];
+        }
         const long long at = first ? ((long long)a * p.R + r0) * p.width[0] + k
                                    : ((long long)a * p.width[1] + k - p.width[0]) * p.R + r0;
         const long long step = first ? p.width[0] : 1;
@@ -359,7 +367,7 @@ struct AdSpace {
             few_S = c.take<float>(z.M * z.R);
             few_T = c.take<float>(bwd ? z.M * z.R : 0);
             few_slot = c.take<int>(z.M);
-            if (bwd) few_dx = c.take<float>(few::down_shares(z.O, z.D, z.dtype) * z.M * z.D);
+            if (bwd) few_dx = c.take<float>(few::down_shares(z.O, z.D) * z.M * z.D);
             bytes = c.used;
             return;
         }
@@ -682,7 +690,7 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
                  f.sp.bytes);
     const bool grads = z.on && (da || db);
     if (M <= few::kFewRows) {
-        const int m = (int)M, shares = few::down_shares(O, D, dtype);
+        const int m = (int)M, shares = few::down_shares(O, D);
         if (z.on) {
             if (int s = few::low_rank({x, ldx, m, D, a, R, scale, req_ptr, req_adapter, nreq,
                                        n_adapters, f.sp.few_S, f.sp.few_slot, dtype}, f.st))

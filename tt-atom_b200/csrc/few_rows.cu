@@ -51,22 +51,23 @@ __device__ __forceinline__ bool rows16(const void* p, int K, long long ld, int d
     return aligned16(p) && K % e == 0 && ld % e == 0;
 }
 
-// The block's sums of 16 rows by 8 columns (red: [warp][matrix][16][8]) into out.
-template <bool GATED>
+// The block's sums of ROWS rows by 8 columns (red: [warp][matrix][ROWS][8]) into out.
+template <bool GATED, int ROWS>
 __device__ __forceinline__ void finish(const Args& p, const float* red, int n0) {
     __syncthreads();
     const int i = threadIdx.x, m = i >> 3, n = n0 + (i & 7);
-    if (i >= 128 || m >= p.M || n >= p.N) return;
+    if (i >= ROWS * 8 || m >= p.M || n >= p.N) return;
     constexpr int kMats = GATED ? 2 : 1;
     float v = 0.f, u = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        v += red[k * kMats * 128 + i];
-        if (GATED) u += red[k * kMats * 128 + 128 + i];
+        v += red[k * kMats * ROWS * 8 + i];
+        if (GATED) u += red[(k * kMats + 1) * ROWS * 8 + i];
     }
     if (GATED && p.dh) {
         float d = 0.f, a, da;
         const long long at = (long long)m * p.N + n, all = (long long)p.M * p.N;
+#pragma unroll 8
         for (int k = 0; k < p.dh_parts; ++k) d += p.dh[k * all + at];
         if (p.act == 2) {
             const float phi = 0.5f * erfcf(-0.70710678f * v);
@@ -154,15 +155,15 @@ __global__ void __launch_bounds__(256) few16_kernel(const __grid_constant__ Args
         *reinterpret_cast<float2*>(r) = make_float2(acc[j][0], acc[j][1]);
         *reinterpret_cast<float2*>(r + 64) = make_float2(acc[j][2], acc[j][3]);
     }
-    finish<GATED>(p, red, n0);
+    finish<GATED, 16>(p, red, n0);
 }
 
-// fp32: 8 rows of W by 8 of x a warp (16 rows in two passes over the block's W, the second from
-// L1), float4 along K, the 64 sums added over the lanes by halves.
+// fp32: 8 rows of W by 8 of x a warp (more rows in passes over the block's W, all but the
+// first from L1), float4 along K, the 64 sums added over the lanes by halves.
 template <bool GATED>
-__global__ void __launch_bounds__(256) few32_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(256, 2) few32_kernel(const __grid_constant__ Args p) {
     constexpr int kMats = GATED ? 2 : 1;
-    __shared__ float red[8 * kMats * 128];
+    __shared__ float red[8 * kMats * kFewRows * 8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n0 = blockIdx.x * 8;
     let_next_start();
     const int chunks = (p.K + 127) / 128, first = chunks * warp / 8, end = chunks * (warp + 1) / 8;
@@ -170,15 +171,15 @@ __global__ void __launch_bounds__(256) few32_kernel(const __grid_constant__ Args
                                                             (!GATED || aligned16(p.w[kMats - 1]));
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
     bool waited = false;
-    for (int m0 = 0; m0 < 16; m0 += 8) {
-#pragma unroll
+    for (int m0 = 0; m0 < p.M; m0 += 8) {
+#pragma unroll 1
         for (int j = 0; j < kMats; ++j) {
             float acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0.f;
             const float* w = static_cast<const float*>(p.w[j]) + (long long)n0 * p.K;
             const float* x = static_cast<const float*>(p.x) + m0 * p.ldx;
-            for (int c = first; m0 < p.M && (c < end || !waited); ++c) {
+            for (int c = first; c < end || !waited; ++c) {
                 const int k = c * 128 + lane * 4;
                 const bool in = c < end && k < p.K;
                 float4 b[8];
@@ -190,21 +191,29 @@ __global__ void __launch_bounds__(256) few32_kernel(const __grid_constant__ Args
                     waited = true;
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (m0 + i >= p.M) break;
-                    const float4 a = in ? load16(x + i * p.ldx, k, p.K, xv) : zero;
+                for (int i0 = 0; i0 < 8; i0 += 4) {          // four rows' loads at once
+                    if (m0 + i0 >= p.M) break;
+                    float4 a[4];
 #pragma unroll
-                    for (int n = 0; n < 8; ++n)
-                        acc[8 * i + n] = fmaf(a.x, b[n].x, fmaf(a.y, b[n].y,
-                                         fmaf(a.z, b[n].z, fmaf(a.w, b[n].w, acc[8 * i + n]))));
+                    for (int i = 0; i < 4; ++i)
+                        a[i] = in && m0 + i0 + i < p.M
+                            ? load16(x + (i0 + i) * p.ldx, k, p.K, xv) : zero;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) {
+                            float& v = acc[8 * (i0 + i) + n];
+                            v = fmaf(a[i].x, b[n].x, fmaf(a[i].y, b[n].y,
+                                fmaf(a[i].z, b[n].z, fmaf(a[i].w, b[n].w, v))));
+                        }
                 }
             }
             sum_halves<64>(acc, lane);
-            *reinterpret_cast<float2*>(red + (warp * kMats + j) * 128 + m0 * 8 + 2 * lane) =
+            *reinterpret_cast<float2*>(red + (warp * kMats + j) * kFewRows * 8 + m0 * 8 + 2 * lane) =
                 make_float2(acc[0], acc[1]);
         }
     }
-    finish<GATED>(p, red, n0);
+    finish<GATED, kFewRows>(p, red, n0);
 }
 
 // One warp a value of S, eight to a block; K along the lanes.
@@ -294,24 +303,21 @@ __global__ void __launch_bounds__(256) low_back_kernel(const __grid_constant__ L
     }
 }
 
-// A block has 32 lanes' columns (8 a lane, fp32 4) and a share of K, of which its 8 warps take
-// every eighth row; the warps' sums are added in order through shared memory.
+// A block has 64 columns, two a lane, and a share of K, of which its 8 warps take every eighth
+// row; the warps' sums meet in shared memory, in order. Bound by loading W: few columns a thread
+// leave registers for 32 warps an SM (8 columns: 178 registers, one block an SM, twice the time).
 template <int DT, int MR>
 __global__ void __launch_bounds__(256) down_kernel(const __grid_constant__ DownArgs p) {
-    constexpr int C = DT == ATOM_F32 ? 4 : 8, kW = 32 * C, kK = 128;
-    __shared__ __align__(16) float as[kK][MR];
-    __shared__ float red[MR][kW];
+    constexpr int kW = 64, kK = 128;
+    __shared__ __align__(16) float as[kK][MR + 4];
+    __shared__ __align__(8) float red[8][MR][kW / 2];
     let_next_start();
     wait_before();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.x * kW + lane * C;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.x * kW + lane * 2;
     const int lo = (int)((long long)p.K * blockIdx.y / p.shares);
     const int hi = (int)((long long)p.K * (blockIdx.y + 1) / p.shares);
-    const bool vec = rows16(p.w[0], p.N, p.N, DT) && (!p.a[1] || aligned16(p.w[1]));
-    float acc[MR][C];
-#pragma unroll
-    for (int m = 0; m < MR; ++m)
-#pragma unroll
-        for (int c = 0; c < C; ++c) acc[m][c] = 0.f;
+    const bool vec = p.N % 2 == 0 && ((uintptr_t)p.w[0] & 7) == 0 && ((uintptr_t)p.w[1] & 7) == 0;
+    float acc[2][MR] = {};
     for (int j = 0; j < (p.a[1] ? 2 : 1); ++j)
         for (int k0 = lo; k0 < hi; k0 += kK) {
             __syncthreads();
@@ -322,73 +328,74 @@ __global__ void __launch_bounds__(256) down_kernel(const __grid_constant__ DownA
             }
             __syncthreads();
             if (n >= p.N) continue;
-#pragma unroll 4
+#pragma unroll 8
             for (int i = warp; i < min(kK, hi - k0); i += 8) {
-                float w[C];
-                const long long at = (long long)(k0 + i) * p.N;
-                if constexpr (DT == ATOM_F32) {
-                    const float4 v = load16(static_cast<const float*>(p.w[j]) + at, n, p.N, vec);
-                    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-                } else {
-                    const uint4 v = load16(static_cast<const unsigned short*>(p.w[j]) + at, n, p.N,
-                                           vec);
-                    const uint32_t ww[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float2 f = pair_f(ww[c], DT);
-                        w[2 * c] = f.x, w[2 * c + 1] = f.y;
-                    }
-                }
+                const long long at = (long long)(k0 + i) * p.N + n;
+                float2 w;
+                if (vec)
+                    w = DT == ATOM_F32
+                        ? *reinterpret_cast<const float2*>(static_cast<const float*>(p.w[j]) + at)
+                        : pair_f(*reinterpret_cast<const uint32_t*>(
+                                     static_cast<const unsigned short*>(p.w[j]) + at), DT);
+                else
+                    w = make_float2(load_f(p.w[j], at, DT),
+                                    n + 1 < p.N ? load_f(p.w[j], at + 1, DT) : 0.f);
 #pragma unroll
                 for (int m = 0; m < MR; m += 4) {
                     const float4 x = *reinterpret_cast<const float4*>(&as[i][m]);
                     const float xx[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int c = 0; c < C; ++c) acc[m + e][c] = fmaf(xx[e], w[c], acc[m + e][c]);
+                    for (int e = 0; e < 4; ++e) {
+                        acc[0][m + e] = fmaf(xx[e], w.x, acc[0][m + e]);
+                        acc[1][m + e] = fmaf(xx[e], w.y, acc[1][m + e]);
+                    }
                 }
             }
         }
-    for (int k = 0; k < 8; ++k) {
+    for (int c = 0; c < 2; ++c) {                    // even columns, odd ones
         __syncthreads();
-        if (warp == k)
 #pragma unroll
-            for (int m = 0; m < MR; ++m)
+        for (int m = 0; m < MR; ++m) red[warp][m][lane] = c ? acc[1][m] : acc[0][m];
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.M * 32; i += 256) {
+            const int m = i >> 5, col = blockIdx.x * kW + 2 * lane + c;
+            float v = 0.f;
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    float* q = &red[m][c * 32 + lane];       // a bank a lane
-                    *q = k ? *q + acc[m][c] : acc[m][c];
-                }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.M * kW; i += 256) {
-        const int m = i / kW, j = i % kW, col = blockIdx.x * kW + j;
-        if (col < p.N)
-            p.part[((long long)blockIdx.y * p.M + m) * p.N + col] = red[m][j % C * 32 + j / C];
+            for (int k = 0; k < 8; ++k) v += red[k][m][lane];
+            if (col < p.N) p.part[((long long)blockIdx.y * p.M + m) * p.N + col] = v;
+        }
     }
 }
+// 32 columns of a row a block; its 8 warps share out the shares and the ranks.
 __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumArgs p) {
+    __shared__ float red[8][32];
     let_next_start();
     wait_before();
-    const int n = blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
-    if (n >= p.N) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.x * 32 + lane;
+    const int m = blockIdx.y, a = p.T ? p.slot[m] : -1;
     float v = 0.f;
+    if (n < p.N) {
 #pragma unroll 8
-    for (int k = 0; k < p.shares; ++k) v += p.part[((long long)k * p.M + m) * p.N + n];
-    const int a = p.T ? p.slot[m] : -1;
-    if (a >= 0) {
-        const long long at = (long long)a * p.R * p.N + n;
-#pragma unroll 8
-        for (int r = 0; r < p.R; ++r)
-            v = fmaf(p.T[m * p.R + r], load_f(p.a, at + (long long)r * p.N, p.dtype), v);
+        for (int k = warp; k < p.shares; k += 8) v += p.part[((long long)k * p.M + m) * p.N + n];
+        if (a >= 0) {
+            const long long at = (long long)a * p.R * p.N + n;
+#pragma unroll 4
+            for (int r = warp; r < p.R; r += 8)
+                v = fmaf(p.T[m * p.R + r], load_f(p.a, at + (long long)r * p.N, p.dtype), v);
+        }
     }
+    red[warp][lane] = v;
+    __syncthreads();
+    if (warp || n >= p.N) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) v += red[k][lane];
     store_f(p.out, m * p.ldo + n, v, p.dtype);
 }
 
-// 32 rows by 256 columns a block, 4 by 8 a thread. Bound by writing.
+// 64 rows by 256 columns a block, twice 4 by 8 a thread. Bound by writing.
 __global__ void __launch_bounds__(256) outer_kernel(const __grid_constant__ OuterArgs p) {
-    __shared__ float ps[kFewRows][32];
+    constexpr int kRows = 64;
+    __shared__ float ps[kFewRows][kRows];
     __shared__ float qs[kFewRows][256];
     let_next_start();
     wait_before();
@@ -396,10 +403,10 @@ __global__ void __launch_bounds__(256) outer_kernel(const __grid_constant__ Oute
     while (k + 1 < p.n && blockIdx.x >= p.first[k + 1]) ++k;
     const OuterItem& it = p.it[k];
     const int tiles = (it.J + 255) / 256, b = blockIdx.x - p.first[k];
-    const int i0 = b / tiles * 32, j0 = b % tiles * 256;
-    for (int i = threadIdx.x; i < p.M * 32; i += 256) {
-        const int m = i >> 5, c = i0 + (i & 31);
-        ps[m][i & 31] = c < it.I ? load_f(it.p, m * it.ldp + c, it.p32 ? ATOM_F32 : p.dtype) : 0.f;
+    const int i0 = b / tiles * kRows, j0 = b % tiles * 256;
+    for (int i = threadIdx.x; i < p.M * kRows; i += 256) {
+        const int m = i / kRows, c = i0 + i % kRows;
+        ps[m][i % kRows] = c < it.I ? load_f(it.p, m * it.ldp + c, it.p32 ? ATOM_F32 : p.dtype) : 0.f;
     }
     for (int i = threadIdx.x; i < p.M * 256; i += 256) {
         const int m = i >> 8, c = j0 + (i & 255);
@@ -407,40 +414,44 @@ __global__ void __launch_bounds__(256) outer_kernel(const __grid_constant__ Oute
     }
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float acc[4][8] = {};
-    for (int m = 0; m < p.M; ++m) {
-        float x[4], y[8];
+    const bool vec = rows16(it.out, it.J, it.J, p.dtype);
+    for (int r0 = 0; r0 < kRows && i0 + r0 < it.I; r0 += 32) {
+        float acc[4][8] = {};
+        for (int m = 0; m < p.M; ++m) {
+            float x[4], y[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = ps[m][warp * 4 + i];
+            for (int i = 0; i < 4; ++i) x[i] = ps[m][r0 + warp * 4 + i];
 #pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(&qs[m][lane * 8 + j]);
-            y[j] = v.x, y[j + 1] = v.y, y[j + 2] = v.z, y[j + 3] = v.w;
+            for (int j = 0; j < 8; j += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(&qs[m][lane * 4 + 32 * j]);
+                y[j] = v.x, y[j + 1] = v.y, y[j + 2] = v.z, y[j + 3] = v.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+            const int r = i0 + r0 + warp * 4 + i;
+            if (r >= it.I) continue;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
-    }
-    const bool vec = rows16(it.out, it.J, it.J, p.dtype);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = i0 + warp * 4 + i, c = j0 + lane * 8;
-        if (r >= it.I || c >= it.J) continue;
-        const long long at = (long long)r * it.J + c;
-        if (vec && c + 8 <= it.J) {
-            if (p.dtype == ATOM_F32) {
-                float4* q = reinterpret_cast<float4*>(static_cast<float*>(it.out) + at);
-                q[0] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-                q[1] = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
-            } else {
-                *reinterpret_cast<uint4*>(static_cast<unsigned short*>(it.out) + at) = make_uint4(
-                    pair_w(acc[i][0], acc[i][1], p.dtype), pair_w(acc[i][2], acc[i][3], p.dtype),
-                    pair_w(acc[i][4], acc[i][5], p.dtype), pair_w(acc[i][6], acc[i][7], p.dtype));
+            for (int h = 0; h < 8; h += 4) {
+                const int c = j0 + lane * 4 + 32 * h;
+                const long long at = (long long)r * it.J + c;
+                const float* v = acc[i] + h;
+                if (c >= it.J) continue;
+                if (!vec) {
+                    for (int j = 0; j < 4; ++j)
+                        if (c + j < it.J) store_f(it.out, at + j, v[j], p.dtype);
+                } else if (p.dtype == ATOM_F32) {
+                    *reinterpret_cast<float4*>(static_cast<float*>(it.out) + at) =
+                        make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                    *reinterpret_cast<uint2*>(static_cast<unsigned short*>(it.out) + at) =
+                        make_uint2(pair_w(v[0], v[1], p.dtype), pair_w(v[2], v[3], p.dtype));
+                }
             }
-        } else {
-            for (int j = 0; j < 8; ++j)
-                if (c + j < it.J) store_f(it.out, at + j, acc[i][j], p.dtype);
         }
     }
 }
@@ -513,28 +524,26 @@ int low_rank_back(const LowBackArgs& p, Chain& st) {
     return st.launch("low-rank part of a few rows", low_back_kernel, dim3(p.M), 256, 0, p);
 }
 
-// Shares of K that give the GPU some three blocks an SM, 64 rows each at least.
-int down_shares(int K, int N, int dtype) {
-    const int w = dtype == ATOM_F32 ? 128 : 256, tiles = (N + w - 1) / w;
-    return std::max(1, std::min({444 / tiles, K / 64, 32}));
+// Shares of K that give the GPU some four blocks an SM, 32 rows each at least.
+int down_shares(int K, int N, int most) {
+    return std::max(1, std::min({592 / ((N + 63) / 64), K / 32, most}));
 }
 int down(const DownArgs& p, Chain& st) {
-    const int w = p.dtype == ATOM_F32 ? 128 : 256;
     const bool half = p.M <= 8;
     void (*k)(DownArgs) =
         p.dtype == ATOM_F32    ? (half ? down_kernel<ATOM_F32, 8> : down_kernel<ATOM_F32, 16>)
         : p.dtype == ATOM_BF16 ? (half ? down_kernel<ATOM_BF16, 8> : down_kernel<ATOM_BF16, 16>)
                                : (half ? down_kernel<ATOM_F16, 8> : down_kernel<ATOM_F16, 16>);
-    return st.launch("product of a few rows", k, dim3((p.N + w - 1) / w, p.shares), 256, 0, p);
+    return st.launch("product of a few rows", k, dim3((p.N + 63) / 64, p.shares), 256, 0, p);
 }
 int sum(const SumArgs& p, Chain& st) {
-    return st.launch("sums of a few rows", sum_kernel, dim3((p.N + 255) / 256, p.M), 256, 0, p);
+    return st.launch("sums of a few rows", sum_kernel, dim3((p.N + 31) / 32, p.M), 256, 0, p);
 }
 int outer(OuterArgs p, Chain& st) {
     int n = 0;
     for (int i = 0; i < p.n; ++i) {
         p.first[i] = n;
-        n += (p.it[i].I + 31) / 32 * ((p.it[i].J + 255) / 256);
+        n += (p.it[i].I + 63) / 64 * ((p.it[i].J + 255) / 256);
     }
     return n ? st.launch("outer products of a few rows", outer_kernel, dim3(n), 256, 0, p) : ATOM_OK;
 }

@@ -1,4 +1,4 @@
-// Products of a few rows (up to kFewRows): streaming a weight matrix past rows that fit registers.
+// Products of a few rows: streaming a weight matrix past rows that fit registers.
 #pragma once
 
 #include "typed.cuh"
@@ -6,6 +6,8 @@
 namespace atom {
 namespace few {
 
+// One tensor-core tile's rows. (fp32 with 32, measured against planes: 75 us for 58 at
+// 22 x 752 x 1280 backward, 248 for 171 at 27 x 1173 x 6032.)
 constexpr int kFewRows = 16;
 
 struct Args {
@@ -71,7 +73,7 @@ struct DownArgs {
     float* part;
     int dtype;
 };
-int down_shares(int K, int N, int dtype);
+int down_shares(int K, int N, int most = 592);
 int down(const DownArgs& p, Chain& st);
 // out[m, n] = the shares' sum (+ T[m, :] . a[slot[m]][:, n])
 struct SumArgs {

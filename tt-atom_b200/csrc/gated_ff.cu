@@ -67,8 +67,8 @@ struct FfSpace {
         const long long M = z.M, k = z.split ? 2 : 1, M32 = up(M, 32);
         if (M <= few::kFewRows) {
             if (bwd) {
-                few_dh = c.take<float>(few::down_shares(z.O, z.F, z.dtype) * M * z.F);
-                few_dx = c.take<float>(few::down_shares(z.F, z.D, z.dtype) * M * z.D);
+                few_dh = c.take<float>(few::down_shares(z.O, z.F, 32) * M * z.F);
+                few_dx = c.take<float>(few::down_shares(z.F, z.D) * M * z.D);
                 few_grads = c.take<float>(3 * M * z.F);
             } else if (z.split) {
                 H32 = c.take<float>(M * z.Fp);
@@ -373,7 +373,7 @@ int few_backward(Ff& f, const void* x, long long ldx, const void* wg, const void
                  void* dwg, void* dwu, void* dwd) {
     const FfSizes& z = f.z;
     const int M = (int)z.M, t = z.dtype;
-    const int s1 = few::down_shares(z.O, z.F, t), s2 = few::down_shares(z.F, z.D, t);
+    const int s1 = few::down_shares(z.O, z.F, 32), s2 = few::down_shares(z.F, z.D);
     if (int s = few::down({{dy, nullptr}, lddy, 0, M, z.O, {wd, nullptr}, z.F, s1, f.sp.few_dh, t},
                           f.st))
         return s;
