@@ -219,3 +219,52 @@ def test_adapted_projection_then_gated_block(t):
     u = max(torch.finfo(t).eps / 2, 2.0 ** -20)
     for got, ref in zip((y, dx, da, db, *dw), want):
         assert float((got.double() - ref).norm() / ref.norm()) <= 4 * u * 4
+
+
+MANY = [
+    # requests of a tile that share adapters, in and out of order, with empty ones between them
+    ([1] * 300, [i % 3 for i in range(300)], 3, 16, 64, 72),
+    ([2, 0] * 400, [(i * 7 // 3) % 9 - 1 for i in range(800)], 8, 8, 40, 136),
+    ([0] * 700 + [30, 0, 30] + [0] * 600 + [40], [i % 2 for i in range(1304)], 2, 4, 64, 64),
+    ([1] * 100 + [400] + [1] * 100, [0, 1] * 50 + [1] + [1, 0] * 50, 2, 40, 72, 64),
+    ([7] * 60, [i % 4 for i in range(60)], 4, 33, 128, 96),
+    ([7] * 60, [i % 4 for i in range(60)], 4, 72, 136, 64),
+    ([5] * 104, list(range(104)), 104, 20, 64, 200),
+]
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_requests_that_share_a_tile_and_an_adapter(case, t):
+    both(make(*MANY[case], t, seed=60 + case))
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("R", [12, 72])
+def test_rows_do_not_depend_on_how_requests_cut_them(R, t):
+    # Blocks that have other requests' rows add zeros to a row's sums, which change nothing. In fp32
+    # the sums leave tensor memory after every second stage of four slices of 16 ranks: a block of
+    # several slices that does not begin on a stage has them cut elsewhere, and its rounding (not
+    # its bound, gamma) depends on that.
+    args = make([600], [1], 2, R, 64, 96, t, seed=70)
+    x, w, a, b, scale, ptr, ids, dy = args
+    y, dx = adapted_linear(*args[:7]), adapted_linear_bwd(*args, adapter_grads=False)[0]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    want = reference(*args)
+    for lengths in ([1] * 600, [250, 20, 330], [0] * 300 + [3, 0] * 200):
+        p = torch.tensor([0] + lengths, **i32).cumsum(0).to(torch.int32)
+        q = torch.ones(len(lengths), **i32)
+        y2 = adapted_linear(x, w, a, b, scale, p, q)
+        dx2 = adapted_linear_bwd(x, w, a, b, scale, p, q, dy, adapter_grads=False)[0]
+        check([y2, dx2], want, ("y", "dx"))
+        if t != torch.float32 or R <= 16:
+            same = torch.equal(y2, y) and torch.equal(dx2, dx)
+            assert same
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("M", [1, 7, 16, 17])
+@pytest.mark.parametrize("R, D, O", [(1, 7, 300), (20, 1000, 33), (128, 72, 136), (9, 264, 8)])
+def test_few_rows_both_ways(M, R, D, O, t):  # noqa: E741
+    lengths = [M // 3, 0, M - M // 3]
+    both(make(lengths, [1, 0, 2 if M > 1 else -1], 4, R, D, O, t, seed=80 + M))

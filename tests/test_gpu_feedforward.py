@@ -270,3 +270,10 @@ def test_wide_and_long():
     want = reference(x, wg, wu, wd, dy, "silu")
     check([gated_ff(x, wg, wu, wd)], want, ["y"])
     check(gated_ff_bwd(x, wg, wu, wd, dy), want, ("dx", "dwg", "dwu", "dwd"))
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("M, D, F, O", [(1, 7, 9, 300), (2, 1000, 33, 5), (9, 65, 700, 136),
+                                        (16, 264, 130, 1), (13, 40, 2000, 24), (17, 264, 130, 8)])
+def test_few_rows_both_ways(M, D, F, O, t):  # noqa: E741
+    test_against_the_definition((M, D, F, O), t)

@@ -3,12 +3,14 @@
 //   y = x W^T + S B^T,  S = s (x A^T) row by row with the row's own A, B and s
 //
 // The requests' rows are cut at every 256th row into pieces: piece t + r holds the rows of request
-// r in row tile t (t + r grows along the requests, so it names a piece without a table). One
-// product gives S: each row tile times the adapters of its pieces, 16 ranks a slice, of which the
-// rows that are not a request's own become zeros in its piece's block of 256 rows. The shared projection's product (pair_product.cu) then takes each piece of its
-// row tile as more of K, S's block times the request's B, in slices of 16 ranks of which four make
-// a stage: the adapters cost their own multiplications and no pass over y. The backward pass is the same with T = s (dy B), W and A in
-// the place of S, W^T and B, and dA = T^T x, dB = dy^T S summed by pieces in their order.
+// r in row tile t (t + r grows along the requests, so it names a piece without a table). Pieces of
+// a tile that have one adapter share a block of 256 rows, which the first of them leads. One product
+// gives S: each row tile times the adapters of its blocks, 16 ranks a slice, of which rows that are
+// not the adapter's become zeros in its block. The shared projection's product (pair_product.cu)
+// then takes each block of its row tile as more of K, S times the adapter's B, in slices of 16
+// ranks of which four make a stage: the adapters cost their own multiplications and no pass over
+// y. The backward pass is the same with T = s (dy B), W and A in the place of S, W^T and B, and
+// dA = T^T x, dB = dy^T S summed by pieces in their order.
 //
 // Zeros in a block keep other requests' rows as they are only where B is finite; an adapter that
 // is not is found when the pieces are, left out, and its own rows are set to NaN.
@@ -22,25 +24,27 @@ namespace {
 
 using namespace pair;
 
-// fp32, more than 64 ranks: the pieces' blocks as planes, scaled row by row, from the low-rank
-// rows. A block a piece.
-__global__ void __launch_bounds__(256) blocks32_kernel(const int4* pieces, const float* rows, int R,
-                                                       int Rs, __half* block, long long plane,
+// fp32, more than 64 ranks: the blocks as planes, scaled row by row, from the low-rank rows. A
+// thread block each.
+__global__ void __launch_bounds__(256) blocks32_kernel(const int* lead, const int* row_lead,
+                                                       const int4* pieces, int M, const float* rows,
+                                                       int R, int Rs, __half* block, long long plane,
                                                        float* rinv) {
     let_next_start();
     wait_before();
-    const int4 c = pieces[blockIdx.x];
-    if (c.x < 0) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m0 = c.y / 256 * 256;
+    if (lead[blockIdx.x] < 0) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = pieces[blockIdx.x].y / 256;
+    const int m0 = t * 256, request = blockIdx.x - t;
     block += (long long)blockIdx.x * 256 * Rs;
     for (int i = threadIdx.x; i < 256 * Rs / 8; i += 256) {
         const int m = m0 + i * 8 / Rs;           // Rs is a multiple of 8
-        if (m >= c.y && m < c.z) continue;
+        if (m < M && row_lead[m] == request) continue;
         *reinterpret_cast<uint4*>(block + i * 8) = make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>(block + plane + i * 8) = make_uint4(0, 0, 0, 0);
     }
 #pragma unroll 4
-    for (int m = c.y + warp; m < c.z; m += 8) {
+    for (int m = m0 + warp; m < min(M, m0 + 256); m += 8) {
+        if (row_lead[m] != request) continue;
         const float4 x = 4 * lane < Rs
             ? *reinterpret_cast<const float4*>(rows + (long long)m * Rs + 4 * lane)
             : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -355,7 +359,7 @@ struct AdSpace {
     float *rinv, *xinv, *wr, *ext_rinv, *part, *gpart, *few_S, *few_T, *few_dx;
     void *S, *T;
     int4 *piece, *bad, *tile_req;
-    int *usable, *few_slot;
+    int *lead, *row_lead, *usable, *few_slot;
     unsigned *max, *maxima[3];       // of w, of the adapters beside it, of those of the low-rank
                                      // rows; and the blocks' own
     size_t bytes;
@@ -387,6 +391,8 @@ struct AdSpace {
             bad = c.take<int4>(z.nad);
             tile_req = c.take<int4>(z.tiles);
             usable = c.take<int>(z.pieces);
+            lead = c.take<int>(z.pieces);
+            row_lead = c.take<int>(z.M);
             first = c.take<__half>(k * (bwd ? b_n : a_n));
             ext = c.take<__half>(k * (bwd ? a_n : b_n));
             block = c.take<__half>(k * z.pieces * 256 * z.Rs);
@@ -416,7 +422,7 @@ struct Ad {
 
     Pieces pieces(const void* other, long long other_n) const {
         return {req_ptr, req_adapter, z.nreq, z.nad, (int)z.M, z.tiles, z.pieces, sp.piece,
-                sp.tile_req, other, other_n, sp.bad, z.dtype};
+                sp.lead, sp.row_lead, sp.tile_req, other, other_n, sp.bad, z.dtype};
     }
 
     // A direction's operands: rows, the shared matrix, the adapters that make the low-rank rows
@@ -436,6 +442,8 @@ struct Ad {
         p.tile_req = sp.tile_req;
         p.piece = sp.piece;
         p.usable = sp.usable;
+        p.lead = sp.lead;
+        p.row_lead = sp.row_lead;
         p.bad = sp.bad;
         return p;
     }
@@ -473,7 +481,8 @@ struct Ad {
         if (int s = launch(kLow, {128, share, 0}, z.split, maps, p, st)) return s;
         if (!z.split || !blocks || planes) return ATOM_OK;
         return st.launch("adapters: blocks", blocks32_kernel, dim3(z.pieces), 256, 0,
-                         (const int4*)sp.piece, (const float*)p.low_rows, z.R, z.Rs, sp.block,
+                         (const int*)sp.lead, (const int*)sp.row_lead,
+                         (const int4*)sp.piece, (int)z.M, (const float*)p.low_rows, z.R, z.Rs, sp.block,
                          (long long)z.pieces * 256 * z.Rs, sp.ext_rinv);
     }
 

@@ -277,12 +277,12 @@ struct Blocks {
     __device__ __forceinline__ int at() const { return (sub - 1) * 16; }     // first rank
 };
 
-// A row tile's pieces, 32 requests at a time, one a lane. Whole warps.
+// A row tile's blocks, 32 requests at a time, one a lane. Whole warps.
 struct Window {
     const Args& p;
     int mt, first, behind, base = 0;
-    int4 c;                  // this lane's piece
-    unsigned mask = 0;       // the lanes whose piece has an adapter
+    int a = -1;              // this lane's adapter where its request leads a block
+    unsigned mask = 0;       // the lanes that have one
     __device__ __forceinline__ Window(const Args& q, int tile) : p(q), mt(tile) {
         const int4 t = p.tile_req[mt];
         first = t.x;
@@ -292,8 +292,8 @@ struct Window {
     __device__ __forceinline__ void look(int r) {
         base = r;
         const int i = r + (threadIdx.x & 31);
-        c = i < behind ? p.piece[mt + i] : make_int4(-1, 0, 0, 0);
-        mask = __ballot_sync(0xffffffffu, c.x >= 0);
+        a = i < behind ? p.lead[mt + i] : -1;
+        mask = __ballot_sync(0xffffffffu, a >= 0);
     }
     __device__ __forceinline__ int count() {         // of all requests; ends on the first again
         int n = __popc(mask);
@@ -306,16 +306,16 @@ struct Window {
         }
         return n;
     }
-    // writes down which pieces the product beside the projection takes
+    // writes down which blocks the product beside the projection takes
     __device__ __forceinline__ void settle() {
         int n = 0, spoilt = 0;
         for (int r = first; r < behind; r += 32) {
             look(r);
-            const bool ok = c.x >= 0 && is_finite(p, c.x);
+            const bool ok = a >= 0 && is_finite(p, a);
             n += __popc(__ballot_sync(0xffffffffu, ok));
-            spoilt |= __ballot_sync(0xffffffffu, c.x >= 0 && !ok) != 0;
+            spoilt |= __ballot_sync(0xffffffffu, a >= 0 && !ok) != 0;
             const int i = r + (threadIdx.x & 31);
-            if (i < behind) p.usable[mt + i] = ok ? c.x : -1;
+            if (i < behind) p.usable[mt + i] = ok ? a : -1;
         }
         if ((threadIdx.x & 31) == 0) {
             p.tile_req[mt].z = n;
@@ -345,8 +345,8 @@ struct Low {
     __device__ __forceinline__ int sub(int i) const {           // which of its piece's slices i is
         return slices > 4 ? i : (i & 3) % slices;
     }
-    // the piece of slice i of group g: its adapter and rows, and its request
-    __device__ __forceinline__ int4 piece(int g, int i) {
+    // the block of slice i of group g: its adapter and the request that leads it
+    __device__ __forceinline__ int2 piece(int g, int i) {
         int j = g * each + (slices > 4 ? 0 : (i >> 2) * half + (i & 3) / slices);
         if (j < before) {
             before = 0;
@@ -359,8 +359,7 @@ struct Low {
         unsigned v = w.mask;
         for (j -= before; j > 0; --j) v &= v - 1;
         const int l = __ffs(v) - 1;
-        return make_int4(__shfl_sync(0xffffffffu, w.c.x, l), __shfl_sync(0xffffffffu, w.c.y, l),
-                         __shfl_sync(0xffffffffu, w.c.z, l), w.base + l);
+        return make_int2(__shfl_sync(0xffffffffu, w.a, l), w.base + l);
     }
 };
 
@@ -596,21 +595,22 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
 // blocks are planes, scaled row by row: a piece's slices are all in one warp then (ranks of 64 at
 // most; larger ones have a kernel of their own, from the rows).
 __device__ __forceinline__ void low_store(const Args& p, Low& low, int g, int part,
-                                          long long m0, int lane, float (*v)[32], float f) {
+                                          long long m0, int lane, int lead, float (*v)[32],
+                                          float f) {
     const int used = low.used(g, part);
     const long long m = m0 + lane;
     float largest = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (i >= used) break;
-        const int4 piece = low.piece(g, part * 4 + i);
+        const int2 piece = low.piece(g, part * 4 + i);
         const int sub = low.sub(part * 4 + i), c0 = sub * 16;
-        const bool in = m >= piece.y && m < piece.z;
+        const bool in = piece.y == lead;
         const float s = p.low_scale[piece.x] * f;
         float* x = v[i >> 1] + (i & 1) * 16;
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = in ? x[j] * s : 0.f;
-        const long long row = ((long long)(low.w.mt + piece.w) * 256 + (m & 255)) * p.Rs;
+        const long long row = ((long long)(low.w.mt + piece.y) * 256 + (m & 255)) * p.Rs;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                // eight ranks at a time: Rs is a multiple of 8
             const int c = c0 + 8 * h;
@@ -984,6 +984,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
             if (EPI == kLow && warp == 2 && rank == 0 && ti.ks == 0 && p.usable)
                 Window(p, ti.mt).settle();
             if constexpr (EPI == kLow && !SPLIT) {
+                const int lead = m + lane < p.M ? p.row_lead[m + lane] : -1;
                 Low low_(p, ti.mt);
                 for (int g = ti.ks; g < low_.groups(); g += p.ksplit) {
                     if (!(ok = filled())) break;
@@ -995,7 +996,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     pin32(v[0]);
                     pin32(v[1]);
                     drained();
-                    low_store(p, low_, g, part, m, lane, v, 1.f);
+                    low_store(p, low_, g, part, m, lane, lead, v, 1.f);
                 }
             } else if constexpr (!SPLIT) {
                 if (!(ok = filled())) break;
@@ -1062,11 +1063,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 const float sb = p.bmax ? pow2_inv(pow2_scale(*p.bmax)) : 1.f;
                 const float sa = p.rinv ? (m + lane < p.M ? p.rinv[m + lane] : 0.f) : *p.factor;
                 if constexpr (EPI == kLow) {
+                    const int lead = m + lane < p.M ? p.row_lead[m + lane] : -1;
                     Low low_(p, ti.mt);
                     for (int g = ti.ks; g < low_.groups(); g += p.ksplit) {
                         clear();
                         if (!(ok = add((p.ph[0].nk + kRound - 1) / kRound, 1.f))) break;
-                        low_store(p, low_, g, part, m, lane, v, sa * sb);
+                        low_store(p, low_, g, part, m, lane, lead, v, sa * sb);
                     }
                     if (!ok) break;
                     continue;
@@ -1372,11 +1374,34 @@ __device__ __forceinline__ void find_pieces(const Pieces& p) {
                 c.z = min(begins(r + 1), m0 + 256);
                 if (c.y < c.z && a >= 0 && a < p.nad) c.x = a;
             }
-            if (lane == 0) p.piece[w] = c;
+            // The requests of a tile that share an adapter share a block: the first of them among
+            // 256 numbers leads it (156 rows of 153 requests, 3 adapters, 16 ranks, forward
+            // and backward: 115 us with a block a request, 65 us so).
+            int lead = r;
+            const int t = w - r;
+            if (c.x >= 0) {
+                int got = r;
+#pragma unroll
+                for (int j = 7; j >= 0; --j) {
+                    const int q = (r & ~255) + 32 * j + lane;
+                    if (q < r && p.adapter[q] == c.x &&
+                        ::max(begins(q), t * 256) < min(begins(q + 1), t * 256 + 256))
+                        got = q;
+                }
+                lead = __reduce_min_sync(0xffffffffu, got);
+            }
+            if (lane == 0) {
+                p.piece[w] = c;
+                p.lead[w] = lead == r ? c.x : -1;
+            }
+            for (int m = c.y + lane; m < c.z; m += 32) p.row_lead[m] = c.x < 0 ? -1 : lead;
         } else if (w < p.pieces + p.tiles) {
             const int t = w - p.pieces;
             const int first = last_le(p.n, t * 256, begins);
             const int last = last_le(p.n, t * 256 + 255, begins);
+            const int head = begins(0), tail = begins(p.n);
+            for (int m = t * 256 + lane; m < min(p.M, t * 256 + 256); m += 32)
+                if (m < head || m >= tail) p.row_lead[m] = -1;
             // a request that begins before the tile reaches into it at most as the last such one
             if (lane == 0) p.tile_req[t] = make_int4(::max(first, 0), last + 1, 0, 0);
         }

@@ -53,14 +53,17 @@ struct Args {
     const float* factor;     // ... and the planes' scales together
     const float* cinv[2];    // 1 / scale of B's rows (columns of C; u's second), or NULL:
     const unsigned* bmax;    // B's tensor was scaled by this finite maximum (bits)
-    // low-rank blocks beside the phases: block t + r holds the rows of request r in 256-row tile
-    // t ([256][R] typed, zeros in other rows), multiplied by the request's adapter
+    // low-rank blocks beside the phases: block t + r holds the rows of 256-row tile t whose requests
+    // have request r's adapter ([256][R] typed, zeros in other rows), r being the first such
     int ext;                 // 16-rank slices a request, 0: none
     int ext_a, ext_b, ext_bmn;
     int4* tile_req;          // of a row tile: its requests' first and behind; and, from kLow on,
-                             // how many pieces count and whether one's adapter is not finite
-    const int4* piece;       // of a block: adapter or -1 (none), its rows
-    int* usable;             // from kLow on: the same adapter, -1 also where it is not finite
+                             // how many blocks count and whether one's adapter is not finite
+    const int4* piece;       // t + r, of request r in tile t: adapter or -1 (none), its rows
+    const int* lead;         // a block's adapter where it is the first of its tile with that
+                             // adapter, which takes the others' rows along; else -1
+    const int* row_lead;     // per row: the request whose block it is in, -1: none
+    int* usable;             // from kLow on: as lead, -1 also where the adapter is not finite
     const int4* bad;         // of an adapter: not all zero = not finite, its rows become NaN
     const float* low_scale;  // kLow: per adapter
     void* low_block;         // kLow: [block][256][Rs] typed (SPLIT: planes low_plane apart, NULL
@@ -133,6 +136,7 @@ struct Pieces {
     int n, nad, M;           // requests, adapters, rows
     int tiles, pieces;       // row tiles; and requests
     int4* piece;             // adapter or -1, first row, behind the last row
+    int *lead, *row_lead;    // as in Args
     int4* tile_req;          // requests first .. behind that reach into a row tile
     const void* other;       // the matrix of each adapter beside the projection: `other_n` values
     long long other_n;
