@@ -277,3 +277,35 @@ def test_wide_and_long():
                                         (16, 264, 130, 1), (13, 40, 2000, 24), (17, 264, 130, 8)])
 def test_few_rows_both_ways(M, D, F, O, t):  # noqa: E741
     test_against_the_definition((M, D, F, O), t)
+
+
+@pytest.mark.parametrize("act", ["silu", "sigmoid", "gelu"])
+def test_fp32_rows_far_below_their_bound(act):
+    """fp32 rows of H and of dG | dU are two 16-bit planes scaled by a bound of the row, below
+    (8 D max|x| max|w|) for g and u (each factor rounded up to a power of two): a plane's last
+    place is 2^-36 where the bound is 2^15, so a value is off by at most 2^-51 of it. Outliers in x
+    and in rows of the weights, and gates that are closed, bring rows far below it."""
+    M, D, F, O = 40, 512, 264, 64  # noqa: E741
+    x, wg, wu, wd, dy = make(M, D, F, O, torch.float32, seed=31)
+    x[:, 5] *= 300
+    x[::4] *= 2.0 ** -20
+    wg[3], wu[7] = wg[3] * 50, wu[7] * 50
+    wg[:, 5] = 0.02 * wg[:, 5].sign() - 0.01
+    dy[::3, 1] *= 100
+    want = reference(x, wg, wu, wd, dy, act)
+    X, WG, WU, WD, DY = (v.double() for v in (x, wg, wu, wd, dy))
+    top = torch.maximum(WG.abs().max(), WU.abs().max())
+    g = 8 * D * X.abs().amax(1, keepdim=True) * top
+    dh = 8 * O * DY.abs().amax(1, keepdim=True) * WD.abs().max()
+    one = torch.ones_like(g)
+    eh = (2.0 ** -51 * (g if act == "sigmoid" else g * g)).expand(M, F)
+    eg = (2.0 ** -51 * dh * (torch.maximum(g, one) if act == "sigmoid" else 2 * g)).expand(M, F)
+    wx = 2.0 ** -51 * M * (eg[:, :1] * 2.0 ** 51 * 2 * X.abs().amax(1, keepdim=True)).max()
+    wy = 2.0 ** -51 * M * (eh[:, :1] * 2.0 ** 51 * 2 * DY.abs().amax(1, keepdim=True)).max()
+    more = {"y": eh @ WD.abs().T, "dx": eg @ (WG.abs() + WU.abs()), "dwg": eg.T @ X.abs() + wx,
+            "dwu": eg.T @ X.abs() + wx, "dwd": DY.abs().T @ eh + wy}
+    want = {k: (v, e + 1.01 * more[k]) for k, (v, e) in want.items()}
+    check([gated_ff(x, wg, wu, wd, act=act)], want, ["y"])
+    y, kept = gated_ff(x, wg, wu, wd, act=act, keep=True)
+    for k in (None, kept):
+        check(gated_ff_bwd(x, wg, wu, wd, dy, act=act, kept=k), want, ("dx", "dwg", "dwu", "dwd"))

@@ -56,7 +56,7 @@ struct FfSizes {
 // always become two planes.
 struct FfSpace {
     __half *x, *wg, *wu, *wd, *dy, *xt, *dyt, *hp, *dgup;
-    float *xr, *wgr, *wur, *wdr, *dyr, *hr, *dgur, *H32, *dgu32, *dh, *part;
+    float *xr, *wgr, *wur, *wdr, *dyr, *hr, *dgur, *H32, *dh, *part;
     __half *H, *dgu;
     float *few_dh, *few_dx, *few_grads;
     unsigned *max, *maxima[4];  // of wg | wu, of wd, x'' factor, dy'' factor; and the blocks' own
@@ -94,9 +94,8 @@ struct FfSpace {
             if (bwd) dgu = c.take<__half>(2 * M * z.Fp);
         } else {
             max = c.take<unsigned>(4);
-            for (unsigned*& m : maxima) m = bwd ? c.take<unsigned>(2 * kPrepBlocks) : nullptr;
+            for (unsigned*& m : maxima) m = c.take<unsigned>(2 * kPrepBlocks);
             xr = c.take<float>(M32);
-            H32 = c.take<float>(M * z.Fp);
             hp = c.take<__half>(2 * M * z.Fp);
             hr = c.take<float>(M32);
             if (!bwd) {
@@ -105,7 +104,6 @@ struct FfSpace {
                 wdr = c.take<float>(up(z.O, 32));
             } else {
                 dyr = c.take<float>(M32);
-                dgu32 = c.take<float>(2 * M * z.Fp);
                 dgup = c.take<__half>(4 * M * z.Fp);
                 dgur = c.take<float>(M32);
                 xt = c.take<__half>(2 * M * z.Dp);
@@ -115,6 +113,12 @@ struct FfSpace {
         bytes = c.used;
     }
 };
+
+int log2_up(int n) {
+    int k = 0;
+    while ((1 << k) < n) ++k;
+    return k;
+}
 
 // Fills a map (and, for two planes, the next one).
 int put(Maps& maps, int i, const Operand& o, bool mn, int box_rows, bool split) {
@@ -156,8 +160,16 @@ struct Ff {
     // G and U, and beside its scales in the weights' gradients later.
     int inputs(const void* xp, long long ldx, const void* g, const void* u, const void* d) {
         x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kRowSplit, sp.xr);
-        wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kRowSplit, sp.wgr);
-        wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kRowSplit, sp.wur);
+        if (z.split) {
+            const long long n = z.F * z.Dp;
+            gather({g, z.F, z.D, z.D, sp.wg, z.Dp, n, sp.wgr, nullptr, kRowSplit, nullptr}, 0);
+            gather({u, z.F, z.D, z.D, sp.wu, z.Dp, n, sp.wur, nullptr, kRowSplit, nullptr}, 0);
+            wg = {sp.wg, z.F, z.D, z.Dp, n};
+            wu = {sp.wu, z.F, z.D, z.Dp, n};
+        } else {
+            wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kPack, nullptr);
+            wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kPack, nullptr);
+        }
         wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kRowSplit, sp.wdr);
         return prepare(list, st);
     }
@@ -176,6 +188,18 @@ struct Ff {
         wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kTensorSplit, nullptr, 0);
         wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kTensorSplit, nullptr, 0);
         wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kTensorSplit, nullptr, 1);
+        if (z.split) {
+            // Scales of dG | dU and H, and the largest that a row of them and its partner in the
+            // weights' gradients have together.
+            PrepItem b{sp.xr, z.M, 0, 0, nullptr, 0, 0, sp.dgur, nullptr, kBounds, sp.xr};
+            b.dy = sp.dyr;
+            for (int k = 0; k < 2; ++k) b.w[k] = sp.maxima[k], b.n[k] = parts[k];
+            b.lg[0] = log2_up(z.D), b.lg[1] = log2_up(z.O);
+            b.sigmoid = act == 1;
+            gather(b, 2);
+            b.dy = nullptr, b.rinv = sp.hr, b.weight = sp.dyr;
+            gather(b, 3);
+        }
         return prepare(list, st);
     }
     Args args(long long M, int N) const {
@@ -198,17 +222,26 @@ struct Ff {
         p.C[0] = C;
         p.ldc = ldc;
     }
-    // a gate epilogue's output, and what it keeps in lane blocks
-    int gate_output(Maps& maps, Args& p, void* C, long long width, void* H) const {
+    // a gate epilogue's output (dgu or, forward, H; and H beside dgu), and what it keeps in lane
+    // blocks; fp32: planes
+    int gate_output(Maps& maps, Args& p, __half* C, long long width, __half* H) const {
         p.gu_half = up(z.M, 32) * z.Fp;
         p.H = H != nullptr;
-        p.used |= 1u << kOutMap | (unsigned)p.H << kHMap;
-        if (H)
-            if (int s = make_out_map(&maps.m[kHMap], H, z.dtype, z.Fp, z.M, z.Fp)) return s;
-        return make_out_map(&maps.m[kOutMap], C, z.dtype, width, z.M, width);
+        p.h_rinv = sp.hr;
+        p.gu_rinv = sp.dgur;
+        const int t = z.split ? ATOM_F16 : z.dtype;
+        for (int k = 0; k < step(); ++k) {
+            p.used |= 1u << (kOutMap + k) | (unsigned)p.H << (kHMap + k);
+            if (int s = make_out_map(&maps.m[kOutMap + k], C + k * z.M * width, t, width, z.M, width))
+                return s;
+            if (!H) continue;
+            if (int s = make_out_map(&maps.m[kHMap + k], H + k * z.M * z.Fp, t, z.Fp, z.M, z.Fp))
+                return s;
+        }
+        return ATOM_OK;
     }
     // [G | U] tiles of X
-    int gates(int epilogue, Args& p, void* C, long long width, void* H) {
+    int gates(int epilogue, Args& p, __half* C, long long width, __half* H) {
         const Choice c = z.gate;
         const int k = step();
         Maps maps;
@@ -226,14 +259,10 @@ struct Ff {
     int forward(void* y, long long ldy, float* kept) {
         Args p = args(z.M, z.F);
         p.gu = kept;
-        if (int s = gates(kGate, p, z.split ? (void*)sp.H32 : sp.H, z.Fp, nullptr)) return s;
-        Operand h{sp.H, z.M, z.F, z.Fp, 0};
-        if (z.split) {
-            list.add({sp.H32, z.M, z.F, z.Fp, sp.hp, z.Fp, z.M * z.Fp, sp.hr, nullptr, kRowSplit,
-                      nullptr});
-            if (int s = prepare(list, st)) return s;
-            h = {sp.hp, z.M, z.F, z.Fp, z.M * z.Fp};
-        }
+        p.w_inv = sp.maxima[0], p.n_w_inv = parts[0], p.lg_k = log2_up(z.D);
+        __half* out = z.split ? sp.hp : sp.H;
+        if (int s = gates(kGate, p, out, z.Fp, nullptr)) return s;
+        const Operand h{out, z.M, z.F, z.Fp, z.M * z.Fp};
         const Choice c = z.down;
         const int k = step();
         Maps maps;
@@ -248,8 +277,9 @@ struct Ff {
     }
     int backward(const float* kept, void* dx, long long lddx, void* dwg, void* dwu, void* dwd) {
         const int k = step();
-        void* dgu = z.split ? (void*)sp.dgu32 : sp.dgu;
-        void* H = !dwd ? nullptr : z.split ? (void*)sp.H32 : sp.H;
+        __half* dgu = z.split ? sp.dgup : sp.dgu;
+        __half* hs = z.split ? sp.hp : sp.H;
+        __half* H = dwd ? hs : nullptr;
         {   // dH, and dG, dU, H either in its epilogue or in that of G and U
             const Choice c = z.dh;
             Maps maps;
@@ -272,21 +302,15 @@ struct Ff {
                 if (int s = gates(kGateBwdGU, q, dgu, 2 * z.Fp, H)) return s;
             }
         }
-        Operand g{sp.dgu, z.M, 2 * z.Fp, 2 * z.Fp, 0}, h{sp.H, z.M, z.F, z.Fp, 0};
+        const Operand g{dgu, z.M, 2 * z.Fp, 2 * z.Fp, z.M * 2 * z.Fp};
+        const Operand h{hs, z.M, z.F, z.Fp, z.M * z.Fp};
         Operand xt = x, dyt = dy;
         if (z.split) {
             // dG | dU and H are scaled row by row. In the weights' gradients, sums over rows, the
             // rows' scales s cancel against x (and dy) rows divided by them: what is left is one
             // power of two, the largest of the rows' x (dy) and dG | dU (H) scales together, and
             // rows lose bits only as far as they are small in the sum.
-            const long long M = z.M, W = 2 * z.Fp;
-            g = {sp.dgup, M, W, W, M * W};
-            h = {sp.hp, M, z.F, z.Fp, M * z.Fp};
-            gather({sp.dgu32, M, W, W, sp.dgup, W, M * W, sp.dgur, nullptr, kRowSplit, sp.xr}, 2);
-            if (dwd)
-                gather({sp.H32, M, z.F, z.Fp, sp.hp, z.Fp, M * z.Fp, sp.hr, nullptr, kRowSplit,
-                        sp.dyr}, 3);
-            if (int s = prepare(list, st)) return s;
+            const long long M = z.M;
             if (dwg || dwu) {
                 xt = {sp.xt, M, z.D, z.Dp, M * z.Dp};
                 list.add({x_src, M, z.D, x_ld, sp.xt, z.Dp, M * z.Dp, nullptr, sp.max + 2, kWeighted,

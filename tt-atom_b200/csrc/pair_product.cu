@@ -213,6 +213,12 @@ __device__ __noinline__ bool spoilt_row(const Args& p, int mt, long long m, int 
     return bad;
 }
 
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
 // What a warp knows of its tiles' requests: a lane a tile, 32 tiles ahead, so that no tile waits
 // for its own (a load takes two microseconds beside the tiles' traffic).
 struct Ahead {
@@ -429,6 +435,25 @@ __device__ __forceinline__ void store_tma(Out& o, int lane, const CUtensorMap* m
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
 }
+// A gate's output: typed, or (SPLIT) as planes in the row's scale s.
+template <bool SPLIT>
+__device__ __forceinline__ void store_typed(Out& o, int lane, const CUtensorMap* map, int x, int y,
+                                            float* v, int dtype, float s) {
+    if constexpr (SPLIT) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] *= s;
+        store_tma(o, lane, map, x, y, -1, v, ATOM_F16);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const float2 hi = __half22float2(__floats2half2_rn(v[i], v[i + 1]));
+            v[i] = (v[i] - hi.x) * 2048.f;
+            v[i + 1] = (v[i + 1] - hi.y) * 2048.f;
+        }
+        store_tma(o, lane, map + 1, x, y, -1, v, ATOM_F16);
+    } else {
+        store_tma(o, lane, map, x, y, -1, v, dtype);
+    }
+}
 // Where rows do not start on 16 bytes, or end inside them: row by row, a column a lane.
 __device__ __forceinline__ void store_rows(Out& o, int lane, void* C, long long off, long long ld,
                                            int rows, int cols, const float* v, int dtype) {
@@ -546,7 +571,8 @@ __device__ __forceinline__ void gate_bwd32(float* g, float* u, float* d, int act
 // v0 (and v1: the u columns of a gate).
 template <int EPI, bool SPLIT>
 __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const Tile& ti, Out& o,
-                                         long long m, int n, int lane, float* v0, float* v1) {
+                                         long long m, int n, int lane, float* v0, float* v1,
+                                         float sh, float sg) {
     if (m >= p.M || n >= p.N) return;
     const int left = p.N - n;
     if constexpr (EPI == kStore) {
@@ -571,7 +597,7 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
             store_block(lane_block(p.gu, m, n, p.Fp, lane) + p.gu_half, v1);
         }
         gate32(v0, v1, p.act);
-        store_tma(o, lane, &maps.m[kOutMap], n, (int)m, -1, v0, p.dtype);
+        store_typed<SPLIT>(o, lane, &maps.m[kOutMap], n, (int)m, v0, p.dtype, sh);
     } else {
         // v0, v1 = g, u (kGateBwdGU, dh from memory) or v0 = dh (kGateBwdDH, g and u from memory)
         float w[32];
@@ -584,9 +610,9 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
             load_block(lane_block(p.gu, m, n, p.Fp, lane) + p.gu_half, v1);
         }
         gate_bwd32(v0, v1, w, p.act);
-        store_tma(o, lane, &maps.m[kOutMap], n, (int)m, -1, v0, p.dtype);
-        store_tma(o, lane, &maps.m[kOutMap], p.Fp + n, (int)m, -1, v1, p.dtype);
-        if (p.H) store_tma(o, lane, &maps.m[kHMap], n, (int)m, -1, w, p.dtype);
+        store_typed<SPLIT>(o, lane, &maps.m[kOutMap], n, (int)m, v0, p.dtype, sg);
+        store_typed<SPLIT>(o, lane, &maps.m[kOutMap], p.Fp + n, (int)m, v1, p.dtype, sg);
+        if (p.H) store_typed<SPLIT>(o, lane, &maps.m[kHMap], n, (int)m, w, p.dtype, sh);
     }
 }
 
@@ -972,6 +998,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
         Out out{outbuf + (warp - 2) * 4096, 0};
         constexpr int kParts = GATED ? 2 * kChunks : kChunks;
         uint32_t low = 2 * BN;
+        int e_w = 0;
+        if constexpr (SPLIT && EPI == kGate) {
+            float w = 0.f;
+#pragma unroll 4
+            for (int i = lane; i < p.n_w_inv; i += 32) w = fmaxf(w, __uint_as_float(p.w_inv[i]));
+            e_w = bound_exp(warp_max(w)) + p.lg_k;
+        }
         Ahead ahead;
         uint32_t mine_k = 0;
         for (long long t = first; ok && t < p.tiles; t += pairs, ++mine_k) {
@@ -1011,7 +1044,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     if (GATED) pin32(v1);
                     if (k == kChunks - 1) drained();
                     if (EPI == kStore && spoilt) spoil32(v0);
-                    finish32<EPI, SPLIT>(maps, p, ti, out, m, nb + 32 * k, lane, v0, v1);
+                    finish32<EPI, SPLIT>(maps, p, ti, out, m, nb + 32 * k, lane, v0, v1, 1.f,
+                                         1.f);
                 }
             } else {
                 // the tile's rounds summed in registers
@@ -1062,6 +1096,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 static_assert(!SPLIT || kParts == 2, "parts of a SPLIT tile");
                 const float sb = p.bmax ? pow2_inv(pow2_scale(*p.bmax)) : 1.f;
                 const float sa = p.rinv ? (m + lane < p.M ? p.rinv[m + lane] : 0.f) : *p.factor;
+                // A gate's scales come from bounds of its sums, K max|x| max|w|, and not from a pass
+                // over the values, which would be written and read once more in fp32 (18,000 x 128 x
+                // 512 training step: 281 us with that pass, 231 without). Planes hold values to 2^-51
+                // of their row's bound, so a row whose largest value is 2^-27 of it still has fp32's
+                // own rounding; Gaussian rows come to 2^-16 at K = 512 (2^-20 at 2,048 at the least).
+                float sh = 1.f, sg = 1.f;
+                if constexpr (EPI == kGate) {
+                    const int e = bound_exp(sa) + e_w;
+                    const float inv = bound_inv(p.act == 1 ? e : 2 * e);
+                    sh = pow2_inv(inv);
+                    if (ti.nt == 0 && part == 0 && m + lane < p.M) p.h_rinv[m + lane] = inv;
+                } else if constexpr (EPI == kGateBwdGU || EPI == kGateBwdDH) {
+                    if (m + lane < p.M) {
+                        sh = pow2_inv(p.h_rinv[m + lane]);
+                        sg = pow2_inv(p.gu_rinv[m + lane]);
+                    }
+                }
                 if constexpr (EPI == kLow) {
                     const int lead = m + lane < p.M ? p.row_lead[m + lane] : -1;
                     Low low_(p, ti.mt);
@@ -1109,7 +1160,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     float u[32];         // kGateBwdDH: room for the u that it reads
                     if (EPI == kStore && spoilt) spoil32(v[k]);
                     finish32<EPI, SPLIT>(maps, p, ti, out, m, nb + 32 * k, lane, v[k],
-                                         GATED ? v[kChunks + k] : u);
+                                         GATED ? v[kChunks + k] : u, sh, sg);
                 }
             }
         }
@@ -1190,18 +1241,13 @@ __device__ __forceinline__ float max_finite(float m, const float4& v) {
     return fmaxf(fmaxf(m, __uint_as_float(max(finite_bits(v.x), finite_bits(v.y)))),
                  __uint_as_float(max(finite_bits(v.z), finite_bits(v.w))));
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
 
 // A row's scale from its maximum; its inverse and what goes into `max` on the way.
 __device__ __forceinline__ float row_scale(const PrepItem& it, long long r, float mx, bool writes,
                                            float& top) {
     const float s = pow2_scale(__float_as_uint(mx)), inv = mx > 0.f ? pow2_inv(s) : 0.f;
     if (writes) it.rinv[r] = inv;
-    if (it.weight) top = fmaxf(top, fminf(inv * it.weight[r], 0x1p126f));
+    top = fmaxf(top, it.weight ? fminf(inv * it.weight[r], 0x1p126f) : inv);
     return s;
 }
 // kTensorSplit's scale, or what kWeighted divides a row's weight by, from the maxima.
@@ -1470,14 +1516,31 @@ __global__ void __launch_bounds__(256, 3)
         if (blockIdx.x == 0 && threadIdx.x == 0) *it.max = max;
     }
     const int blocks = l.blocks[blockIdx.y];
-    if (it.mode == kPack) prep_pack(it, blocks);
+    if (it.mode == kBounds) {
+        int e[2] = {};
+        for (int k = 0; k < (it.dy ? 2 : 1); ++k) {
+            float v = 0.f;
+            for (int i = threadIdx.x; i < it.n[k]; i += 256)
+                v = fmaxf(v, __uint_as_float(it.w[k][i]));
+            e[k] = bound_exp(pow2_inv(pow2_scale(__float_as_uint(over_block(v))))) + it.lg[k];
+        }
+        for (long long r = blockIdx.x * 256LL + threadIdx.x; r < it.rows; r += blocks * 256LL) {
+            // |g|, |u| < 2^g; |act(g)| <= |g| or 1, |act'(g)| < 2 (sigmoid: 1/4)
+            const int g = bound_exp(static_cast<const float*>(it.src)[r]) + e[0];
+            const float inv = bound_inv(
+                it.dy ? bound_exp(it.dy[r]) + e[1] + (it.sigmoid ? ::max(g - 2, 0) : g + 1)
+                      : it.sigmoid ? g : 2 * g);
+            it.rinv[r] = inv;
+            top = fmaxf(top, fminf(inv * it.weight[r], 0x1p126f));
+        }
+    } else if (it.mode == kPack) prep_pack(it, blocks);
     else if (prep_wide(it)) prep_block(it, blocks, part, max, top);
     else prep_narrow(it, blocks, max, top);
     // the epilogue reads scales of columns 32 at a time
     if (it.mode == kRowSplit && blockIdx.x == 0 && threadIdx.x < 32 &&
         it.rows + lane < (it.rows + 31) / 32 * 32)
         it.rinv[it.rows + lane] = 0.f;
-    if (it.part && (it.mode == kMax || it.mode == kRowSplit)) {
+    if (it.part && (it.mode == kMax || it.mode == kRowSplit || it.mode == kBounds)) {
         __syncthreads();
         top = over_block(top);
         if (threadIdx.x == 0) it.part[blockIdx.x] = __float_as_uint(top);
@@ -1485,7 +1548,7 @@ __global__ void __launch_bounds__(256, 3)
 }
 
 int prep_blocks(const PrepItem& it) {
-    const int rows = it.mode == kPack ? 8 : prep_wide(it) ? 1 : 8 * (kNV / prep_slots(it));
+    const int rows = it.mode == kBounds ? 256 : it.mode == kPack ? 8 : prep_wide(it) ? 1 : 8 * (kNV / prep_slots(it));
     return (int)std::max(1LL, std::min((it.rows + rows - 1) / rows, (long long)kPrepBlocks));
 }
 int prepare(PrepList& l, Chain& st, const Pieces* pieces) {

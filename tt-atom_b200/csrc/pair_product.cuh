@@ -53,6 +53,12 @@ struct Args {
     const float* factor;     // ... and the planes' scales together
     const float* cinv[2];    // 1 / scale of B's rows (columns of C; u's second), or NULL:
     const unsigned* bmax;    // B's tensor was scaled by this finite maximum (bits)
+    // SPLIT gates write planes (maps kOutMap, kHMap, the lo plane's behind each) in scales that are
+    // known before their values are:
+    float* h_rinv;           // 1 / scale of H's rows (kGate makes and writes it)
+    const float* gu_rinv;    // of dG | dU's
+    const unsigned* w_inv;   // kGate: n_w_inv values whose largest is Wg's and Wu's 1 / scale (bits)
+    int n_w_inv, lg_k;       // ... and 2^lg_k >= K
     // low-rank blocks beside the phases: block t + r holds the rows of 256-row tile t whose requests
     // have request r's adapter ([256][R] typed, zeros in other rows), r being the first such
     int ext;                 // 16-rank slices a request, 0: none
@@ -104,22 +110,28 @@ int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain
 // Operand preparation, up to 6 matrices a launch.
 // kPack: 16-bit copy. kRowSplit: planes scaled row by row. kRowScale: the scales alone. kMax: the
 // largest finite magnitude. kTensorSplit: planes scaled by that. kWeighted: planes of row r times
-// weight[r] / max (a power of two).
-enum Prep { kPack = 0, kRowSplit = 1, kMax = 2, kTensorSplit = 3, kRowScale = 4, kWeighted = 5 };
+// weight[r] / max (a power of two). kBounds: 1 / scale of a gate's rows from what bounds them.
+enum Prep { kPack = 0, kRowSplit = 1, kMax = 2, kTensorSplit = 3, kRowScale = 4, kWeighted = 5,
+            kBounds = 6 };
 struct PrepItem {
     const void* src;
     long long rows, cols, ld;
     void* dst;               // [rows][dld], the lo plane `plane` elements behind
     long long dld, plane;
     float* rinv;             // kRowSplit, kRowScale: 1 / scale of each row, 0 for a row of zeros
-    // kMax, and kRowSplit with a weight (the largest rinv[r] * weight[r]): a maximum of each block
-    // goes to part[block]. kTensorSplit, kWeighted: the largest of part[0 .. parts - 1], which its
+    // kMax, kRowSplit (the largest rinv[r]) and both it and kBounds with a weight (the largest
+    // rinv[r] * weight[r]): a maximum of each block goes to part[block]. kTensorSplit, kWeighted: the largest of part[0 .. parts - 1], which its
     // first block leaves in *max for the products
     unsigned* max;
     int mode;
     const float* weight;
     unsigned* part = nullptr;
     int parts = 0;
+    // kBounds, of H (dy = NULL) or dG | dU: src and dy are 1 / scale of x's and dy's rows; the
+    // maxima of the weights beside them; 2^lg >= their sums' lengths
+    const float* dy = nullptr;
+    const unsigned* w[2] = {};
+    int n[2] = {}, lg[2] = {}, sigmoid = 0;
 };
 constexpr int kPrepBlocks = 1184;            // of one launch and item, at most
 int prep_blocks(const PrepItem& it);          // how many maxima an item writes

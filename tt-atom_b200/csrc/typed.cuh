@@ -39,6 +39,14 @@ __device__ __forceinline__ float pow2_scale(unsigned bits) {
 __device__ __forceinline__ float pow2_inv(float s) {
     return __uint_as_float((254u << 23) - (__float_as_uint(s) & 0x7F800000u));
 }
+// What is scaled to 1 / inv lies below 2^bound_exp(inv); and 1 / scale for values below 2^e.
+__device__ __forceinline__ int bound_exp(float inv) {
+    return (int)(__float_as_uint(inv) >> 23) - 127 + 15;
+}
+__device__ __forceinline__ float bound_inv(int e) {
+    const int sh = e - 15 < -126 ? -126 : (e - 15 > 126 ? 126 : e - 15);
+    return __uint_as_float((unsigned)(sh + 127) << 23);
+}
 // y = hi + lo 2^-11 to 22 bits (lo is NaN where y is not finite).
 __device__ __forceinline__ void split_half2(float y0, float y1, __half2& hi, __half2& lo) {
     hi = __floats2half2_rn(y0, y1);
