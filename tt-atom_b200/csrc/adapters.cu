@@ -25,44 +25,43 @@ namespace {
 using namespace pair;
 
 // fp32, more than 64 ranks: the blocks as planes, scaled row by row, from the low-rank rows. A
-// thread block each.
-__global__ void __launch_bounds__(256) blocks32_kernel(const int* lead, const int* row_lead,
-                                                       const int4* pieces, int M, const float* rows,
-                                                       int R, int Rs, __half* block, long long plane,
-                                                       float* rinv) {
+// thread block each, a warp a row, four ranks a lane.
+__global__ void __launch_bounds__(256) blocks32_kernel(const __grid_constant__ Args p,
+                                                       const float* rows, int Rs, __half* block,
+                                                       long long plane, float* rinv) {
     let_next_start();
     wait_before();
-    if (lead[blockIdx.x] < 0) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = pieces[blockIdx.x].y / 256;
-    const int m0 = t * 256, request = blockIdx.x - t;
-    block += (long long)blockIdx.x * 256 * Rs;
-    for (int i = threadIdx.x; i < 256 * Rs / 8; i += 256) {
-        const int m = m0 + i * 8 / Rs;           // Rs is a multiple of 8
-        if (m < M && row_lead[m] == request) continue;
-        *reinterpret_cast<uint4*>(block + i * 8) = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(block + plane + i * 8) = make_uint4(0, 0, 0, 0);
-    }
+    if (p.lead[blockIdx.x] < 0) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = p.piece[blockIdx.x].y / 256;
+    const int m0 = t * 256, request = blockIdx.x - t, first = p.tile_req[t].x;
+    int before = 0;                              // blocks that the tile has before this one
+    for (int i = t + first; i < (int)blockIdx.x; i += 32)
+        before += __popc(__ballot_sync(0xffffffffu, i + lane < (int)blockIdx.x &&
+                                                        p.lead[i + lane] >= 0));
+    const int slice = before * p.ext + lane / 4;
+    if (4 * lane >= 16 * p.ext) return;
+    __half* q0 = block + ((first_stage(t, first, p.ext) + (slice >> 2)) * 256) * 64 +
+                 (slice & 3) * 16 + (lane & 3) * 4;
+    const unsigned lanes = p.ext == 8 ? 0xffffffffu : (1u << 4 * p.ext) - 1;
 #pragma unroll 4
-    for (int m = m0 + warp; m < min(M, m0 + 256); m += 8) {
-        if (row_lead[m] != request) continue;
-        const float4 x = 4 * lane < Rs
+    for (int m = m0 + warp; m < m0 + 256; m += 8) {
+        const bool in = m < p.M && p.row_lead[m] == request;
+        const float4 x = in && 4 * lane < Rs
             ? *reinterpret_cast<const float4*>(rows + (long long)m * Rs + 4 * lane)
             : make_float4(0.f, 0.f, 0.f, 0.f);
         const unsigned mx = __reduce_max_sync(
-            0xffffffffu, max(max(finite_bits(x.x), finite_bits(x.y)),
-                             max(finite_bits(x.z), finite_bits(x.w))));
+            lanes, max(max(finite_bits(x.x), finite_bits(x.y)),
+                       max(finite_bits(x.z), finite_bits(x.w))));
         const float s = pow2_scale(mx);
-        if (lane == 0) rinv[m] = pow2_inv(s);
-        if (4 * lane >= Rs) continue;
+        if (in && lane == 0) rinv[m] = pow2_inv(s);
         __half2 h[2], l[2];
         split_half2(x.x * s, x.y * s, h[0], l[0]);
         split_half2(x.z * s, x.w * s, h[1], l[1]);
-        __half* q = block + (m - m0) * Rs + 4 * lane;
+        __half* q = q0 + (m - m0) * 64;
         *reinterpret_cast<uint2*>(q) = *reinterpret_cast<uint2*>(h);
         *reinterpret_cast<uint2*>(q + plane) = *reinterpret_cast<uint2*>(l);
     }
 }
-
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -335,13 +334,15 @@ struct AdSizes {
     int dtype;
     long long M;
     int D, O, nad, R, nreq;
-    int tiles, pieces, Rs;
+    int tiles, pieces, Rs, ext;      // ext: slices of 16 ranks
+    long long stages;                // of four slices, in all row tiles' blocks
     long long Dp, Op;
     bool split, on;
     Choice product;
     AdSizes(int t, long long m, int d, int o, int n, int r, int q, bool bwd)
         : dtype(t), M(m), D(d), O(o), nad(n), R(r), nreq(q), tiles((int)((m + 255) / 256)),
-          pieces(tiles + q), Rs((int)up(r, 8)), Dp(up(d, 8)), Op(up(o, 8)), split(t == ATOM_F32),
+          pieces(tiles + q), Rs((int)up(r, 8)), ext((r + 15) / 16),
+          stages(first_stage(tiles, q, ext) + 1), Dp(up(d, 8)), Op(up(o, 8)), split(t == ATOM_F32),
           on(n > 0 && q > 0),
           product(choose(m, bwd ? d : o, ((bwd ? o : d) + 63) / 64, 1, false, t == ATOM_F32, true)) {}
     int grad_split() const {
@@ -395,7 +396,7 @@ struct AdSpace {
             row_lead = c.take<int>(z.M);
             first = c.take<__half>(k * (bwd ? b_n : a_n));
             ext = c.take<__half>(k * (bwd ? a_n : b_n));
-            block = c.take<__half>(k * z.pieces * 256 * z.Rs);
+            block = c.take<__half>(k * z.stages * 256 * 64);
             if (bwd || z.split) T = c.take<char>(z.M * z.Rs * e);
             if (bwd) {
                 x = c.take<__half>(k * z.M * z.Dp);
@@ -438,7 +439,8 @@ struct Ad {
         p.M = z.M, p.N = N, p.groups = 1, p.nphase = 1;
         p.bf16 = z.dtype == ATOM_BF16;
         p.dtype = z.dtype;
-        p.ext = (z.R + 15) / 16;
+        p.ext = z.ext;
+        p.nad = z.nad;
         p.tile_req = sp.tile_req;
         p.piece = sp.piece;
         p.usable = sp.usable;
@@ -468,7 +470,7 @@ struct Ad {
         p.low_scale = scale;
         const bool planes = z.split && z.R <= 64;        // written by the product
         p.low_block = !z.split || (blocks && planes) ? sp.block : nullptr;
-        p.low_plane = (long long)z.pieces * 256 * z.Rs;
+        p.low_plane = z.stages * 256 * 64;
         p.low_rinv = sp.ext_rinv;
         p.low_rows = z.split && !planes && !kept ? sp.T : kept;
         if (!blocks) p.usable = nullptr;
@@ -480,10 +482,8 @@ struct Ad {
         const int share = std::max(1, std::min(groups, 74 / z.tiles));
         if (int s = launch(kLow, {128, share, 0}, z.split, maps, p, st)) return s;
         if (!z.split || !blocks || planes) return ATOM_OK;
-        return st.launch("adapters: blocks", blocks32_kernel, dim3(z.pieces), 256, 0,
-                         (const int*)sp.lead, (const int*)sp.row_lead,
-                         (const int4*)sp.piece, (int)z.M, (const float*)p.low_rows, z.R, z.Rs, sp.block,
-                         (long long)z.pieces * 256 * z.Rs, sp.ext_rinv);
+        return st.launch("adapters: blocks", blocks32_kernel, dim3(z.pieces), 256, 0, p,
+                         (const float*)p.low_rows, z.Rs, sp.block, p.low_plane, sp.ext_rinv);
     }
 
     int run(const void* rows, long long ld, bool bwd, void* out, long long ldo, void* kept) {
@@ -561,9 +561,8 @@ struct Ad {
                                  bwd ? 64 : c.bn / 2))
                 return s;
             if (!z.on) continue;
-            if (int s = make_slice_map(&maps.m[2 * k + pl],
-                                       at(sp.block, (long long)z.pieces * 256 * z.Rs), z.R,
-                                       (long long)z.pieces * 256, z.Rs, 128, false, 0, 0))
+            if (int s = make_map(&maps.m[2 * k + pl], at(sp.block, z.stages * 256 * 64), 64,
+                                 z.stages * 256, 64, 128))
                 return s;
             if (int s = make_slice_map(&maps.m[3 * k + pl], at(o.second, o.second_plane), scols,
                                        bwd ? z.R : z.O, o.second_ld, c.bn / 2, bwd, z.nad,
@@ -617,10 +616,11 @@ int check_ad(int dtype, int64_t M, int D, int O, int nad, int R, int nreq) {
     ATOM_REQUIRE(M >= 0 && M < (1LL << 31) - 256 && D > 0 && O > 0 && nad >= 0 && nreq >= 0,
                  "adapted_linear: bad sizes");
     ATOM_REQUIRE(D < (1 << 24) && O < (1 << 24), "adapted_linear: widths above 2^24");
-    ATOM_REQUIRE(nad < (1 << 14) && nreq < (1 << 22) && (M + 255) / 256 + nreq < (1 << 23),
-                 "adapted_linear: sizes above 2^14 adapters, 2^22 requests or 2^23 pieces of 256 "
-                 "rows");
     ATOM_REQUIRE(R >= 1 && R <= 128, "adapted_linear: the rank must be 1..128");
+    ATOM_REQUIRE(nad < (1 << 14) && nreq < (1 << 22) &&
+                     first_stage((M + 255) / 256, nreq, (R + 15) / 16) < (1 << 23) - 1,
+                 "adapted_linear: sizes above 2^14 adapters, 2^22 requests or 2^25 slices of 256 "
+                 "rows by 16 ranks");
     return ATOM_OK;
 }
 

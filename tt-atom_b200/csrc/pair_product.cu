@@ -244,12 +244,12 @@ struct Share {
         end = p.ksplit == 1 ? nk : (int)((long long)(ti.ks + 1) * nk / p.ksplit);
     }
 };
-// Walks the low-rank blocks of a row tile in slices of 16 ranks, p.ext of them each; four slices of
-// whatever blocks make a stage. The adapters of the first 32 requests, one a lane, are asked for
-// when the walk is made and needed when it begins.
+// Walks the low-rank blocks of a row tile in slices of 16 ranks, p.ext of them each, four to a
+// stage. The adapters of the first 32 requests, one a lane, are asked for when the walk is made and
+// needed when it begins.
 struct Blocks {
     const Args& p;
-    int mt, base, behind, mine, left_in = -1, sub = 0, r = 0, slot = 0;
+    int mt, base, behind, mine, left_in = -1, sub = 0, slot = 0;
     unsigned left = 0;
     __device__ __forceinline__ Blocks(const Args& q, int tile, const int4& t)
         : p(q), mt(tile), base(t.x), behind(t.z ? t.y : t.x) {
@@ -259,7 +259,7 @@ struct Blocks {
         const int i = base + (threadIdx.x & 31);
         mine = i < behind ? p.usable[mt + i] : -1;
     }
-    // the next slice (r, at(), slot); false when there is none
+    // the next slice (at(), slot); false when there is none
     __device__ __forceinline__ bool next() {
         if (sub > 0 && sub < p.ext) {
             ++sub;
@@ -275,7 +275,6 @@ struct Blocks {
         }
         const int i = __ffs(left) - 1;
         left &= left - 1;
-        r = base + i;
         slot = __shfl_sync(0xffffffffu, mine, i);
         sub = 1;
         return true;
@@ -312,16 +311,17 @@ struct Window {
         }
         return n;
     }
-    // writes down which blocks the product beside the projection takes
+    // Writes down which adapters the product beside the projection takes. Adapter nad, past the
+    // tensor map's end, reads as zeros: what is not finite leaves the other rows as they are.
     __device__ __forceinline__ void settle() {
         int n = 0, spoilt = 0;
         for (int r = first; r < behind; r += 32) {
             look(r);
-            const bool ok = a >= 0 && is_finite(p, a);
-            n += __popc(__ballot_sync(0xffffffffu, ok));
-            spoilt |= __ballot_sync(0xffffffffu, a >= 0 && !ok) != 0;
+            const bool ok = a < 0 || is_finite(p, a);
+            n += __popc(mask);
+            spoilt |= __any_sync(0xffffffffu, !ok);
             const int i = r + (threadIdx.x & 31);
-            if (i < behind) p.usable[mt + i] = ok ? a : -1;
+            if (i < behind) p.usable[mt + i] = ok ? a : p.nad;
         }
         if ((threadIdx.x & 31) == 0) {
             p.tile_req[mt].z = n;
@@ -351,9 +351,10 @@ struct Low {
     __device__ __forceinline__ int sub(int i) const {           // which of its piece's slices i is
         return slices > 4 ? i : (i & 3) % slices;
     }
-    // the block of slice i of group g: its adapter and the request that leads it
-    __device__ __forceinline__ int2 piece(int g, int i) {
-        int j = g * each + (slices > 4 ? 0 : (i >> 2) * half + (i & 3) / slices);
+    // the block of slice i of group g: which one of the tile's, its adapter, the request that leads it
+    __device__ __forceinline__ int3 piece(int g, int i) {
+        const int block = g * each + (slices > 4 ? 0 : (i >> 2) * half + (i & 3) / slices);
+        int j = block;
         if (j < before) {
             before = 0;
             w.look(w.first);
@@ -365,7 +366,7 @@ struct Low {
         unsigned v = w.mask;
         for (j -= before; j > 0; --j) v &= v - 1;
         const int l = __ffs(v) - 1;
-        return make_int2(__shfl_sync(0xffffffffu, w.a, l), w.base + l);
+        return make_int3(block, __shfl_sync(0xffffffffu, w.a, l), w.base + l);
     }
 };
 
@@ -617,33 +618,37 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
 }
 
 // kLow: a lane's row of the four slices that a warp has of group g, times the adapter's scale and f:
-// into the pieces' blocks (zeros outside a piece's rows), and into the rows' own places. fp32
-// blocks are planes, scaled row by row: a piece's slices are all in one warp then (ranks of 64 at
-// most; larger ones have a kernel of their own, from the rows).
+// into the tile's blocks (zeros where the row is of another one), and into the rows' own places.
+// fp32 blocks are planes, scaled row by row: a block's slices are all in one warp then (ranks of 64
+// at most; larger ones have a kernel of their own, from the rows).
 __device__ __forceinline__ void low_store(const Args& p, Low& low, int g, int part,
                                           long long m0, int lane, int lead, float (*v)[32],
                                           float f) {
     const int used = low.used(g, part);
     const long long m = m0 + lane;
+    const long long stage0 = first_stage(low.w.mt, low.w.first, p.ext);
+    // a slice's 16 values of this row, in 16-bit elements
+    auto place = [&](int slice) {
+        return ((stage0 + (slice >> 2)) * 256 + (m & 255)) * 64 + (slice & 3) * 16;
+    };
     float largest = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (i >= used) break;
-        const int2 piece = low.piece(g, part * 4 + i);
+        const int3 piece = low.piece(g, part * 4 + i);
         const int sub = low.sub(part * 4 + i), c0 = sub * 16;
-        const bool in = piece.y == lead;
-        const float s = p.low_scale[piece.x] * f;
+        const bool in = piece.z == lead;
+        const float s = p.low_scale[piece.y] * f;
         float* x = v[i >> 1] + (i & 1) * 16;
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = in ? x[j] * s : 0.f;
-        const long long row = ((long long)(low.w.mt + piece.y) * 256 + (m & 255)) * p.Rs;
+        const long long at = place(piece.x * p.ext + sub);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                // eight ranks at a time: Rs is a multiple of 8
             const int c = c0 + 8 * h;
-            if (c >= p.Rs) break;
             const float* y = x + 8 * h;
             if (p.dtype == ATOM_F32) {
-                if (p.low_rows && in) {
+                if (p.low_rows && in && c < p.Rs) {
                     float* q = static_cast<float*>(p.low_rows) + m * p.Rs + c;
                     *reinterpret_cast<float4*>(q) = make_float4(y[0], y[1], y[2], y[3]);
                     *reinterpret_cast<float4*>(q + 4) = make_float4(y[4], y[5], y[6], y[7]);
@@ -652,31 +657,29 @@ __device__ __forceinline__ void low_store(const Args& p, Low& low, int g, int pa
             }
             const uint4 w = make_uint4(pair_w(y[0], y[1], p.dtype), pair_w(y[2], y[3], p.dtype),
                                        pair_w(y[4], y[5], p.dtype), pair_w(y[6], y[7], p.dtype));
-            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.low_block) + row + c) = w;
-            if (p.low_rows && in)
+            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.low_block) + at + 8 * h) = w;
+            if (p.low_rows && in && c < p.Rs)
                 *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.low_rows) + m * p.Rs + c) = w;
         }
         if (p.dtype != ATOM_F32 || !p.low_block) continue;
 #pragma unroll
         for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(x[j]));
-        if (sub < p.ext - 1) continue;               // the piece's last slice: its planes
+        if (sub < p.ext - 1) continue;               // the block's last slice: its planes
         const float scale = pow2_scale(finite_bits(largest));
         if (in) p.low_rinv[m] = pow2_inv(scale);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if (k > i || k < i - sub) continue;
             const float* y = v[k >> 1] + (k & 1) * 16;
-            const int c = (k - i + sub) * 16;
+            __half* q = static_cast<__half*>(p.low_block) + place(piece.x * p.ext + k - i + sub);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (c + 8 * h >= p.Rs) break;
                 __half2 hi[4], lo[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     split_half2(y[8 * h + 2 * j] * scale, y[8 * h + 2 * j + 1] * scale, hi[j], lo[j]);
-                __half* q = static_cast<__half*>(p.low_block) + row + c + 8 * h;
-                *reinterpret_cast<uint4*>(q) = *reinterpret_cast<uint4*>(hi);
-                *reinterpret_cast<uint4*>(q + p.low_plane) = *reinterpret_cast<uint4*>(lo);
+                *reinterpret_cast<uint4*>(q + 8 * h) = *reinterpret_cast<uint4*>(hi);
+                *reinterpret_cast<uint4*>(q + 8 * h + p.low_plane) = *reinterpret_cast<uint4*>(lo);
             }
         }
         largest = 0.f;
@@ -771,7 +774,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                         int slot[4], r16[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            slot[i] = i < mine ? low.piece(g, 4 * rank + i).x : 0;
+                            slot[i] = i < mine ? low.piece(g, 4 * rank + i).y : 0;
                             r16[i] = low.sub(4 * rank + i) * 16;
                         }
                         for (int kt = 0; kt < p.ph[0].nk; ++kt) {
@@ -826,30 +829,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 }
                 if (!p.ext) continue;
                 const int n0 = ti.nt * BN + rank * CF::HB;
-                while (ok) {
-                    int rs[4], slots[4], ks[4], n = 0;
+                long long y = first_stage(ti.mt, req.x, p.ext) * 256 + rank * 128;
+                for (; ok; y += 256) {
+                    int slots[4], ks[4], n = 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (n == i && st.next()) rs[i] = st.r, slots[i] = st.slot, ks[i] = st.at(), ++n;
+                        if (n == i && st.next()) slots[i] = st.slot, ks[i] = st.at(), ++n;
                     uint32_t dst, bar;
-                    if (n == 0 || !(ok = open(dst, bar, n * (CF::kStage / 4)))) break;
+                    if (n == 0 || !(ok = open(dst, bar, P * (CF::kA + n * (CF::kB / 4))))) break;
                     if (!elect_one()) continue;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (i >= n) break;
-                        const int y = (ti.mt + rs[i]) * 256 + rank * 128, k0 = ks[i];
+                    for (int pl = 0; pl < P; ++pl) {
+                        tma_load(dst + pl * CF::kA, &maps.m[p.ext_a + pl], 0, (int)y, bar);
 #pragma unroll
-                        for (int pl = 0; pl < P; ++pl) {
-                            tma_load(dst + pl * CF::kA + i * (CF::kA / 4), &maps.m[p.ext_a + pl],
-                                     k0, y, bar);
+                        for (int i = 0; i < 4; ++i) {
+                            if (i >= n) break;
                             const uint32_t db = dst + P * CF::kA + pl * CF::kB + i * (CF::kB / 4);
                             const CUtensorMap* mb = &maps.m[p.ext_b + pl];
                             if (p.ext_bmn) {
 #pragma unroll
                                 for (int j = 0; j < CF::HB / 64; ++j)
-                                    tma_load3(db + j * 2048, mb, n0 + 64 * j, k0, slots[i], bar);
+                                    tma_load3(db + j * 2048, mb, n0 + 64 * j, ks[i], slots[i], bar);
                             } else {
-                                tma_load3(db, mb, k0, n0, slots[i], bar);
+                                tma_load3(db, mb, ks[i], n0, slots[i], bar);
                             }
                         }
                     }
@@ -954,13 +956,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 }
                 if (SPLIT && ok && open) end(), next_low(), n = 0;
                 if (p.ext) {
-                    const uint64_t a = sdesc_slice(base, 0);
                     const uint64_t b = sdesc_slice(base + P * CF::kA, p.ext_bmn);
                     const uint32_t id = idesc(BN, SPLIT ? 0 : p.bf16, 0, p.ext_bmn);
                     for (; ok && left > 0; left -= 4, ++n) {
                         if (SPLIT && open && n == kRound) end(), n = 0;
                         ok = (open || begin()) &&
-                             stage(a, b, CF::kA >> 6, CF::kB >> 6, id, min(4, left));
+                             stage(base_k, b, 32 >> 4, CF::kB >> 6, id, min(4, left));
                     }
                 }
                 if (ok && open) {

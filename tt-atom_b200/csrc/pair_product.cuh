@@ -26,6 +26,12 @@ struct Phase {
 // 16 columns a slice (ph[0].b0: the adapters' map).
 enum Epilogue { kStore = 0, kGate = 1, kGateBwdGU = 2, kGateBwdDH = 3, kLow = 4 };
 
+// A row tile's first stage of low-rank blocks, by its number and its first request's: tiles need at
+// most a stage more than a quarter of their pieces' slices.
+__host__ __device__ inline long long first_stage(long long tile, long long request, int ext) {
+    return (tile + request) * ext / 4 + tile;
+}
+
 struct Args {
     long long M;             // rows of the output (of one group)
     int N;                   // its columns (gate epilogues: F)
@@ -59,20 +65,21 @@ struct Args {
     const float* gu_rinv;    // of dG | dU's
     const unsigned* w_inv;   // kGate: n_w_inv values whose largest is Wg's and Wu's 1 / scale (bits)
     int n_w_inv, lg_k;       // ... and 2^lg_k >= K
-    // low-rank blocks beside the phases: block t + r holds the rows of 256-row tile t whose requests
-    // have request r's adapter ([256][R] typed, zeros in other rows), r being the first such
-    int ext;                 // 16-rank slices a request, 0: none
+    // Low-rank blocks beside the phases: a row tile's requests that share an adapter have one, led
+    // by the first of them, of `ext` slices of 16 ranks, zero in the other rows. A tile's blocks lie
+    // slice by slice, four to a stage of 256 rows x 64, from stage first_stage() on.
+    int ext;                 // slices a block, 0: none
+    int nad;                 // adapters
     int ext_a, ext_b, ext_bmn;
     int4* tile_req;          // of a row tile: its requests' first and behind; and, from kLow on,
                              // how many blocks count and whether one's adapter is not finite
     const int4* piece;       // t + r, of request r in tile t: adapter or -1 (none), its rows
-    const int* lead;         // a block's adapter where it is the first of its tile with that
-                             // adapter, which takes the others' rows along; else -1
+    const int* lead;         // ... and the adapter again where request r leads a block, else -1
     const int* row_lead;     // per row: the request whose block it is in, -1: none
-    int* usable;             // from kLow on: as lead, -1 also where the adapter is not finite
+    int* usable;             // from kLow on: as lead, but nad where the adapter is not finite
     const int4* bad;         // of an adapter: not all zero = not finite, its rows become NaN
     const float* low_scale;  // kLow: per adapter
-    void* low_block;         // kLow: [block][256][Rs] typed (SPLIT: planes low_plane apart, NULL
+    void* low_block;         // kLow: [stage][256][64] typed (SPLIT: planes low_plane apart, NULL
     long long low_plane;     // for more than 64 ranks), and SPLIT 1 / scale of the rows
     float* low_rinv;
     void* low_rows;          // kLow: [M][Rs] typed, or NULL
