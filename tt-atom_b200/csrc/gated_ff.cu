@@ -144,7 +144,7 @@ struct Ff {
                  long long pitch, int mode, float* rinv, int m = 0) {
         if (!z.split && tma_ready(p, ld)) return {p, rows, cols, ld, 0};
         list.add({p, rows, cols, ld, buf, pitch, rows * pitch, rinv, sp.max + m,
-                  z.split ? mode : kPack, nullptr, sp.maxima[m], parts[m]});
+                  z.split ? mode : kPack, sp.maxima[m], parts[m]});
         if (mode == kRowSplit || !z.split) list.it[list.n - 1].part = nullptr;
         return {buf, rows, cols, pitch, rows * pitch};
     }
@@ -162,8 +162,8 @@ struct Ff {
         x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kRowSplit, sp.xr);
         if (z.split) {
             const long long n = z.F * z.Dp;
-            gather({g, z.F, z.D, z.D, sp.wg, z.Dp, n, sp.wgr, nullptr, kRowSplit, nullptr}, 0);
-            gather({u, z.F, z.D, z.D, sp.wu, z.Dp, n, sp.wur, nullptr, kRowSplit, nullptr}, 0);
+            gather({g, z.F, z.D, z.D, sp.wg, z.Dp, n, sp.wgr, nullptr, kRowSplit}, 0);
+            gather({u, z.F, z.D, z.D, sp.wu, z.Dp, n, sp.wur, nullptr, kRowSplit}, 0);
             wg = {sp.wg, z.F, z.D, z.Dp, n};
             wu = {sp.wu, z.F, z.D, z.Dp, n};
         } else {
@@ -174,33 +174,43 @@ struct Ff {
         return prepare(list, st);
     }
     int inputs_bwd(const void* xp, long long ldx, const void* g, const void* u, const void* d,
-                   const void* dyp, long long lddy, bool kept) {
+                   const void* dyp, long long lddy, bool kept, bool dwgu, bool dwd) {
         if (z.split) {
-            gather({g, z.F, z.D, z.D, nullptr, 0, 0, nullptr, nullptr, kMax, nullptr}, 0);
-            gather({u, z.F, z.D, z.D, nullptr, 0, 0, nullptr, nullptr, kMax, nullptr}, 0);
-            gather({d, z.O, z.F, z.F, nullptr, 0, 0, nullptr, nullptr, kMax, nullptr}, 1);
+            gather({g, z.F, z.D, z.D, nullptr, 0, 0, nullptr, nullptr, kMax}, 0);
+            gather({u, z.F, z.D, z.D, nullptr, 0, 0, nullptr, nullptr, kMax}, 0);
+            gather({d, z.O, z.F, z.F, nullptr, 0, 0, nullptr, nullptr, kMax}, 1);
         }
-        x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kept ? kRowScale : kRowSplit, sp.xr);
-        if (z.split) list.it[list.n - 1].part = nullptr;
-        dy = take(dyp, z.M, z.O, lddy, sp.dy, z.Op, kRowSplit, sp.dyr);
+        if (z.split) {
+            x = {sp.x, z.M, z.D, z.Dp, z.M * z.Dp};
+            dy = {sp.dy, z.M, z.O, z.Op, z.M * z.Op};
+            gather({xp, z.M, z.D, ldx, sp.x, z.Dp, x.plane, sp.xr, nullptr,
+                    kept ? kRowScale : kRowSplit}, 2);
+            gather({dyp, z.M, z.O, lddy, sp.dy, z.Op, dy.plane, sp.dyr, nullptr, kRowSplit}, 3);
+        } else {
+            x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kPack, nullptr);
+            dy = take(dyp, z.M, z.O, lddy, sp.dy, z.Op, kPack, nullptr);
+        }
         if (z.split)
             if (int s = prepare(list, st)) return s;
         wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kTensorSplit, nullptr, 0);
         wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kTensorSplit, nullptr, 0);
         wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kTensorSplit, nullptr, 1);
-        if (z.split) {
-            // Scales of dG | dU and H, and the largest that a row of them and its partner in the
-            // weights' gradients have together.
-            PrepItem b{sp.xr, z.M, 0, 0, nullptr, 0, 0, sp.dgur, nullptr, kBounds, sp.xr};
-            b.dy = sp.dyr;
-            for (int k = 0; k < 2; ++k) b.w[k] = sp.maxima[k], b.n[k] = parts[k];
-            b.lg[0] = log2_up(z.D), b.lg[1] = log2_up(z.O);
-            b.sigmoid = act == 1;
-            gather(b, 2);
-            b.dy = nullptr, b.rinv = sp.hr, b.weight = sp.dyr;
-            gather(b, 3);
-        }
+        // dG | dU and H are scaled row by row. In the weights' gradients, sums over rows, the rows'
+        // scales s cancel against x (and dy) rows divided by them: what is left is one power of two
+        // for all rows, and rows lose bits only as far as they are small in the sum.
+        auto weighted = [&](const void* p, int n, long long ld, __half* buf, long long pitch, int k) {
+            PrepItem it{p, z.M, n, ld, buf, pitch, z.M * pitch, nullptr, sp.max + 2 + k, kWeighted};
+            it.bounds = bounds();
+            for (int i = 0; i < 4; ++i) it.top[i] = sp.maxima[i], it.tops[i] = parts[i];
+            it.of_h = k;
+            list.add(it);
+        };
+        if (z.split && dwgu) weighted(xp, z.D, ldx, sp.xt, z.Dp, 0);
+        if (z.split && dwd) weighted(dyp, z.O, lddy, sp.dyt, z.Op, 1);
         return prepare(list, st);
+    }
+    Bounds bounds() const {
+        return {sp.xr, sp.dyr, sp.max, {log2_up(z.D), log2_up(z.O)}, act == 1};
     }
     Args args(long long M, int N) const {
         Args p;
@@ -229,6 +239,7 @@ struct Ff {
         p.H = H != nullptr;
         p.h_rinv = sp.hr;
         p.gu_rinv = sp.dgur;
+        p.bounds = bounds();
         const int t = z.split ? ATOM_F16 : z.dtype;
         for (int k = 0; k < step(); ++k) {
             p.used |= 1u << (kOutMap + k) | (unsigned)p.H << (kHMap + k);
@@ -259,7 +270,7 @@ struct Ff {
     int forward(void* y, long long ldy, float* kept) {
         Args p = args(z.M, z.F);
         p.gu = kept;
-        p.w_inv = sp.maxima[0], p.n_w_inv = parts[0], p.lg_k = log2_up(z.D);
+        p.w_inv = sp.maxima[0], p.n_w_inv = parts[0];
         __half* out = z.split ? sp.hp : sp.H;
         if (int s = gates(kGate, p, out, z.Fp, nullptr)) return s;
         const Operand h{out, z.M, z.F, z.Fp, z.M * z.Fp};
@@ -305,24 +316,7 @@ struct Ff {
         const Operand g{dgu, z.M, 2 * z.Fp, 2 * z.Fp, z.M * 2 * z.Fp};
         const Operand h{hs, z.M, z.F, z.Fp, z.M * z.Fp};
         Operand xt = x, dyt = dy;
-        if (z.split) {
-            // dG | dU and H are scaled row by row. In the weights' gradients, sums over rows, the
-            // rows' scales s cancel against x (and dy) rows divided by them: what is left is one
-            // power of two, the largest of the rows' x (dy) and dG | dU (H) scales together, and
-            // rows lose bits only as far as they are small in the sum.
-            const long long M = z.M;
-            if (dwg || dwu) {
-                xt = {sp.xt, M, z.D, z.Dp, M * z.Dp};
-                list.add({x_src, M, z.D, x_ld, sp.xt, z.Dp, M * z.Dp, nullptr, sp.max + 2, kWeighted,
-                          sp.dgur, sp.maxima[2], parts[2]});
-            }
-            if (dwd) {
-                dyt = {sp.dyt, M, z.O, z.Op, M * z.Op};
-                list.add({dy_src, M, z.O, dy_ld, sp.dyt, z.Op, M * z.Op, nullptr, sp.max + 3,
-                          kWeighted, sp.hr, sp.maxima[3], parts[3]});
-            }
-            if (int s = prepare(list, st)) return s;
-        }
+        if (z.split) xt.p = sp.xt, dyt.p = sp.dyt;
         if (dx) {
             const Choice c = z.dx;
             Maps maps;
@@ -368,8 +362,6 @@ struct Ff {
         }
         return ATOM_OK;
     }
-    const void *x_src = nullptr, *dy_src = nullptr;
-    long long x_ld = 0, dy_ld = 0;
 };
 
 // A few rows: two products forward, which keep nothing; back, dH, then G and U again with dG, dU
@@ -484,9 +476,10 @@ extern "C" int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t 
     Ff f{z, FfSpace(ws, z, true), st, act};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
                  f.sp.bytes);
-    f.x_src = x, f.x_ld = ldx, f.dy_src = dy, f.dy_ld = lddy;
     if (M <= few::kFewRows)
         return few_backward(f, x, ldx, wg, wu, wd, dy, lddy, dx, lddx, dwg, dwu, dwd);
-    if (int s = f.inputs_bwd(x, ldx, wg, wu, wd, dy, lddy, kept != nullptr)) return s;
+    if (int s = f.inputs_bwd(x, ldx, wg, wu, wd, dy, lddy, kept != nullptr, dwg || dwu,
+                             dwd != nullptr))
+        return s;
     return f.backward(static_cast<const float*>(kept), dx, lddx, dwg, dwu, dwd);
 }

@@ -18,6 +18,11 @@
 // (added there to nearest) every kRound stages: 8 additions, which holds an fp32 result near 5e-7
 // of itself (2-norm) at any K; one accumulator at K = 1024 is 3.5e-6 off, 16 additions 9.7e-7.
 //
+// Bound by the tensor core where K and the tiles are many: the whole training step of 8,192 x 2,048
+// x 8,192 in bf16 (2.47 PFLOP in 8 launches) runs at 1.34 PFLOP/s, 95 % of what a library product
+// sustains under the power cap; 60,000 x 256 -> 2 x 1,024 with the gate at 1.05, bound by its
+// epilogue; a SPLIT product does three, at 0.9 of 1.7 PFLOP/s together at 4,011 x 672 x 2,632.
+//
 // Warp 0 has TMA, warp 1 tensor memory and the products (CTA 0's issues for both), warps 2.. the
 // epilogue. Every wait is bounded: on expiry the kernel records a code, lets copies in
 // flight land, frees its tensor memory and returns.
@@ -999,12 +1004,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
         Out out{outbuf + (warp - 2) * 4096, 0};
         constexpr int kParts = GATED ? 2 * kChunks : kChunks;
         uint32_t low = 2 * BN;
-        int e_w = 0;
+        int e_g = 0, e_d = 0;        // of g and u, and of dh, beside x's and dy's rows
         if constexpr (SPLIT && EPI == kGate) {
             float w = 0.f;
 #pragma unroll 4
             for (int i = lane; i < p.n_w_inv; i += 32) w = fmaxf(w, __uint_as_float(p.w_inv[i]));
-            e_w = bound_exp(warp_max(w)) + p.lg_k;
+            e_g = bound_exp(warp_max(w)) + p.bounds.lg[0];
+        } else if constexpr (SPLIT && (EPI == kGateBwdGU || EPI == kGateBwdDH)) {
+            e_g = bound_exp(pow2_inv(pow2_scale(p.bounds.w[0]))) + p.bounds.lg[0];
+            e_d = bound_exp(pow2_inv(pow2_scale(p.bounds.w[1]))) + p.bounds.lg[1];
         }
         Ahead ahead;
         uint32_t mine_k = 0;
@@ -1103,15 +1111,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 // of their row's bound, so a row whose largest value is 2^-27 of it still has fp32's
                 // own rounding; Gaussian rows come to 2^-16 at K = 512 (2^-20 at 2,048 at the least).
                 float sh = 1.f, sg = 1.f;
-                if constexpr (EPI == kGate) {
-                    const int e = bound_exp(sa) + e_w;
-                    const float inv = bound_inv(p.act == 1 ? e : 2 * e);
+                if constexpr (EPI == kGate || EPI == kGateBwdGU || EPI == kGateBwdDH) {
+                    const bool in = m + lane < p.M, writes = in && ti.nt == 0 && part == 0;
+                    const int g = bound_exp(in ? p.bounds.x[m + lane] : 0.f) + e_g;
+                    const float inv = bound_inv(p.bounds.h(g));
                     sh = pow2_inv(inv);
-                    if (ti.nt == 0 && part == 0 && m + lane < p.M) p.h_rinv[m + lane] = inv;
-                } else if constexpr (EPI == kGateBwdGU || EPI == kGateBwdDH) {
-                    if (m + lane < p.M) {
-                        sh = pow2_inv(p.h_rinv[m + lane]);
-                        sg = pow2_inv(p.gu_rinv[m + lane]);
+                    if (writes) p.h_rinv[m + lane] = inv;
+                    if constexpr (EPI != kGate) {
+                        const int d = bound_exp(in ? p.bounds.dy[m + lane] : 0.f) + e_d;
+                        const float gu = bound_inv(p.bounds.gu(g, d));
+                        sg = pow2_inv(gu);
+                        if (writes) p.gu_rinv[m + lane] = gu;
                     }
                 }
                 if constexpr (EPI == kLow) {
@@ -1213,7 +1223,8 @@ __global__ void __launch_bounds__(256) reduce_kernel(const __grid_constant__ Arg
 // stay in registers between their maximum and their planes (up to 8192 columns) and are read once.
 // Planes and packed rows are zero past the row's end up to the pitch. Bound by memory: the two
 // halves of a value cost five instructions, since what is not finite needs no care (its results are
-// not finite either way) except that a maximum leaves it out.
+// not finite either way) except that a maximum leaves it out. 18,000 x 1,536 values: 43 us, 5.2 TB/s
+// read and written.
 constexpr int kNV = 8;
 __host__ __device__ inline int prep_slots(const PrepItem& it) {      // float4 a lane of one row
     const long long c = it.dld > it.cols ? it.dld : it.cols;
@@ -1248,17 +1259,27 @@ __device__ __forceinline__ float row_scale(const PrepItem& it, long long r, floa
                                            float& top) {
     const float s = pow2_scale(__float_as_uint(mx)), inv = mx > 0.f ? pow2_inv(s) : 0.f;
     if (writes) it.rinv[r] = inv;
-    top = fmaxf(top, it.weight ? fminf(inv * it.weight[r], 0x1p126f) : inv);
+    top = fmaxf(top, inv);
     return s;
 }
-// kTensorSplit's scale, or what kWeighted divides a row's weight by, from the maxima.
-__device__ __forceinline__ float fixed_scale(const PrepItem& it, long long r, unsigned max) {
-    if (it.mode == kTensorSplit) return pow2_scale(max);
-    // a row whose partner is zero may have any weight
-    return fminf(it.weight[r] * pow2_inv(__uint_as_float(max)), 0x1p126f);
+// What a launch knows of all its rows: kTensorSplit's largest magnitude; kWeighted's power of two
+// 2^power, and the exponents that the weights and the sums' lengths put on g and u and on dh.
+struct Fixed {
+    unsigned max;
+    int power, g, d;
+};
+template <bool WEIGHTED>
+__device__ __forceinline__ float fixed_scale(const PrepItem& it, long long r, const Fixed& f) {
+    if (!WEIGHTED || it.mode == kTensorSplit) return pow2_scale(f.max);
+    const int g = bound_exp(it.bounds.x[r]) + f.g;
+    const float inv = bound_inv(it.of_h ? it.bounds.h(g)
+                                        : it.bounds.gu(g, bound_exp(it.bounds.dy[r]) + f.d));
+    const int k = (int)(__float_as_uint(inv) >> 23) - 127 - f.power;
+    return __uint_as_float((unsigned)(min(::max(k, -126), 126) + 127) << 23);
 }
 
-__device__ __forceinline__ void prep_narrow(const PrepItem& it, int blocks, unsigned max,
+template <bool WEIGHTED>
+__device__ __forceinline__ void prep_narrow(const PrepItem& it, int blocks, const Fixed& fixed,
                                             float& top) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int nv = prep_slots(it), rows = kNV / nv, shift = 31 - __clz(nv);
@@ -1323,15 +1344,16 @@ __device__ __forceinline__ void prep_narrow(const PrepItem& it, int blocks, unsi
             const long long r = r0 + i;
             if (r >= it.rows) continue;
             const float s = scans ? row_scale(it, r, m[j], k == 0 && lane == 0, top)
-                                  : fixed_scale(it, r, max);
+                                  : fixed_scale<WEIGHTED>(it, r, fixed);
             if (mode != kRowScale && c < dld)
                 prep_put(static_cast<__half*>(it.dst) + r * dld + c, it.plane, x[j], s);
         }
     }
 }
 
+template <bool WEIGHTED>
 __device__ __forceinline__ void prep_block(const PrepItem& it, int blocks, float* part,
-                                           unsigned max, float& top) {
+                                           const Fixed& fixed, float& top) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = threadIdx.x;
     const int cols = (int)it.cols, dld = (int)it.dld, mode = it.mode;
     const bool scans = mode == kRowSplit || mode == kMax || mode == kRowScale;
@@ -1373,7 +1395,7 @@ __device__ __forceinline__ void prep_block(const PrepItem& it, int blocks, float
             s = row_scale(it, r, mx, me == 0, top);
             if (mode == kRowScale) continue;
         } else {
-            s = fixed_scale(it, r, max);
+            s = fixed_scale<WEIGHTED>(it, r, fixed);
         }
         __half* hi = static_cast<__half*>(it.dst) + r * dld;
 #pragma unroll
@@ -1487,6 +1509,10 @@ __device__ __forceinline__ void find_pieces(const Pieces& p) {
     if (threadIdx.x == 0) reinterpret_cast<int*>(p.bad + a)[part] = found;
 }
 
+// KIND 0: 16-bit copies; 1: planes; 2: planes with kWeighted items. Small operands are prepared in the
+// time of a launch and of their code's first fetch: all in one kernel costs 1,002 x 256 x 1,024 in
+// fp32 2 us of 26, 4,000 x 256 adapters forward and backward 4 of 101.
+template <int KIND>
 __global__ void __launch_bounds__(256, 3)
     prep_kernel(const __grid_constant__ PrepList l, const __grid_constant__ Pieces pieces) {
     __shared__ float part[8];
@@ -1499,6 +1525,10 @@ __global__ void __launch_bounds__(256, 3)
     const PrepItem& it = l.it[blockIdx.y];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (blockIdx.x >= l.blocks[blockIdx.y]) return;
+    if constexpr (KIND == 0) {
+        prep_pack(it, l.blocks[blockIdx.y]);
+        return;
+    }
     float top = 0.f;
     auto over_block = [&](float v) {             // the block's largest, in every thread
         v = warp_max(v);
@@ -1508,40 +1538,37 @@ __global__ void __launch_bounds__(256, 3)
         __syncthreads();
         return warp_max(v);
     };
-    unsigned max = 0;
-    if (it.mode == kTensorSplit || it.mode == kWeighted) {
+    auto largest = [&](const unsigned* of, int n) {
         float v = 0.f;
 #pragma unroll 4
-        for (int i = threadIdx.x; i < it.parts; i += 256) v = fmaxf(v, __uint_as_float(it.part[i]));
-        max = __float_as_uint(over_block(v));
-        if (blockIdx.x == 0 && threadIdx.x == 0) *it.max = max;
+        for (int i = threadIdx.x; i < n; i += 256) v = fmaxf(v, __uint_as_float(of[i]));
+        return over_block(v);
+    };
+    Fixed fixed{};
+    if (it.mode == kTensorSplit) {
+        fixed.max = __float_as_uint(largest(it.part, it.parts));
+        if (blockIdx.x == 0 && threadIdx.x == 0) *it.max = fixed.max;
+    } else if (KIND == 2 && it.mode == kWeighted) {
+        // 2^power is no less than what a row's magnitude, in its scale, and its weight can come to
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = largest(it.top[k], it.tops[k]);
+        fixed.g = bound_exp(pow2_inv(pow2_scale(__float_as_uint(v[0])))) + it.bounds.lg[0];
+        fixed.d = bound_exp(pow2_inv(pow2_scale(__float_as_uint(v[1])))) + it.bounds.lg[1];
+        const int x = bound_exp(v[2]), dy = bound_exp(v[3]), g = x + fixed.g;
+        const int weight = it.of_h ? it.bounds.h(g) : it.bounds.gu(g, dy + fixed.d);
+        fixed.power = min(::max(weight + (it.of_h ? dy : x) - 30, -126), 126);
+        if (blockIdx.x == 0 && threadIdx.x == 0)
+            *it.max = (unsigned)(fixed.power + 127) << 23;
     }
     const int blocks = l.blocks[blockIdx.y];
-    if (it.mode == kBounds) {
-        int e[2] = {};
-        for (int k = 0; k < (it.dy ? 2 : 1); ++k) {
-            float v = 0.f;
-            for (int i = threadIdx.x; i < it.n[k]; i += 256)
-                v = fmaxf(v, __uint_as_float(it.w[k][i]));
-            e[k] = bound_exp(pow2_inv(pow2_scale(__float_as_uint(over_block(v))))) + it.lg[k];
-        }
-        for (long long r = blockIdx.x * 256LL + threadIdx.x; r < it.rows; r += blocks * 256LL) {
-            // |g|, |u| < 2^g; |act(g)| <= |g| or 1, |act'(g)| < 2 (sigmoid: 1/4)
-            const int g = bound_exp(static_cast<const float*>(it.src)[r]) + e[0];
-            const float inv = bound_inv(
-                it.dy ? bound_exp(it.dy[r]) + e[1] + (it.sigmoid ? ::max(g - 2, 0) : g + 1)
-                      : it.sigmoid ? g : 2 * g);
-            it.rinv[r] = inv;
-            top = fmaxf(top, fminf(inv * it.weight[r], 0x1p126f));
-        }
-    } else if (it.mode == kPack) prep_pack(it, blocks);
-    else if (prep_wide(it)) prep_block(it, blocks, part, max, top);
-    else prep_narrow(it, blocks, max, top);
+    if (prep_wide(it)) prep_block<KIND == 2>(it, blocks, part, fixed, top);
+    else prep_narrow<KIND == 2>(it, blocks, fixed, top);
     // the epilogue reads scales of columns 32 at a time
     if (it.mode == kRowSplit && blockIdx.x == 0 && threadIdx.x < 32 &&
         it.rows + lane < (it.rows + 31) / 32 * 32)
         it.rinv[it.rows + lane] = 0.f;
-    if (it.part && (it.mode == kMax || it.mode == kRowSplit || it.mode == kBounds)) {
+    if (it.part && (it.mode == kMax || it.mode == kRowSplit || it.mode == kRowScale)) {
         __syncthreads();
         top = over_block(top);
         if (threadIdx.x == 0) it.part[blockIdx.x] = __float_as_uint(top);
@@ -1549,7 +1576,7 @@ __global__ void __launch_bounds__(256, 3)
 }
 
 int prep_blocks(const PrepItem& it) {
-    const int rows = it.mode == kBounds ? 256 : it.mode == kPack ? 8 : prep_wide(it) ? 1 : 8 * (kNV / prep_slots(it));
+    const int rows = it.mode == kPack ? 8 : prep_wide(it) ? 1 : 8 * (kNV / prep_slots(it));
     return (int)std::max(1LL, std::min((it.rows + rows - 1) / rows, (long long)kPrepBlocks));
 }
 int prepare(PrepList& l, Chain& st, const Pieces* pieces) {
@@ -1560,8 +1587,15 @@ int prepare(PrepList& l, Chain& st, const Pieces* pieces) {
     if (pieces)
         grid = std::max(grid, (pieces->pieces + pieces->tiles + 7) / 8 +
                                   (pieces->other ? 4 * pieces->nad : 0));
-    const int s = st.launch("operand preparation", prep_kernel, dim3(grid, l.n + (pieces != nullptr)),
-                            256, 0, l, pieces ? *pieces : none);
+    bool weighted = false, split = false;        // a list is of one type
+    for (int i = 0; i < l.n; ++i) {
+        weighted |= l.it[i].mode == kWeighted;
+        split |= l.it[i].mode != kPack;
+    }
+    const int s = st.launch("operand preparation",
+                            weighted ? prep_kernel<2> : split ? prep_kernel<1> : prep_kernel<0>,
+                            dim3(grid, l.n + (pieces != nullptr)), 256, 0, l,
+                            pieces ? *pieces : none);
     l.n = 0;
     return s;
 }

@@ -26,6 +26,20 @@ struct Phase {
 // 16 columns a slice (ph[0].b0: the adapters' map).
 enum Epilogue { kStore = 0, kGate = 1, kGateBwdGU = 2, kGateBwdDH = 3, kLow = 4 };
 
+// What bounds a gate's rows: those of x and dy, by 1 / scale, the largest magnitudes (bits) of
+// Wg | Wu and of Wd, and lg[k], 2^lg[k] being no less than D and O.
+struct Bounds {
+    const float *x, *dy;
+    const unsigned* w;
+    int lg[2], sigmoid;
+    // exponents of bounds of H and of dG | dU from those of g and u (x, W and D alone) and of dh:
+    // |act(g)| <= |g|, |act'(g)| < 2, or for the sigmoid 1 and 1/4
+    __device__ __forceinline__ int h(int g) const { return sigmoid ? g : 2 * g; }
+    __device__ __forceinline__ int gu(int g, int d) const {
+        return d + (sigmoid ? max(g - 2, 0) : g + 1);
+    }
+};
+
 // A row tile's first stage of low-rank blocks, by its number and its first request's: tiles need at
 // most a stage more than a quarter of their pieces' slices.
 __host__ __device__ inline long long first_stage(long long tile, long long request, int ext) {
@@ -61,10 +75,11 @@ struct Args {
     const unsigned* bmax;    // B's tensor was scaled by this finite maximum (bits)
     // SPLIT gates write planes (maps kOutMap, kHMap, the lo plane's behind each) in scales that are
     // known before their values are:
-    float* h_rinv;           // 1 / scale of H's rows (kGate makes and writes it)
-    const float* gu_rinv;    // of dG | dU's
+    float* h_rinv;           // out: 1 / scale of H's rows
+    float* gu_rinv;          // out, backward: of dG | dU's
     const unsigned* w_inv;   // kGate: n_w_inv values whose largest is Wg's and Wu's 1 / scale (bits)
-    int n_w_inv, lg_k;       // ... and 2^lg_k >= K
+    int n_w_inv;
+    Bounds bounds;           // kGate: lg and sigmoid alone
     // Low-rank blocks beside the phases: a row tile's requests that share an adapter have one, led
     // by the first of them, of `ext` slices of 16 ranks, zero in the other rows. A tile's blocks lie
     // slice by slice, four to a stage of 256 rows x 64, from stage first_stage() on.
@@ -117,28 +132,26 @@ int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain
 // Operand preparation, up to 6 matrices a launch.
 // kPack: 16-bit copy. kRowSplit: planes scaled row by row. kRowScale: the scales alone. kMax: the
 // largest finite magnitude. kTensorSplit: planes scaled by that. kWeighted: planes of row r times
-// weight[r] / max (a power of two). kBounds: 1 / scale of a gate's rows from what bounds them.
-enum Prep { kPack = 0, kRowSplit = 1, kMax = 2, kTensorSplit = 3, kRowScale = 4, kWeighted = 5,
-            kBounds = 6 };
+// the 1 / scale of what they are summed with, dG | dU's or H's, over a power of two.
+enum Prep { kPack = 0, kRowSplit = 1, kMax = 2, kTensorSplit = 3, kRowScale = 4, kWeighted = 5 };
 struct PrepItem {
     const void* src;
     long long rows, cols, ld;
     void* dst;               // [rows][dld], the lo plane `plane` elements behind
     long long dld, plane;
     float* rinv;             // kRowSplit, kRowScale: 1 / scale of each row, 0 for a row of zeros
-    // kMax, kRowSplit (the largest rinv[r]) and both it and kBounds with a weight (the largest
-    // rinv[r] * weight[r]): a maximum of each block goes to part[block]. kTensorSplit, kWeighted: the largest of part[0 .. parts - 1], which its
-    // first block leaves in *max for the products
+    // kMax, kRowSplit and kRowScale (the largest rinv[r]): a maximum of each block goes to
+    // part[block]. kTensorSplit: the largest of part[0 .. parts - 1], which its first block leaves
+    // in *max for the products, as kWeighted's does its power of two.
     unsigned* max;
     int mode;
-    const float* weight;
     unsigned* part = nullptr;
     int parts = 0;
-    // kBounds, of H (dy = NULL) or dG | dU: src and dy are 1 / scale of x's and dy's rows; the
-    // maxima of the weights beside them; 2^lg >= their sums' lengths
-    const float* dy = nullptr;
-    const unsigned* w[2] = {};
-    int n[2] = {}, lg[2] = {}, sigmoid = 0;
+    // kWeighted: rows of x (dy where `of_h`); the maxima over blocks of the weights' magnitudes and
+    // of the rows' 1 / scale
+    Bounds bounds{};
+    const unsigned* top[4] = {};         // Wg | Wu, Wd, x, dy
+    int tops[4] = {}, of_h = 0;
 };
 constexpr int kPrepBlocks = 1184;            // of one launch and item, at most
 int prep_blocks(const PrepItem& it);          // how many maxima an item writes
