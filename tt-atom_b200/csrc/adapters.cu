@@ -580,11 +580,10 @@ struct Ad {
         p.rinv = sp.rinv;
         p.cinv[0] = sp.wr;
         if (z.split && bwd) p.bmax = sp.max;
-        if (!z.on) p.ext = 0;
         p.ext_a = 2 * k, p.ext_b = 3 * k, p.ext_bmn = bwd ? 1 : 0;
         p.ext_rinv = sp.ext_rinv;
         p.ext_bmax = sp.max + 1;
-        return launch(kStore, c, z.split, maps, p, st);
+        return launch(z.on ? kStoreLow : kStore, c, z.split, maps, p, st);
     }
 
     // S alone, in the backward pass: x's and a's own copies, the pieces as they are

@@ -581,8 +581,8 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
                                          float sh, float sg) {
     if (m >= p.M || n >= p.N) return;
     const int left = p.N - n;
-    if constexpr (EPI == kStore) {
-        if (p.blocked) {
+    if constexpr (EPI == kStore || EPI == kStoreLow) {
+        if (EPI == kStore && p.blocked) {
             store_block(lane_block(p.blocked, m, n, p.Fp, lane), v0);
         } else if (p.ksplit > 1) {
             const int z = ti.ks * p.groups + ti.grp;
@@ -766,7 +766,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 const Tile ti = tile_of(p, t);
                 const int m0 = ti.mt * 256 + rank * 128;
                 int4 req = make_int4(0, 0, 0, 0);
-                if (EPI == kStore && p.ext) {
+                if (EPI == kStoreLow) {
                     req = ahead.get(p, mine_k, first, pairs);
                     if (ti.ks != p.ksplit - 1) req.z = 0;
                 }
@@ -832,7 +832,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                         }
                     }
                 }
-                if (!p.ext) continue;
+                if constexpr (EPI != kStoreLow) continue;
                 const int n0 = ti.nt * BN + rank * CF::HB;
                 long long y = first_stage(ti.mt, req.x, p.ext) * 256 + rank * 128;
                 for (; ok; y += 256) {
@@ -927,7 +927,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
             for (long long t = first; ok && t < p.tiles; t += pairs, ++mine_k) {
                 const Tile ti = tile_of(p, t);
                 int n = 0, left = 0;
-                if (EPI == kStore && p.ext) {
+                if (EPI == kStoreLow) {
                     left = ahead.get(p, mine_k, first, pairs).z * p.ext;
                     if (ti.ks != p.ksplit - 1) left = 0;
                 }
@@ -960,7 +960,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     }
                 }
                 if (SPLIT && ok && open) end(), next_low(), n = 0;
-                if (p.ext) {
+                if constexpr (EPI == kStoreLow) {
                     const uint64_t b = sdesc_slice(base + P * CF::kA, p.ext_bmn);
                     const uint32_t id = idesc(BN, SPLIT ? 0 : p.bf16, 0, p.ext_bmn);
                     for (; ok && left > 0; left -= 4, ++n) {
@@ -1021,8 +1021,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
             const long long m = (long long)ti.mt * 256 + rank * 128 + q * 32;
             const int nb = ti.nt * (GATED ? BN / 2 : BN) + c0;
             int4 req = make_int4(0, 0, 0, 0);
-            if (EPI == kStore && p.ext) req = ahead.get(p, mine_k, first, pairs);
-            const bool spoilt = EPI == kStore && req.w && spoilt_row(p, ti.mt, m + lane, lane);
+            if (EPI == kStoreLow) req = ahead.get(p, mine_k, first, pairs);
+            const bool spoilt = EPI == kStoreLow && req.w && spoilt_row(p, ti.mt, m + lane, lane);
             if (EPI == kLow && warp == 2 && rank == 0 && ti.ks == 0 && p.usable)
                 Window(p, ti.mt).settle();
             if constexpr (EPI == kLow && !SPLIT) {
@@ -1052,7 +1052,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     pin32(v0);
                     if (GATED) pin32(v1);
                     if (k == kChunks - 1) drained();
-                    if (EPI == kStore && spoilt) spoil32(v0);
+                    if (EPI == kStoreLow && spoilt) spoil32(v0);
                     finish32<EPI, SPLIT>(maps, p, ti, out, m, nb + 32 * k, lane, v0, v1, 1.f,
                                          1.f);
                 }
@@ -1159,7 +1159,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                         }
                     }
                 }
-                if (p.ext) {
+                if constexpr (EPI == kStoreLow) {
                     const int es = ti.ks == p.ksplit - 1 ? (req.z * p.ext + 3) >> 2 : 0;
                     // rows of no piece have no scale, and sums of zero
                     float f = m + lane < p.M ? p.ext_rinv[m + lane] : 0.f;
@@ -1169,7 +1169,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
 #pragma unroll
                 for (int k = 0; k < kChunks; ++k) {
                     float u[32];         // kGateBwdDH: room for the u that it reads
-                    if (EPI == kStore && spoilt) spoil32(v[k]);
+                    if (EPI == kStoreLow && spoilt) spoil32(v[k]);
                     finish32<EPI, SPLIT>(maps, p, ti, out, m, nb + 32 * k, lane, v[k],
                                          GATED ? v[kChunks + k] : u, sh, sg);
                 }
@@ -1751,7 +1751,7 @@ int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain
     if (p.tiles == 0) return ATOM_OK;
     if (epilogue == kLow)
         return split ? run<128, kLow, true>(maps, p, st) : run<128, kLow, false>(maps, p, st);
-    if (epilogue == kStore && !p.blocked) {
+    if ((epilogue == kStore || epilogue == kStoreLow) && !p.blocked) {
         // TMA stores clip at 16 bytes, so columns have to end there too
         const int e = p.ksplit > 1 ? 4 : dtype_size(p.dtype);
         p.tma = p.N * e % 16 == 0;
@@ -1776,6 +1776,7 @@ int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain
                            : run<128, E, false>(maps, p, st);   \
     }
     ATOM_PAIR(kStore)
+    ATOM_PAIR(kStoreLow)
     ATOM_PAIR(kGate)
     ATOM_PAIR(kGateBwdGU)
     ATOM_PAIR(kGateBwdDH)

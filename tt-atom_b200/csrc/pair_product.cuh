@@ -23,8 +23,9 @@ struct Phase {
 };
 
 // kLow: the requests' low-rank rows themselves: of each row tile, times the adapters of its pieces,
-// 16 columns a slice (ph[0].b0: the adapters' map).
-enum Epilogue { kStore = 0, kGate = 1, kGateBwdGU = 2, kGateBwdDH = 3, kLow = 4 };
+// 16 columns a slice (ph[0].b0: the adapters' map). kStoreLow: kStore with low-rank blocks beside the
+// phases.
+enum Epilogue { kStore = 0, kGate = 1, kGateBwdGU = 2, kGateBwdDH = 3, kLow = 4, kStoreLow = 5 };
 
 // What bounds a gate's rows: those of x and dy, by 1 / scale, the largest magnitudes (bits) of
 // Wg | Wu and of Wd, and lg[k], 2^lg[k] being no less than D and O.
