@@ -79,6 +79,7 @@ __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uin
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+constexpr int kStages = 4;           // of grads16_kernel
 // dA[a] = T^T x and dB[a] = (S^T dy)^T over the pieces of adapter a, in their order: blocks have
 // all ranks by 128 columns of x or dy, and the pieces are shared out over blocks (`split`) whose
 // sums are added in order by a second pass. Bound by reading x and dy once.
@@ -143,7 +144,7 @@ __device__ __forceinline__ void put_grad(const Grads& p, int which, int a, int r
 // columns, 8 adapters of 16 ranks: 20 us (2.4 TB/s; floor 7.6), bound by the latency of its stages.
 template <bool BF16, int MT>
 __global__ void __launch_bounds__(256) grads16_kernel(const __grid_constant__ Grads p) {
-    constexpr int kX = 32 * 272, kT = 32 * (32 * MT + 16), kStages = 4;
+    constexpr int kX = 32 * 272, kT = 32 * (32 * MT + 16);
     extern __shared__ __align__(16) uint8_t smem[];
     let_next_start();
     wait_before();
@@ -270,8 +271,7 @@ __global__ void __launch_bounds__(256) grads32_kernel(const __grid_constant__ Gr
             put_grad(p, which, a, r0 + ty * 4 + i, c0 + lane * 4 + j, acc[i][j]);
 }
 // A thread has a column and four ranks: it reads along rows of columns and writes dB's ranks,
-// which lie side by side, together. 32 loads in flight a thread (16 shares of 3 x 1,850 x 16 values:
-// 18 us with 16, 5.5 us so).
+// which lie side by side, together. Bound by the latency of its loads, 16 in flight a thread.
 __global__ void __launch_bounds__(256) grads_sum_kernel(const __grid_constant__ Grads p) {
     let_next_start();
     wait_before();
@@ -284,16 +284,16 @@ __global__ void __launch_bounds__(256) grads_sum_kernel(const __grid_constant__ 
         const int a = i / groups, r0 = (i - a * groups) * 4, n = min(4, p.R - r0);
         const float* part = p.part + a * per + (long long)r0 * W + k;
         float v[4] = {};
-        for (int s0 = 0; s0 < p.split; s0 += 8) {    // 32 loads at once
-            float t[8][4];
+        for (int s0 = 0; s0 < p.split; s0 += 4) {    // 16 loads at once
+            float t[4][4];
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
+            for (int s = 0; s < 4; ++s)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     t[s][j] = j < n && s0 + s < p.split
                         ? part[(s0 + s) * all + (long long)j * W] : 0.f;
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
+            for (int s = 0; s < 4; ++s)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] += t[s][j];
         }
@@ -319,7 +319,7 @@ template <bool BF16>
 int grads16(const Grads& p, dim3 grid, Chain& st) {
 #define ATOM_GRADS(N)                                                                             \
     if (p.R <= 16 * N) {                                                                          \
-        constexpr int smem = 4 * (32 * 272 + 32 * (32 * N + 16));                                 \
+        constexpr int smem = kStages * (32 * 272 + 32 * (32 * N + 16));                           \
         if (smem > 48 * 1024)                                                                     \
             cudaFuncSetAttribute(grads16_kernel<BF16, N>,                                         \
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem);              \
