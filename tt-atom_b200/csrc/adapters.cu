@@ -423,6 +423,7 @@ struct Ad {
     const int *req_ptr, *req_adapter;
     const float* scale;
     const void *w, *a, *b;
+    Sums sums{};
 
     Pieces pieces(const void* other, long long other_n) const {
         return {req_ptr, req_adapter, z.nreq, z.nad, (int)z.M, z.tiles, z.pieces, sp.piece,
@@ -483,7 +484,7 @@ struct Ad {
         // as many items as pairs of SMs, but no more than a tile may have groups
         const int groups = std::min(16, (z.nreq * p.ext + 7) / 8);
         const int share = std::max(1, std::min(groups, 74 / z.tiles));
-        if (int s = launch(kLow, {128, share, 0}, z.split, maps, p, st)) return s;
+        if (int s = launch(kLow, {128, share, 0}, z.split, maps, p, st, sums)) return s;
         if (!z.split || !blocks || planes) return ATOM_OK;
         return st.launch("adapters: blocks", blocks32_kernel, dim3(z.pieces), 256, 0, p,
                          (const float*)p.low_rows, z.Rs, sp.block, p.low_plane, sp.ext_rinv);
@@ -583,7 +584,8 @@ struct Ad {
         p.ext_a = 2 * k, p.ext_b = 3 * k, p.ext_bmn = bwd ? 1 : 0;
         p.ext_rinv = sp.ext_rinv;
         p.ext_bmax = sp.max + 1;
-        return launch(z.on ? kStoreLow : kStore, c, z.split, maps, p, st);
+        if (int s = launch(z.on ? kStoreLow : kStore, c, z.split, maps, p, st, sums)) return s;
+        return add_up(sums, st);
     }
 
     // S alone, in the backward pass: x's and a's own copies, the pieces as they are

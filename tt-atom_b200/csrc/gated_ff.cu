@@ -56,7 +56,7 @@ struct FfSizes {
 // always become two planes.
 struct FfSpace {
     __half *x, *wg, *wu, *wd, *dy, *xt, *dyt, *hp, *dgup;
-    float *xr, *wgr, *wur, *wdr, *dyr, *hr, *dgur, *H32, *dh, *part;
+    float *xr, *wgr, *wur, *wdr, *dyr, *hr, *dgur, *H32, *dh, *part, *part_gu, *part_d;
     __half *H, *dgu;
     float *few_dh, *few_dx, *few_grads;
     unsigned *max, *maxima[4];  // of wg | wu, of wd, x'' factor, dy'' factor; and the blocks' own
@@ -82,13 +82,13 @@ struct FfSpace {
         wg = c.take<__half>(k * z.F * z.Dp);
         wu = c.take<__half>(k * z.F * z.Dp);
         wd = c.take<__half>(k * z.O * z.Fp);
-        size_t pf = z.down.part;
         if (bwd) {
-            pf = std::max({z.dx.part, z.dwgu.part, z.dwd.part});
             dy = c.take<__half>(k * M * z.Op);
             dh = c.take<float>(M32 * z.Fp);
         }
-        part = c.take<float>(pf);
+        part = c.take<float>(bwd ? z.dx.part : z.down.part);
+        part_gu = c.take<float>(z.dwgu.part);
+        part_d = c.take<float>(z.dwd.part);
         if (!z.split) {
             H = c.take<__half>(M * z.Fp);
             if (bwd) dgu = c.take<__half>(2 * M * z.Fp);
@@ -137,6 +137,7 @@ struct Ff {
     Operand x, wg, wu, wd, dy;
     PrepList list;
     int parts[4] = {};          // blocks' maxima so far
+    Sums sums{};
 
     // an operand of this call: as it lies, or through the list's packing / planes; kTensorSplit:
     // by maximum `m` of parts[m] blocks
@@ -265,7 +266,7 @@ struct Ff {
         else if (z.split) p.bmax = sp.max;
         p.used = z.split ? 0x3f : 0x7;
         if (int s = gate_output(maps, p, C, width, H)) return s;
-        return launch(epilogue, c, z.split, maps, p, st);
+        return launch(epilogue, c, z.split, maps, p, st, sums);
     }
     int forward(void* y, long long ldy, float* kept) {
         Args p = args(z.M, z.F);
@@ -284,7 +285,8 @@ struct Ff {
         q.rinv = sp.hr;
         q.cinv[0] = sp.wdr;
         output(q, y, ldy);
-        return launch(kStore, c, z.split, maps, q, st);
+        if (int s = launch(kStore, c, z.split, maps, q, st, sums)) return s;
+        return add_up(sums, st);
     }
     int backward(const float* kept, void* dx, long long lddx, void* dwg, void* dwu, void* dwd) {
         const int k = step();
@@ -304,10 +306,10 @@ struct Ff {
             if (kept) {
                 p.gu = const_cast<float*>(kept);
                 if (int s = gate_output(maps, p, dgu, 2 * z.Fp, H)) return s;
-                if (int s = launch(kGateBwdDH, c, z.split, maps, p, st)) return s;
+                if (int s = launch(kGateBwdDH, c, z.split, maps, p, st, sums)) return s;
             } else {
                 p.blocked = sp.dh;
-                if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
+                if (int s = launch(kStore, c, z.split, maps, p, st, sums)) return s;
                 Args q = args(z.M, z.F);
                 q.dh = sp.dh;
                 if (int s = gates(kGateBwdGU, q, dgu, 2 * z.Fp, H)) return s;
@@ -331,7 +333,7 @@ struct Ff {
             p.rinv = sp.dgur;
             if (z.split) p.bmax = sp.max;
             output(p, dx, lddx);
-            if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
+            if (int s = launch(kStore, c, z.split, maps, p, st, sums)) return s;
         }
         if (dwg || dwu) {
             Choice c = z.dwgu;
@@ -344,10 +346,11 @@ struct Ff {
             Args p = args(z.F, z.D);
             p.groups = two ? 2 : 1;
             p.ph[0] = {0, 2 * k, 2 * k, z.nk(z.M), 1, 1, c.bn, c.bn / 2};
+            p.part = sp.part_gu;
             p.factor = reinterpret_cast<const float*>(sp.max + 2);
             output(p, dwg ? dwg : dwu, z.D);
             p.C[1] = dwu;
-            if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
+            if (int s = launch(kStore, c, z.split, maps, p, st, sums)) return s;
         }
         if (dwd) {
             const Choice c = z.dwd;
@@ -356,11 +359,12 @@ struct Ff {
             if (int s = put(maps, k, h, true, 64, z.split)) return s;
             Args p = args(z.O, z.F);
             p.ph[0] = {0, k, k, z.nk(z.M), 1, 1, c.bn, c.bn / 2};
+            p.part = sp.part_d;
             p.factor = reinterpret_cast<const float*>(sp.max + 3);
             output(p, dwd, z.F);
-            if (int s = launch(kStore, c, z.split, maps, p, st)) return s;
+            if (int s = launch(kStore, c, z.split, maps, p, st, sums)) return s;
         }
-        return ATOM_OK;
+        return add_up(sums, st);
     }
 };
 

@@ -1199,10 +1199,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
 
 // C[g][m, n] = sum over the splits, in order. Split products are small (fewer tiles than pairs of
 // SMs), so 32-bit indexes do.
-__global__ void __launch_bounds__(256) reduce_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(256) reduce_kernel(const __grid_constant__ Sums sums) {
     let_next_start();
     wait_before();
-    const uint32_t M = (uint32_t)p.M, N = p.N, all = M * N * p.groups;
+    const Sums::Item& p = sums.it[blockIdx.y];
+    const uint32_t N = p.N, all = p.M * N * p.groups;
     const uint32_t step = N % 4 ? 1 : 4;
     for (uint32_t i = (blockIdx.x * 256u + threadIdx.x) * step; i < all; i += gridDim.x * 256u * step) {
         float v[4] = {};
@@ -1216,10 +1217,22 @@ __global__ void __launch_bounds__(256) reduce_kernel(const __grid_constant__ Arg
 #pragma unroll 4
             for (int s = 0; s < p.ksplit; ++s) v[0] += p.part[(long long)s * all + i];
         }
-        const uint32_t row = i / N, n = i - row * N, g = row >= M;
-        const long long at = (row - g * M) * p.ldc + n;
-        for (uint32_t j = 0; j < step; ++j) store_f(p.C[g], at + j, v[j], p.dtype);
+        const uint32_t row = i / N, n = i - row * N, g = row >= p.M;
+        const long long at = (row - g * p.M) * p.ldc + n;
+        for (uint32_t j = 0; j < step; ++j) store_f(p.C[g], at + j, v[j], sums.dtype);
     }
+}
+int add_up(Sums& sums, Chain& st) {
+    long long blocks = 0;
+    for (int i = 0; i < sums.n; ++i) {
+        const Sums::Item& p = sums.it[i];
+        blocks = std::max(blocks, ((long long)p.M * p.N * p.groups / (p.N % 4 ? 1 : 4) + 255) / 256);
+    }
+    if (sums.n == 0) return ATOM_OK;
+    const int s = st.launch("pair product sums", reduce_kernel,
+                            dim3((unsigned)std::min(blocks, 1184LL), sums.n), 256, 0, sums);
+    sums.n = 0;
+    return s;
 }
 
 // Operand preparation. A warp has eight float4 a lane: one row of up to 1024 columns, or two, four
@@ -1707,7 +1720,7 @@ Choice choose(long long M, int N, int nk, int groups, bool gated, bool split, bo
 }
 
 template <int BN, int EPI, bool SPLIT, int OUT>
-static int run(const Maps& maps, const Args& p, Chain& st) {
+static int run(const Maps& maps, const Args& p, Chain& st, Sums& sums) {
     using CF = Cfg<BN, EPI, SPLIT>;
     static std::atomic<bool> set[64];
     int dev = 0;
@@ -1729,14 +1742,14 @@ static int run(const Maps& maps, const Args& p, Chain& st) {
                           CF::kSmem, maps, p))
         return s;
     if (EPI != kLow && p.ksplit > 1) {
-        const long long blocks = (p.M * p.N * p.groups / (p.N % 4 ? 1 : 4) + 255) / 256;
-        return st.launch("pair product sums", reduce_kernel,
-                         dim3((unsigned)std::min(std::max(blocks, 1LL), 1184LL)), 256, 0, p);
+        sums.dtype = p.dtype;
+        sums.it[sums.n++] = {p.part, (uint32_t)p.M, (uint32_t)p.N, (uint32_t)p.groups, p.ksplit,
+                             {p.C[0], p.C[1]}, p.ldc};
     }
     return ATOM_OK;
 }
 
-int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain& st) {
+int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain& st, Sums& sums) {
     const bool gated = epilogue == kGate || epilogue == kGateBwdGU;
     const int w = gated ? c.bn / 2 : c.bn;
     p.mtiles = ceil_div(p.M, 256);
@@ -1754,8 +1767,8 @@ int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain
     }
     if (p.tiles == 0) return ATOM_OK;
     if (epilogue == kLow)
-        return split ? run<128, kLow, true, kOut>(maps, p, st)
-                     : run<128, kLow, false, kOut>(maps, p, st);
+        return split ? run<128, kLow, true, kOut>(maps, p, st, sums)
+                     : run<128, kLow, false, kOut>(maps, p, st, sums);
     if ((epilogue == kStore || epilogue == kStoreLow) && !p.blocked) {
         // TMA stores clip at 16 bytes, so columns have to end there too
         const int e = p.ksplit > 1 ? 4 : dtype_size(p.dtype);
@@ -1780,9 +1793,9 @@ int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain
                      : p.ksplit > 1                  ? kPart : kOut;
 #define ATOM_PAIR(E, O)                                            \
     if (epilogue == E && form == O) {                              \
-        if (split) return run<128, E, true, O>(maps, p, st);       \
-        return c.bn == 256 ? run<256, E, false, O>(maps, p, st)    \
-                           : run<128, E, false, O>(maps, p, st);   \
+        if (split) return run<128, E, true, O>(maps, p, st, sums);       \
+        return c.bn == 256 ? run<256, E, false, O>(maps, p, st, sums)    \
+                           : run<128, E, false, O>(maps, p, st, sums);   \
     }
     ATOM_PAIR(kStore, kOut)
     ATOM_PAIR(kStore, kRows)

@@ -127,8 +127,22 @@ int make_low_map(CUtensorMap* m, const void* p, long long cols, long long rows, 
 int make_out_map(CUtensorMap* m, const void* p, int dtype, long long cols, long long rows,
                  long long ld);
 
-// Launches the product: tiles, C's maps (kStore) etc. are filled in from M, N, C and the choice.
-int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain& st);
+// The outputs of products whose K was split, to be added up in one launch.
+struct Sums {
+    struct Item {
+        const float* part;
+        uint32_t M, N, groups;
+        int ksplit;
+        void* C[2];
+        long long ldc;
+    } it[3];
+    int n = 0, dtype = 0;
+};
+int add_up(Sums& sums, Chain& st);
+
+// Launches the product: tiles, C's maps (kStore) etc. are filled in from M, N, C and the choice. The
+// sums of a split K go into the list.
+int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain& st, Sums& sums);
 
 // Operand preparation, up to 6 matrices a launch.
 // kPack: 16-bit copy. kRowSplit: planes scaled row by row. kRowScale: the scales alone. kMax: the
