@@ -505,7 +505,8 @@ int atom_orb_zbl(const float* ev, const int* Z, const int* src, const int* tgt, 
  * and adapter gradients are zeroed. Results do not change from call to call (no atomics in any
  * sum). A wait that expires leaves ATOM_PAIR_WAIT_CODE for atom_device_error. fp16 values past
  * 65504 become infinities, as everywhere in that type: the gated row is such a value.
- * Up to 16 rows nothing is kept and `kept` is not read.
+ * Up to 16 rows nothing is kept and `kept` is not read. Outputs overlap neither inputs nor each
+ * other.
  * ---------------------------------------------------------------------------------------- */
 
 /* Sizes in bytes, to bytes_host[3]: the workspace of atom_gated_ff_fwd, that of

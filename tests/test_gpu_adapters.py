@@ -268,3 +268,22 @@ def test_rows_do_not_depend_on_how_requests_cut_them(R, t):
 def test_few_rows_both_ways(M, R, D, O, t):  # noqa: E741
     lengths = [M // 3, 0, M - M // 3]
     both(make(lengths, [1, 0, 2 if M > 1 else -1], 4, R, D, O, t, seed=80 + M))
+
+
+def test_offsets_past_32_bits():
+    # 2.2e9 outputs: the last rows and their adapter against the definition of those rows alone
+    M, D, O, R, last = 1_050_000, 64, 2104, 16, 300  # noqa: E741
+    t, g = torch.bfloat16, torch.Generator(device="cuda").manual_seed(5)
+
+    def r(*shape, s=1.0):
+        return (torch.randn(*shape, generator=g, device="cuda") * s).to(t)
+    x, w, a, b = r(M, D), r(O, D, s=D ** -0.5), r(2, R, D, s=D ** -0.5), r(2, O, R, s=R ** -0.5)
+    scale = torch.tensor([0.5, 1.5], device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    ptr, ids = torch.tensor([0, 500, M - last, M], **i32), torch.tensor([0, -1, 1], **i32)
+    dy = r(M, O)
+    want = reference(x[-last:], w, a, b, scale, torch.tensor([0, last], **i32), ids[2:], dy[-last:])
+    check([adapted_linear(x, w, a, b, scale, ptr, ids)[-last:]], want, ["y"])
+    dx, da, db = adapted_linear_bwd(x, w, a, b, scale, ptr, ids, dy)
+    want = {"dx": want["dx"], **{k: tuple(v[1] for v in want[k]) for k in ("da", "db")}}
+    check([dx[-last:], da[1], db[1]], want, ("dx", "da", "db"))

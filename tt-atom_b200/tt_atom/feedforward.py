@@ -5,6 +5,7 @@ case of, for any widths, in fp32, bf16 and fp16, with the gradients of its weigh
 program needs to train or fine-tune a block and to run it in 16 bits. No counterpart in the
 reference, whose feed-forwards are ungated MLPs (tt_atom/grid.py) or the spectral block
 (tt_atom/spectral.py). The kernels are behind ``atom_gated_ff_fwd`` / ``atom_gated_ff_bwd``.
+As everywhere in this package gradients are functions of their own: autograd does not see them.
 """
 from __future__ import annotations
 
