@@ -31,16 +31,13 @@ __global__ void __launch_bounds__(256) blocks32_kernel(const __grid_constant__ A
                                                        long long plane, float* rinv) {
     let_next_start();
     wait_before();
-    if (p.lead[blockIdx.x] < 0) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = p.piece[blockIdx.x].y / 256;
-    const int m0 = t * 256, request = blockIdx.x - t, first = p.tile_req[t].x;
-    int before = 0;                              // blocks that the tile has before this one
-    for (int i = t + first; i < (int)blockIdx.x; i += 32)
-        before += __popc(__ballot_sync(0xffffffffu, i + lane < (int)blockIdx.x &&
-                                                        p.lead[i + lane] >= 0));
-    const int slice = before * p.ext + lane / 4;
+    const int4 req = p.tile_req[t];
+    const int m0 = t * 256, j = blockIdx.x - t - req.x;      // the tile's j-th block
+    if (j < 0 || j >= req.z) return;
+    const int request = p.lead[blockIdx.x].y, slice = j * p.ext + lane / 4;
     if (4 * lane >= 16 * p.ext) return;
-    __half* q0 = block + ((first_stage(t, first, p.ext) + (slice >> 2)) * 256) * 64 +
+    __half* q0 = block + ((first_stage(t, req.x, p.ext) + (slice >> 2)) * 256) * 64 +
                  (slice & 3) * 16 + (lane & 3) * 4;
     const unsigned lanes = p.ext == 8 ? 0xffffffffu : (1u << 4 * p.ext) - 1;
 #pragma unroll 4
@@ -363,7 +360,8 @@ struct AdSpace {
     float *rinv, *xinv, *wr, *ext_rinv, *part, *gpart, *few_S, *few_T, *few_dx;
     void *S, *T;
     int4 *piece, *bad, *tile_req;
-    int *lead, *row_lead, *usable, *few_slot;
+    int2* lead;
+    int *row_lead, *usable, *few_slot;
     unsigned *max, *maxima[3];       // of w, of the adapters beside it, of those of the low-rank
                                      // rows; and the blocks' own
     size_t bytes;
@@ -395,7 +393,7 @@ struct AdSpace {
             bad = c.take<int4>(z.nad);
             tile_req = c.take<int4>(z.tiles);
             usable = c.take<int>(z.pieces);
-            lead = c.take<int>(z.pieces);
+            lead = c.take<int2>(z.pieces);
             row_lead = c.take<int>(z.M);
             first = c.take<__half>(k * (bwd ? b_n : a_n));
             ext = c.take<__half>(k * (bwd ? a_n : b_n));

@@ -250,19 +250,19 @@ struct Share {
     }
 };
 // Walks the low-rank blocks of a row tile in slices of 16 ranks, p.ext of them each, four to a
-// stage. The adapters of the first 32 requests, one a lane, are asked for when the walk is made and
-// needed when it begins.
+// stage. The adapters of 32 blocks, one a lane, are asked for when the walk is made and needed when
+// it begins.
 struct Blocks {
     const Args& p;
-    int mt, base, behind, mine, left_in = -1, sub = 0, slot = 0;
-    unsigned left = 0;
+    const int* usable;
+    int n, j = -1, mine, sub = 0, slot = 0;
     __device__ __forceinline__ Blocks(const Args& q, int tile, const int4& t)
-        : p(q), mt(tile), base(t.x), behind(t.z ? t.y : t.x) {
-        ask();
+        : p(q), usable(q.usable + tile + t.x), n(t.z) {
+        ask(0);
     }
-    __device__ __forceinline__ void ask() {
-        const int i = base + (threadIdx.x & 31);
-        mine = i < behind ? p.usable[mt + i] : -1;
+    __device__ __forceinline__ void ask(int k) {
+        k += threadIdx.x & 31;
+        mine = k < n ? usable[k] : 0;
     }
     // the next slice (at(), slot); false when there is none
     __device__ __forceinline__ bool next() {
@@ -270,82 +270,43 @@ struct Blocks {
             ++sub;
             return true;
         }
-        if (left_in != base) left = __ballot_sync(0xffffffffu, mine >= 0), left_in = base;
-        while (left == 0) {
-            if (base + 32 >= behind) return false;
-            base += 32;
-            ask();
-            left = __ballot_sync(0xffffffffu, mine >= 0);
-            left_in = base;
-        }
-        const int i = __ffs(left) - 1;
-        left &= left - 1;
-        slot = __shfl_sync(0xffffffffu, mine, i);
+        if (++j >= n) return false;
+        if (j && (j & 31) == 0) ask(j);
+        slot = __shfl_sync(0xffffffffu, mine, j & 31);
         sub = 1;
         return true;
     }
     __device__ __forceinline__ int at() const { return (sub - 1) * 16; }     // first rank
 };
 
-// A row tile's blocks, 32 requests at a time, one a lane. Whole warps.
-struct Window {
-    const Args& p;
-    int mt, first, behind, base = 0;
-    int a = -1;              // this lane's adapter where its request leads a block
-    unsigned mask = 0;       // the lanes that have one
-    __device__ __forceinline__ Window(const Args& q, int tile) : p(q), mt(tile) {
-        const int4 t = p.tile_req[mt];
-        first = t.x;
-        behind = t.y;
-        look(first);
+// Writes down which adapters the product beside the projection takes for a row tile's blocks.
+// Adapter nad, past the tensor map's end, reads as zeros: what is not finite leaves the other rows
+// as they are. A whole warp.
+__device__ __forceinline__ void settle(const Args& p, int mt) {
+    const int4 t = p.tile_req[mt];
+    bool spoilt = false;
+    for (int j = threadIdx.x & 31; j < t.z; j += 32) {
+        const int a = p.lead[mt + t.x + j].x;
+        const bool ok = is_finite(p, a);
+        p.usable[mt + t.x + j] = ok ? a : p.nad;
+        spoilt |= !ok;
     }
-    __device__ __forceinline__ void look(int r) {
-        base = r;
-        const int i = r + (threadIdx.x & 31);
-        a = i < behind ? p.lead[mt + i] : -1;
-        mask = __ballot_sync(0xffffffffu, a >= 0);
-    }
-    __device__ __forceinline__ int count() {         // of all requests; ends on the first again
-        int n = __popc(mask);
-        if (behind - first > 32) {
-            for (int r = first + 32; r < behind; r += 32) {
-                look(r);
-                n += __popc(mask);
-            }
-            look(first);
-        }
-        return n;
-    }
-    // Writes down which adapters the product beside the projection takes. Adapter nad, past the
-    // tensor map's end, reads as zeros: what is not finite leaves the other rows as they are.
-    __device__ __forceinline__ void settle() {
-        int n = 0, spoilt = 0;
-        for (int r = first; r < behind; r += 32) {
-            look(r);
-            const bool ok = a < 0 || is_finite(p, a);
-            n += __popc(mask);
-            spoilt |= __any_sync(0xffffffffu, !ok);
-            const int i = r + (threadIdx.x & 31);
-            if (i < behind) p.usable[mt + i] = ok ? a : p.nad;
-        }
-        if ((threadIdx.x & 31) == 0) {
-            p.tile_req[mt].z = n;
-            p.tile_req[mt].w = spoilt;
-        }
-        look(first);
-    }
-};
+    spoilt = __any_sync(0xffffffffu, spoilt);
+    if ((threadIdx.x & 31) == 0) p.tile_req[mt].w = spoilt;
+}
 
-// kLow: groups of a row tile's pieces whose slices of 16 ranks fill 128 columns (a piece's slices
+// kLow: groups of a row tile's blocks whose slices of 16 ranks fill 128 columns (a block's slices
 // stay together); with few row tiles, `ksplit` work items share a tile's groups.
 struct Low {
-    Window w;
-    int count, slices, half, each, before = 0;   // pieces; slices a piece; pieces a half, a group
-    __device__ __forceinline__ Low(const Args& p, int tile) : w(p, tile) {
+    const Args& p;
+    int mt, first, count, slices, half, each;    // blocks; slices a block; blocks a half, a group
+    __device__ __forceinline__ Low(const Args& q, int tile) : p(q), mt(tile) {
+        const int4 t = p.tile_req[mt];
+        first = t.x;
+        count = t.z;
         slices = p.ext;
         half = slices <= 4 ? 4 / slices : 0;
         each = slices <= 4 ? 2 * half : 1;
-        count = w.count();
     }
     __device__ __forceinline__ int groups() const { return (count + each - 1) / each; }
     // slices of group g in half h (64 columns; slice i of a group is i % 4 of half i / 4)
@@ -353,25 +314,14 @@ struct Low {
         if (slices > 4) return h ? slices - 4 : 4;
         return max(0, min(half, count - g * each - h * half)) * slices;
     }
-    __device__ __forceinline__ int sub(int i) const {           // which of its piece's slices i is
+    __device__ __forceinline__ int sub(int i) const {           // which of its block's slices i is
         return slices > 4 ? i : (i & 3) % slices;
     }
     // the block of slice i of group g: which one of the tile's, its adapter, the request that leads it
-    __device__ __forceinline__ int3 piece(int g, int i) {
-        const int block = g * each + (slices > 4 ? 0 : (i >> 2) * half + (i & 3) / slices);
-        int j = block;
-        if (j < before) {
-            before = 0;
-            w.look(w.first);
-        }
-        while (j >= before + __popc(w.mask)) {
-            before += __popc(w.mask);
-            w.look(w.base + 32);
-        }
-        unsigned v = w.mask;
-        for (j -= before; j > 0; --j) v &= v - 1;
-        const int l = __ffs(v) - 1;
-        return make_int3(block, __shfl_sync(0xffffffffu, w.a, l), w.base + l);
+    __device__ __forceinline__ int3 block(int g, int i) const {
+        const int j = g * each + (slices > 4 ? 0 : (i >> 2) * half + (i & 3) / slices);
+        const int2 l = p.lead[mt + first + j];
+        return make_int3(j, l.x, l.y);
     }
 };
 
@@ -630,12 +580,12 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
 // fp32 blocks are planes, scaled row by row: a block's slices are all in one warp then (ranks of 64
 // at most; larger ones have a kernel of their own, from the rows).
 template <bool SPLIT>
-__device__ __forceinline__ void low_store(const Args& p, Low& low, int g, int part,
+__device__ __forceinline__ void low_store(const Args& p, const Low& low, int g, int part,
                                           long long m0, int lane, int lead, float (*v)[32],
                                           float f) {
     const int used = low.used(g, part);
     const long long m = m0 + lane;
-    const long long stage0 = first_stage(low.w.mt, low.w.first, p.ext);
+    const long long stage0 = first_stage(low.mt, low.first, p.ext);
     // a slice's 16 values of this row, in 16-bit elements
     auto place = [&](int slice) {
         return ((stage0 + (slice >> 2)) * 256 + (m & 255)) * 64 + (slice & 3) * 16;
@@ -644,14 +594,14 @@ __device__ __forceinline__ void low_store(const Args& p, Low& low, int g, int pa
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (i >= used) break;
-        const int3 piece = low.piece(g, part * 4 + i);
+        const int3 block = low.block(g, part * 4 + i);
         const int sub = low.sub(part * 4 + i), c0 = sub * 16;
-        const bool in = piece.z == lead;
-        const float s = p.low_scale[piece.y] * f;
+        const bool in = block.z == lead;
+        const float s = p.low_scale[block.y] * f;
         float* x = v[i >> 1] + (i & 1) * 16;
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = in ? x[j] * s : 0.f;
-        const long long at = place(piece.x * p.ext + sub);
+        const long long at = place(block.x * p.ext + sub);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                // eight ranks at a time: Rs is a multiple of 8
             const int c = c0 + 8 * h;
@@ -680,7 +630,7 @@ __device__ __forceinline__ void low_store(const Args& p, Low& low, int g, int pa
         for (int k = 0; k < 4; ++k) {
             if (k > i || k < i - sub) continue;
             const float* y = v[k >> 1] + (k & 1) * 16;
-            __half* q = static_cast<__half*>(p.low_block) + place(piece.x * p.ext + k - i + sub);
+            __half* q = static_cast<__half*>(p.low_block) + place(block.x * p.ext + k - i + sub);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 __half2 hi[4], lo[4];
@@ -783,7 +733,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                         int slot[4], r16[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            slot[i] = i < mine ? low.piece(g, 4 * rank + i).y : 0;
+                            slot[i] = i < mine ? low.block(g, 4 * rank + i).y : 0;
                             r16[i] = low.sub(4 * rank + i) * 16;
                         }
                         for (int kt = 0; kt < p.ph[0].nk; ++kt) {
@@ -1028,7 +978,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
             if (EPI == kStoreLow) req = ahead.get(p, mine_k, first, pairs);
             const bool spoilt = EPI == kStoreLow && req.w && spoilt_row(p, ti.mt, m + lane, lane);
             if (EPI == kLow && warp == 2 && rank == 0 && ti.ks == 0 && p.usable)
-                Window(p, ti.mt).settle();
+                settle(p, ti.mt);
             if constexpr (EPI == kLow && !SPLIT) {
                 const int lead = m + lane < p.M ? p.row_lead[m + lane] : -1;
                 Low low_(p, ti.mt);
@@ -1445,6 +1395,7 @@ __device__ __forceinline__ void prep_pack(const PrepItem& it, int blocks) {
 
 // Finds pieces: a piece a warp, a row tile a warp, then four blocks an adapter.
 __device__ __forceinline__ void find_pieces(const Pieces& p) {
+    __shared__ unsigned seen[8][1 << 14 >> 5];       // adapters, of a warp's tile
     const int lane = threadIdx.x & 31, w = blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lookups = (p.pieces + p.tiles + 7) / 8;
     // rows are kept within 0 .. M whatever the table holds
@@ -1476,10 +1427,7 @@ __device__ __forceinline__ void find_pieces(const Pieces& p) {
                 }
                 lead = __reduce_min_sync(0xffffffffu, got);
             }
-            if (lane == 0) {
-                p.piece[w] = c;
-                p.lead[w] = lead == r ? c.x : -1;
-            }
+            if (lane == 0) p.piece[w] = c;
             for (int m = c.y + lane; m < c.z; m += 32) p.row_lead[m] = c.x < 0 ? -1 : lead;
         } else if (w < p.pieces + p.tiles) {
             const int t = w - p.pieces;
@@ -1488,8 +1436,33 @@ __device__ __forceinline__ void find_pieces(const Pieces& p) {
             const int head = begins(0), tail = begins(p.n);
             for (int m = t * 256 + lane; m < min(p.M, t * 256 + 256); m += 32)
                 if (m < head || m >= tail) p.row_lead[m] = -1;
-            // a request that begins before the tile reaches into it at most as the last such one
-            if (lane == 0) p.tile_req[t] = make_int4(::max(first, 0), last + 1, 0, 0);
+            // The tile's blocks in order: of each 256 numbers, the first requests with an adapter. (A
+            // request that begins before the tile reaches into it at most as the last such one.)
+            unsigned* bits = seen[threadIdx.x >> 5];
+            int n = 0;
+            for (int r0 = ::max(first, 0) & ~31; r0 <= last; r0 += 32) {
+                const int r = r0 + lane;
+                if (r0 <= ::max(first, 0) || (r0 & 255) == 0) {
+                    __syncwarp();
+                    for (int i = lane; i < (p.nad + 31) / 32; i += 32) bits[i] = 0;
+                    __syncwarp();
+                }
+                int a = -1;
+                if (r >= first && r >= 0 && r <= last && p.adapter[r] < p.nad &&
+                    ::max(begins(r), t * 256) < min(begins(r + 1), t * 256 + 256))
+                    a = p.adapter[r];
+                const unsigned same = __match_any_sync(0xffffffffu, a);
+                const bool leads = a >= 0 && __ffs(same) - 1 == lane && !(bits[a >> 5] >> (a & 31) & 1);
+                const unsigned all = __ballot_sync(0xffffffffu, leads);
+                if (leads) {
+                    atomicOr(&bits[a >> 5], 1u << (a & 31));
+                    p.lead[t + ::max(first, 0) + n + __popc(all & ((1u << lane) - 1))] =
+                        make_int2(a, r);
+                }
+                n += __popc(all);
+                __syncwarp();
+            }
+            if (lane == 0) p.tile_req[t] = make_int4(::max(first, 0), last + 1, n, 0);
         }
         return;
     }
@@ -1526,19 +1499,20 @@ __device__ __forceinline__ void find_pieces(const Pieces& p) {
     if (threadIdx.x == 0) reinterpret_cast<int*>(p.bad + a)[part] = found;
 }
 
-// KIND 0: 16-bit copies; 1: planes; 2: planes with kWeighted items. Small operands are prepared in the
+// KIND 0: 16-bit copies; 1: planes; 2: planes with kWeighted items. FINDS: and an adapters call's pieces. Small operands are prepared in the
 // time of a launch and of their code's first fetch: all in one kernel costs 1,002 x 256 x 1,024 in
 // fp32 2 us of 26, 4,000 x 256 adapters forward and backward 4 of 101.
-template <int KIND>
+template <int KIND, bool FINDS>
 __global__ void __launch_bounds__(256, 3)
     prep_kernel(const __grid_constant__ PrepList l, const __grid_constant__ Pieces pieces) {
     __shared__ float part[8];
     let_next_start();
     wait_before();
-    if (blockIdx.y == l.n) {
-        find_pieces(pieces);
-        return;
-    }
+    if constexpr (FINDS)
+        if (blockIdx.y == l.n) {
+            find_pieces(pieces);
+            return;
+        }
     const PrepItem& it = l.it[blockIdx.y];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (blockIdx.x >= l.blocks[blockIdx.y]) return;
@@ -1610,7 +1584,9 @@ int prepare(PrepList& l, Chain& st, const Pieces* pieces) {
         split |= l.it[i].mode != kPack;
     }
     const int s = st.launch("operand preparation",
-                            weighted ? prep_kernel<2> : split ? prep_kernel<1> : prep_kernel<0>,
+                            weighted ? prep_kernel<2, false>
+                            : split  ? pieces ? prep_kernel<1, true> : prep_kernel<1, false>
+                                     : pieces ? prep_kernel<0, true> : prep_kernel<0, false>,
                             dim3(grid, l.n + (pieces != nullptr)), 256, 0, l,
                             pieces ? *pieces : none);
     l.n = 0;

@@ -87,10 +87,11 @@ struct Args {
     int ext;                 // slices a block, 0: none
     int nad;                 // adapters
     int ext_a, ext_b, ext_bmn;
-    int4* tile_req;          // of a row tile: its requests' first and behind; and, from kLow on,
-                             // how many blocks count and whether one's adapter is not finite
+    int4* tile_req;          // of a row tile: its requests' first and behind, its blocks; and, from
+                             // kLow on, whether one's adapter is not finite
     const int4* piece;       // t + r, of request r in tile t: adapter or -1 (none), its rows
-    const int* lead;         // ... and the adapter again where request r leads a block, else -1
+    const int2* lead;        // t + first + j, of tile t's j-th block: its adapter, the request that
+                             // leads it
     const int* row_lead;     // per row: the request whose block it is in, -1: none
     int* usable;             // from kLow on: as lead, but nad where the adapter is not finite
     const int4* bad;         // of an adapter: not all zero = not finite, its rows become NaN
@@ -183,8 +184,9 @@ struct Pieces {
     int n, nad, M;           // requests, adapters, rows
     int tiles, pieces;       // row tiles; and requests
     int4* piece;             // adapter or -1, first row, behind the last row
-    int *lead, *row_lead;    // as in Args
-    int4* tile_req;          // requests first .. behind that reach into a row tile
+    int2* lead;              // as in Args, like the next two
+    int* row_lead;
+    int4* tile_req;
     const void* other;       // the matrix of each adapter beside the projection: `other_n` values
     long long other_n;
     int4* bad;               // per adapter: a quarter of them is not finite
