@@ -1499,9 +1499,11 @@ __device__ __forceinline__ void find_pieces(const Pieces& p) {
     if (threadIdx.x == 0) reinterpret_cast<int*>(p.bad + a)[part] = found;
 }
 
-// KIND 0: 16-bit copies; 1: planes; 2: planes with kWeighted items. FINDS: and an adapters call's pieces. Small operands are prepared in the
-// time of a launch and of their code's first fetch: all in one kernel costs 1,002 x 256 x 1,024 in
-// fp32 2 us of 26, 4,000 x 256 adapters forward and backward 4 of 101.
+// KIND 0: 16-bit copies; 1: planes; 2: planes with kWeighted items. FINDS: and an adapters call's
+// pieces. Small operands are prepared in the time of a launch and of their code's first fetch: with
+// all of it in one kernel, 1,002 x 256 x 1,024 in fp32 took 26.2 us and 4,000 rows of adapters forward
+// and backward 101, with KIND alone 24.4 and 97, so 21.8 and 91 (with instances for wide rows and for
+// items that look for maxima as well, 21.6 and 90, but 12,011 rows of adapters 78.1 for 76.5).
 template <int KIND, bool FINDS>
 __global__ void __launch_bounds__(256, 3)
     prep_kernel(const __grid_constant__ PrepList l, const __grid_constant__ Pieces pieces) {
