@@ -19,7 +19,7 @@
 // of itself (2-norm) at any K; one accumulator at K = 1024 is 3.5e-6 off, 16 additions 9.7e-7.
 //
 // Bound by the tensor core where K and the tiles are many: the whole training step of 8,192 x 2,048
-// x 8,192 in bf16 (2.47 PFLOP in 8 launches) runs at 1.34 PFLOP/s, 95 % of what a library product
+// x 8,192 in bf16 (2.47 PFLOP in 6 launches) runs at 1.34 PFLOP/s, 95 % of what a library product
 // sustains under the power cap; 60,000 x 256 -> 2 x 1,024 with the gate at 1.05, bound by its
 // epilogue; a SPLIT product does three, at 0.9 of 1.7 PFLOP/s together at 4,011 x 672 x 2,632.
 //
