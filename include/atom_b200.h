@@ -313,8 +313,9 @@ int atom_wait_selftest(int64_t budget_cycles, void* stream);
 #define ATOM_EDGE_WAIT_CODE 8
 int atom_ring_wait_selftest(int64_t budget_cycles, void* stream);
 
-/* The code of an expired wait inside the products of the typed operators (last section). */
+/* The same for the products of the typed operators (last section). */
 #define ATOM_PAIR_WAIT_CODE 9
+int atom_pair_wait_selftest(int64_t budget_cycles, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Edge-side fused ops of the edgewise block (tt_atom/edgewise.py:39-87, forces.py:352-418).

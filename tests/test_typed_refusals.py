@@ -117,3 +117,24 @@ def test_python_wrappers_refuse_on_the_gpu():
         with pytest.raises(ValueError):
             call()
     assert torch.cuda.current_device() == 0
+
+
+def test_pair_wait_selftest_rejects_bad_budget():
+    for budget in (0, 2_000_000_001):
+        with pytest.raises(L.AtomError):
+            L.call("atom_pair_wait_selftest", budget, None)
+
+
+@pytest.mark.gpu
+def test_expired_pair_wait_is_reported_and_cleared():
+    """A product's bounded wait gives up, records its code, and the context stays usable."""
+    st, code = L.stream_ptr(), ctypes.c_int(-1)
+    L.call("atom_device_error", ctypes.byref(code), st)
+    L.call("atom_pair_wait_selftest", 2_000_000, st)          # ~1 ms
+    L.call("atom_device_error", ctypes.byref(code), st)
+    assert code.value == 9
+    L.call("atom_device_error", ctypes.byref(code), st)
+    assert code.value == 0
+    x = torch.ones(40, 64, device="cuda", dtype=torch.bfloat16)
+    y = gated_ff(x, x, x, x.T.contiguous(), act="sigmoid")
+    assert torch.equal(y, torch.full_like(y, float(y[0, 0])))

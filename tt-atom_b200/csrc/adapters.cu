@@ -13,7 +13,7 @@
 // dA = T^T x, dB = dy^T S summed by pieces in their order.
 //
 // Zeros in a block keep other requests' rows as they are only where B is finite; an adapter that
-// is not is found when the pieces are, left out, and its own rows are set to NaN.
+// is not is found when the pieces are, read as zeros, and its own rows are set to NaN.
 #include <algorithm>
 
 #include "few_rows.cuh"

@@ -20,7 +20,7 @@
 //
 // Bound by the tensor core where K and the tiles are many: the whole training step of 8,192 x 2,048
 // x 8,192 in bf16 (2.47 PFLOP in 6 launches) runs at 1.34 PFLOP/s, 95 % of what a library product
-// sustains under the power cap; 60,000 x 256 -> 2 x 1,024 with the gate at 1.05, bound by its
+// sustains under the power cap; 60,000 x 256 -> 2 x 1,024 with the gate at 1.1, bound by its
 // epilogue; a SPLIT product does three, at 0.9 of 1.7 PFLOP/s together at 4,011 x 672 x 2,632.
 //
 // Warp 0 has TMA, warp 1 tensor memory and the products (CTA 0's issues for both), warps 2.. the
@@ -62,13 +62,14 @@ __device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
 }
 // Bounded wait; false once the budget is spent or any CTA has failed. The clock and the error
 // word (a trip to L2) are looked at every 256 tries only.
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, int* err) {
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, int* err,
+                                          long long budget = kWaitCycles) {
     if (mbar_try(b, parity)) return true;
     const long long t0 = clock64();
     for (uint32_t n = 1;; ++n) {
         if (mbar_try(b, parity)) return true;
         if ((n & 255) == 0) {
-            if (clock64() - t0 > kWaitCycles) {
+            if (clock64() - t0 > budget) {
                 atomicCAS(err, 0, ATOM_PAIR_WAIT_CODE);
                 return false;
             }
@@ -1792,5 +1793,22 @@ int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain
     return ATOM_ERR_UNSUPPORTED;
 }
 
+// Test hook: one thread waits, as the products do, on a barrier that nothing arrives on.
+__global__ void wait_selftest_kernel(long long budget, int* err) {
+    __shared__ uint64_t b;
+    mbar_init(&b, 1);
+    mbar_wait(&b, 0, err, budget);
+}
+
 }  // namespace pair
 }  // namespace atom
+
+extern "C" int atom_pair_wait_selftest(int64_t budget_cycles, void* stream) {
+    using namespace atom;
+    ATOM_REQUIRE(budget_cycles > 0 && budget_cycles <= pair::kWaitCycles,
+                 "atom_pair_wait_selftest: budget_cycles must be in [1, %lld]", pair::kWaitCycles);
+    int* err = device_error_word();
+    ATOM_REQUIRE(err, "atom_pair_wait_selftest: no device error word");
+    pair::wait_selftest_kernel<<<1, 1, 0, (cudaStream_t)stream>>>(budget_cycles, err);
+    return check_launch("atom_pair_wait_selftest");
+}
