@@ -348,6 +348,8 @@ struct AdSizes {
     int grad_split() const {
         const long long blocks = (long long)nad * (split ? (R + 31) / 32 : 1) *
                                  ((D + 127) / 128 + (O + 127) / 128);
+        // shares of the rows, for some four (16-bit: eight) blocks an SM: 6,007 rows, 8 adapters, bf16,
+        // forward and backward took 162, 149, 134 and 145 us with 1, 2, 4 and 8
         const long long s = blocks ? (split ? 592 : 1184) / blocks : 1;
         return (int)std::max(1LL, std::min({s, 16LL, (long long)pieces}));
     }
@@ -699,6 +701,7 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "adapted_linear: the workspace needs %zu bytes",
                  f.sp.bytes);
     const bool grads = z.on && (da || db);
+    // (2,048 x 2,048, rank 16, bf16: 20.5 us at 1 row and 31.2 at 16, against 33.2 and 43.2 by tiles)
     if (M <= few::kFewRows) {
         const int m = (int)M, shares = few::down_shares(O, D);
         if (z.on) {

@@ -526,7 +526,8 @@ int low_rank_back(const LowBackArgs& p, Chain& st) {
     return st.launch("low-rank part of a few rows", low_back_kernel, dim3(p.M), 256, 0, p);
 }
 
-// Shares of K that give the GPU some four blocks an SM, 32 rows each at least.
+// Shares of K that give the GPU some four blocks an SM, 32 rows each at least (11 rows, 2 x 7,688 x
+// 224 in bf16: 27 us with 148, 52 with 32).
 int down_shares(int K, int N, int most) {
     return std::max(1, std::min({592 / ((N + 63) / 64), K / 32, most}));
 }

@@ -29,16 +29,28 @@ struct Operand {
     }
 };
 
+// Whether a call's rows are streamed past: 16 at most, where a tile of 256 would be all but empty
+// (1,024 x 4,096 in bf16, forward: 8.7 us at 1 row and 11.1 at 16 against 21.6 and 17.1 by tiles;
+// 256 x 1,024 in fp32, backward: 16 and 32 against 45 and 46). A 16-bit backward pass multiplies on
+// the FMA pipe there: from 7 rows on, or 80 million products of rows and weights, tiles are faster
+// (1,024 x 4,096: 31 against 43 us at 1 row, 39 and 39 at 6, 63 and 36 at 16; 2,048 x 8,192: 92 and
+// 91 at 1 row, 97 and 83 at 2).
+bool few_rows(int dtype, long long M, int D, int F, int O, bool bwd) {
+    if (M > few::kFewRows) return false;
+    return !bwd || dtype == ATOM_F32 || (M <= 6 && M * F * (2LL * D + O) <= 80000000);
+}
+
 struct FfSizes {
     int dtype;
     long long M;
     int D, F, O;
     long long Dp, Fp, Op;       // widths of packed rows
-    bool split;
+    bool split, few;
     Choice gate{}, down{}, dh{}, dx{}, dwgu{}, dwd{};
     FfSizes(int t, long long m, int d, int f, int o, bool bwd)
         : dtype(t), M(m), D(d), F(f), O(o), Dp(up(d, 8)), Fp(up(f, 32)), Op(up(o, 8)),
-          split(t == ATOM_F32) {
+          split(t == ATOM_F32), few(few_rows(t, m, d, f, o, bwd)) {
+        if (few) return;
         gate = choose(M, F, nk(D), 1, true, split, false);
         if (!bwd) {
             down = choose(M, O, nk(F), 1, false, split, true);
@@ -65,7 +77,7 @@ struct FfSpace {
         memset(this, 0, sizeof(*this));
         Cursor c(ws);
         const long long M = z.M, k = z.split ? 2 : 1, M32 = up(M, 32);
-        if (M <= few::kFewRows) {
+        if (z.few) {
             if (bwd) {
                 few_dh = c.take<float>(few::down_shares(z.O, z.F, 32) * M * z.F);
                 few_dx = c.take<float>(few::down_shares(z.F, z.D) * M * z.D);
@@ -455,7 +467,7 @@ extern "C" int atom_gated_ff_fwd(int dtype, const void* x, int64_t ldx, int64_t 
     Ff f{z, FfSpace(ws, z, false), (cudaStream_t)stream, act};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
                  f.sp.bytes);
-    if (M <= few::kFewRows) return few_forward(f, x, ldx, wg, wu, wd, y, ldy);
+    if (z.few) return few_forward(f, x, ldx, wg, wu, wd, y, ldy);
     if (int s = f.inputs(x, ldx, wg, wu, wd)) return s;
     return f.forward(y, ldy, static_cast<float*>(kept));
 }
@@ -480,8 +492,9 @@ extern "C" int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t 
     Ff f{z, FfSpace(ws, z, true), st, act};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
                  f.sp.bytes);
-    if (M <= few::kFewRows)
+    if (z.few)
         return few_backward(f, x, ldx, wg, wu, wd, dy, lddy, dx, lddx, dwg, dwu, dwd);
+    if (M <= few::kFewRows) kept = nullptr;          // the forward pass kept nothing
     if (int s = f.inputs_bwd(x, ldx, wg, wu, wd, dy, lddy, kept != nullptr, dwg || dwu,
                              dwd != nullptr))
         return s;

@@ -1673,7 +1673,9 @@ static int sm_count() {
 // The tile width and split that a count of clocks prefers: rounds of work items over the SM
 // pairs, each a tile's stages (512 clocks of tensor work at width 256, 256 at 128 but fed no
 // faster than ~300; SPLIT 12 products of 64) and its fill and drain, and for a split the pass
-// over the partial sums.
+// over the partial sums. Width 256 against 128: 60,000 x 256 x 1,024 bf16 forward 91 and 103 us,
+// 8,192 x 2,048 x 8,192 559 and 622; splits against none: 18,000 x 128 x 512 fp32 backward 139 and
+// 343 us, 200 x 1,024 x 4,096 bf16 forward 16.7 and 19.7.
 Choice choose(long long M, int N, int nk, int groups, bool gated, bool split, bool may_split) {
     const int pairs = sm_count() / 2;
     const long long mt = (M + 255) / 256 * groups;
