@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(256) grads16_kernel(const __grid_constant__ Gr
 }
 
 // fp32: 32 ranks by 128 columns a block, 4 x 4 a thread, 32 rows at a time. On the FMA pipe: it is
-// exact without planes, and 4,000 x 512 columns x 20 ranks take 15 us, 2,124 x 4,150 x 32 take 51.
+// exact without planes, and 4,000 x 512 columns x 20 ranks take 14 us, 2,124 x 4,150 x 32 take 42.
 __global__ void __launch_bounds__(256) grads32_kernel(const __grid_constant__ Grads p) {
     __shared__ __align__(16) float ts[32][36], xs[32][132];
     let_next_start();
@@ -348,10 +348,12 @@ struct AdSizes {
     int grad_split() const {
         const long long blocks = (long long)nad * (split ? (R + 31) / 32 : 1) *
                                  ((D + 127) / 128 + (O + 127) / 128);
-        // shares of the rows, for some four (16-bit: eight) blocks an SM: 6,007 rows, 8 adapters, bf16,
-        // forward and backward took 162, 149, 134 and 145 us with 1, 2, 4 and 8
-        const long long s = blocks ? (split ? 592 : 1184) / blocks : 1;
-        return (int)std::max(1LL, std::min({s, 16LL, (long long)pieces}));
+        // shares of the rows, for some eight blocks an SM, forward and backward: 6,007 rows, 8 adapters
+        // in bf16 took 162, 149, 134 and 145 us with 1, 2, 4 and 8; in fp32, 7,882 rows of 1,146 + 336
+        // columns, 2 adapters 280 us with 16 and 252 with 32, and 2,124 of 1,486 + 2,664 331 with 8 and
+        // 292 with 12
+        const long long s = blocks ? 1184 / blocks : 1;
+        return (int)std::max(1LL, std::min({s, split ? 32LL : 16LL, (long long)pieces}));
     }
 };
 
