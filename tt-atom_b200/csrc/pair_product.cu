@@ -1116,9 +1116,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 }
                 if constexpr (EPI == kStoreLow) {
                     const int es = ti.ks == p.ksplit - 1 ? (req.z * p.ext + 3) >> 2 : 0;
-                    // rows of no piece have no scale, and sums of zero
-                    float f = m + lane < p.M ? p.ext_rinv[m + lane] : 0.f;
-                    f = (finite_bits(f) ? f : 0.f) * pow2_inv(pow2_scale(*p.ext_bmax));
+                    // a row without an adapter has no scale (the workspace holds anything there)
+                    float f = m + lane < p.M && p.row_lead[m + lane] >= 0 ? p.ext_rinv[m + lane] : 0.f;
+                    f *= pow2_inv(pow2_scale(*p.ext_bmax));
                     if (!(ok = add((es + kRound - 1) / kRound, f))) break;
                 }
 #pragma unroll
