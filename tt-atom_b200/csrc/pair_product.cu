@@ -470,14 +470,14 @@ __device__ __forceinline__ void normal(float g, float& cdf, float& bell) {
     cdf = g < 0.f ? tail : 1.f - tail;
 }
 // Two sigmoids with one reciprocal, 1 / (a b): a multiprocessor has 16 results of ex2 and rcp a
-// clock, and a gate needs both for every value. Exponentials stay below 2^60, where a sigmoid is
-// nothing beside its own rounding, so that a b is finite.
+// clock, and a gate needs both for every value. From e = exp(-|g|) <= 1, so that a b is at most 4 and
+// a closed gate (e / (1 + e)) keeps its value down to the smallest normal one. A NaN in one of the
+// two is in both: they are columns of one row of H, and each of y's sums over that row is NaN anyway.
 __device__ __forceinline__ void sigmoid2(float g0, float g1, float& s0, float& s1) {
-    const float a = 1.f + exp2_fast(fminf(-1.4426950f * g0, 60.f));
-    const float b = 1.f + exp2_fast(fminf(-1.4426950f * g1, 60.f));
-    const float r = rcp_fast(a * b);
-    s0 = r * b;
-    s1 = r * a;
+    const float e0 = exp2_fast(-1.4426950f * fabsf(g0)), e1 = exp2_fast(-1.4426950f * fabsf(g1));
+    const float a = 1.f + e0, b = 1.f + e1, r = rcp_fast(a * b);
+    s0 = (g0 >= 0.f ? b : e0 * b) * r;
+    s1 = (g1 >= 0.f ? a : e1 * a) * r;
 }
 // h = act(g) u
 template <bool GELU>
