@@ -1,11 +1,13 @@
-"""Where the typed operators could lose what the definition keeps, with 16 rows and with more (which
-other kernels take)."""
+"""Where the typed operators could lose what the definition keeps: a NaN in a gate's weights, gates
+that are closed or open, fp32 values far below others of their row, weight or call, and the same
+call with 16 rows and with more (which other kernels take)."""
 import pytest
 import torch
 
 import test_gpu_adapters as ad
 import test_gpu_feedforward as ff
 from tt_atom import _lib as L
+from tt_atom.adapters import adapted_linear, adapted_linear_bwd
 from tt_atom.feedforward import gated_ff, gated_ff_bwd
 
 pytestmark = pytest.mark.gpu
@@ -73,7 +75,7 @@ def test_nan_in_a_gates_weights(M, act, t):
 
 
 @pytest.mark.parametrize("M", [16, 40])
-@pytest.mark.parametrize("t", [torch.bfloat16], ids=str)
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float32], ids=str)
 def test_sigmoid_gates_that_are_closed(t, M):
     # sigmoid(-50) = 2e-22. A product's error in g, gamma(D) of its terms' magnitudes (64 at most),
     # is a relative error of the sigmoid; beside it half steps of the type for h and y, both ways
@@ -81,6 +83,77 @@ def test_sigmoid_gates_that_are_closed(t, M):
     y = gated_ff(*args[:4], act="sigmoid")
     bound = 64 * ff.gamma(32) + 3 * torch.finfo(t).eps
     assert off(y, exact(*args, "sigmoid")["y"])[0] <= bound
+
+
+def outliers(kind, M, D, F, O):  # noqa: E741
+    x, wg, wu, wd, dy = ff.make(M, D, F, O, torch.float32, seed=4)
+    if kind == "a weight of 16":
+        wg[5, 7] = 16
+    elif kind == "a weight of 100 and a feature of 100":
+        wg[5, 7] = 100
+        x[:, 9] *= 100
+    elif kind == "a feature of 1,000 with small weights":
+        x[:, 9] *= 1000
+        wg[:, 9] /= 1000
+        wu[:, 9] /= 1000
+    elif kind == "a constant feature without weights":
+        x[:, 9] = 1e4
+        wg[:, 9] = wu[:, 9] = 0
+    elif kind == "closed gates":
+        x[:, 9] = 1
+        wg[:, 9] = -12
+    elif kind == "a large row":
+        x[1] *= 1e5
+        dy[1] = 0
+    elif kind == "a large weight beside small ones":
+        wd[0, 0] = 1e6
+        dy[:, 0] = 0
+    return x, wg, wu, wd, dy
+
+
+@pytest.mark.parametrize("kind", [
+    "a weight of 16", "a weight of 100 and a feature of 100", "a feature of 1,000 with small weights",
+    "a constant feature without weights", "closed gates", "a large row",
+    "a large weight beside small ones"])
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+@pytest.mark.parametrize("M", [16, 17, 130])
+def test_fp32_keeps_fp32s_accuracy_beside_outliers(M, act, kind):
+    """Every output keeps its bound of fp32, element by element, and is as a whole (y and dx, whose rows
+    sum over all gates, also in the worst row; a row of dwg may hang on one gate, and is then as far
+    off as chance has it) at most twice as far off as the same formulas in fp32 steps: an addition
+    here may be off by a whole step (the tensor core's, toward zero) where those are off by half.
+    Beside it what the activation's own arithmetic may add, 8 + g^2 steps (|g| <= 20 where a gate is
+    neither 0 nor 1 nor the value itself)."""
+    args = outliers(kind, M, 1024, 264, 72)
+    bounds = ff.reference(*args, act)
+    want, plain = exact(*args, act), exact(*args, act, torch.float32)
+    g = float((args[0] @ args[1].T).abs().max().clamp_max(20))
+    own = (8 + g * g) * 2.0 ** -23
+    for got in run(*args, act):
+        ff.check(got.values(), bounds, got)
+        for name, v in got.items():
+            a, b = off(v, want[name]), off(plain[name], want[name])
+            assert a[0] <= 2 * b[0] + own, (name, a, b)
+            assert name[:2] == "dw" or a[1] <= 2 * b[1] + own, (name, a, b)
+
+
+@pytest.mark.parametrize("size", [1e3, 1e9, 1e15])
+@pytest.mark.parametrize("R", [8, 72])
+@pytest.mark.parametrize("rows", [3, 70])
+def test_an_adapters_size_stays_with_its_requests(rows, R, size):
+    # fp32: one adapter many times larger than the others; the other requests keep their bounds
+    args = ad.make([rows] * 3, [0, 1, 2], 3, R, 64, 96, torch.float32, seed=5)
+    x, w, a, b, scale, ptr, ids, dy = args
+    a[1] *= size
+    b[1] *= size
+    want = ad.reference(*args)
+    rest = [i for i in range(3 * rows) if not rows <= i < 2 * rows]
+    y, kept = adapted_linear(*args[:7], keep=True)
+    ad.check([y[rest]], {"y": [v[rest] for v in want["y"]]}, ["y"])
+    want = {k: [v[rest if k == "dx" else [0, 2]] for v in want[k]] for k in ("dx", "da", "db")}
+    for k in (kept, None):
+        dx, da, db = adapted_linear_bwd(*args, kept=k)
+        ad.check([dx[rest], da[[0, 2]], db[[0, 2]]], want, ("dx", "da", "db"))
 
 
 def test_a_row_without_an_adapter_beside_large_ones_and_an_old_workspace():

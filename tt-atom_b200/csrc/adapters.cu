@@ -24,41 +24,6 @@ namespace {
 
 using namespace pair;
 
-// fp32, more than 64 ranks: the blocks as planes, scaled row by row, from the low-rank rows. A
-// thread block each, a warp a row, four ranks a lane.
-__global__ void __launch_bounds__(256) blocks32_kernel(const __grid_constant__ Args p,
-                                                       const float* rows, int Rs, __half* block,
-                                                       long long plane, float* rinv) {
-    let_next_start();
-    wait_before();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = p.piece[blockIdx.x].y / 256;
-    const int4 req = p.tile_req[t];
-    const int m0 = t * 256, j = blockIdx.x - t - req.x;      // the tile's j-th block
-    if (j < 0 || j >= req.z) return;
-    const int request = p.lead[blockIdx.x].y, slice = j * p.ext + lane / 4;
-    if (4 * lane >= 16 * p.ext) return;
-    __half* q0 = block + ((first_stage(t, req.x, p.ext) + (slice >> 2)) * 256) * 64 +
-                 (slice & 3) * 16 + (lane & 3) * 4;
-    const unsigned lanes = p.ext == 8 ? 0xffffffffu : (1u << 4 * p.ext) - 1;
-#pragma unroll 4
-    for (int m = m0 + warp; m < m0 + 256; m += 8) {
-        const bool in = m < p.M && p.row_lead[m] == request;
-        const float4 x = in && 4 * lane < Rs
-            ? *reinterpret_cast<const float4*>(rows + (long long)m * Rs + 4 * lane)
-            : make_float4(0.f, 0.f, 0.f, 0.f);
-        const unsigned mx = __reduce_max_sync(
-            lanes, max(max(finite_bits(x.x), finite_bits(x.y)),
-                       max(finite_bits(x.z), finite_bits(x.w))));
-        const float s = pow2_scale(mx);
-        if (in && lane == 0) rinv[m] = pow2_inv(s);
-        __half2 h[2], l[2];
-        split_half2(x.x * s, x.y * s, h[0], l[0]);
-        split_half2(x.z * s, x.w * s, h[1], l[1]);
-        __half* q = q0 + (m - m0) * 64;
-        *reinterpret_cast<uint2*>(q) = *reinterpret_cast<uint2*>(h);
-        *reinterpret_cast<uint2*>(q + plane) = *reinterpret_cast<uint2*>(l);
-    }
-}
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -345,6 +310,7 @@ struct AdSizes {
           stages(first_stage(tiles, q, ext) + 1), Dp(up(d, 8)), Op(up(o, 8)), split(t == ATOM_F32),
           on(n > 0 && q > 0),
           product(choose(m, bwd ? d : o, ((bwd ? o : d) + 63) / 64, 1, false, t == ATOM_F32, true)) {}
+    int planes() const { return split ? kPlanes : 1; }
     int grad_split() const {
         const long long blocks = (long long)nad * (split ? (R + 31) / 32 : 1) *
                                  ((D + 127) / 128 + (O + 127) / 128);
@@ -360,19 +326,17 @@ struct AdSizes {
 // One call's buffers. Copies and planes of one direction's operands; the backward pass has x's a
 // second time where the forward pass kept no S.
 struct AdSpace {
-    __half *rows, *x, *w, *first, *first2, *ext, *block;
-    float *rinv, *xinv, *wr, *ext_rinv, *part, *gpart, *few_S, *few_T, *few_dx;
+    uint16_t *rows, *x, *w, *first, *first2, *ext, *block;
+    float *part, *gpart, *few_S, *few_T, *few_dx;
     void *S, *T;
     int4 *piece, *bad, *tile_req;
     int2* lead;
     int *row_lead, *usable, *few_slot;
-    unsigned *max, *maxima[3];       // of w, of the adapters beside it, of those of the low-rank
-                                     // rows; and the blocks' own
     size_t bytes;
     AdSpace(void* ws, const AdSizes& z, bool bwd) {
         memset(this, 0, sizeof(*this));
         Cursor c(ws);
-        const long long k = z.split ? 2 : 1, e = dtype_size(z.dtype);
+        const long long k = z.planes(), e = dtype_size(z.dtype);
         if (z.M <= few::kFewRows) {
             few_S = c.take<float>(z.M * z.R);
             few_T = c.take<float>(bwd ? z.M * z.R : 0);
@@ -382,16 +346,9 @@ struct AdSpace {
             return;
         }
         const long long a_n = (long long)z.nad * z.R * z.Dp, b_n = (long long)z.nad * z.O * z.Rs;
-        rows = c.take<__half>(k * z.M * (bwd ? z.Op : z.Dp));
-        w = c.take<__half>(k * z.O * z.Dp);
+        rows = c.take<uint16_t>(k * z.M * (bwd ? z.Op : z.Dp));
+        w = c.take<uint16_t>(k * z.O * z.Dp);
         part = c.take<float>(z.product.part);
-        if (z.split) {
-            rinv = c.take<float>(up(z.M, 32));
-            if (!bwd) wr = c.take<float>(up(z.O, 32));
-            max = c.take<unsigned>(4);
-            for (unsigned*& m : maxima) m = c.take<unsigned>(kPrepBlocks);
-            ext_rinv = c.take<float>(z.on ? z.M : 0);
-        }
         if (z.on) {
             piece = c.take<int4>(z.pieces);
             bad = c.take<int4>(z.nad);
@@ -399,14 +356,13 @@ struct AdSpace {
             usable = c.take<int>(z.pieces);
             lead = c.take<int2>(z.pieces);
             row_lead = c.take<int>(z.M);
-            first = c.take<__half>(k * (bwd ? b_n : a_n));
-            ext = c.take<__half>(k * (bwd ? a_n : b_n));
-            block = c.take<__half>(k * z.stages * 256 * 64);
-            if (bwd || z.split) T = c.take<char>(z.M * z.Rs * e);
+            first = c.take<uint16_t>(k * (bwd ? b_n : a_n));
+            ext = c.take<uint16_t>(k * (bwd ? a_n : b_n));
+            block = c.take<uint16_t>(k * z.stages * 256 * 64);
             if (bwd) {
-                x = c.take<__half>(k * z.M * z.Dp);
-                first2 = c.take<__half>(k * a_n);
-                if (z.split) xinv = c.take<float>(up(z.M, 32));
+                T = c.take<char>(z.M * z.Rs * e);
+                x = c.take<uint16_t>(k * z.M * z.Dp);
+                if (!z.split) first2 = c.take<uint16_t>(a_n);
                 S = c.take<char>(z.M * z.Rs * e);
                 const long long s = z.grad_split();
                 gpart = c.take<float>(s > 1 ? s * z.nad * z.R * (z.D + z.O) : 0);
@@ -458,13 +414,12 @@ struct Ad {
 
     // The low-rank rows of `rows` [M, K] and a (forward) or b (backward): s rows first^T into
     // `kept` (may be NULL) and, as the product beside the projection takes them, the blocks.
-    int low_rows(const Operands& o, bool bwd, const float* rinv, const unsigned* max, void* kept,
-                 bool blocks) {
-        const int K = bwd ? z.O : z.D, k = z.split ? 2 : 1;
+    int low_rows(const Operands& o, bool bwd, void* kept, bool blocks) {
+        const int K = bwd ? z.O : z.D, k = z.planes();
         Maps maps;
         for (int pl = 0; pl < k; ++pl) {
-            const __half* r = static_cast<const __half*>(o.rows) + pl * o.rows_plane;
-            const __half* f = static_cast<const __half*>(o.first) + pl * o.first_plane;
+            const uint16_t* r = static_cast<const uint16_t*>(o.rows) + pl * o.rows_plane;
+            const uint16_t* f = static_cast<const uint16_t*>(o.first) + pl * o.first_plane;
             if (int s = make_map(&maps.m[pl], r, K, z.M, o.ld, 128)) return s;
             if (int s = make_low_map(&maps.m[k + pl], f, bwd ? z.R : K, bwd ? K : z.R, o.first_ld,
                                      bwd, z.nad, (bwd ? K : z.R) * o.first_ld))
@@ -474,26 +429,19 @@ struct Ad {
         p.ph[0] = {0, k, k, (K + 63) / 64, 0, bwd ? 1 : 0, 0, 0};
         p.used = (1u << 2 * k) - 1;
         p.low_scale = scale;
-        const bool planes = z.split && z.R <= 64;        // written by the product
-        p.low_block = !z.split || (blocks && planes) ? sp.block : nullptr;
+        p.low_block = !z.split || blocks ? sp.block : nullptr;
         p.low_plane = z.stages * 256 * 64;
-        p.low_rinv = sp.ext_rinv;
-        p.low_rows = z.split && !planes && !kept ? sp.T : kept;
+        p.low_rows = kept;
         if (!blocks) p.usable = nullptr;
         p.Rs = z.Rs;
-        p.rinv = rinv;
-        p.bmax = max;
         // as many items as pairs of SMs, but no more than a tile may have groups
         const int groups = std::min(16, (z.nreq * p.ext + 7) / 8);
         const int share = std::max(1, std::min(groups, 74 / z.tiles));
-        if (int s = launch(kLow, {128, share, 0}, z.split, maps, p, st, sums)) return s;
-        if (!z.split || !blocks || planes) return ATOM_OK;
-        return st.launch("adapters: blocks", blocks32_kernel, dim3(z.pieces), 256, 0, p,
-                         (const float*)p.low_rows, z.Rs, sp.block, p.low_plane, sp.ext_rinv);
+        return launch(kLow, {128, share, 0}, z.split, maps, p, st, sums);
     }
 
     int run(const void* rows, long long ld, bool bwd, void* out, long long ldo, void* kept) {
-        const int K = bwd ? z.O : z.D, N = bwd ? z.D : z.O, k = z.split ? 2 : 1;
+        const int K = bwd ? z.O : z.D, N = bwd ? z.D : z.O, k = z.planes();
         const long long Kp = bwd ? z.Op : z.Dp;
         const void* first = bwd ? b : a;         // forward [nad][R][D], backward [nad][O][R]
         const void* second = bwd ? a : b;
@@ -505,61 +453,30 @@ struct Ad {
         Operands o{rows, w, first, second, ld, z.D, fcols, scols, 0, 0, 0, 0};
         PrepList l;
         const Pieces found = pieces(product ? second : nullptr, (long long)z.R * (bwd ? z.D : z.O));
-        if (z.split) {
-            o = {sp.rows, sp.w, sp.first, sp.ext, Kp, z.Dp, fp, spp,
-                 z.M * Kp, z.O * z.Dp, frows * fp, srows * spp};
-            int parts[3] = {};
-            auto largest = [&](const void* p, long long n, long long cols, int m) {
-                PrepItem it{p, n, cols, cols, nullptr, 0, 0, nullptr, nullptr, kMax,
-                            sp.maxima[m], 0};
-                parts[m] = prep_blocks(it);
-                l.add(it);
-            };
-            auto planes = [&](const void* p, long long n, long long cols, __half* dst,
-                              long long pitch, int m) {
-                l.add({p, n, cols, cols, dst, pitch, n * pitch, nullptr, sp.max + m, kTensorSplit,
-                       sp.maxima[m], parts[m]});
-            };
-            l.add({rows, z.M, K, ld, sp.rows, Kp, z.M * Kp, sp.rinv, nullptr, kRowSplit});
-            if (product && bwd) largest(w, z.O, z.D, 0);
-            if (product && !bwd)
-                l.add({w, z.O, z.D, z.D, sp.w, z.Dp, z.O * z.Dp, sp.wr, nullptr, kRowSplit});
-            if (z.on) {
-                largest(second, srows, scols, 1);
-                largest(first, frows, fcols, 2);
-            }
-            if (int s = prepare(l, st, z.on ? &found : nullptr)) return s;
-            if (product && bwd) planes(w, z.O, z.D, sp.w, z.Dp, 0);
-            if (z.on) {
-                planes(second, srows, scols, sp.ext, spp, 1);
-                planes(first, frows, fcols, sp.first, fp, 2);
-            }
-            if (int s = prepare(l, st)) return s;
-        } else {
-            auto take = [&](const void*& p, long long& pld, long long n, long long cols, __half* buf,
-                            long long pitch) {
-                if (tma_ready(p, pld)) return;
-                l.add({p, n, cols, pld, buf, pitch, 0, nullptr, nullptr, kPack});
-                p = buf, pld = pitch;
-            };
-            take(o.rows, o.ld, z.M, K, sp.rows, Kp);
-            if (product) take(o.w, o.w_ld, z.O, z.D, sp.w, z.Dp);
-            if (z.on) {
-                take(o.first, o.first_ld, frows, fcols, sp.first, fp);
-                if (product) take(o.second, o.second_ld, srows, scols, sp.ext, spp);
-            }
+        auto take = [&](const void*& p, long long& pld, long long& plane, long long n, long long cols,
+                        uint16_t* buf, long long pitch) {
+            if (!z.split && tma_ready(p, pld)) return;
+            plane = n * pitch;
+            l.add({p, n, cols, pld, buf, pitch, plane, z.split ? kSplit : kPack});
+            p = buf, pld = pitch;
+        };
+        take(o.rows, o.ld, o.rows_plane, z.M, K, sp.rows, Kp);
+        if (product) take(o.w, o.w_ld, o.w_plane, z.O, z.D, sp.w, z.Dp);
+        if (z.on) {
+            take(o.first, o.first_ld, o.first_plane, frows, fcols, sp.first, fp);
+            // (fp32: a's planes serve the gradients as well)
+            if (product || z.split)
+                take(o.second, o.second_ld, o.second_plane, srows, scols, sp.ext, spp);
         }
-        if (!z.split)
-            if (int s = prepare(l, st, z.on ? &found : nullptr)) return s;
+        if (int s = prepare(l, st, z.on ? &found : nullptr)) return s;
         if (z.on)
-            if (int s = low_rows(o, bwd, sp.rinv, z.split ? sp.max + 2 : nullptr, kept, product))
-                return s;
+            if (int s = low_rows(o, bwd, kept, product)) return s;
         if (!product) return ATOM_OK;
         const Choice c = z.product;
         Maps maps;
         for (int pl = 0; pl < k; ++pl) {
             auto at = [&](const void* base, long long plane) {
-                return static_cast<const __half*>(base) + pl * plane;
+                return static_cast<const uint16_t*>(base) + pl * plane;
             };
             if (int s = make_map(&maps.m[pl], at(o.rows, o.rows_plane), K, z.M, o.ld, 128)) return s;
             if (int s = make_map(&maps.m[k + pl], at(o.w, o.w_plane), z.D, z.O, o.w_ld,
@@ -580,39 +497,29 @@ struct Ad {
         p.ldc = ldo;
         p.used = z.on ? (1u << 4 * k) - 1 : (1u << 2 * k) - 1;
         p.part = sp.part;
-        p.rinv = sp.rinv;
-        p.cinv[0] = sp.wr;
-        if (z.split && bwd) p.bmax = sp.max;
         p.ext_a = 2 * k, p.ext_b = 3 * k, p.ext_bmn = bwd ? 1 : 0;
-        p.ext_rinv = sp.ext_rinv;
-        p.ext_bmax = sp.max + 1;
         if (int s = launch(z.on ? kStoreLow : kStore, c, z.split, maps, p, st, sums)) return s;
         return add_up(sums, st);
     }
 
-    // S alone, in the backward pass: x's and a's own copies, the pieces as they are
+    // S alone, in the backward pass: x's own copy (and a's: fp32 has it beside the projection), the
+    // pieces as they are
     int low_again(const void* x, long long ldx) {
         const long long an = (long long)z.nad * z.R;
         Operands o{x, nullptr, a, nullptr, ldx, 0, z.D, 0, 0, 0, 0, 0};
         PrepList l;
+        if (z.split || !tma_ready(x, ldx)) {
+            o.rows = sp.x, o.ld = z.Dp, o.rows_plane = z.M * z.Dp;
+            l.add({x, z.M, z.D, ldx, sp.x, z.Dp, o.rows_plane, z.split ? kSplit : kPack});
+        }
         if (z.split) {
-            o = {sp.x, nullptr, sp.first2, nullptr, z.Dp, 0, z.Dp, 0, z.M * z.Dp, 0, an * z.Dp, 0};
-            l.add({x, z.M, z.D, ldx, sp.x, z.Dp, z.M * z.Dp, sp.xinv, nullptr, kRowSplit});
-            // a's maximum is there: a is beside the projection in this direction
-            l.add({a, an, z.D, z.D, sp.first2, z.Dp, an * z.Dp, nullptr, sp.max + 3, kTensorSplit,
-                   sp.max + 1, 1});
-        } else {
-            if (!tma_ready(x, ldx)) {
-                l.add({x, z.M, z.D, ldx, sp.x, z.Dp, 0, nullptr, nullptr, kPack});
-                o.rows = sp.x, o.ld = z.Dp;
-            }
-            if (!tma_ready(a, z.D)) {
-                l.add({a, an, z.D, z.D, sp.first2, z.Dp, 0, nullptr, nullptr, kPack});
-                o.first = sp.first2, o.first_ld = z.Dp;
-            }
+            o.first = sp.ext, o.first_ld = z.Dp, o.first_plane = an * z.Dp;
+        } else if (!tma_ready(a, z.D)) {
+            l.add({a, an, z.D, z.D, sp.first2, z.Dp, 0, kPack});
+            o.first = sp.first2, o.first_ld = z.Dp;
         }
         if (int s = prepare(l, st)) return s;
-        return low_rows(o, false, sp.xinv, z.split ? sp.max + 3 : nullptr, sp.S, false);
+        return low_rows(o, false, sp.S, false);
     }
 };
 
@@ -743,7 +650,7 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
         if (!tma_ready(x, ldx)) {
             if (!again) {
                 PrepList l;
-                l.add({x, M, D, ldx, f.sp.x, z.Dp, 0, nullptr, nullptr, kPack});
+                l.add({x, M, D, ldx, f.sp.x, z.Dp, 0, kPack});
                 if (int s = prepare(l, f.st)) return s;
             }
             p.rows[0] = f.sp.x, p.ld[0] = z.Dp;

@@ -17,13 +17,13 @@ namespace {
 
 using namespace pair;
 
-// A 16-bit operand ready for TMA (fp32: its hi plane, the lo plane `plane` elements behind).
+// A 16-bit operand ready for TMA (fp32: the first of its planes, `plane` elements apart).
 struct Operand {
     const void* p = nullptr;
     long long rows = 0, cols = 0, ld = 0, plane = 0;
     Operand columns(long long c0, long long n) const {
         Operand o = *this;
-        o.p = static_cast<const __half*>(p) + c0;
+        o.p = static_cast<const uint16_t*>(p) + c0;
         o.cols = n;
         return o;
     }
@@ -62,80 +62,54 @@ struct FfSizes {
         }
     }
     int nk(long long k) const { return (int)((k + 63) / 64); }
+    int planes() const { return split ? kPlanes : 1; }
 };
 
 // One call's buffers. 16-bit operands are packed only where TMA cannot read them; fp32 ones
-// always become two planes.
+// always become planes.
 struct FfSpace {
-    __half *x, *wg, *wu, *wd, *dy, *xt, *dyt, *hp, *dgup;
-    float *xr, *wgr, *wur, *wdr, *dyr, *hr, *dgur, *H32, *dh, *part, *part_gu, *part_d;
-    __half *H, *dgu;
-    float *few_dh, *few_dx, *few_grads;
-    unsigned *max, *maxima[4];  // of wg | wu, of wd, x'' factor, dy'' factor; and the blocks' own
+    uint16_t *x, *wg, *wu, *wd, *dy, *H, *dgu;
+    float *dh, *part, *part_gu, *part_d;
+    float *few_H, *few_dh, *few_dx, *few_grads;
     size_t bytes;
     FfSpace(void* ws, const FfSizes& z, bool bwd) {
         memset(this, 0, sizeof(*this));
         Cursor c(ws);
-        const long long M = z.M, k = z.split ? 2 : 1, M32 = up(M, 32);
+        const long long M = z.M, k = z.planes();
         if (z.few) {
             if (bwd) {
                 few_dh = c.take<float>(few::down_shares(z.O, z.F, 32) * M * z.F);
                 few_dx = c.take<float>(few::down_shares(z.F, z.D) * M * z.D);
                 few_grads = c.take<float>(3 * M * z.F);
             } else if (z.split) {
-                H32 = c.take<float>(M * z.Fp);
+                few_H = c.take<float>(M * z.Fp);
             } else {
-                H = c.take<__half>(M * z.Fp);
+                H = c.take<uint16_t>(M * z.Fp);
             }
             bytes = c.used;
             return;
         }
-        x = c.take<__half>(k * M * z.Dp);
-        wg = c.take<__half>(k * z.F * z.Dp);
-        wu = c.take<__half>(k * z.F * z.Dp);
-        wd = c.take<__half>(k * z.O * z.Fp);
+        x = c.take<uint16_t>(k * M * z.Dp);
+        wg = c.take<uint16_t>(k * z.F * z.Dp);
+        wu = c.take<uint16_t>(k * z.F * z.Dp);
+        wd = c.take<uint16_t>(k * z.O * z.Fp);
+        H = c.take<uint16_t>(k * M * z.Fp);
         if (bwd) {
-            dy = c.take<__half>(k * M * z.Op);
-            dh = c.take<float>(M32 * z.Fp);
+            dy = c.take<uint16_t>(k * M * z.Op);
+            dh = c.take<float>(up(M, 32) * z.Fp);
+            dgu = c.take<uint16_t>(k * M * 2 * z.Fp);
         }
         part = c.take<float>(bwd ? z.dx.part : z.down.part);
         part_gu = c.take<float>(z.dwgu.part);
         part_d = c.take<float>(z.dwd.part);
-        if (!z.split) {
-            H = c.take<__half>(M * z.Fp);
-            if (bwd) dgu = c.take<__half>(2 * M * z.Fp);
-        } else {
-            max = c.take<unsigned>(4);
-            for (unsigned*& m : maxima) m = c.take<unsigned>(2 * kPrepBlocks);
-            xr = c.take<float>(M32);
-            hp = c.take<__half>(2 * M * z.Fp);
-            hr = c.take<float>(M32);
-            if (!bwd) {
-                wgr = c.take<float>(up(z.F, 32));
-                wur = c.take<float>(up(z.F, 32));
-                wdr = c.take<float>(up(z.O, 32));
-            } else {
-                dyr = c.take<float>(M32);
-                dgup = c.take<__half>(4 * M * z.Fp);
-                dgur = c.take<float>(M32);
-                xt = c.take<__half>(2 * M * z.Dp);
-                dyt = c.take<__half>(2 * M * z.Op);
-            }
-        }
         bytes = c.used;
     }
 };
 
-int log2_up(int n) {
-    int k = 0;
-    while ((1 << k) < n) ++k;
-    return k;
-}
-
-// Fills a map (and, for two planes, the next one).
-int put(Maps& maps, int i, const Operand& o, bool mn, int box_rows, bool split) {
-    for (int pl = 0; pl < (split ? 2 : 1); ++pl)
-        if (int s = make_map(&maps.m[i + pl], static_cast<const __half*>(o.p) + pl * o.plane, o.cols,
+// Fills a map (and, for further planes, the next ones).
+int put(Maps& maps, int i, const Operand& o, bool mn, int box_rows, int planes) {
+    for (int pl = 0; pl < planes; ++pl)
+        if (int s = make_map(&maps.m[i + pl], static_cast<const uint16_t*>(o.p) + pl * o.plane, o.cols,
                              o.rows, o.ld, mn ? 64 : box_rows))
             return s;
     return ATOM_OK;
@@ -148,82 +122,26 @@ struct Ff {
     int act;
     Operand x, wg, wu, wd, dy;
     PrepList list;
-    int parts[4] = {};          // blocks' maxima so far
     Sums sums{};
 
-    // an operand of this call: as it lies, or through the list's packing / planes; kTensorSplit:
-    // by maximum `m` of parts[m] blocks
-    Operand take(const void* p, long long rows, long long cols, long long ld, __half* buf,
-                 long long pitch, int mode, float* rinv, int m = 0) {
+    // an operand of this call: as it lies, or through the list's packing / planes
+    Operand take(const void* p, long long rows, long long cols, long long ld, uint16_t* buf,
+                 long long pitch) {
         if (!z.split && tma_ready(p, ld)) return {p, rows, cols, ld, 0};
-        list.add({p, rows, cols, ld, buf, pitch, rows * pitch, rinv, sp.max + m,
-                  z.split ? mode : kPack, sp.maxima[m], parts[m]});
-        if (mode == kRowSplit || !z.split) list.it[list.n - 1].part = nullptr;
-        return {buf, rows, cols, pitch, rows * pitch};
+        const long long plane = rows * pitch;
+        list.add({p, rows, cols, ld, buf, pitch, plane, z.split ? kSplit : kPack});
+        return {buf, rows, cols, pitch, plane};
     }
-    // an item whose blocks' maxima go behind those that maximum m has
-    void gather(PrepItem it, int m) {
-        it.part = sp.maxima[m] + parts[m];
-        parts[m] += prep_blocks(it);
-        list.add(it);
-    }
-    // Weights and rows brought into the form that the products read. fp32 forward: every operand
-    // scaled row by row, in one launch. fp32 backward: the weights are read across their rows, so
-    // each of them (Wg and Wu together) has one scale, from a launch before; x is needed only for
-    // G and U, and beside its scales in the weights' gradients later.
-    int inputs(const void* xp, long long ldx, const void* g, const void* u, const void* d) {
-        x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kRowSplit, sp.xr);
-        if (z.split) {
-            const long long n = z.F * z.Dp;
-            gather({g, z.F, z.D, z.D, sp.wg, z.Dp, n, sp.wgr, nullptr, kRowSplit}, 0);
-            gather({u, z.F, z.D, z.D, sp.wu, z.Dp, n, sp.wur, nullptr, kRowSplit}, 0);
-            wg = {sp.wg, z.F, z.D, z.Dp, n};
-            wu = {sp.wu, z.F, z.D, z.Dp, n};
-        } else {
-            wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kPack, nullptr);
-            wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kPack, nullptr);
-        }
-        wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kRowSplit, sp.wdr);
+    // What the products read, in one launch; dyp: a backward pass, which reads x for G and U and for
+    // the weights' gradients alone.
+    int inputs(const void* xp, long long ldx, const void* g, const void* u, const void* d,
+               const void* dyp = nullptr, long long lddy = 0, bool reads_x = true) {
+        if (reads_x) x = take(xp, z.M, z.D, ldx, sp.x, z.Dp);
+        wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp);
+        wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp);
+        wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8));
+        if (dyp) dy = take(dyp, z.M, z.O, lddy, sp.dy, z.Op);
         return prepare(list, st);
-    }
-    int inputs_bwd(const void* xp, long long ldx, const void* g, const void* u, const void* d,
-                   const void* dyp, long long lddy, bool kept, bool dwgu, bool dwd) {
-        if (z.split) {
-            gather({g, z.F, z.D, z.D, nullptr, 0, 0, nullptr, nullptr, kMax}, 0);
-            gather({u, z.F, z.D, z.D, nullptr, 0, 0, nullptr, nullptr, kMax}, 0);
-            gather({d, z.O, z.F, z.F, nullptr, 0, 0, nullptr, nullptr, kMax}, 1);
-        }
-        if (z.split) {
-            x = {sp.x, z.M, z.D, z.Dp, z.M * z.Dp};
-            dy = {sp.dy, z.M, z.O, z.Op, z.M * z.Op};
-            gather({xp, z.M, z.D, ldx, sp.x, z.Dp, x.plane, sp.xr, nullptr,
-                    kept ? kRowScale : kRowSplit}, 2);
-            gather({dyp, z.M, z.O, lddy, sp.dy, z.Op, dy.plane, sp.dyr, nullptr, kRowSplit}, 3);
-        } else {
-            x = take(xp, z.M, z.D, ldx, sp.x, z.Dp, kPack, nullptr);
-            dy = take(dyp, z.M, z.O, lddy, sp.dy, z.Op, kPack, nullptr);
-        }
-        if (z.split)
-            if (int s = prepare(list, st)) return s;
-        wg = take(g, z.F, z.D, z.D, sp.wg, z.Dp, kTensorSplit, nullptr, 0);
-        wu = take(u, z.F, z.D, z.D, sp.wu, z.Dp, kTensorSplit, nullptr, 0);
-        wd = take(d, z.O, z.F, z.F, sp.wd, up(z.F, 8), kTensorSplit, nullptr, 1);
-        // dG | dU and H are scaled row by row. In the weights' gradients, sums over rows, the rows'
-        // scales s cancel against x (and dy) rows divided by them: what is left is one power of two
-        // for all rows, and rows lose bits only as far as they are small in the sum.
-        auto weighted = [&](const void* p, int n, long long ld, __half* buf, long long pitch, int k) {
-            PrepItem it{p, z.M, n, ld, buf, pitch, z.M * pitch, nullptr, sp.max + 2 + k, kWeighted};
-            it.bounds = bounds();
-            for (int i = 0; i < 4; ++i) it.top[i] = sp.maxima[i], it.tops[i] = parts[i];
-            it.of_h = k;
-            list.add(it);
-        };
-        if (z.split && dwgu) weighted(xp, z.D, ldx, sp.xt, z.Dp, 0);
-        if (z.split && dwd) weighted(dyp, z.O, lddy, sp.dyt, z.Op, 1);
-        return prepare(list, st);
-    }
-    Bounds bounds() const {
-        return {sp.xr, sp.dyr, sp.max, {log2_up(z.D), log2_up(z.O)}, act == 1};
     }
     Args args(long long M, int N) const {
         Args p;
@@ -240,81 +158,65 @@ struct Ff {
         p.used = 0;
         return p;
     }
-    int step() const { return z.split ? 2 : 1; }
     void output(Args& p, void* C, long long ldc) const {
         p.C[0] = C;
         p.ldc = ldc;
     }
-    // a gate epilogue's output (dgu or, forward, H; and H beside dgu), and what it keeps in lane
-    // blocks; fp32: planes
-    int gate_output(Maps& maps, Args& p, __half* C, long long width, __half* H) const {
+    // a gate epilogue's output (dgu or, forward, H; and H beside dgu); fp32: planes
+    int gate_output(Maps& maps, Args& p, uint16_t* C, long long width, uint16_t* H) const {
         p.gu_half = up(z.M, 32) * z.Fp;
         p.H = H != nullptr;
-        p.h_rinv = sp.hr;
-        p.gu_rinv = sp.dgur;
-        p.bounds = bounds();
-        const int t = z.split ? ATOM_F16 : z.dtype;
-        for (int k = 0; k < step(); ++k) {
-            p.used |= 1u << (kOutMap + k) | (unsigned)p.H << (kHMap + k);
-            if (int s = make_out_map(&maps.m[kOutMap + k], C + k * z.M * width, t, width, z.M, width))
+        const int n = z.planes(), t = z.split ? ATOM_BF16 : z.dtype;
+        for (int k = 0; k < n; ++k) {
+            p.used |= 1u << (out_map(n) + k) | (unsigned)p.H << (h_map(n) + k);
+            if (int s = make_out_map(&maps.m[out_map(n) + k], C + k * z.M * width, t, width, z.M, width))
                 return s;
             if (!H) continue;
-            if (int s = make_out_map(&maps.m[kHMap + k], H + k * z.M * z.Fp, t, z.Fp, z.M, z.Fp))
+            if (int s = make_out_map(&maps.m[h_map(n) + k], H + k * z.M * z.Fp, t, z.Fp, z.M, z.Fp))
                 return s;
         }
         return ATOM_OK;
     }
     // [G | U] tiles of X
-    int gates(int epilogue, Args& p, __half* C, long long width, __half* H) {
+    int gates(int epilogue, Args& p, uint16_t* C, long long width, uint16_t* H) {
         const Choice c = z.gate;
-        const int k = step();
+        const int k = z.planes();
         Maps maps;
-        if (int s = put(maps, 0, x, false, 128, z.split)) return s;
-        if (int s = put(maps, k, wg, false, c.bn / 2, z.split)) return s;
-        if (int s = put(maps, 2 * k, wu, false, c.bn / 2, z.split)) return s;
+        if (int s = put(maps, 0, x, false, 128, k)) return s;
+        if (int s = put(maps, k, wg, false, c.bn / 2, k)) return s;
+        if (int s = put(maps, 2 * k, wu, false, c.bn / 2, k)) return s;
         p.ph[0] = {0, k, 2 * k, z.nk(z.D), 0, 0, c.bn / 2, 0};
-        p.rinv = sp.xr;
-        if (sp.wgr) p.cinv[0] = sp.wgr, p.cinv[1] = sp.wur;
-        else if (z.split) p.bmax = sp.max;
-        p.used = z.split ? 0x3f : 0x7;
+        p.used = (1u << 3 * k) - 1;
         if (int s = gate_output(maps, p, C, width, H)) return s;
         return launch(epilogue, c, z.split, maps, p, st, sums);
     }
     int forward(void* y, long long ldy, float* kept) {
         Args p = args(z.M, z.F);
         p.gu = kept;
-        p.w_inv = sp.maxima[0], p.n_w_inv = parts[0];
-        __half* out = z.split ? sp.hp : sp.H;
-        if (int s = gates(kGate, p, out, z.Fp, nullptr)) return s;
-        const Operand h{out, z.M, z.F, z.Fp, z.M * z.Fp};
+        if (int s = gates(kGate, p, sp.H, z.Fp, nullptr)) return s;
+        const Operand h{sp.H, z.M, z.F, z.Fp, z.M * z.Fp};
         const Choice c = z.down;
-        const int k = step();
+        const int k = z.planes();
         Maps maps;
-        if (int s = put(maps, 0, h, false, 128, z.split)) return s;
-        if (int s = put(maps, k, wd, false, c.bn / 2, z.split)) return s;
+        if (int s = put(maps, 0, h, false, 128, k)) return s;
+        if (int s = put(maps, k, wd, false, c.bn / 2, k)) return s;
         Args q = args(z.M, z.O);
         q.ph[0] = {0, k, k, z.nk(z.F), 0, 0, c.bn, c.bn / 2};
-        q.rinv = sp.hr;
-        q.cinv[0] = sp.wdr;
         output(q, y, ldy);
         if (int s = launch(kStore, c, z.split, maps, q, st, sums)) return s;
         return add_up(sums, st);
     }
     int backward(const float* kept, void* dx, long long lddx, void* dwg, void* dwu, void* dwd) {
-        const int k = step();
-        __half* dgu = z.split ? sp.dgup : sp.dgu;
-        __half* hs = z.split ? sp.hp : sp.H;
-        __half* H = dwd ? hs : nullptr;
+        const int k = z.planes();
+        uint16_t *dgu = sp.dgu, *H = dwd ? sp.H : nullptr;
         {   // dH, and dG, dU, H either in its epilogue or in that of G and U
             const Choice c = z.dh;
             Maps maps;
-            if (int s = put(maps, 0, dy, false, 128, z.split)) return s;
-            if (int s = put(maps, k, wd, true, 64, z.split)) return s;
+            if (int s = put(maps, 0, dy, false, 128, k)) return s;
+            if (int s = put(maps, k, wd, true, 64, k)) return s;
             Args p = args(z.M, z.F);
             p.ph[0] = {0, k, k, z.nk(z.O), 0, 1, c.bn, c.bn / 2};
-            p.rinv = sp.dyr;
-            if (z.split) p.bmax = sp.max + 1;
-            p.used = z.split ? 0xf : 0x3;
+            p.used = (1u << 2 * k) - 1;
             if (kept) {
                 p.gu = const_cast<float*>(kept);
                 if (int s = gate_output(maps, p, dgu, 2 * z.Fp, H)) return s;
@@ -328,22 +230,18 @@ struct Ff {
             }
         }
         const Operand g{dgu, z.M, 2 * z.Fp, 2 * z.Fp, z.M * 2 * z.Fp};
-        const Operand h{hs, z.M, z.F, z.Fp, z.M * z.Fp};
-        Operand xt = x, dyt = dy;
-        if (z.split) xt.p = sp.xt, dyt.p = sp.dyt;
+        const Operand h{sp.H, z.M, z.F, z.Fp, z.M * z.Fp};
         if (dx) {
             const Choice c = z.dx;
             Maps maps;
-            if (int s = put(maps, 0, g.columns(0, z.F), false, 128, z.split)) return s;
-            if (int s = put(maps, k, g.columns(z.Fp, z.F), false, 128, z.split)) return s;
-            if (int s = put(maps, 2 * k, wg, true, 64, z.split)) return s;
-            if (int s = put(maps, 3 * k, wu, true, 64, z.split)) return s;
+            if (int s = put(maps, 0, g.columns(0, z.F), false, 128, k)) return s;
+            if (int s = put(maps, k, g.columns(z.Fp, z.F), false, 128, k)) return s;
+            if (int s = put(maps, 2 * k, wg, true, 64, k)) return s;
+            if (int s = put(maps, 3 * k, wu, true, 64, k)) return s;
             Args p = args(z.M, z.D);
             p.nphase = 2;
             p.ph[0] = {0, 2 * k, 2 * k, z.nk(z.F), 0, 1, c.bn, c.bn / 2};
             p.ph[1] = {k, 3 * k, 3 * k, z.nk(z.F), 0, 1, c.bn, c.bn / 2};
-            p.rinv = sp.dgur;
-            if (z.split) p.bmax = sp.max;
             output(p, dx, lddx);
             if (int s = launch(kStore, c, z.split, maps, p, st, sums)) return s;
         }
@@ -351,15 +249,14 @@ struct Ff {
             Choice c = z.dwgu;
             const bool two = dwg && dwu;
             Maps maps;
-            if (int s = put(maps, 0, g.columns(dwg ? 0 : z.Fp, z.F), true, 64, z.split)) return s;
+            if (int s = put(maps, 0, g.columns(dwg ? 0 : z.Fp, z.F), true, 64, k)) return s;
             if (two)
-                if (int s = put(maps, k, g.columns(z.Fp, z.F), true, 64, z.split)) return s;
-            if (int s = put(maps, 2 * k, xt, true, 64, z.split)) return s;
+                if (int s = put(maps, k, g.columns(z.Fp, z.F), true, 64, k)) return s;
+            if (int s = put(maps, 2 * k, x, true, 64, k)) return s;
             Args p = args(z.F, z.D);
             p.groups = two ? 2 : 1;
             p.ph[0] = {0, 2 * k, 2 * k, z.nk(z.M), 1, 1, c.bn, c.bn / 2};
             p.part = sp.part_gu;
-            p.factor = reinterpret_cast<const float*>(sp.max + 2);
             output(p, dwg ? dwg : dwu, z.D);
             p.C[1] = dwu;
             if (int s = launch(kStore, c, z.split, maps, p, st, sums)) return s;
@@ -367,12 +264,11 @@ struct Ff {
         if (dwd) {
             const Choice c = z.dwd;
             Maps maps;
-            if (int s = put(maps, 0, dyt, true, 64, z.split)) return s;
-            if (int s = put(maps, k, h, true, 64, z.split)) return s;
+            if (int s = put(maps, 0, dy, true, 64, k)) return s;
+            if (int s = put(maps, k, h, true, 64, k)) return s;
             Args p = args(z.O, z.F);
             p.ph[0] = {0, k, k, z.nk(z.M), 1, 1, c.bn, c.bn / 2};
             p.part = sp.part_d;
-            p.factor = reinterpret_cast<const float*>(sp.max + 3);
             output(p, dwd, z.F);
             if (int s = launch(kStore, c, z.split, maps, p, st, sums)) return s;
         }
@@ -385,7 +281,7 @@ struct Ff {
 int few_forward(Ff& f, const void* x, long long ldx, const void* wg, const void* wu, const void* wd,
                 void* y, long long ldy) {
     const FfSizes& z = f.z;
-    void* h = z.split ? (void*)f.sp.H32 : f.sp.H;
+    void* h = z.split ? (void*)f.sp.few_H : f.sp.H;
     few::Args p{};
     p.x = x, p.ldx = ldx, p.M = (int)z.M, p.K = z.D, p.N = z.F;
     p.w[0] = wg, p.w[1] = wu;
@@ -495,8 +391,6 @@ extern "C" int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t 
     if (z.few)
         return few_backward(f, x, ldx, wg, wu, wd, dy, lddy, dx, lddx, dwg, dwu, dwd);
     if (M <= few::kFewRows) kept = nullptr;          // the forward pass kept nothing
-    if (int s = f.inputs_bwd(x, ldx, wg, wu, wd, dy, lddy, kept != nullptr, dwg || dwu,
-                             dwd != nullptr))
-        return s;
+    if (int s = f.inputs(x, ldx, wg, wu, wd, dy, lddy, !kept || dwg || dwu)) return s;
     return f.backward(static_cast<const float*>(kept), dx, lddx, dwg, dwu, dwd);
 }

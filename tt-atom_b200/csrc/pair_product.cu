@@ -11,12 +11,13 @@
 // of B's, CTA 1 the others. Accumulators are fp32 in tensor memory, two buffers, so that the
 // epilogue of one tile runs beside the products of the next.
 //
-// fp32 operands (SPLIT) come as two fp16 planes: x = (hi + lo 2^-11) / s with s a power of two
-// per row or per tensor (22 significant bits for what lies within 2^-28 of the largest entry),
-// and hi hi + 2^-11 (hi lo + lo hi) is kept in two accumulators. The tensor core rounds every
-// addition toward zero, some 2^-24 of the sum a step, so a SPLIT tile is drained into registers
-// (added there to nearest) every kRound stages: 8 additions, which holds an fp32 result near 5e-7
-// of itself (2-norm) at any K; one accumulator at K = 1024 is 3.5e-6 off, 16 additions 9.7e-7.
+// fp32 operands (SPLIT) come as three bf16 planes, hi + mid + lo (typed.cuh), without scales: a result
+// does not depend on how large other rows, columns or requests are. A sum is six products: lo hi,
+// hi lo, mid mid, mid hi, hi mid and hi hi (what is left out is below 2^-23 of a term). The tensor core
+// rounds every addition toward zero, some 2^-24 of the sum a step, so a SPLIT tile is drained into
+// registers (added there to nearest) after every stage, and a stage begins with the small products:
+// four additions to a large sum. A slot of the ring holds one plane of a stage, lo first, and is free
+// again when its products are done.
 //
 // Bound by the tensor core where K and the tiles are many: the whole training step of 8,192 x 2,048
 // x 8,192 in bf16 (2.47 PFLOP in 6 launches) runs at 1.34 PFLOP/s, 95 % of what a library product
@@ -29,6 +30,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cstring>
 
 #include "pair_product.cuh"
 
@@ -37,7 +39,6 @@
 namespace atom {
 namespace pair {
 
-constexpr int kRound = 2;                            // stages between two drains of a SPLIT tile
 constexpr long long kWaitCycles = 2000000000LL;      // ~1 s
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -219,12 +220,6 @@ __device__ __noinline__ bool spoilt_row(const Args& p, int mt, long long m, int 
     return bad;
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-
 // What a warp knows of its tiles' requests: a lane a tile, 32 tiles ahead, so that no tile waits
 // for its own (a load takes two microseconds beside the tiles' traffic).
 struct Ahead {
@@ -336,12 +331,12 @@ struct Cfg {
     static constexpr int kThreads = 64 + 32 * EW;
     static constexpr int HB = BN / 2;
     static constexpr uint32_t kA = 128 * 128, kB = HB * 128;
-    static constexpr uint32_t kStage = (SPLIT ? 2 : 1) * (kA + kB);
-    static constexpr int S = SPLIT ? 4 : (EW == 16 ? 160 : 192) * 1024 / kStage;
-    // tensor memory: two accumulator buffers of BN columns, and SPLIT two for hi lo + lo hi
-    static_assert((SPLIT ? 4 : 2) * BN <= 512, "tensor memory");
+    static constexpr uint32_t kSlot = kA + kB;       // a stage (SPLIT: of one plane)
+    static constexpr int S = (EW == 16 ? 160 : 192) * 1024 / kSlot;
+    static constexpr int kBufs = SPLIT ? 4 : 2;      // accumulators in tensor memory
+    static_assert(kBufs * BN <= 512, "tensor memory");
     static constexpr uint32_t kOut = EW * 4096;
-    static constexpr uint32_t kSmem = S * kStage + kOut + 512 + 1024;
+    static constexpr uint32_t kSmem = S * kSlot + kOut + 512 + 1024;
     static_assert(kSmem <= 232448, "shared memory");
 };
 
@@ -358,26 +353,10 @@ __device__ __forceinline__ void stage_f32(uint8_t* buf, int lane, const float* v
         *reinterpret_cast<float4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) =
             make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
 }
-// By TMA, which leaves out what lies past the map's rows and columns. 16-bit blocks take the
-// two halves of the buffer in turn.
-template <bool F32, bool DEEP = false>
-__device__ __forceinline__ void store_tma(Out& o, int lane, const CUtensorMap* map, int x, int y,
-                                          int z, const float* v, int dtype) {
-    uint8_t* b = o.buf;
-    if constexpr (F32) {
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        __syncwarp();
-        stage_f32(b, lane, v);
-    } else {
-        b += (o.turn++ & 1u) * 2048;
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        __syncwarp();
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint4*>(b + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = make_uint4(
-                pair_w(v[8 * c], v[8 * c + 1], dtype), pair_w(v[8 * c + 2], v[8 * c + 3], dtype),
-                pair_w(v[8 * c + 4], v[8 * c + 5], dtype), pair_w(v[8 * c + 6], v[8 * c + 7], dtype));
-    }
+// By TMA, which leaves out what lies past the map's rows and columns.
+template <bool DEEP>
+__device__ __forceinline__ void send(const uint8_t* b, int lane, const CUtensorMap* map, int x, int y,
+                                     int z) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) {
@@ -393,23 +372,37 @@ __device__ __forceinline__ void store_tma(Out& o, int lane, const CUtensorMap* m
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
 }
-// A gate's output: typed, or (SPLIT) as planes in the row's scale s.
+template <bool DEEP = false>
+__device__ __forceinline__ void store_f32(Out& o, int lane, const CUtensorMap* map, int x, int y, int z,
+                                          const float* v) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+    stage_f32(o.buf, lane, v);
+    send<DEEP>(o.buf, lane, map, x, y, z);
+}
+// 16-bit blocks, `word(i)` columns 2 i and 2 i + 1, take the two halves of the buffer in turn.
+template <typename W>
+__device__ __forceinline__ void store_16(Out& o, int lane, const CUtensorMap* map, int x, int y, W word) {
+    uint8_t* b = o.buf + (o.turn++ & 1u) * 2048;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4*>(b + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+            make_uint4(word(4 * c), word(4 * c + 1), word(4 * c + 2), word(4 * c + 3));
+    send<false>(b, lane, map, x, y, 0);
+}
+// Typed, or (SPLIT) as planes, which uses up v.
 template <bool SPLIT>
 __device__ __forceinline__ void store_typed(Out& o, int lane, const CUtensorMap* map, int x, int y,
-                                            float* v, int dtype, float s) {
+                                            float* v, int dtype) {
     if constexpr (SPLIT) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] *= s;
-        store_tma<false>(o, lane, map, x, y, -1, v, ATOM_F16);
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-            const float2 hi = __half22float2(__floats2half2_rn(v[i], v[i + 1]));
-            v[i] = (v[i] - hi.x) * 2048.f;
-            v[i + 1] = (v[i + 1] - hi.y) * 2048.f;
-        }
-        store_tma<false>(o, lane, map + 1, x, y, -1, v, ATOM_F16);
+        for (int k = 0; k < kPlanes; ++k)
+            store_16(o, lane, map + k, x, y,
+                     [&](int i) { return take_plane(v[2 * i], v[2 * i + 1], k); });
     } else {
-        store_tma<false>(o, lane, map, x, y, -1, v, dtype);
+        store_16(o, lane, map, x, y, [&](int i) { return pair_w(v[2 * i], v[2 * i + 1], dtype); });
     }
 }
 // Where rows do not start on 16 bytes, or end inside them: row by row, a column a lane.
@@ -533,18 +526,20 @@ enum Form { kOut = 0, kRows = 1, kPart = 2, kBlocked = 3, kGelu = 1 };     // kG
 // The epilogue's last step on 32 columns n.. of the warp's rows m.. (m + lane is this lane's);
 // v0 (and v1: the u columns of a gate).
 template <int EPI, bool SPLIT, int OUT>
-__device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const Tile& ti, Out& o,
-                                         long long m, int n, int lane, float* v0, float* v1,
-                                         float sh, float sg) {
+__device__ __forceinline__ void finish32(const CUtensorMap* maps, const Args& p, const Tile& ti, Out& o,
+                                         long long m, int n, int lane, float* v0, float* v1) {
+    constexpr int P = SPLIT ? kPlanes : 1;
     if (m >= p.M || n >= p.N) return;
     if constexpr (EPI == kStore || EPI == kStoreLow) {
         const int z = ti.ks * p.groups + ti.grp;
         if constexpr (OUT == kBlocked)
             store_block(lane_block(p.blocked, m, n, p.Fp, lane), v0);
         else if constexpr (OUT == kPart)
-            store_tma<true, true>(o, lane, &maps.m[kPartMap], n, (int)m, z, v0, ATOM_F32);
+            store_f32<true>(o, lane, maps + part_map(P), n, (int)m, z, v0);
+        else if constexpr (OUT == kOut && SPLIT)
+            store_f32(o, lane, maps + out_map(P) + ti.grp, n, (int)m, 0, v0);
         else if constexpr (OUT == kOut)
-            store_tma<SPLIT>(o, lane, &maps.m[kOutMap + ti.grp], n, (int)m, -1, v0, p.dtype);
+            store_typed<false>(o, lane, maps + out_map(P) + ti.grp, n, (int)m, v0, p.dtype);
         else if (p.ksplit > 1)
             store_rows(o, lane, p.part, (z * p.M + m) * p.N + n, p.N, (int)min(32LL, p.M - m),
                        p.N - n, v0, ATOM_F32);
@@ -557,7 +552,7 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
             store_block(lane_block(p.gu, m, n, p.Fp, lane) + p.gu_half, v1);
         }
         gate32<OUT == kGelu>(v0, v1, p.act);
-        store_typed<SPLIT>(o, lane, &maps.m[kOutMap], n, (int)m, v0, p.dtype, sh);
+        store_typed<SPLIT>(o, lane, maps + out_map(P), n, (int)m, v0, p.dtype);
     } else {
         // v0, v1 = g, u (kGateBwdGU, dh from memory) or v0 = dh (kGateBwdDH, g and u from memory)
         float w[32];
@@ -570,98 +565,77 @@ __device__ __forceinline__ void finish32(const Maps& maps, const Args& p, const 
             load_block(lane_block(p.gu, m, n, p.Fp, lane) + p.gu_half, v1);
         }
         gate_bwd32<OUT == kGelu>(v0, v1, w, p.act);
-        store_typed<SPLIT>(o, lane, &maps.m[kOutMap], n, (int)m, v0, p.dtype, sg);
-        store_typed<SPLIT>(o, lane, &maps.m[kOutMap], p.Fp + n, (int)m, v1, p.dtype, sg);
-        if (p.H) store_typed<SPLIT>(o, lane, &maps.m[kHMap], n, (int)m, w, p.dtype, sh);
+        store_typed<SPLIT>(o, lane, maps + out_map(P), n, (int)m, v0, p.dtype);
+        store_typed<SPLIT>(o, lane, maps + out_map(P), p.Fp + n, (int)m, v1, p.dtype);
+        if (p.H) store_typed<SPLIT>(o, lane, maps + h_map(P), n, (int)m, w, p.dtype);
     }
 }
 
-// kLow: a lane's row of the four slices that a warp has of group g, times the adapter's scale and f:
-// into the tile's blocks (zeros where the row is of another one), and into the rows' own places.
-// fp32 blocks are planes, scaled row by row: a block's slices are all in one warp then (ranks of 64
-// at most; larger ones have a kernel of their own, from the rows).
+// kLow: a lane's row of the four slices that a warp has of group g, times the adapter's scale: into the
+// tile's blocks (zeros where the row is of another one), and into the rows' own places.
 template <bool SPLIT>
 __device__ __forceinline__ void low_store(const Args& p, const Low& low, int g, int part,
-                                          long long m0, int lane, int lead, float (*v)[32],
-                                          float f) {
+                                          long long m0, int lane, int lead, float (*v)[32]) {
     const int used = low.used(g, part);
     const long long m = m0 + lane;
     const long long stage0 = first_stage(low.mt, low.first, p.ext);
-    // a slice's 16 values of this row, in 16-bit elements
-    auto place = [&](int slice) {
-        return ((stage0 + (slice >> 2)) * 256 + (m & 255)) * 64 + (slice & 3) * 16;
-    };
-    float largest = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (i >= used) break;
         const int3 block = low.block(g, part * 4 + i);
-        const int sub = low.sub(part * 4 + i), c0 = sub * 16;
+        const int sub = low.sub(part * 4 + i), c0 = sub * 16, slice = block.x * p.ext + sub;
         const bool in = block.z == lead;
-        const float s = p.low_scale[block.y] * f;
+        const float s = p.low_scale[block.y];
         float* x = v[i >> 1] + (i & 1) * 16;
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = in ? x[j] * s : 0.f;
-        const long long at = place(block.x * p.ext + sub);
+        // the slice's 16 values of this row, in 16-bit elements
+        const long long at = ((stage0 + (slice >> 2)) * 256 + (m & 255)) * 64 + (slice & 3) * 16;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                // eight ranks at a time: Rs is a multiple of 8
             const int c = c0 + 8 * h;
-            const float* y = x + 8 * h;
+            float* y = x + 8 * h;
+            uint16_t* q = static_cast<uint16_t*>(p.low_block) + at + 8 * h;
             if constexpr (SPLIT) {
                 if (p.low_rows && in && c < p.Rs) {
-                    float* q = static_cast<float*>(p.low_rows) + m * p.Rs + c;
-                    *reinterpret_cast<float4*>(q) = make_float4(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<float4*>(q + 4) = make_float4(y[4], y[5], y[6], y[7]);
+                    float* r = static_cast<float*>(p.low_rows) + m * p.Rs + c;
+                    *reinterpret_cast<float4*>(r) = make_float4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<float4*>(r + 4) = make_float4(y[4], y[5], y[6], y[7]);
                 }
+                if (!p.low_block) continue;
+#pragma unroll
+                for (int k = 0; k < kPlanes; ++k, q += p.low_plane)
+                    *reinterpret_cast<uint4*>(q) =
+                        make_uint4(take_plane(y[0], y[1], k), take_plane(y[2], y[3], k),
+                                   take_plane(y[4], y[5], k), take_plane(y[6], y[7], k));
                 continue;
             }
             const uint4 w = make_uint4(pair_w(y[0], y[1], p.dtype), pair_w(y[2], y[3], p.dtype),
                                        pair_w(y[4], y[5], p.dtype), pair_w(y[6], y[7], p.dtype));
-            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.low_block) + at + 8 * h) = w;
+            *reinterpret_cast<uint4*>(q) = w;
             if (p.low_rows && in && c < p.Rs)
                 *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.low_rows) + m * p.Rs + c) = w;
         }
-        if (!SPLIT || !p.low_block) continue;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(x[j]));
-        if (sub < p.ext - 1) continue;               // the block's last slice: its planes
-        const float scale = pow2_scale(finite_bits(largest));
-        if (in) p.low_rinv[m] = pow2_inv(scale);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (k > i || k < i - sub) continue;
-            const float* y = v[k >> 1] + (k & 1) * 16;
-            __half* q = static_cast<__half*>(p.low_block) + place(block.x * p.ext + k - i + sub);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                __half2 hi[4], lo[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    split_half2(y[8 * h + 2 * j] * scale, y[8 * h + 2 * j + 1] * scale, hi[j], lo[j]);
-                *reinterpret_cast<uint4*>(q + 8 * h) = *reinterpret_cast<uint4*>(hi);
-                *reinterpret_cast<uint4*>(q + 8 * h + p.low_plane) = *reinterpret_cast<uint4*>(lo);
-            }
-        }
-        largest = 0.f;
     }
 }
 
 template <int BN, int EPI, bool SPLIT, int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>::kThreads, 1)
-    pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
+    pair_kernel(const __grid_constant__ MapArray<part_map(SPLIT ? kPlanes : 1) + 1> maps,
+                const __grid_constant__ Args p) {
     using CF = Cfg<BN, EPI, SPLIT>;
-    constexpr int S = CF::S, P = SPLIT ? 2 : 1;      // stages, planes
+    constexpr int S = CF::S, P = SPLIT ? kPlanes : 1, kBufs = CF::kBufs;
     // a gate's tile: columns 0 .. BN/2 of the accumulator are g, the others u
     constexpr bool GATED = EPI == kGate || EPI == kGateBwdGU;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* outbuf = smem + S * CF::kStage;
+    uint8_t* outbuf = smem + S * CF::kSlot;
     uint64_t* full = reinterpret_cast<uint64_t*>(outbuf + CF::kOut);
     uint64_t* empty = full + S;
-    uint64_t* accf = empty + S;      // [2] accumulator buffer full
-    uint64_t* acce = accf + 2;       // [2] and free again (CTA 0's: both CTAs' epilogue warps)
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acce + 2);
+    uint64_t* accf = empty + S;      // [kBufs] accumulator full
+    uint64_t* acce = accf + kBufs;   // [kBufs] and free again (CTA 0's: both CTAs' epilogue warps)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acce + kBufs);
     int* failed = reinterpret_cast<int*>(tmem_slot + 1);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -674,14 +648,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < kBufs; ++b) {
             mbar_init(&accf[b], 1);
             mbar_init(&acce[b], 2 * CF::EW);
         }
         *failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 2 && lane < kMaps && (p.used >> lane & 1))
+    if (warp == 2 && lane <= part_map(P) && (p.used >> lane & 1))
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.m[lane]))
                      : "memory");
     if (warp == 1) {
@@ -702,14 +676,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
             uint32_t it = 0, slot = 0, turn = 0;
             bool ok = true;
             const uint32_t full0 = peer_addr(smem_u32(full), 0);
-            // waits for a free stage and names its barrier of CTA 0
-            auto open = [&](uint32_t& dst, uint32_t& bar, uint32_t bytes = CF::kStage) {
+            // waits for a free slot and names its barrier of CTA 0
+            auto open = [&](uint32_t& dst, uint32_t& bar, uint32_t bytes = CF::kSlot) {
                 const uint32_t s = slot;
                 if (!mbar_wait(&empty[s], turn ^ 1u, p.err)) return false;
                 if (rank == 0 && elect_one())
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
                                      smem_u32(&full[s])), "r"(2 * bytes) : "memory");
-                dst = base + s * CF::kStage;
+                dst = base + s * CF::kSlot;
                 bar = full0 + s * 8;
                 ++it;
                 if (++slot == S) slot = 0, turn ^= 1u;
@@ -737,21 +711,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                             slot[i] = i < mine ? low.block(g, 4 * rank + i).y : 0;
                             r16[i] = low.sub(4 * rank + i) * 16;
                         }
-                        for (int kt = 0; kt < p.ph[0].nk; ++kt) {
-                            uint32_t dst, bar;
-                            if (!(ok = open(dst, bar, P * (CF::kA + n * 1024)))) break;
-                            if (!elect_one()) continue;
+                        for (int kt = 0; ok && kt < p.ph[0].nk; ++kt) {
                             const int k0 = kt * 64;
 #pragma unroll
-                            for (int pl = 0; pl < P; ++pl) {
-                                tma_load(dst + pl * CF::kA, &maps.m[p.ph[0].a + pl], k0, m0, bar);
+                            for (int pl = P - 1; pl >= 0; --pl) {
+                                uint32_t dst, bar;
+                                if (!(ok = open(dst, bar, CF::kA + n * 1024))) break;
+                                if (!elect_one()) continue;
+                                tma_load(dst, &maps.m[p.ph[0].a + pl], k0, m0, bar);
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const uint32_t db = dst + P * CF::kA + pl * CF::kB + i * 2048;
+                                for (int i = 0; i < 4; ++i)
                                     if (i < mine)
-                                        tma_load3(db, &maps.m[p.ph[0].b0 + pl], mn ? r16[i] : k0,
+                                        tma_load3(dst + CF::kA + i * 2048,
+                                                  &maps.m[p.ph[0].b0 + pl], mn ? r16[i] : k0,
                                                   mn ? k0 : r16[i], slot[i], bar);
-                                }
                             }
                         }
                     }
@@ -763,14 +736,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     const int n0 = ti.nt * ph.bstep + rank * ph.brank;
                     const CUtensorMap* ma = &maps.m[ph.a + P * ti.grp];
                     const CUtensorMap* mb = &maps.m[rank ? ph.b1 : ph.b0];
-                    for (int kt = sh.kt; kt < sh.end; ++kt) {
-                        uint32_t dst, bar;
-                        if (!(ok = open(dst, bar))) break;
+                    for (int kt = sh.kt; ok && kt < sh.end; ++kt) {
                         const int k0 = kt * 64;
-                        if (!elect_one()) continue;
 #pragma unroll
-                        for (int pl = 0; pl < P; ++pl) {
-                            const uint32_t da = dst + pl * CF::kA, db = dst + P * CF::kA + pl * CF::kB;
+                        for (int pl = P - 1; pl >= 0; --pl) {
+                            uint32_t da, bar;
+                            if (!(ok = open(da, bar))) break;
+                            if (!elect_one()) continue;
+                            const uint32_t db = da + CF::kA;
                             if (ph.a_mn) {
                                 tma_load(da, ma + pl, m0, k0, bar);
                                 tma_load(da + 8192, ma + pl, m0 + 64, k0, bar);
@@ -795,16 +768,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (n == i && st.next()) slots[i] = st.slot, ks[i] = st.at(), ++n;
-                    uint32_t dst, bar;
-                    if (n == 0 || !(ok = open(dst, bar, P * (CF::kA + n * (CF::kB / 4))))) break;
-                    if (!elect_one()) continue;
+                    if (n == 0) break;
 #pragma unroll
-                    for (int pl = 0; pl < P; ++pl) {
-                        tma_load(dst + pl * CF::kA, &maps.m[p.ext_a + pl], 0, (int)y, bar);
+                    for (int pl = P - 1; pl >= 0; --pl) {
+                        uint32_t dst, bar;
+                        if (!(ok = open(dst, bar, CF::kA + n * (CF::kB / 4)))) break;
+                        if (!elect_one()) continue;
+                        tma_load(dst, &maps.m[p.ext_a + pl], 0, (int)y, bar);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             if (i >= n) break;
-                            const uint32_t db = dst + P * CF::kA + pl * CF::kB + i * (CF::kB / 4);
+                            const uint32_t db = dst + CF::kA + i * (CF::kB / 4);
                             const CUtensorMap* mb = &maps.m[p.ext_b + pl];
                             if (p.ext_bmn) {
 #pragma unroll
@@ -817,7 +791,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     }
                 }
             }
-            // the last stages are read before this CTA may end
+            // the last slots are read before this CTA may end
             for (uint32_t k = it > S ? it - S : 0; ok && k < it; ++k)
                 ok = mbar_wait(&empty[k % S], (k / S) & 1u, p.err);
             if (!ok) *(volatile int*)failed = 1;
@@ -827,78 +801,79 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
             uint32_t slot = 0, turn = 0, round = 0;
             bool ok = true, open = false;
             uint32_t acc = 0, fresh = 0;
-            // SPLIT: hi lo + lo hi gather over all rounds of a tile's phases (and of its blocks),
-            // in two buffers by turns; the rounds' waits cover them
-            uint32_t low = tmem + 2 * BN, low_fresh = 0;
             const uint64_t base_k = sdesc(base, 0), base_mn = sdesc(base, 1);
-            auto begin = [&]() {         // a free accumulator buffer for the next round
-                const uint32_t b = round & 1u;
-                if (!mbar_wait(&acce[b], ((round >> 1) & 1u) ^ 1u, p.err)) return false;
+            auto begin = [&]() {         // a free accumulator for the next round
+                const uint32_t b = round % kBufs;
+                if (!mbar_wait(&acce[b], ((round / kBufs) & 1u) ^ 1u, p.err)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 acc = tmem + b * BN;
                 fresh = 0;
                 return open = true;
             };
             auto end = [&]() {
-                if (elect_one()) mma_commit(&accf[round & 1u]);
+                if (elect_one()) mma_commit(&accf[round % kBufs]);
                 ++round;
                 open = false;
             };
-            // One stage's products. Descriptors only add to their address field: one thread issues
-            // a product every ~40 clocks this way, against ~160 building each anew, which had
-            // bound the whole kernel (a product of 256 x 256 x 16 takes 128 clocks).
+            // One stage's products (SPLIT: a round of their own). Descriptors only add to their address
+            // field: one thread issues a product every ~40 clocks this way, against ~160 building each
+            // anew, which had bound the whole kernel (a product of 256 x 256 x 16 takes 128 clocks).
             auto stage = [&](uint64_t a, uint64_t b, uint32_t as, uint32_t bs, uint32_t id,
                              int steps) {
-                if (!mbar_wait(&full[slot], turn, p.err)) return false;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                a += slot * (CF::kStage >> 4);
-                b += slot * (CF::kStage >> 4);
-                if (elect_one()) {
+                if (!open && !begin()) return false;
+                uint64_t at[P], bt[P], *done[P];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (k < steps) {
-                            const uint64_t ad = a + k * as, bd = b + k * bs;
-                            const uint32_t add = k ? 1u : fresh;
-                            mma(acc, ad, bd, id, add);
-                            if constexpr (SPLIT) {
-                                mma(low, ad, bd + (CF::kB >> 4), id, k ? 1u : low_fresh);
-                                mma(low, ad + (CF::kA >> 4), bd, id, 1u);
+                for (int pl = P - 1; pl >= 0; --pl) {
+                    if (!mbar_wait(&full[slot], turn, p.err)) return false;
+                    at[pl] = a + slot * (CF::kSlot >> 4);
+                    bt[pl] = b + slot * (CF::kSlot >> 4);
+                    done[pl] = &empty[slot];
+                    if (++slot == S) slot = 0, turn ^= 1u;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (elect_one()) {
+                    auto product = [&](int i, int j) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (k < steps) {
+                                mma(acc, at[i] + k * as, bt[j] + k * bs, id, k ? 1u : fresh);
+                                fresh = 1;
                             }
-                        }
+                    };
+                    if constexpr (SPLIT) {
+                        product(2, 0);
+                        product(0, 2);
+                        mma_commit(done[2]);
+                        product(1, 1);
+                        product(1, 0);
+                        product(0, 1);
+                        mma_commit(done[1]);
                     }
-                    mma_commit(&empty[slot]);
+                    product(0, 0);
+                    mma_commit(done[0]);
                 }
                 __syncwarp();
-                fresh = low_fresh = 1;
-                if (++slot == S) slot = 0, turn ^= 1u;
+                fresh = 1;
+                if constexpr (SPLIT) end();
                 return true;
-            };
-            auto next_low = [&]() {
-                low = tmem + 2 * BN + (low == tmem + 2 * BN ? BN : 0);
-                low_fresh = 0;
             };
             Ahead ahead;
             uint32_t mine_k = 0;
             for (long long t = first; ok && t < p.tiles; t += pairs, ++mine_k) {
                 const Tile ti = tile_of(p, t);
-                int n = 0, left = 0;
+                int left = 0;
                 if (EPI == kStoreLow) {
                     left = ahead.get(p, mine_k, first, pairs).z * p.ext;
                     if (ti.ks != p.ksplit - 1) left = 0;
                 }
                 if constexpr (EPI == kLow) {
                     const int groups = Low(p, ti.mt).groups(), mn = p.ph[0].b_mn;
-                    const uint64_t b = mn ? sdesc_low(base + P * CF::kA)
-                                          : base_k + (P * CF::kA >> 4);
-                    const uint32_t id = idesc(BN, SPLIT ? 0 : p.bf16, 0, mn);
+                    const uint64_t b = mn ? sdesc_low(base + CF::kA) : base_k + (CF::kA >> 4);
+                    const uint32_t id = idesc(BN, SPLIT ? 1 : p.bf16, 0, mn);
                     for (int g = ti.ks; ok && g < groups; g += p.ksplit) {
-                        for (int kt = 0; ok && kt < p.ph[0].nk; ++kt, ++n) {
-                            if (SPLIT && open && n == kRound) end(), n = 0;
-                            ok = (open || begin()) &&
-                                 stage(base_k, b, 32 >> 4, mn ? 512 >> 4 : 32 >> 4, id, 4);
-                        }
-                        if (ok) end(), n = 0;
-                        if (SPLIT) next_low();
+                        for (int kt = 0; ok && kt < p.ph[0].nk; ++kt)
+                            ok = stage(base_k, b, 32 >> 4, mn ? 512 >> 4 : 32 >> 4, id, 4);
+                        if (ok && open) end();
                     }
                     continue;
                 }
@@ -906,28 +881,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     const int a_mn = p.ph[f].a_mn, b_mn = p.ph[f].b_mn;
                     const Share sh(p, ti, f);
                     const uint64_t a = a_mn ? base_mn : base_k;
-                    const uint64_t b = (b_mn ? base_mn : base_k) + (P * CF::kA >> 4);
+                    const uint64_t b = (b_mn ? base_mn : base_k) + (CF::kA >> 4);
                     const uint32_t as = a_mn ? 2048 >> 4 : 32 >> 4, bs = b_mn ? 2048 >> 4 : 32 >> 4;
-                    const uint32_t id = idesc(BN, SPLIT ? 0 : p.bf16, a_mn, b_mn);
-                    for (int kt = sh.kt; ok && kt < sh.end; ++kt, ++n) {
-                        if (SPLIT && open && n == kRound) end(), n = 0;
-                        ok = (open || begin()) && stage(a, b, as, bs, id, 4);
-                    }
+                    const uint32_t id = idesc(BN, SPLIT ? 1 : p.bf16, a_mn, b_mn);
+                    for (int kt = sh.kt; ok && kt < sh.end; ++kt) ok = stage(a, b, as, bs, id, 4);
                 }
-                if (SPLIT && ok && open) end(), next_low(), n = 0;
                 if constexpr (EPI == kStoreLow) {
-                    const uint64_t b = sdesc_slice(base + P * CF::kA, p.ext_bmn);
-                    const uint32_t id = idesc(BN, SPLIT ? 0 : p.bf16, 0, p.ext_bmn);
-                    for (; ok && left > 0; left -= 4, ++n) {
-                        if (SPLIT && open && n == kRound) end(), n = 0;
-                        ok = (open || begin()) &&
-                             stage(base_k, b, 32 >> 4, CF::kB >> 6, id, min(4, left));
-                    }
+                    const uint64_t b = sdesc_slice(base + CF::kA, p.ext_bmn);
+                    const uint32_t id = idesc(BN, SPLIT ? 1 : p.bf16, 0, p.ext_bmn);
+                    for (; ok && left > 0; left -= 4)
+                        ok = stage(base_k, b, 32 >> 4, CF::kB >> 6, id, min(4, left));
                 }
-                if (ok && open) {
-                    end();
-                    if (SPLIT) next_low();
-                }
+                if (ok && open) end();
             }
             if (!ok) *(volatile int*)failed = 1;
         }
@@ -943,12 +908,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
             __syncwarp();
             if (lane == 0)
                 asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                                 acce0 + 8 * (round & 1u)) : "memory");
+                                 acce0 + 8 * (round % kBufs)) : "memory");
             ++round;
         };
         auto filled = [&]() {
             const bool ok = __all_sync(0xffffffffu,
-                                       mbar_wait(&accf[round & 1u], (round >> 1) & 1u, p.err));
+                                       mbar_wait(&accf[round % kBufs], (round / kBufs) & 1u, p.err));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             return ok;
         };
@@ -958,17 +923,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
         bool ok = true;
         Out out{outbuf + (warp - 2) * 4096, 0};
         constexpr int kParts = GATED ? 2 * kChunks : kChunks;
-        uint32_t low = 2 * BN;
-        int e_g = 0, e_d = 0;        // of g and u, and of dh, beside x's and dy's rows
-        if constexpr (SPLIT && EPI == kGate) {
-            float w = 0.f;
-#pragma unroll 4
-            for (int i = lane; i < p.n_w_inv; i += 32) w = fmaxf(w, __uint_as_float(p.w_inv[i]));
-            e_g = bound_exp(warp_max(w)) + p.bounds.lg[0];
-        } else if constexpr (SPLIT && (EPI == kGateBwdGU || EPI == kGateBwdDH)) {
-            e_g = bound_exp(pow2_inv(pow2_scale(p.bounds.w[0]))) + p.bounds.lg[0];
-            e_d = bound_exp(pow2_inv(pow2_scale(p.bounds.w[1]))) + p.bounds.lg[1];
-        }
         Ahead ahead;
         uint32_t mine_k = 0;
         for (long long t = first; ok && t < p.tiles; t += pairs, ++mine_k) {
@@ -985,7 +939,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 Low low_(p, ti.mt);
                 for (int g = ti.ks; g < low_.groups(); g += p.ksplit) {
                     if (!(ok = filled())) break;
-                    const uint32_t ta = tmem + lanes + (round & 1u) * BN + c0;
+                    const uint32_t ta = tmem + lanes + (round % kBufs) * BN + c0;
                     float v[2][32];
                     tmem_ld32(ta, v[0]);
                     tmem_ld32(ta + 32, v[1]);
@@ -993,11 +947,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     pin32(v[0]);
                     pin32(v[1]);
                     drained();
-                    low_store<SPLIT>(p, low_, g, part, m, lane, lead, v, 1.f);
+                    low_store<SPLIT>(p, low_, g, part, m, lane, lead, v);
                 }
             } else if constexpr (!SPLIT) {
                 if (!(ok = filled())) break;
-                const uint32_t ta = tmem + lanes + (round & 1u) * BN + c0;
+                const uint32_t ta = tmem + lanes + (round % kBufs) * BN + c0;
 #pragma unroll 1
                 for (int k = 0; k < kChunks; ++k) {
                     float v0[32], v1[32];
@@ -1008,8 +962,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     if (GATED) pin32(v1);
                     if (k == kChunks - 1) drained();
                     if (EPI == kStoreLow && spoilt) spoil32(v0);
-                    finish32<EPI, SPLIT, OUT>(maps, p, ti, out, m, nb + 32 * k, lane, v0, v1, 1.f,
-                                         1.f);
+                    finish32<EPI, SPLIT, OUT>(maps.m, p, ti, out, m, nb + 32 * k, lane, v0, v1);
                 }
             } else {
                 // the tile's rounds summed in registers
@@ -1024,68 +977,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                 auto column = [&](int k) {
                     return GATED ? (k / kChunks) * (BN / 2) + (k % kChunks) * 32 : 32 * k;
                 };
-                // adds f times the next `rounds` rounds
-                auto add = [&](int rounds, float f) {
-                    const uint32_t tl = tmem + lanes + c0;
+                auto add = [&](int rounds) {
                     for (int r = 0; r < rounds; ++r) {
                         if (!filled()) return false;
-                        const uint32_t ta = tl + (round & 1u) * BN;
+                        const uint32_t ta = tmem + lanes + (round % kBufs) * BN + c0;
                         float x[2][32];
 #pragma unroll
                         for (int k = 0; k < kParts; ++k) tmem_ld32(ta + column(k), x[k]);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int k = 0; k < kParts; ++k) {
-                            pin32(x[k]);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[k][i] = fmaf(f, x[k][i], v[k][i]);
-                        }
-                        if (r == rounds - 1) {
-#pragma unroll
-                            for (int k = 0; k < kParts; ++k) tmem_ld32(tl + low + column(k), x[k]);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int k = 0; k < kParts; ++k) {
-                                pin32(x[k]);
-#pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    v[k][i] = fmaf(f * (1.f / 2048.f), x[k][i], v[k][i]);
-                            }
-                            low = low == 2 * BN ? 3 * BN : 2 * BN;
-                        }
+                        for (int k = 0; k < kParts; ++k) pin32(x[k]);
                         drained();
+#pragma unroll
+                        for (int k = 0; k < kParts; ++k)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[k][i] += x[k][i];
                     }
                     return true;
                 };
                 static_assert(!SPLIT || kParts == 2, "parts of a SPLIT tile");
-                const float sb = p.bmax ? pow2_inv(pow2_scale(*p.bmax)) : 1.f;
-                const float sa = p.rinv ? (m + lane < p.M ? p.rinv[m + lane] : 0.f) : *p.factor;
-                // A gate's scales come from bounds of its sums, K max|x| max|w|, and not from a pass
-                // over the values, which would be written and read once more in fp32 (18,000 x 128 x
-                // 512 training step: 281 us with that pass, 231 without). Planes hold values to 2^-51
-                // of their row's bound, so a row whose largest value is 2^-27 of it still has fp32's
-                // own rounding; Gaussian rows come to 2^-16 at K = 512 (2^-20 at 2,048 at the least).
-                float sh = 1.f, sg = 1.f;
-                if constexpr (EPI == kGate || EPI == kGateBwdGU || EPI == kGateBwdDH) {
-                    const bool in = m + lane < p.M, writes = in && ti.nt == 0 && part == 0;
-                    const int g = bound_exp(in ? p.bounds.x[m + lane] : 0.f) + e_g;
-                    const float inv = bound_inv(p.bounds.h(g));
-                    sh = pow2_inv(inv);
-                    if (writes) p.h_rinv[m + lane] = inv;
-                    if constexpr (EPI != kGate) {
-                        const int d = bound_exp(in ? p.bounds.dy[m + lane] : 0.f) + e_d;
-                        const float gu = bound_inv(p.bounds.gu(g, d));
-                        sg = pow2_inv(gu);
-                        if (writes) p.gu_rinv[m + lane] = gu;
-                    }
-                }
                 if constexpr (EPI == kLow) {
                     const int lead = m + lane < p.M ? p.row_lead[m + lane] : -1;
                     Low low_(p, ti.mt);
                     for (int g = ti.ks; g < low_.groups(); g += p.ksplit) {
                         clear();
-                        if (!(ok = add((p.ph[0].nk + kRound - 1) / kRound, 1.f))) break;
-                        low_store<SPLIT>(p, low_, g, part, m, lane, lead, v, sa * sb);
+                        if (!(ok = add(p.ph[0].nk))) break;
+                        low_store<SPLIT>(p, low_, g, part, m, lane, lead, v);
                     }
                     if (!ok) break;
                     continue;
@@ -1095,38 +1012,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<BN, EPI, SPLIT>:
                     const Share sh(p, ti, f);
                     stages += sh.end - sh.kt;
                 }
-                if (!(ok = add((stages + kRound - 1) / kRound, 1.f))) break;
-#pragma unroll
-                for (int k = 0; k < kParts; ++k)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[k][i] = v[k][i] * sa * sb;
-                if (p.cinv[0]) {
-#pragma unroll
-                    for (int k = 0; k < kParts; ++k) {
-                        const int n = nb + 32 * (GATED ? k % kChunks : k);
-                        const float* c = p.cinv[GATED && k >= kChunks] + n;
-                        if (n >= p.N) continue;
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const float4 x = __ldg(reinterpret_cast<const float4*>(c + i));
-                            v[k][i] *= x.x, v[k][i + 1] *= x.y;
-                            v[k][i + 2] *= x.z, v[k][i + 3] *= x.w;
-                        }
-                    }
-                }
-                if constexpr (EPI == kStoreLow) {
-                    const int es = ti.ks == p.ksplit - 1 ? (req.z * p.ext + 3) >> 2 : 0;
-                    // a row without an adapter has no scale (the workspace holds anything there)
-                    float f = m + lane < p.M && p.row_lead[m + lane] >= 0 ? p.ext_rinv[m + lane] : 0.f;
-                    f *= pow2_inv(pow2_scale(*p.ext_bmax));
-                    if (!(ok = add((es + kRound - 1) / kRound, f))) break;
-                }
+                if (EPI == kStoreLow && ti.ks == p.ksplit - 1) stages += (req.z * p.ext + 3) >> 2;
+                if (!(ok = add(stages))) break;
 #pragma unroll
                 for (int k = 0; k < kChunks; ++k) {
                     float u[32];         // kGateBwdDH: room for the u that it reads
                     if (EPI == kStoreLow && spoilt) spoil32(v[k]);
-                    finish32<EPI, SPLIT, OUT>(maps, p, ti, out, m, nb + 32 * k, lane, v[k],
-                                         GATED ? v[kChunks + k] : u, sh, sg);
+                    finish32<EPI, SPLIT, OUT>(maps.m, p, ti, out, m, nb + 32 * k, lane, v[k],
+                                              GATED ? v[kChunks + k] : u);
                 }
             }
         }
@@ -1186,193 +1079,49 @@ int add_up(Sums& sums, Chain& st) {
     return s;
 }
 
-// Operand preparation. A warp has eight float4 a lane: one row of up to 1024 columns, or two, four
-// or eight narrower ones, so that narrow rows keep as much in flight; wider rows take a block. Rows
-// stay in registers between their maximum and their planes (up to 8192 columns) and are read once.
-// Planes and packed rows are zero past the row's end up to the pitch. Bound by memory: the two
-// halves of a value cost five instructions, since what is not finite needs no care (its results are
-// not finite either way) except that a maximum leaves it out. 18,000 x 1,536 values: 43 us, 5.2 TB/s
-// read and written.
+// Operand preparation. A warp has eight float4 a lane: one row of up to 1024 columns, two, four or
+// eight narrower ones, so that narrow rows keep as much in flight, or 1024 columns of a wider one.
+// Planes and packed rows are zero past the row's end up to the pitch. Bound by memory.
 constexpr int kNV = 8;
 __host__ __device__ inline int prep_slots(const PrepItem& it) {      // float4 a lane of one row
-    const long long c = it.dld > it.cols ? it.dld : it.cols;
-    return c <= 128 ? 1 : c <= 256 ? 2 : c <= 512 ? 4 : 8;
+    return it.dld <= 128 ? 1 : it.dld <= 256 ? 2 : it.dld <= 512 ? 4 : 8;
 }
-__host__ __device__ inline bool prep_wide(const PrepItem& it) {
-    return it.dld > 1024 || it.cols > 1024;
+__host__ __device__ inline int prep_chunks(const PrepItem& it) {     // warps a row
+    return (int)((it.dld + 1023) / 1024);
 }
-__device__ __forceinline__ float4 prep_load(const float* src, int c, int cols, bool four) {
-    if (four) return c < cols ? *reinterpret_cast<const float4*>(src + c)
-                              : make_float4(0.f, 0.f, 0.f, 0.f);
-    return make_float4(c < cols ? src[c] : 0.f, c + 1 < cols ? src[c + 1] : 0.f,
-                       c + 2 < cols ? src[c + 2] : 0.f, c + 3 < cols ? src[c + 3] : 0.f);
-}
-__device__ __forceinline__ void prep_put(__half* hi, long long plane, const float4& v, float s) {
-    __half2 h[2], g[2];
-    split_half2(v.x * s, v.y * s, h[0], g[0]);
-    split_half2(v.z * s, v.w * s, h[1], g[1]);
-    *reinterpret_cast<uint2*>(hi) = *reinterpret_cast<uint2*>(h);
-    *reinterpret_cast<uint2*>(hi + plane) = *reinterpret_cast<uint2*>(g);
-}
-__device__ __forceinline__ float max_abs(float m, const float4& v) {      // passes over NaN
-    return fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-}
-__device__ __forceinline__ float max_finite(float m, const float4& v) {
-    return fmaxf(fmaxf(m, __uint_as_float(max(finite_bits(v.x), finite_bits(v.y)))),
-                 __uint_as_float(max(finite_bits(v.z), finite_bits(v.w))));
-}
-
-// A row's scale from its maximum; its inverse and what goes into `max` on the way.
-__device__ __forceinline__ float row_scale(const PrepItem& it, long long r, float mx, bool writes,
-                                           float& top) {
-    const float s = pow2_scale(__float_as_uint(mx)), inv = mx > 0.f ? pow2_inv(s) : 0.f;
-    if (writes) it.rinv[r] = inv;
-    top = fmaxf(top, inv);
-    return s;
-}
-// What a launch knows of all its rows: kTensorSplit's largest magnitude; kWeighted's power of two
-// 2^power, and the exponents that the weights and the sums' lengths put on g and u and on dh.
-struct Fixed {
-    unsigned max;
-    int power, g, d;
-};
-template <bool WEIGHTED>
-__device__ __forceinline__ float fixed_scale(const PrepItem& it, long long r, const Fixed& f) {
-    if (!WEIGHTED || it.mode == kTensorSplit) return pow2_scale(f.max);
-    const int g = bound_exp(it.bounds.x[r]) + f.g;
-    const float inv = bound_inv(it.of_h ? it.bounds.h(g)
-                                        : it.bounds.gu(g, bound_exp(it.bounds.dy[r]) + f.d));
-    const int k = (int)(__float_as_uint(inv) >> 23) - 127 - f.power;
-    return __uint_as_float((unsigned)(min(::max(k, -126), 126) + 127) << 23);
-}
-
-template <bool WEIGHTED>
-__device__ __forceinline__ void prep_narrow(const PrepItem& it, int blocks, const Fixed& fixed,
-                                            float& top) {
+__device__ __forceinline__ void prep_split(const PrepItem& it, int blocks) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int nv = prep_slots(it), rows = kNV / nv, shift = 31 - __clz(nv);
-    const int cols = (int)it.cols, dld = (int)it.dld, mode = it.mode;
-    const bool scans = mode == kRowSplit || mode == kMax || mode == kRowScale;
-    for (long long r0 = (blockIdx.x * 8LL + warp) * rows; r0 < it.rows; r0 += blocks * 8LL * rows) {
-        float4 x[kNV];
+    const int nv = prep_slots(it), rows = kNV / nv, shift = 31 - __clz(nv), chunks = prep_chunks(it);
+    const int cols = (int)it.cols, dld = (int)it.dld;
+    const long long units = (it.rows + rows - 1) / rows * chunks;
+    const bool four = aligned16(it.src) && it.ld % 4 == 0 && cols % 4 == 0;
+    for (long long u = blockIdx.x * 8LL + warp; u < units; u += blocks * 8LL) {
+        const long long r0 = chunks == 1 ? u * rows : u / chunks;
+        const int c0 = chunks == 1 ? 0 : (int)(u - r0 * chunks) * 1024;
         const float* src = static_cast<const float*>(it.src) + r0 * it.ld;
-        const bool four = aligned16(it.src) && it.ld % 4 == 0 && cols % 4 == 0;
-        // slot j: row r0 + j / nv, columns 4 (j % nv * 32 + lane) ..
-        if (four) {
-#pragma unroll
-            for (int j = 0; j < kNV; ++j) {
-                const int i = j >> shift, c = (((j & (nv - 1)) << 5) + lane) * 4;
-                x[j] = r0 + i < it.rows && c < cols
-                           ? *reinterpret_cast<const float4*>(src + i * it.ld + c)
-                           : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kNV; ++j) {
-                const int i = j >> shift, c = (((j & (nv - 1)) << 5) + lane) * 4;
-                x[j] = prep_load(src + i * it.ld, c, r0 + i < it.rows ? cols : 0, false);
-            }
-        }
-        float m[kNV];
-        if (scans) {
-            bool wild = false;
-#pragma unroll
-            for (int j = 0; j < kNV; ++j) {
-                m[j] = max_abs(0.f, x[j]);
-                wild |= isinf(m[j]);
-            }
-            if (__any_sync(0xffffffffu, wild))
-#pragma unroll
-                for (int j = 0; j < kNV; ++j) m[j] = max_finite(0.f, x[j]);
-            // over a row's slots, then over the lanes
-#pragma unroll
-            for (int o = 1; o < kNV; o *= 2)
-                if (o < nv)
-#pragma unroll
-                    for (int j = 0; j < kNV; ++j)
-                        if (!(j & o)) m[j] = m[j | o] = fmaxf(m[j], m[j | o]);
-#pragma unroll
-            for (int j = 0; j < kNV; ++j)
-                if ((j & (nv - 1)) == 0) m[j] = warp_max(m[j]);
-#pragma unroll
-            for (int o = kNV / 2; o > 0; o /= 2)
-                if (o < nv)
-#pragma unroll
-                    for (int j = 0; j < kNV; ++j)
-                        if ((j & (2 * o - 1)) == o) m[j] = m[j ^ o];
-            if (mode == kMax) {
-#pragma unroll
-                for (int j = 0; j < kNV; ++j) top = fmaxf(top, m[j]);
-                continue;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < kNV; ++j) {
-            const int i = j >> shift, k = j & (nv - 1), c = ((k << 5) + lane) * 4;
-            const long long r = r0 + i;
-            if (r >= it.rows) continue;
-            const float s = scans ? row_scale(it, r, m[j], k == 0 && lane == 0, top)
-                                  : fixed_scale<WEIGHTED>(it, r, fixed);
-            if (mode != kRowScale && c < dld)
-                prep_put(static_cast<__half*>(it.dst) + r * dld + c, it.plane, x[j], s);
-        }
-    }
-}
-
-template <bool WEIGHTED>
-__device__ __forceinline__ void prep_block(const PrepItem& it, int blocks, float* part,
-                                           const Fixed& fixed, float& top) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = threadIdx.x;
-    const int cols = (int)it.cols, dld = (int)it.dld, mode = it.mode;
-    const bool scans = mode == kRowSplit || mode == kMax || mode == kRowScale;
-    for (long long r = blockIdx.x; r < it.rows; r += blocks) {
-        const float* src = static_cast<const float*>(it.src) + r * it.ld;
-        const bool four = aligned16(src) && cols % 4 == 0;
         float4 x[kNV];
-        if (four) {
-#pragma unroll
-            for (int j = 0; j < kNV; ++j) x[j] = prep_load(src, 4 * (j * 256 + me), cols, true);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kNV; ++j) x[j] = prep_load(src, 4 * (j * 256 + me), cols, false);
-        }
-        const int held = 4 * kNV * 256;
-        float s;
-        if (scans) {
-            float mx = 0.f;
-            for (int pass = 0; pass < 2; ++pass) {
-                mx = 0.f;
-#pragma unroll
-                for (int j = 0; j < kNV; ++j) mx = pass ? max_finite(mx, x[j]) : max_abs(mx, x[j]);
-                for (int c = held + 4 * me; c < cols; c += 1024) {
-                    const float4 v = prep_load(src, c, cols, four);
-                    mx = pass ? max_finite(mx, v) : max_abs(mx, v);
-                }
-                mx = warp_max(mx);
-                __syncthreads();
-                if (lane == 0) part[warp] = mx;
-                __syncthreads();
-#pragma unroll
-                for (int k = 0; k < 8; ++k) mx = fmaxf(mx, part[k]);
-                if (!isinf(mx)) break;
-            }
-            if (mode == kMax) {
-                top = fmaxf(top, mx);
-                continue;
-            }
-            s = row_scale(it, r, mx, me == 0, top);
-            if (mode == kRowScale) continue;
-        } else {
-            s = fixed_scale<WEIGHTED>(it, r, fixed);
-        }
-        __half* hi = static_cast<__half*>(it.dst) + r * dld;
+        // slot j: row r0 + j / nv, columns c0 + 4 (j % nv * 32 + lane) ..
 #pragma unroll
         for (int j = 0; j < kNV; ++j) {
-            const int c = 4 * (j * 256 + me);
-            if (c < dld) prep_put(hi + c, it.plane, x[j], s);
+            const int i = j >> shift, c = c0 + (((j & (nv - 1)) << 5) + lane) * 4;
+            const int end = r0 + i < it.rows ? cols : 0;
+            const float* q = src + i * it.ld + c;
+            if (four)
+                x[j] = c < end ? *reinterpret_cast<const float4*>(q) : make_float4(0.f, 0.f, 0.f, 0.f);
+            else
+                x[j] = make_float4(c < end ? q[0] : 0.f, c + 1 < end ? q[1] : 0.f,
+                                   c + 2 < end ? q[2] : 0.f, c + 3 < end ? q[3] : 0.f);
         }
-        for (int c = held + 4 * me; c < dld; c += 1024)
-            prep_put(hi + c, it.plane, prep_load(src, c, cols, four), s);
+#pragma unroll
+        for (int j = 0; j < kNV; ++j) {
+            const int i = j >> shift, c = c0 + (((j & (nv - 1)) << 5) + lane) * 4;
+            if (r0 + i >= it.rows || c >= dld) continue;
+            uint16_t* q = static_cast<uint16_t*>(it.dst) + (r0 + i) * dld + c;
+#pragma unroll
+            for (int k = 0; k < kPlanes; ++k, q += it.plane)
+                *reinterpret_cast<uint2*>(q) =
+                    make_uint2(take_plane(x[j].x, x[j].y, k), take_plane(x[j].z, x[j].w, k));
+        }
     }
 }
 
@@ -1500,15 +1249,11 @@ __device__ __forceinline__ void find_pieces(const Pieces& p) {
     if (threadIdx.x == 0) reinterpret_cast<int*>(p.bad + a)[part] = found;
 }
 
-// KIND 0: 16-bit copies; 1: planes; 2: planes with kWeighted items. FINDS: and an adapters call's
-// pieces. Small operands are prepared in the time of a launch and of their code's first fetch: with
-// all of it in one kernel, 1,002 x 256 x 1,024 in fp32 took 26.2 us and 4,000 rows of adapters forward
-// and backward 101, with KIND alone 24.4 and 97, so 21.8 and 91 (with instances for wide rows and for
-// items that look for maxima as well, 21.6 and 90, but 12,011 rows of adapters 78.1 for 76.5).
-template <int KIND, bool FINDS>
+// SPLIT: planes, else 16-bit copies. FINDS: and an adapters call's pieces. Small operands are prepared
+// in the time of a launch and of their code's first fetch, so each has an instance.
+template <bool SPLIT, bool FINDS>
 __global__ void __launch_bounds__(256, 3)
     prep_kernel(const __grid_constant__ PrepList l, const __grid_constant__ Pieces pieces) {
-    __shared__ float part[8];
     let_next_start();
     wait_before();
     if constexpr (FINDS)
@@ -1516,80 +1261,31 @@ __global__ void __launch_bounds__(256, 3)
             find_pieces(pieces);
             return;
         }
-    const PrepItem& it = l.it[blockIdx.y];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (blockIdx.x >= l.blocks[blockIdx.y]) return;
-    if constexpr (KIND == 0) {
-        prep_pack(it, l.blocks[blockIdx.y]);
-        return;
-    }
-    float top = 0.f;
-    auto over_block = [&](float v) {             // the block's largest, in every thread
-        v = warp_max(v);
-        if (lane == 0) part[warp] = v;
-        __syncthreads();
-        v = part[lane & 7];
-        __syncthreads();
-        return warp_max(v);
-    };
-    auto largest = [&](const unsigned* of, int n) {
-        float v = 0.f;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += 256) v = fmaxf(v, __uint_as_float(of[i]));
-        return over_block(v);
-    };
-    Fixed fixed{};
-    if (it.mode == kTensorSplit) {
-        fixed.max = __float_as_uint(largest(it.part, it.parts));
-        if (blockIdx.x == 0 && threadIdx.x == 0) *it.max = fixed.max;
-    } else if (KIND == 2 && it.mode == kWeighted) {
-        // 2^power is no less than what a row's magnitude, in its scale, and its weight can come to
-        float v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = largest(it.top[k], it.tops[k]);
-        fixed.g = bound_exp(pow2_inv(pow2_scale(__float_as_uint(v[0])))) + it.bounds.lg[0];
-        fixed.d = bound_exp(pow2_inv(pow2_scale(__float_as_uint(v[1])))) + it.bounds.lg[1];
-        const int x = bound_exp(v[2]), dy = bound_exp(v[3]), g = x + fixed.g;
-        const int weight = it.of_h ? it.bounds.h(g) : it.bounds.gu(g, dy + fixed.d);
-        fixed.power = min(::max(weight + (it.of_h ? dy : x) - 30, -126), 126);
-        if (blockIdx.x == 0 && threadIdx.x == 0)
-            *it.max = (unsigned)(fixed.power + 127) << 23;
-    }
     const int blocks = l.blocks[blockIdx.y];
-    if (prep_wide(it)) prep_block<KIND == 2>(it, blocks, part, fixed, top);
-    else prep_narrow<KIND == 2>(it, blocks, fixed, top);
-    // the epilogue reads scales of columns 32 at a time
-    if (it.mode == kRowSplit && blockIdx.x == 0 && threadIdx.x < 32 &&
-        it.rows + lane < (it.rows + 31) / 32 * 32)
-        it.rinv[it.rows + lane] = 0.f;
-    if (it.part && (it.mode == kMax || it.mode == kRowSplit || it.mode == kRowScale)) {
-        __syncthreads();
-        top = over_block(top);
-        if (threadIdx.x == 0) it.part[blockIdx.x] = __float_as_uint(top);
-    }
+    if (blockIdx.x >= blocks) return;
+    if constexpr (SPLIT) prep_split(l.it[blockIdx.y], blocks);
+    else prep_pack(l.it[blockIdx.y], blocks);
 }
 
-int prep_blocks(const PrepItem& it) {
-    const int rows = it.mode == kPack ? 8 : prep_wide(it) ? 1 : 8 * (kNV / prep_slots(it));
-    return (int)std::max(1LL, std::min((it.rows + rows - 1) / rows, (long long)kPrepBlocks));
-}
 int prepare(PrepList& l, Chain& st, const Pieces* pieces) {
     if (l.n == 0 && !pieces) return ATOM_OK;
     int grid = 1;
-    for (int i = 0; i < l.n; ++i) grid = std::max(grid, l.blocks[i] = prep_blocks(l.it[i]));
+    bool split = false;              // a list is of one type
+    for (int i = 0; i < l.n; ++i) {
+        const PrepItem& it = l.it[i];
+        split = it.mode == kSplit;
+        const int rows = split ? kNV / prep_slots(it) : 1, chunks = split ? prep_chunks(it) : 1;
+        const long long warps = (it.rows + rows - 1) / rows * chunks;
+        l.blocks[i] = (int)std::max(1LL, std::min((warps + 7) / 8, (long long)kPrepBlocks));
+        grid = std::max(grid, l.blocks[i]);
+    }
     Pieces none{};
     if (pieces)
         grid = std::max(grid, (pieces->pieces + pieces->tiles + 7) / 8 +
                                   (pieces->other ? 4 * pieces->nad : 0));
-    bool weighted = false, split = false;        // a list is of one type
-    for (int i = 0; i < l.n; ++i) {
-        weighted |= l.it[i].mode == kWeighted;
-        split |= l.it[i].mode != kPack;
-    }
     const int s = st.launch("operand preparation",
-                            weighted ? prep_kernel<2, false>
-                            : split  ? pieces ? prep_kernel<1, true> : prep_kernel<1, false>
-                                     : pieces ? prep_kernel<0, true> : prep_kernel<0, false>,
+                            split ? pieces ? prep_kernel<true, true> : prep_kernel<true, false>
+                                  : pieces ? prep_kernel<false, true> : prep_kernel<false, false>,
                             dim3(grid, l.n + (pieces != nullptr)), 256, 0, l,
                             pieces ? *pieces : none);
     l.n = 0;
@@ -1672,7 +1368,7 @@ static int sm_count() {
 
 // The tile width and split that a count of clocks prefers: rounds of work items over the SM
 // pairs, each a tile's stages (512 clocks of tensor work at width 256, 256 at 128 but fed no
-// faster than ~300; SPLIT 12 products of 64) and its fill and drain, and for a split the pass
+// faster than ~300; SPLIT 24 products of 64) and its fill and drain, and for a split the pass
 // over the partial sums. Width 256 against 128: 60,000 x 256 x 1,024 bf16 forward 91 and 103 us,
 // 8,192 x 2,048 x 8,192 559 and 622; splits against none: 18,000 x 128 x 512 fp32 backward 139 and
 // 343 us, 200 x 1,024 x 4,096 bf16 forward 16.7 and 19.7.
@@ -1685,7 +1381,7 @@ Choice choose(long long M, int N, int nk, int groups, bool gated, bool split, bo
         if (split && bn == 256) continue;
         const int w = gated ? bn / 2 : bn;
         const long long tiles = mt * ((N + w - 1) / w);
-        const double stage = split ? 800 : bn == 256 ? 530 : 310;
+        const double stage = split ? 1600 : bn == 256 ? 530 : 310;
         for (int ks = 1; ks <= 32 && ks * 2 <= nk + 1; ++ks) {
             if (ks > 1 && (!may_split || tiles >= pairs)) break;
             const double fill = 2500 + (split || bn == 256 ? 1200 : 600);
@@ -1719,8 +1415,10 @@ static int run(const Maps& maps, const Args& p, Chain& st, Sums& sums) {
     }
     const long long pairs = sm_count() / 2;
     const int grid = 2 * (int)(p.tiles < pairs ? p.tiles : pairs);
+    MapArray<part_map(SPLIT ? kPlanes : 1) + 1> its;
+    memcpy(&its, &maps, sizeof(its));
     if (int s = st.launch("pair product", pair_kernel<BN, EPI, SPLIT, OUT>, dim3(grid), CF::kThreads,
-                          CF::kSmem, maps, p))
+                          CF::kSmem, its, p))
         return s;
     if (EPI != kLow && p.ksplit > 1) {
         sums.dtype = p.dtype;
@@ -1752,19 +1450,20 @@ int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain
                      : run<128, kLow, false, kOut>(maps, p, st, sums);
     if ((epilogue == kStore || epilogue == kStoreLow) && !p.blocked) {
         // TMA stores clip at 16 bytes, so columns have to end there too
+        const int planes = split ? kPlanes : 1, part = part_map(planes), out = out_map(planes);
         const int e = p.ksplit > 1 ? 4 : dtype_size(p.dtype);
         p.tma = p.N * e % 16 == 0;
         for (int g = 0; g < p.groups && p.ksplit == 1; ++g)
             p.tma = p.tma && aligned16(p.C[g]) && p.ldc * e % 16 == 0;
         if (p.tma && p.ksplit > 1) {
-            p.used |= 1u << kPartMap;
-            if (int s = encode_map(&maps.m[kPartMap], p.part, true, p.N, p.M, p.ksplit * p.groups,
+            p.used |= 1u << part;
+            if (int s = encode_map(&maps.m[part], p.part, true, p.N, p.M, p.ksplit * p.groups,
                                    p.N, p.M * p.N, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B))
                 return s;
         }
         for (int g = 0; p.tma && p.ksplit == 1 && g < p.groups; ++g) {
-            p.used |= 1u << (kOutMap + g);
-            if (int s = make_out_map(&maps.m[kOutMap + g], p.C[g], p.dtype, p.N, p.M, p.ldc))
+            p.used |= 1u << (out + g);
+            if (int s = make_out_map(&maps.m[out + g], p.C[g], p.dtype, p.N, p.M, p.ldc))
                 return s;
         }
     }

@@ -8,13 +8,18 @@
 namespace atom {
 namespace pair {
 
-constexpr int kMaps = 12;
-constexpr int kOutMap = 8, kHMap = 10, kPartMap = 11;   // outputs (two groups), H, partial sums
-struct Maps {
-    CUtensorMap m[kMaps];
+// Tensor maps of a product whose operands have `planes` planes (16-bit: one): up to four operands,
+// the outputs (two groups, or a gate's planes), H, partial sums.
+constexpr int out_map(int planes) { return 4 * planes; }
+constexpr int h_map(int planes) { return 5 * planes; }
+constexpr int part_map(int planes) { return 6 * planes; }
+template <int N>
+struct MapArray {
+    CUtensorMap m[N];
 };
+using Maps = MapArray<part_map(kPlanes) + 1>;
 
-// One run of K stages: operands by map index (SPLIT: the lo plane's map is the next one).
+// One run of K stages: operands by map index (SPLIT: the other planes' maps are the next ones).
 struct Phase {
     int a, b0, b1;           // A; B of CTA 0 and of CTA 1
     int nk;                  // 64-deep stages
@@ -26,20 +31,6 @@ struct Phase {
 // 16 columns a slice (ph[0].b0: the adapters' map). kStoreLow: kStore with low-rank blocks beside the
 // phases.
 enum Epilogue { kStore = 0, kGate = 1, kGateBwdGU = 2, kGateBwdDH = 3, kLow = 4, kStoreLow = 5 };
-
-// What bounds a gate's rows: those of x and dy, by 1 / scale, the largest magnitudes (bits) of
-// Wg | Wu and of Wd, and lg[k], 2^lg[k] being no less than D and O.
-struct Bounds {
-    const float *x, *dy;
-    const unsigned* w;
-    int lg[2], sigmoid;
-    // exponents of bounds of H and of dG | dU from those of g and u (x, W and D alone) and of dh:
-    // |act(g)| <= |g|, |act'(g)| < 2, or for the sigmoid 1 and 1/4
-    __device__ __forceinline__ int h(int g) const { return sigmoid ? g : 2 * g; }
-    __device__ __forceinline__ int gu(int g, int d) const {
-        return d + (sigmoid ? max(g - 2, 0) : g + 1);
-    }
-};
 
 // A row tile's first stage of low-rank blocks, by its number and its first request's: tiles need at
 // most a stage more than a quarter of their pieces' slices.
@@ -68,19 +59,8 @@ struct Args {
     float* gu;               // gate: kept g, and u gu_half further, lane blocks, or NULL
     long long gu_half;
     float* dh;               // kGateBwdGU: lane blocks
-    int H;                   // gate backward: H wanted (map kHMap; dG | dU: kOutMap, u at Fp)
+    int H;                   // gate backward: H wanted (its map; dG | dU: the output's, u at Fp)
     int Fp;
-    const float* rinv;       // SPLIT: 1 / scale of A's rows; NULL: `factor` for all of them
-    const float* factor;     // ... and the planes' scales together
-    const float* cinv[2];    // 1 / scale of B's rows (columns of C; u's second), or NULL:
-    const unsigned* bmax;    // B's tensor was scaled by this finite maximum (bits)
-    // SPLIT gates write planes (maps kOutMap, kHMap, the lo plane's behind each) in scales that are
-    // known before their values are:
-    float* h_rinv;           // out: 1 / scale of H's rows
-    float* gu_rinv;          // out, backward: of dG | dU's
-    const unsigned* w_inv;   // kGate: n_w_inv values whose largest is Wg's and Wu's 1 / scale (bits)
-    int n_w_inv;
-    Bounds bounds;           // kGate: lg and sigmoid alone
     // Low-rank blocks beside the phases: a row tile's requests that share an adapter have one, led
     // by the first of them, of `ext` slices of 16 ranks, zero in the other rows. A tile's blocks lie
     // slice by slice, four to a stage of 256 rows x 64, from stage first_stage() on.
@@ -96,13 +76,10 @@ struct Args {
     int* usable;             // from kLow on: as lead, but nad where the adapter is not finite
     const int4* bad;         // of an adapter: not all zero = not finite, its rows become NaN
     const float* low_scale;  // kLow: per adapter
-    void* low_block;         // kLow: [stage][256][64] typed (SPLIT: planes low_plane apart, NULL
-    long long low_plane;     // for more than 64 ranks), and SPLIT 1 / scale of the rows
-    float* low_rinv;
+    void* low_block;         // kLow: [stage][256][64] 16-bit (SPLIT: planes low_plane apart), or NULL
+    long long low_plane;
     void* low_rows;          // kLow: [M][Rs] typed, or NULL
     int Rs;
-    const float* ext_rinv;   // SPLIT: of the low-rank rows
-    const unsigned* ext_bmax;
     int* err;
 };
 
@@ -145,32 +122,17 @@ int add_up(Sums& sums, Chain& st);
 // sums of a split K go into the list.
 int launch(int epilogue, const Choice& c, bool split, Maps& maps, Args& p, Chain& st, Sums& sums);
 
-// Operand preparation, up to 6 matrices a launch.
-// kPack: 16-bit copy. kRowSplit: planes scaled row by row. kRowScale: the scales alone. kMax: the
-// largest finite magnitude. kTensorSplit: planes scaled by that. kWeighted: planes of row r times
-// the 1 / scale of what they are summed with, dG | dU's or H's, over a power of two.
-enum Prep { kPack = 0, kRowSplit = 1, kMax = 2, kTensorSplit = 3, kRowScale = 4, kWeighted = 5 };
+// Operand preparation, up to 6 matrices a launch: 16-bit copies (kPack) or an fp32 matrix's planes
+// (kSplit).
+enum Prep { kPack = 0, kSplit = 1 };
 struct PrepItem {
     const void* src;
     long long rows, cols, ld;
-    void* dst;               // [rows][dld], the lo plane `plane` elements behind
+    void* dst;               // [rows][dld], planes `plane` elements apart
     long long dld, plane;
-    float* rinv;             // kRowSplit, kRowScale: 1 / scale of each row, 0 for a row of zeros
-    // kMax, kRowSplit and kRowScale (the largest rinv[r]): a maximum of each block goes to
-    // part[block]. kTensorSplit: the largest of part[0 .. parts - 1], which its first block leaves
-    // in *max for the products, as kWeighted's does its power of two.
-    unsigned* max;
     int mode;
-    unsigned* part = nullptr;
-    int parts = 0;
-    // kWeighted: rows of x (dy where `of_h`); the maxima over blocks of the weights' magnitudes and
-    // of the rows' 1 / scale
-    Bounds bounds{};
-    const unsigned* top[4] = {};         // Wg | Wu, Wd, x, dy
-    int tops[4] = {}, of_h = 0;
 };
 constexpr int kPrepBlocks = 1184;            // of one launch and item, at most
-int prep_blocks(const PrepItem& it);          // how many maxima an item writes
 struct PrepList {
     PrepItem it[6];
     int n = 0, blocks[6];

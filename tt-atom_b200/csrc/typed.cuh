@@ -1,5 +1,5 @@
 // Shared by the typed operators (gated feed-forward, adapters): element types, their loads and
-// stores, the workspace cursor and a plain product.
+// stores, launches and the workspace cursor.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -24,34 +24,23 @@ __device__ __forceinline__ void store_f(void* p, long long i, float v, int dtype
     else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-// Bits of |x| where x is finite, else 0.
-__device__ __forceinline__ unsigned finite_bits(float x) {
-    const unsigned u = __float_as_uint(x) & 0x7FFFFFFFu;
-    return u < 0x7F800000u ? u : 0u;
-}
-// Power-of-two scale that puts a largest magnitude (its bits, finite) into [2^14, 2^15).
-__device__ __forceinline__ float pow2_scale(unsigned bits) {
-    if (bits == 0) return 1.f;
-    int sh = 141 - (int)(bits >> 23);
-    sh = sh < -126 ? -126 : (sh > 126 ? 126 : sh);
-    return __uint_as_float((unsigned)(sh + 127) << 23);
-}
-__device__ __forceinline__ float pow2_inv(float s) {
-    return __uint_as_float((254u << 23) - (__float_as_uint(s) & 0x7F800000u));
-}
-// What is scaled to 1 / inv lies below 2^bound_exp(inv); and 1 / scale for values below 2^e.
-__device__ __forceinline__ int bound_exp(float inv) {
-    return (int)(__float_as_uint(inv) >> 23) - 127 + 15;
-}
-__device__ __forceinline__ float bound_inv(int e) {
-    const int sh = e - 15 < -126 ? -126 : (e - 15 > 126 ? 126 : e - 15);
-    return __uint_as_float((unsigned)(sh + 127) << 23);
-}
-// y = hi + lo 2^-11 to 22 bits (lo is NaN where y is not finite).
-__device__ __forceinline__ void split_half2(float y0, float y1, __half2& hi, __half2& lo) {
-    hi = __floats2half2_rn(y0, y1);
-    const float2 back = __half22float2(hi);
-    lo = __floats2half2_rn((y0 - back.x) * 2048.f, (y1 - back.y) * 2048.f);
+// fp32 as three bf16 planes, x = hi + mid + lo exactly (8 significant bits each; hi is truncated, so
+// that it is finite where x is). They have fp32's range, so nothing is scaled and a value keeps its
+// bits whatever lies beside it, down to 2^-110 (where lo leaves the normal numbers). An infinity has a
+// NaN in mid, so what is not finite comes out as NaN.
+constexpr int kPlanes = 3;
+// Plane `k` of two values, the first in the lower half; takes it off them, planes in order.
+__device__ __forceinline__ uint32_t take_plane(float& x0, float& x1, int k) {
+    uint32_t w;
+    if (k == 0) {
+        w = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x0, x1);
+        w = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    x0 -= __uint_as_float(w << 16);
+    x1 -= __uint_as_float(w & 0xFFFF0000u);
+    return w;
 }
 
 // The last r in 0 .. n - 1 with value(r) <= key, or -1; value ascending, one warp.
