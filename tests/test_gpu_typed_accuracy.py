@@ -85,6 +85,16 @@ def test_sigmoid_gates_that_are_closed(t, M):
     assert off(y, exact(*args, "sigmoid")["y"])[0] <= bound
 
 
+@pytest.mark.parametrize("M", [5, 40])
+def test_sigmoid_gates_that_are_open(M):
+    # sigmoid'(14) = 8e-7 = s (1 - s), where 1 - s has no more than 4 bits left in fp32 once s is
+    # rounded; dwg is proportional to it. Bound as above, with the terms' magnitudes below 20.
+    args = closed_gates(M, 32, 64, 24, torch.float32, 14.0)
+    want = exact(*args, "sigmoid")["dwg"]
+    for got in run(*args, "sigmoid"):
+        assert off(got["dwg"], want)[0] <= 20 * ff.gamma(32) + 2.0 ** -20
+
+
 def outliers(kind, M, D, F, O):  # noqa: E741
     x, wg, wu, wd, dy = ff.make(M, D, F, O, torch.float32, seed=4)
     if kind == "a weight of 16":

@@ -77,7 +77,7 @@ __device__ __forceinline__ void finish(const Args& p, const float* red, int n0) 
         } else {
             const float s = sigmoid_f(v);
             a = p.act == 1 ? s : v * s;
-            da = p.act == 1 ? s * (1.f - s) : s * (1.f + v * (1.f - s));
+            da = s * (p.act == 1 ? sigmoid_f(-v) : 1.f + v * (1.f - s));
         }
         p.grads[at] = d * u * da;
         p.grads[all + at] = d * a;

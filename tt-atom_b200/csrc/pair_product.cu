@@ -506,7 +506,9 @@ __device__ __forceinline__ void gate_bwd32(float* g, float* u, float* d, int act
         const bool silu = act == 0;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            const float x = g[i], s = sigmoid_gate(x), ds = s * (1.f - s);
+            // s' = e / (1 + e)^2: of s (1 - s) an open gate's s, rounded, leaves nothing
+            const float x = g[i], e = __expf(-fabsf(x)), r = __fdividef(1.f, 1.f + e);
+            const float s = x >= 0.f ? r : e * r, ds = e * r * r;
             out(i, silu ? x * s : s, silu ? fmaf(x, ds, s) : ds);
         }
     } else {
