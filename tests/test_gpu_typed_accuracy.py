@@ -95,6 +95,20 @@ def test_sigmoid_gates_that_are_open(M):
         assert off(got["dwg"], want)[0] <= 20 * ff.gamma(32) + 2.0 ** -20
 
 
+@pytest.mark.parametrize("M", [5, 40])
+@pytest.mark.parametrize("level", [-3.0, -6.0, -9.0])
+def test_gelu_gates_that_are_closed(level, M):
+    # a Gaussian's tail: an error e in g is one of |g| e in it (1 + g^2 / 2 steps of fp32 for the
+    # exponential's own argument), |g| below 1.5 |level| and its terms' magnitudes below 2 |level|
+    args = closed_gates(M, 32, 64, 24, torch.float32, level)
+    want = exact(*args, "gelu")
+    top = 1.5 * abs(level)
+    bound = (top + 1) * 2 * abs(level) * ff.gamma(32) + (4 + top * top) * 2.0 ** -23
+    for got in run(*args, "gelu"):
+        for name in ("y", "dwu", "dwd"):
+            assert off(got[name], want[name])[0] <= bound, name
+
+
 def outliers(kind, M, D, F, O):  # noqa: E741
     x, wg, wu, wd, dy = ff.make(M, D, F, O, torch.float32, seed=4)
     if kind == "a weight of 16":
@@ -125,7 +139,7 @@ def outliers(kind, M, D, F, O):  # noqa: E741
     "a weight of 16", "a weight of 100 and a feature of 100", "a feature of 1,000 with small weights",
     "a constant feature without weights", "closed gates", "a large row",
     "a large weight beside small ones"])
-@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+@pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("M", [16, 17, 130])
 def test_fp32_keeps_fp32s_accuracy_beside_outliers(M, act, kind):
     """Every output keeps its bound of fp32, element by element, and is as a whole (y and dx, whose rows
