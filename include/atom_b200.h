@@ -501,8 +501,9 @@ int atom_orb_zbl(const float* ev, const int* Z, const int* src, const int* tgt, 
  * x, y, dy, dx are [M, width] with a leading dimension of at least the width (in elements);
  * weights and their gradients are dense; one call's operands have one type. Sums are fp32.
  * Any sizes and element-aligned pointers: operands whose rows do not start on 16 bytes are
- * copied to the workspace first. `ws`: ws_bytes of device memory, 256-byte aligned, as large as
- * the *_bytes query says, not used by two calls at a time. M = 0: no rows are written, weight
+ * copied to the workspace first. `ws`: ws_bytes of device memory, 256-byte aligned (other addresses
+ * are refused, as they are for `kept`), as large as the *_bytes query says, not used by two calls at
+ * a time. M = 0: no rows are written, weight
  * and adapter gradients are zeroed. Results do not change from call to call (no atomics in any
  * sum). A wait that expires leaves ATOM_PAIR_WAIT_CODE for atom_device_error. fp16 values past
  * 65504 become infinities, as everywhere in that type: the gated row is such a value.
@@ -543,8 +544,8 @@ int atom_adapted_linear_bytes(int dtype, int64_t M, int D, int O, int n_adapters
  * [nreq + 1] ascending and req_adapter [nreq] int32 on the device (bounds outside 0 .. M are
  * clamped). Requests may be empty, and several may have the same adapter. At most 2^14 adapters
  * and 2^22 requests. A NaN or infinity in an adapter stays with the requests that use it: where b
- * (in the backward pass a) is not finite, their rows may be NaN as a whole. kept (may be NULL):
- * what atom_adapted_linear_bwd needs to spare the product x a^T. */
+ * (in the backward pass a) is not finite, their rows may be NaN as a whole. kept (NULL, or device
+ * memory, 256-byte aligned): what atom_adapted_linear_bwd needs to spare the product x a^T. */
 int atom_adapted_linear_fwd(int dtype, const void* x, int64_t ldx, int64_t M, int D, int O,
                             const void* w, const void* a, const void* b, const float* scale,
                             int n_adapters, int R, const int* req_ptr, const int* req_adapter,

@@ -567,6 +567,8 @@ extern "C" int atom_adapted_linear_fwd(int dtype, const void* x, int64_t ldx, in
     Ad f{z, AdSpace(ws, z, false), (cudaStream_t)stream, req_ptr, req_adapter, scale, w, a, b};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "adapted_linear: the workspace needs %zu bytes",
                  f.sp.bytes);
+    ATOM_REQUIRE(aligned256(ws) && (M <= few::kFewRows || aligned256(kept)),
+                 "adapted_linear: ws and kept must be 256-byte aligned");
     if (M <= few::kFewRows) {
         // a few rows: the low-rank values first, then the projection with them in its epilogue;
         // nothing is kept, the backward pass computes S again
@@ -609,6 +611,8 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
     Ad f{z, AdSpace(ws, z, true), st, req_ptr, req_adapter, scale, w, a, b};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "adapted_linear: the workspace needs %zu bytes",
                  f.sp.bytes);
+    ATOM_REQUIRE(aligned256(ws) && (M <= few::kFewRows || aligned256(kept)),
+                 "adapted_linear: ws and kept must be 256-byte aligned");
     const bool grads = z.on && (da || db);
     // (2,048 x 2,048, rank 16, bf16: 20.5 us at 1 row and 31.2 at 16, against 33.2 and 43.2 by tiles)
     if (M <= few::kFewRows) {

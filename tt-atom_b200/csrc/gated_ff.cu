@@ -363,6 +363,8 @@ extern "C" int atom_gated_ff_fwd(int dtype, const void* x, int64_t ldx, int64_t 
     Ff f{z, FfSpace(ws, z, false), (cudaStream_t)stream, act};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
                  f.sp.bytes);
+    ATOM_REQUIRE(aligned256(ws) && (M <= few::kFewRows || aligned256(kept)),
+                 "gated_ff: ws and kept must be 256-byte aligned");
     if (z.few) return few_forward(f, x, ldx, wg, wu, wd, y, ldy);
     if (int s = f.inputs(x, ldx, wg, wu, wd)) return s;
     return f.forward(y, ldy, static_cast<float*>(kept));
@@ -388,6 +390,8 @@ extern "C" int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t 
     Ff f{z, FfSpace(ws, z, true), st, act};
     ATOM_REQUIRE(ws && ws_bytes >= f.sp.bytes, "gated_ff: the workspace needs %zu bytes",
                  f.sp.bytes);
+    ATOM_REQUIRE(aligned256(ws) && (M <= few::kFewRows || aligned256(kept)),
+                 "gated_ff: ws and kept must be 256-byte aligned");
     if (z.few)
         return few_backward(f, x, ldx, wg, wu, wd, dy, lddy, dx, lddx, dwg, dwu, dwd);
     if (M <= few::kFewRows) kept = nullptr;          // the forward pass kept nothing

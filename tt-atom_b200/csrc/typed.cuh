@@ -123,6 +123,8 @@ __device__ __forceinline__ void let_next_start() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+inline bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255u) == 0; }
+
 // Pieces of a caller's workspace, 256-byte aligned; with base NULL it only adds up the sizes.
 struct Cursor {
     char* base;
