@@ -1,8 +1,9 @@
-"""Where the typed operators' C entries end: alignments that a kernel would fault on are refused on the
-host, before any work."""
+"""Where the typed operators end: alignments that a kernel would fault on are refused on the host, before
+any work, and the largest sizes that the header names are taken."""
 import ctypes
 
 import pytest
+import torch
 
 from tt_atom import _lib as L
 
@@ -28,3 +29,24 @@ def test_workspace_and_kept_have_to_be_aligned(odd, dtype):
                 8, kept, ws, n, None)
         refused("256-byte", "atom_adapted_linear_bwd", dtype, P, 8, M, 8, 8, P, P, P, P, 2, 8, P, P, 2, P,
                 8, kept, P, 8, P, P, ws, n, None)
+
+
+@pytest.mark.parametrize("n, R, nreq, fits", [
+    (1 << 14, 8, 1 << 22, True), ((1 << 14) + 1, 8, 5, False), (5, 8, (1 << 22) + 1, False),
+    # (T + requests) ceil(R / 16) + 4 T < 2^25 - 4 with T = 1
+    (5, 128, (1 << 22) - 3, True), (5, 128, (1 << 22) - 2, False)])
+def test_the_most_adapters_and_requests(n, R, nreq, fits):
+    size = (L.c_size_t * 3)()
+    code = L.lib().atom_adapted_linear_bytes(1, 40, 8, 8, n, R, nreq, size)
+    assert code == (0 if fits else 1)
+    assert fits or "2^14 adapters, 2^22 requests" in L.last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("M", [4, 60])
+def test_as_many_adapters_as_there_may_be(M, t):
+    import test_gpu_adapters as ad
+    n = 1 << 14
+    args = ad.make([1] * M, [(n - 1 - 37 * i) % n for i in range(M)], n, 128, 8, 16, t, seed=M)
+    ad.both(args)

@@ -188,10 +188,10 @@ __global__ void __launch_bounds__(256) grads32_kernel(const __grid_constant__ Gr
     __shared__ __align__(16) float ts[32][36], xs[32][132];
     let_next_start();
     wait_before();
-    const int which = blockIdx.x >= p.tiles0;
-    const int c0 = (blockIdx.x - (which ? p.tiles0 : 0)) * 128, W = p.width[which];
-    const int chunks = (p.R + 31) / 32;
-    const int a = blockIdx.y / chunks, r0 = (blockIdx.y - a * chunks) * 32;
+    const int chunks = (p.R + 31) / 32, tile = blockIdx.x / chunks;
+    const int a = blockIdx.y, r0 = (blockIdx.x - tile * chunks) * 32;
+    const int which = tile >= p.tiles0;
+    const int c0 = (tile - (which ? p.tiles0 : 0)) * 128, W = p.width[which];
     const float* rows = static_cast<const float*>(p.rows[which]) + c0;
     const float* low = static_cast<const float*>(p.low[which]) + r0;
     const long long ld = p.ld[which];
@@ -529,7 +529,7 @@ int check_ad(int dtype, int64_t M, int D, int O, int nad, int R, int nreq) {
                  "adapted_linear: bad sizes");
     ATOM_REQUIRE(D < (1 << 24) && O < (1 << 24), "adapted_linear: widths above 2^24");
     ATOM_REQUIRE(R >= 1 && R <= 128, "adapted_linear: the rank must be 1..128");
-    ATOM_REQUIRE(nad < (1 << 14) && nreq < (1 << 22) &&
+    ATOM_REQUIRE(nad <= (1 << 14) && nreq <= (1 << 22) &&
                      first_stage((M + 255) / 256, nreq, (R + 15) / 16) < (1 << 23) - 1,
                  "adapted_linear: sizes above 2^14 adapters, 2^22 requests or 2^25 slices of 256 "
                  "rows by 16 ranks");
@@ -667,7 +667,7 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
     p.split = z.grad_split();
     p.dtype = dtype;
     const int tiles = p.tiles0 + ceil_div(p.width[1], 128);
-    const dim3 grid(tiles, (unsigned)n_adapters * (z.split ? (R + 31) / 32 : 1), p.split);
+    const dim3 grid(tiles * (z.split ? (R + 31) / 32 : 1), n_adapters, p.split);
     int rc;
     if (dtype == ATOM_BF16) rc = grads16<true>(p, grid, f.st);
     else if (dtype == ATOM_F16) rc = grads16<false>(p, grid, f.st);

@@ -52,7 +52,7 @@ def adapted_linear(x, w, a, b, scale, req_ptr, req_adapter, keep=False):
     w [O, D], a [n, R, D], b [n, O, R], scale [n] float32, req_ptr [nreq + 1] ascending and
     req_adapter [nreq] int32, all on x's device: a replayed graph sees what they hold then.
     Requests may be empty and may share an adapter; 1 <= R <= 128, at most 2^14 adapters and
-    2^22 requests. What is not finite in an adapter stays with its requests (whose rows may be
+    2^22 requests (above 96 ranks 2^22 - 3: include/atom_b200.h has the sum that has to fit). What is not finite in an adapter stays with its requests (whose rows may be
     NaN as a whole). Sums in float32. With ``keep`` returns
     (y, kept): what ``adapted_linear_bwd`` needs to spare the product x a^T."""
     sizes = code, M, D, O, n, R, nreq = _shapes(x, w, a, b, scale, req_ptr,  # noqa: E741
