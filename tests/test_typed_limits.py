@@ -50,3 +50,19 @@ def test_as_many_adapters_as_there_may_be(M, t):
     n = 1 << 14
     args = ad.make([1] * M, [(n - 1 - 37 * i) % n for i in range(M)], n, 128, 8, 16, t, seed=M)
     ad.both(args)
+
+
+@pytest.mark.gpu
+def test_a_wait_that_ran_out_raises_where_results_are_read_back():
+    import tt_atom
+    from tt_atom.feedforward import gated_ff
+    x = torch.ones(40, 64, device="cuda", dtype=torch.bfloat16)
+    gated_ff(x, x, x, x.T.contiguous())
+    tt_atom.check_device()
+    L.call("atom_pair_wait_selftest", 2_000_000, L.stream_ptr())          # ~1 ms
+    gated_ff(x, x, x, x.T.contiguous())
+    with pytest.raises(RuntimeError, match="bounded device-side wait"):
+        tt_atom.check_device()
+    y = gated_ff(x, x, x, x.T.contiguous())
+    tt_atom.check_device()
+    assert (y == y[0, 0]).all()

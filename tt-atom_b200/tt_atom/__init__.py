@@ -8,6 +8,9 @@ Drop-in surface of the reference package for this path:
   MultiCard, MultiCardSim        one process per GPU (tt_atom/batch.py:218,338)
   simulate.relax_atoms, md_atoms FIRE / Langevin, GPU-resident without ASE (simulate.py:15-74)
   radius_graph                   device neighbour list (tt_atom/geometry.py:48)
+  check_device                   raises if a kernel gave up a wait since the last check; what calls
+                                 feedforward or adapters, which return without synchronising, asks it
+                                 where it reads results back (the calculators do so by themselves)
   bundle_cache                   the reference's bundle cache layout (bundle_cache.py)
 """
 from .calculator import TTAtomCalculator
@@ -96,6 +99,9 @@ def __getattr__(name):
     if name in ("MultiCard", "MultiCardSim"):
         from . import batch
         return getattr(batch, name)
+    if name == "check_device":
+        from ._lib import check_device
+        return check_device
     if name == "radius_graph":
         from .graph import radius_graph
         return radius_graph

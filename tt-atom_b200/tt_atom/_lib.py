@@ -193,15 +193,16 @@ def call(name, *args):
 
 
 def check_device(stream=None):
-    """Reads (and clears) the device-side error code of the tensor-core kernels and raises
-    RuntimeError if a bounded wait expired since the last check: the results of every launch
-    since then are incomplete and must not be returned. Synchronises the stream."""
+    """Reads (and clears) the device-side error code of the current device's kernels that wait (the
+    tensor-core GEMMs, the streamed edge kernels, the typed operators) and raises RuntimeError if
+    a bounded wait expired since the last check: the results of every launch since then are
+    incomplete and must not be used. Synchronises the stream."""
     code = ctypes.c_int(0)
     call("atom_device_error", ctypes.byref(code), stream_ptr(stream))
     if code.value != 0:
         raise RuntimeError(
-            f"a bounded device-side wait in the tensor-core GEMM expired (code {code.value}); "
-            "the results of this evaluation are incomplete and were discarded")
+            f"a bounded device-side wait expired (code {code.value}); the results since the last "
+            "check are incomplete")
 
 
 def ptr(t):

@@ -54,7 +54,8 @@ def adapted_linear(x, w, a, b, scale, req_ptr, req_adapter, keep=False):
     Requests may be empty and may share an adapter; 1 <= R <= 128, at most 2^14 adapters and
     2^22 requests (above 96 ranks 2^22 - 3: include/atom_b200.h has the sum that has to fit). What is not finite in an adapter stays with its requests (whose rows may be
     NaN as a whole). Sums in float32. With ``keep`` returns
-    (y, kept): what ``adapted_linear_bwd`` needs to spare the product x a^T."""
+    (y, kept): what ``adapted_linear_bwd`` needs to spare the product x a^T. Does not synchronise;
+    ``tt_atom.check_device`` tells whether a kernel gave up a wait."""
     sizes = code, M, D, O, n, R, nreq = _shapes(x, w, a, b, scale, req_ptr,  # noqa: E741
                                                 req_adapter)
     ldx = row_stride("x", x)

@@ -102,7 +102,8 @@ def gated_ff(x, wg, wu, wd, act="silu", keep=False):
     dense. float32, bfloat16 or float16, sums in float32; the gated row h is rounded to the
     inputs' type before the second product (float32: it is not). With ``keep`` returns
     (y, kept): what ``gated_ff_bwd`` needs to spare the first two products. Runs on the current
-    stream of x's device, without synchronising."""
+    stream of x's device, without synchronising: call ``tt_atom.check_device`` where results are
+    read back, which raises if a kernel gave up a wait."""
     code, M, D, F, O = _shapes(x, wg, wu, wd, act)  # noqa: E741
     ldx = row_stride("x", x)
     here, stream = on_device(x)
