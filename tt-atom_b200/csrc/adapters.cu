@@ -24,23 +24,6 @@ namespace {
 
 using namespace pair;
 
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (BF16)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
-            "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
-            "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 constexpr int kStages = 4;           // of grads16_kernel
 // dA[a] = T^T x and dB[a] = (S^T dy)^T over the pieces of adapter a, in their order: blocks have
 // all ranks by 128 columns of x or dy, and the pieces are shared out over blocks (`split`) whose
@@ -436,7 +419,7 @@ struct Ad {
         p.Rs = z.Rs;
         // as many items as pairs of SMs, but no more than a tile may have groups
         const int groups = std::min(16, (z.nreq * p.ext + 7) / 8);
-        const int share = std::max(1, std::min(groups, 74 / z.tiles));
+        const int share = std::max(1, std::min(groups, pair_count() / z.tiles));
         return launch(kLow, {128, share, 0}, z.split, maps, p, st, sums);
     }
 

@@ -15,22 +15,6 @@
 namespace atom {
 namespace few {
 
-template <bool BF16>
-__device__ __forceinline__ void mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                    uint32_t b0, uint32_t b1) {
-    if constexpr (BF16)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
-            "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
-            "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // 8 (fp32: 4) elements of a row from k on, zeros past its end.
 __device__ __forceinline__ uint4 load16(const unsigned short* row, int k, int K, bool vec) {
     if (vec) return *reinterpret_cast<const uint4*>(row + k);
@@ -146,8 +130,8 @@ __global__ void __launch_bounds__(256) few16_kernel(const __grid_constant__ Args
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int j = 0; j < kMats; ++j) {
-                mma<BF16>(acc[j], a[u].x, b[u].x, a[u].y, b[u].y, v[u][j].x, v[u][j].y);
-                mma<BF16>(acc[j], a[u].z, b[u].z, a[u].w, b[u].w, v[u][j].z, v[u][j].w);
+                mma16816<BF16>(acc[j], a[u].x, b[u].x, a[u].y, b[u].y, v[u][j].x, v[u][j].y);
+                mma16816<BF16>(acc[j], a[u].z, b[u].z, a[u].w, b[u].w, v[u][j].z, v[u][j].w);
             }
     }
 #pragma unroll

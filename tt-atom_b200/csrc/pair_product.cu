@@ -1360,16 +1360,16 @@ int make_out_map(CUtensorMap* m, const void* p, int dtype, long long cols, long 
                       f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-static int sm_count() {
+int pair_count() {
     static std::atomic<int> count[64];
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 74;
     int n = count[dev].load(std::memory_order_relaxed);
     if (n == 0) {
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n = 148;
         count[dev].store(n, std::memory_order_relaxed);
     }
-    return n;
+    return n / 2;
 }
 
 // The tile width and split that a count of clocks prefers: rounds of work items over the SM
@@ -1379,7 +1379,7 @@ static int sm_count() {
 // 8,192 x 2,048 x 8,192 559 and 622; splits against none: 18,000 x 128 x 512 fp32 backward 139 and
 // 343 us, 200 x 1,024 x 4,096 bf16 forward 16.7 and 19.7.
 Choice choose(long long M, int N, int nk, int groups, bool gated, bool split, bool may_split) {
-    const int pairs = sm_count() / 2;
+    const int pairs = pair_count();
     const long long mt = (M + 255) / 256 * groups;
     Choice best{128, 1, 0};
     double least = 1e30;
@@ -1419,7 +1419,7 @@ static int run(const Maps& maps, const Args& p, Chain& st, Sums& sums) {
         }
         if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_relaxed);
     }
-    const long long pairs = sm_count() / 2;
+    const long long pairs = pair_count();
     const int grid = 2 * (int)(p.tiles < pairs ? p.tiles : pairs);
     MapArray<part_map(SPLIT ? kPlanes : 1) + 1> its;
     memcpy(&its, &maps, sizeof(its));

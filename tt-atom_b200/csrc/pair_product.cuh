@@ -105,6 +105,8 @@ int make_low_map(CUtensorMap* m, const void* p, long long cols, long long rows, 
 int make_out_map(CUtensorMap* m, const void* p, int dtype, long long cols, long long rows,
                  long long ld);
 
+int pair_count();            // CTA pairs that the current device runs at a time
+
 // The outputs of products whose K was split, to be added up in one launch.
 struct Sums {
     struct Item {
