@@ -499,7 +499,9 @@ int atom_orb_zbl(const float* ev, const int* Z, const int* src, const int* tgt, 
  * tt_atom/bundle_cache.py, and input adjoints only).
  *
  * x, y, dy, dx are [M, width] with a leading dimension of at least the width (in elements);
- * weights and their gradients are dense; one call's operands have one type. Sums are fp32. M is
+ * weights and their gradients are dense; one call's operands have one type. Sums are fp32; fp32
+ * products of more than 16 rows are made of three bf16 parts of each operand, all 24 bits of what is
+ * above 2^-110 in magnitude, and an infinity there comes out as NaN. M is
  * below 2^31 (adapters: less 256), widths are below 2^24.
  * Any sizes and element-aligned pointers: operands whose rows do not start on 16 bytes are
  * copied to the workspace first. `ws`: ws_bytes of device memory, 256-byte aligned (other addresses
@@ -526,7 +528,9 @@ int atom_gated_ff_fwd(int dtype, const void* x, int64_t ldx, int64_t M, int D, i
 
 /* VJP of atom_gated_ff_fwd: from dy [M, O], dx [M, D], dwg, dwu [F, D] and dwd [O, F]
  * (overwritten; each may be NULL). kept: as the forward call on the same inputs left it, or
- * NULL (the first two products are computed again). */
+ * NULL (the first two products are computed again). The gradients of the gate's two factors, and
+ * the gated row, are rounded to the type before the products that take them (fp32 and a few rows:
+ * not). */
 int atom_gated_ff_bwd(int dtype, const void* x, int64_t ldx, int64_t M, int D, int F, int O,
                       const void* wg, const void* wu, const void* wd, int act, const void* dy,
                       int64_t lddy, const void* kept, void* dx, int64_t lddx, void* dwg,
@@ -546,7 +550,9 @@ int atom_adapted_linear_bytes(int dtype, int64_t M, int D, int O, int n_adapters
  * clamped). Requests may be empty, and several may have the same adapter. At most 2^14 adapters,
  * 2^22 requests and, with T = ceil(M / 256), (T + requests) ceil(R / 16) + 4 T < 2^25 - 4. A NaN or infinity in an adapter stays with the requests that use it: where b
  * (in the backward pass a) is not finite, their rows may be NaN as a whole. kept (NULL, or device
- * memory, 256-byte aligned): what atom_adapted_linear_bwd needs to spare the product x a^T. */
+ * memory, 256-byte aligned): what atom_adapted_linear_bwd needs to spare the product x a^T. In 16
+ * bits and above 16 rows the low-rank row, scale and all, is rounded to the type before the product
+ * with b, and so is the backward pass's, before those with a and x. */
 int atom_adapted_linear_fwd(int dtype, const void* x, int64_t ldx, int64_t M, int D, int O,
                             const void* w, const void* a, const void* b, const float* scale,
                             int n_adapters, int R, const int* req_ptr, const int* req_adapter,

@@ -299,8 +299,8 @@ struct AdSizes {
                                  ((D + 127) / 128 + (O + 127) / 128);
         // shares of the rows, for some eight blocks an SM, forward and backward: 6,007 rows, 8 adapters
         // in bf16 took 162, 149, 134 and 145 us with 1, 2, 4 and 8; in fp32, 7,882 rows of 1,146 + 336
-        // columns, 2 adapters 280 us with 16 and 252 with 32, and 2,124 of 1,486 + 2,664 331 with 8 and
-        // 292 with 12
+        // columns, 2 adapters 287, 247 and 251 us with 8, 16 and 32, and 2,124 of 1,486 + 2,664 344,
+        // 336 and 337
         const long long s = blocks ? 1184 / blocks : 1;
         return (int)std::max(1LL, std::min({s, split ? 32LL : 16LL, (long long)pieces}));
     }
@@ -417,7 +417,9 @@ struct Ad {
         p.low_rows = kept;
         if (!blocks) p.usable = nullptr;
         p.Rs = z.Rs;
-        // as many items as pairs of SMs, but no more than a tile may have groups
+        // as many items as pairs of SMs, but no more than a tile may have groups (300 requests in 512
+        // rows, an adapter each, 1,024 x 1,024 in bf16: 69 us so, 96 with four a tile, 208 with one;
+        // 2,000 rows of 40 requests, rank 64, 512 x 512: 20.5, 20.5 and 26.7)
         const int groups = std::min(16, (z.nreq * p.ext + 7) / 8);
         const int share = std::max(1, std::min(groups, pair_count() / z.tiles));
         return launch(kLow, {128, share, 0}, z.split, maps, p, st, sums);
@@ -597,7 +599,9 @@ extern "C" int atom_adapted_linear_bwd(int dtype, const void* x, int64_t ldx, in
     ATOM_REQUIRE(aligned256(ws) && (M <= few::kFewRows || aligned256(kept)),
                  "adapted_linear: ws and kept must be 256-byte aligned");
     const bool grads = z.on && (da || db);
-    // (2,048 x 2,048, rank 16, bf16: 20.5 us at 1 row and 31.2 at 16, against 33.2 and 43.2 by tiles)
+    // (2,048 x 2,048, rank 16, bf16: 20.5 us at 1 row and 31.2 at 16, against 33.2 and 43.2 by tiles;
+    // an adapter a row, 16 rows against 17 by tiles: fp32 44 and 121 us, fp16 45 and 53, forward 16 and
+    // 72 in fp32, 10 and 27 in 16 bits)
     if (M <= few::kFewRows) {
         const int m = (int)M, shares = few::down_shares(O, D);
         if (z.on) {

@@ -6,8 +6,8 @@
 namespace atom {
 namespace few {
 
-// One tensor-core tile's rows. (fp32 with 32, measured against planes: 75 us for 58 at
-// 22 x 752 x 1280 backward, 248 for 171 at 27 x 1173 x 6032.)
+// One tensor-core tile's rows. (fp32 with 32, measured against planes: 75 us for 62 at
+// 22 x 752 x 1280 backward, 248 for 196 at 27 x 1173 x 6032.)
 constexpr int kFewRows = 16;
 
 struct Args {

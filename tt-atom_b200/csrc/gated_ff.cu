@@ -31,7 +31,8 @@ struct Operand {
 
 // Whether a call's rows are streamed past: 16 at most, where a tile of 256 would be all but empty
 // (1,024 x 4,096 in bf16, forward: 8.7 us at 1 row and 11.1 at 16 against 21.6 and 17.1 by tiles;
-// 256 x 1,024 in fp32, backward: 16 and 32 against 45 and 46). A 16-bit backward pass multiplies on
+// fp32, 16 rows against 17 by tiles: 41 and 55 us forward, 92 and 104 backward, at 256 x 1,024 14 and
+// 20, 34 and 45). A 16-bit backward pass multiplies on
 // the FMA pipe there: from 7 rows on, or 80 million products of rows and weights, tiles are faster
 // (1,024 x 4,096: 31 against 43 us at 1 row, 39 and 39 at 6, 63 and 36 at 16; 2,048 x 8,192: 92 and
 // 91 at 1 row, 97 and 83 at 2).

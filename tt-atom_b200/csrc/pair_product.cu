@@ -8,7 +8,7 @@
 // Operands are 16-bit, K-major (rows of K elements) or M/N-major (rows of M/N elements: the
 // transposed products of a backward pass, read as they lie), in 128-byte swizzled tiles that
 // TMA fetches and zero-fills past the ends. CTA 0 of a pair has rows 0..127 of the tile and half
-// of B's, CTA 1 the others. Accumulators are fp32 in tensor memory, two buffers, so that the
+// of B's, CTA 1 the others. Accumulators are fp32 in tensor memory, two buffers (SPLIT: four), so that the
 // epilogue of one tile runs beside the products of the next.
 //
 // fp32 operands (SPLIT) come as three bf16 planes, hi + mid + lo (typed.cuh), without scales: a result
@@ -20,9 +20,10 @@
 // again when its products are done.
 //
 // Bound by the tensor core where K and the tiles are many: the whole training step of 8,192 x 2,048
-// x 8,192 in bf16 (2.47 PFLOP in 6 launches) runs at 1.34 PFLOP/s, 95 % of what a library product
+// x 8,192 in bf16 (2.47 TFLOP in 6 launches) runs at 1.34 PFLOP/s, 95 % of what a library product
 // sustains under the power cap; 60,000 x 256 -> 2 x 1,024 with the gate at 1.1, bound by its
-// epilogue; a SPLIT product does three, at 0.9 of 1.7 PFLOP/s together at 4,011 x 672 x 2,632.
+// epilogue; a SPLIT sum's six products run at 1.19 PFLOP/s together at 4,011 x 672 x 2,632 forward and
+// at 1.49 at 8,192 x 2,048 x 4,096, bound by reading planes from L2 and by the tensor core.
 //
 // Warp 0 has TMA, warp 1 tensor memory and the products (CTA 0's issues for both), warps 2.. the
 // epilogue. Every wait is bounded: on expiry the kernel records a code, lets copies in
@@ -440,8 +441,7 @@ __device__ __forceinline__ void spoil32(float* v) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(0x7FC00000u);
 }
 // The gate and its gradient. Sigmoids from ex2.approx and rcp.approx, each good to 2 units in the
-// last place; what the exponent's own rounding adds, |g| 2^-24, is far below the products' own
-// error of 5e-7.
+// last place, beside |g| 2^-24 from the exponent's own rounding.
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -527,7 +527,7 @@ __device__ __forceinline__ void gate_bwd32(float* g, float* u, float* d, int act
 }
 
 // What an epilogue does is in the instance, since a launch begins with fetching its code: with all
-// of it in one, the training step of 18,000 x 128 x 512 in fp32 took 226 us, 209 so.
+// of it in one, the training step of 18,000 x 128 x 512 in fp32 took 8 % longer.
 enum Form { kOut = 0, kRows = 1, kPart = 2, kBlocked = 3, kGelu = 1 };     // kGelu: of gates
 // The epilogue's last step on 32 columns n.. of the warp's rows m.. (m + lane is this lane's);
 // v0 (and v1: the u columns of a gate).
@@ -1087,7 +1087,8 @@ int add_up(Sums& sums, Chain& st) {
 
 // Operand preparation. A warp has eight float4 a lane: one row of up to 1024 columns, two, four or
 // eight narrower ones, so that narrow rows keep as much in flight, or 1024 columns of a wider one.
-// Planes and packed rows are zero past the row's end up to the pitch. Bound by memory.
+// Planes and packed rows are zero past the row's end up to the pitch. Bound by memory: planes of
+// 18,000 x 1,536 values take 42 us, 6.6 TB/s read and written.
 constexpr int kNV = 8;
 __host__ __device__ inline int prep_slots(const PrepItem& it) {      // float4 a lane of one row
     return it.dld <= 128 ? 1 : it.dld <= 256 ? 2 : it.dld <= 512 ? 4 : 8;
@@ -1376,8 +1377,8 @@ int pair_count() {
 // pairs, each a tile's stages (512 clocks of tensor work at width 256, 256 at 128 but fed no
 // faster than ~300; SPLIT 24 products of 64) and its fill and drain, and for a split the pass
 // over the partial sums. Width 256 against 128: 60,000 x 256 x 1,024 bf16 forward 91 and 103 us,
-// 8,192 x 2,048 x 8,192 559 and 622; splits against none: 18,000 x 128 x 512 fp32 backward 139 and
-// 343 us, 200 x 1,024 x 4,096 bf16 forward 16.7 and 19.7.
+// 8,192 x 2,048 x 8,192 559 and 622; splits against none: 18,000 x 128 x 512 fp32 backward 159 and
+// 582 us, 200 x 1,024 x 4,096 bf16 forward 16.7 and 19.7.
 Choice choose(long long M, int N, int nk, int groups, bool gated, bool split, bool may_split) {
     const int pairs = pair_count();
     const long long mt = (M + 255) / 256 * groups;

@@ -48,12 +48,13 @@ def _bytes(device, *sizes):
 def adapted_linear(x, w, a, b, scale, req_ptr, req_adapter, keep=False):
     """y [M, O]: for the rows req_ptr[r] .. req_ptr[r + 1] - 1 of request r, with
     k = req_adapter[r], y = x w^T + scale[k] (x a[k]^T) b[k]^T; a request whose k is not in
-    0 .. n - 1 (-1, say) and rows of no request have x w^T alone. x [M, D] with any row stride,
-    w [O, D], a [n, R, D], b [n, O, R], scale [n] float32, req_ptr [nreq + 1] ascending and
+    0 .. n - 1 (-1, say) and rows of no request have x w^T alone. x [M, D] with any row stride from
+    D on, w [O, D], a [n, R, D], b [n, O, R], scale [n] float32, req_ptr [nreq + 1] ascending and
     req_adapter [nreq] int32, all on x's device: a replayed graph sees what they hold then.
     Requests may be empty and may share an adapter; 1 <= R <= 128, at most 2^14 adapters and
     2^22 requests (above 96 ranks 2^22 - 3: include/atom_b200.h has the sum that has to fit). What is not finite in an adapter stays with its requests (whose rows may be
-    NaN as a whole). Sums in float32. With ``keep`` returns
+    NaN as a whole). Sums in float32; 16-bit types round the low-rank row, scale and all, before the
+    product with b (above 16 rows). With ``keep`` returns
     (y, kept): what ``adapted_linear_bwd`` needs to spare the product x a^T. Does not synchronise;
     ``tt_atom.check_device`` tells whether a kernel gave up a wait."""
     sizes = code, M, D, O, n, R, nreq = _shapes(x, w, a, b, scale, req_ptr,  # noqa: E741
@@ -75,7 +76,8 @@ def adapted_linear_bwd(x, w, a, b, scale, req_ptr, req_adapter, dy, kept=None,
                        adapter_grads=True):
     """(dx, da, db) of ``adapted_linear`` from dy [M, O], in the inputs' type; the shared w has
     no gradient here (it is what the adapters leave fixed). An adapter of no request has zeros.
-    Without ``adapter_grads`` the last two are None. ``kept``: what
+    Without ``adapter_grads`` the last two are None. 16-bit types round the low-rank rows before
+    the products that take them (above 16 rows). ``kept``: what
     ``adapted_linear(..., keep=True)`` returned for the same inputs."""
     sizes = code, M, D, O, n, R, nreq = _shapes(x, w, a, b, scale, req_ptr,  # noqa: E741
                                                 req_adapter)

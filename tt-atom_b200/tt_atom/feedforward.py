@@ -1,10 +1,10 @@
 """The gated feed-forward block y = (act(x Wg^T) * (x Wu^T)) Wd^T and its backward pass.
 
-The block that the spectral feed-forward's gate (``atom_spectral_gate_fwd``) is the fixed-shape
-case of, for any widths, in fp32, bf16 and fp16, with the gradients of its weights: what a
-program needs to train or fine-tune a block and to run it in 16 bits. No counterpart in the
-reference, whose feed-forwards are ungated MLPs (tt_atom/grid.py) or the spectral block
-(tt_atom/spectral.py). The kernels are behind ``atom_gated_ff_fwd`` / ``atom_gated_ff_bwd``.
+For any widths, in fp32, bf16 and fp16, with the gradients of its weights: what a program needs
+to train or fine-tune such a block and to run it in 16 bits. It stands beside the feed-forwards
+of the models, which have gates of their own in fixed shapes and fp32
+(``atom_spectral_gate_fwd``) and do not call it. No counterpart in the reference, whose
+feed-forwards are ungated MLPs (tt_atom/grid.py) or the spectral block (tt_atom/spectral.py). The kernels are behind ``atom_gated_ff_fwd`` / ``atom_gated_ff_bwd``.
 As everywhere in this package gradients are functions of their own: autograd does not see them.
 """
 from __future__ import annotations
@@ -98,8 +98,8 @@ def _bytes(device, *sizes):
 
 def gated_ff(x, wg, wu, wd, act="silu", keep=False):
     """y [M, O] = (act(x wg^T) * (x wu^T)) wd^T for x [M, D], wg and wu [F, D], wd [O, F]; act:
-    "silu", "sigmoid" or "gelu" (the erf form). x may have any row stride; the weights are
-    dense. float32, bfloat16 or float16, sums in float32; the gated row h is rounded to the
+    "silu", "sigmoid" or "gelu" (the erf form). x may have any row stride from its width on; the
+    weights are dense. float32, bfloat16 or float16, sums in float32; the gated row h is rounded to the
     inputs' type before the second product (float32: it is not). With ``keep`` returns
     (y, kept): what ``gated_ff_bwd`` needs to spare the first two products. Runs on the current
     stream of x's device, without synchronising: call ``tt_atom.check_device`` where results are
@@ -121,7 +121,8 @@ def gated_ff_bwd(x, wg, wu, wd, dy, act="silu", kept=None, weight_grads=True):
     """(dx, dwg, dwu, dwd) of ``gated_ff`` from dy [M, O], in the inputs' type; the last three
     are None without ``weight_grads`` (the adjoint of the rows alone, as forces need it).
     ``kept`` is what ``gated_ff(..., keep=True)`` returned for the same inputs; without it the
-    first two products are computed again."""
+    first two products are computed again. 16-bit types round h and the gradients of the gate's
+    two factors before the products that take them (a few rows: not)."""
     code, M, D, F, O = _shapes(x, wg, wu, wd, act)  # noqa: E741
     check_like("dy", dy, (M, O), x, dense=False)
     ldx, lddy = row_stride("x", x), row_stride("dy", dy)
