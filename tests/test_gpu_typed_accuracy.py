@@ -196,3 +196,40 @@ def test_a_row_without_an_adapter_beside_large_ones_and_an_old_workspace():
            None, ws.data_ptr(), n[0], L.stream_ptr())
     want = ad.reference(x, w, a, b, scale, ptr, ids, dy)
     ad.check([y[15:]], {"y": [v[15:] for v in want["y"]]}, ["y"])
+
+
+def test_fp32_captured_and_replayed():
+    # two graphs at a time, each with its own workspace, on rows that change under them
+    a, b = ff.make(400, 128, 256, 128, torch.float32, seed=9), ff.make(400, 128, 256, 128, torch.float32, seed=8)
+    p = ad.make([90] * 4, [0, 1, 2, -1], 3, 72, 128, 64, torch.float32, seed=7)
+
+    def everything():
+        y, kept = gated_ff(*a[:4], keep=True)
+        z, kept2 = adapted_linear(*p[:7], keep=True)
+        return (y, *gated_ff_bwd(*a, kept=kept), z, *adapted_linear_bwd(*p, kept=kept2))
+    everything()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(everything())
+        graphs.append(g)
+    a[0].copy_(b[0])
+    p[6].copy_(torch.tensor([2, 2, -1, 0], dtype=torch.int32))
+    for g in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    want = everything()
+    for o in outs:
+        assert all(torch.equal(u, v) for u, v in zip(o, want))
+
+
+def test_fp32_offsets_past_32_bits():
+    # 2.2e9 values of H: the last rows against the definition of those rows alone
+    M, D, F, O, last = 540_000, 64, 4104, 32, 300  # noqa: E741
+    x, wg, wu, wd, dy = ff.make(M, D, F, O, torch.float32, seed=5)
+    want = ff.reference(x[-last:], wg, wu, wd, dy[-last:], "silu")
+    ff.check([gated_ff(x, wg, wu, wd)[-last:]], want, ["y"])
+    dx = gated_ff_bwd(x, wg, wu, wd, dy, weight_grads=False)[0]
+    ff.check([dx[-last:]], want, ["dx"])
