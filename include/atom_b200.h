@@ -501,8 +501,8 @@ int atom_orb_zbl(const float* ev, const int* Z, const int* src, const int* tgt, 
  * x, y, dy, dx are [M, width] with a leading dimension of at least the width (in elements);
  * weights and their gradients are dense; one call's operands have one type. Sums are fp32; fp32
  * products of more than 16 rows are made of three bf16 parts of each operand, all 24 bits of what is
- * above 2^-110 in magnitude, and an infinity there comes out as NaN. M is
- * below 2^31 (adapters: less 256), widths are below 2^24.
+ * above 2^-110 in magnitude, and an infinity there comes out as NaN. M is below 2^31 (adapters: less
+ * 256), widths are below 2^24.
  * Any sizes and element-aligned pointers: operands whose rows do not start on 16 bytes are
  * copied to the workspace first. `ws`: ws_bytes of device memory, 256-byte aligned (other addresses
  * are refused, as they are for `kept`), as large as the *_bytes query says, not used by two calls at
@@ -548,11 +548,12 @@ int atom_adapted_linear_bytes(int dtype, int64_t M, int D, int O, int n_adapters
  * a [n_adapters, R, D], b [n_adapters, O, R], scale [n_adapters] fp32, 1 <= R <= 128; req_ptr
  * [nreq + 1] ascending and req_adapter [nreq] int32 on the device (bounds outside 0 .. M are
  * clamped). Requests may be empty, and several may have the same adapter. At most 2^14 adapters,
- * 2^22 requests and, with T = ceil(M / 256), (T + requests) ceil(R / 16) + 4 T < 2^25 - 4. A NaN or infinity in an adapter stays with the requests that use it: where b
- * (in the backward pass a) is not finite, their rows may be NaN as a whole. kept (NULL, or device
- * memory, 256-byte aligned): what atom_adapted_linear_bwd needs to spare the product x a^T. In 16
- * bits and above 16 rows the low-rank row, scale and all, is rounded to the type before the product
- * with b, and so is the backward pass's, before those with a and x. */
+ * 2^22 requests and, with T = ceil(M / 256), (T + requests) ceil(R / 16) + 4 T < 2^25 - 4. A NaN or
+ * infinity in an adapter stays with the requests that use it: where b (in the backward pass a) is
+ * not finite, their rows may be NaN as a whole. kept (NULL, or device memory, 256-byte aligned):
+ * what atom_adapted_linear_bwd needs to spare the product x a^T. In 16 bits and above 16 rows the
+ * low-rank row, scale and all, is rounded to the type before the product with b, and so is the
+ * backward pass's, before those with a and x. */
 int atom_adapted_linear_fwd(int dtype, const void* x, int64_t ldx, int64_t M, int D, int O,
                             const void* w, const void* a, const void* b, const float* scale,
                             int n_adapters, int R, const int* req_ptr, const int* req_adapter,

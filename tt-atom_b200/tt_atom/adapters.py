@@ -52,11 +52,12 @@ def adapted_linear(x, w, a, b, scale, req_ptr, req_adapter, keep=False):
     D on, w [O, D], a [n, R, D], b [n, O, R], scale [n] float32, req_ptr [nreq + 1] ascending and
     req_adapter [nreq] int32, all on x's device: a replayed graph sees what they hold then.
     Requests may be empty and may share an adapter; 1 <= R <= 128, at most 2^14 adapters and
-    2^22 requests (above 96 ranks 2^22 - 3: include/atom_b200.h has the sum that has to fit). What is not finite in an adapter stays with its requests (whose rows may be
-    NaN as a whole). Sums in float32; 16-bit types round the low-rank row, scale and all, before the
-    product with b (above 16 rows). With ``keep`` returns
-    (y, kept): what ``adapted_linear_bwd`` needs to spare the product x a^T. Does not synchronise;
-    ``tt_atom.check_device`` tells whether a kernel gave up a wait."""
+    2^22 requests (a little less above 112 ranks: include/atom_b200.h has the sum that has to fit).
+    What is not finite in an adapter stays with its requests (whose rows may be NaN as a whole).
+    Sums in float32; 16-bit types round the low-rank row, scale and all, before the product with b
+    (above 16 rows). With ``keep`` returns (y, kept): what ``adapted_linear_bwd`` needs to spare
+    the product x a^T. Does not synchronise; ``tt_atom.check_device`` tells whether a kernel gave up
+    a wait."""
     sizes = code, M, D, O, n, R, nreq = _shapes(x, w, a, b, scale, req_ptr,  # noqa: E741
                                                 req_adapter)
     ldx = row_stride("x", x)

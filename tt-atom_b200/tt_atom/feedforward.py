@@ -4,7 +4,8 @@ For any widths, in fp32, bf16 and fp16, with the gradients of its weights: what 
 to train or fine-tune such a block and to run it in 16 bits. It stands beside the feed-forwards
 of the models, which have gates of their own in fixed shapes and fp32
 (``atom_spectral_gate_fwd``) and do not call it. No counterpart in the reference, whose
-feed-forwards are ungated MLPs (tt_atom/grid.py) or the spectral block (tt_atom/spectral.py). The kernels are behind ``atom_gated_ff_fwd`` / ``atom_gated_ff_bwd``.
+feed-forwards are ungated MLPs (tt_atom/grid.py) or the spectral block (tt_atom/spectral.py).
+The kernels are behind ``atom_gated_ff_fwd`` / ``atom_gated_ff_bwd``.
 As everywhere in this package gradients are functions of their own: autograd does not see them.
 """
 from __future__ import annotations
